@@ -27,9 +27,12 @@ SOURCES = [
     "attn_tc_kernels.cu",
     "w8a16_kernels.cu",
     "w4a16_kernels.cu",
+    "kv4_kernels.cu",
+    "serve_kernels.cu",
     "backend.cc",
     "binding.cc",
     "binding_extra.cc",
+    "binding_serve.cc",
 ]
 
 NVCC_FLAGS = [

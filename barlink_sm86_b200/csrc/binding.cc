@@ -1049,6 +1049,7 @@ at::Tensor rope_attn_decode(const at::Tensor& qkv, const c10::optional<at::Tenso
 }  // namespace
 
 void bind_extra(py::module_& m);  // binding_extra.cc: attention prefill, W8A16, fused TP linears
+void bind_serve(py::module_& m);  // binding_serve.cc: 4-bit cache, request layouts, rules on logits
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "barlink for B200: NVLink peer-memory collectives, tcgen05 linears, decode kernels";
@@ -1144,4 +1145,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_readonly("n_host_staged", &blpg::BarlinkBackend::n_host_staged);
 
   bind_extra(m);
+  bind_serve(m);
 }

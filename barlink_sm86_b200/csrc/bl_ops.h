@@ -434,6 +434,60 @@ int bl_dlin_cluster(int n, int k, int tokens, int want);
 size_t bl_dlin_local_link_bytes(int tokens, int hidden);
 int bl_dlin_local_link_init(void* buf, int tokens, int hidden, void* stream, char* err, size_t errlen);
 
+/* ---- key/value cache in 4 bits (kv4_kernels.cu; layout: kv4.cuh) ----------------------------------
+ * cache: [n_blocks][nkv][block_size / 16] tiles of bl_kv4_tile_bytes(hd) bytes, hd 64 or 128, 16-byte aligned. */
+size_t bl_kv4_tile_bytes(int hd);
+/* RoPE on the q and k heads of rows [(nq + 2 nkv) * hd] (bf16 qkv, dense; or, with qkv null, the sum of nsplit fp32 slabs
+ * `slab` floats apart plus a bias), written to out (may be qkv); rows with a slot >= 0 go into the cache.  Angles in
+ * 64 bits.  Two rows of a call must not name the same slot. */
+int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nsplit, size_t slab, const void* bias, void* out,
+                        const int* positions, const int* slots, void* cache, int rows, int nq, int nkv, int hd, int block_size,
+                        int n_blocks, double theta, void* stream, char* err, size_t errlen);
+/* the cache's values at `slots` as bf16 k, v [rows][nkv][hd]; zeros for a slot below 0 or behind the cache */
+int bl_kv4_read(const void* cache, const int* slots, void* k, void* v, int rows, int nkv, int hd, int block_size, int n_blocks,
+                void* stream, char* err, size_t errlen);
+/* One query token per request against the cache; q rows q_stride elements apart.  A block-table entry that names no
+ * block leaves its tokens out; a request without tokens gets zeros. */
+int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, const int* block_tables, const int* ctx_lens, void* out,
+                            int batch, int nq, int nkv, int hd, int block_size, int n_blocks, int max_blocks, float scale, void* ws,
+                            size_t ws_bytes, void* stream, char* err, size_t errlen);
+
+/* ---- serving steps (serve_kernels.cu) ---------------------------------------------------------------
+ * Request lengths to row offsets cu [batch + 1], positions and slots [tokens], context lengths and block tables.  new_lens:
+ * tokens that a request gets now, below 0: it has ended and its blocks go back.  free_list: ring of n_free entries, free_range
+ * (first, count, missing); free_range_out may be free_range, ctx_lens may be past_lens. */
+int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range, int* cu,
+                    int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks, int n_free, int tokens,
+                    int block_size, void* stream, char* err, size_t errlen);
+/* counts int32 [rows][vocab] += 1 for every id behind a row's first prompt_lens ids; seen (bits) |= every id */
+int bl_count_tokens(const int* ids, const int* cu, const int* prompt_lens, int* counts, void* seen, int rows, int n_ids, int vocab,
+                    int reset, void* stream, char* err, size_t errlen);
+/* Rules on logits [rows][n] (bf16, or fp32): token id = column + offset.  seen: x / r or x * r; counted: - f * count - p; biases;
+ * mask bits (1: allowed).  out: the result in the logits' type (may be logits); part: bl_rules_chunks(rows, n) x rows (value, token)
+ * pairs, as bl_argmax_merge takes them; idx, val: arg max (lowest token; -1 where nothing is left). */
+typedef struct blRulesArgs {
+  const void* logits;
+  size_t ld;
+  int rows, n, fp32;
+  int vocab, offset;
+  void* out;
+  size_t ld_out;
+  void* part;
+  void* idx; /* int32 [rows], with val fp32 [rows]; or null */
+  void* val;
+  const void* penalties; /* fp32 [rows][3]: repetition, presence, frequency; or null (then counts and seen are not read) */
+  const void* counts;    /* int32 [rows][vocab] */
+  const void* seen;      /* bits [rows][ceil(vocab / 32)] */
+  const void* bias_ids;  /* int32 [rows][n_bias], below 0: none */
+  const void* bias;      /* fp32 [rows][n_bias] */
+  int n_bias;
+  const void* mask; /* bits, rows ld_mask words apart, mask_words of them valid; or null */
+  int mask_words;
+  size_t ld_mask;
+} blRulesArgs;
+int bl_rules_chunks(int rows, int n);
+int bl_logit_rules(const blRulesArgs* a, void* stream, char* err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

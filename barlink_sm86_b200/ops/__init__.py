@@ -9,6 +9,7 @@ reference's op surface is `w8a16_quant_act` / `w8a16_gemm`
 library or eager-framework kernels that its demos call.
 """
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -383,7 +384,195 @@ def w8a16_linear_split(x, wq, scale, bias=None, digits=None):
     return w8a16_linear(x, wq, scale, bias, digits=digits)
 
 
+# ---------------------------------------------------------------- the key/value cache in 4 bits
+def kv4_cache(n_blocks, nkv, hd, block_size=16, device="cuda"):
+    """An empty key/value cache of one layer in 4 bits: uint8 [n_blocks, nkv, block_size / 16, bytes of a tile].  hd 64 or 128,
+    block_size a multiple of 16.  Per token and head 20 / 16 * hd bytes (keys and values; bf16: 4 * hd): a group of 32 dims has codes
+    0..15 beside its least element and its step, both bf16.  What it holds is known to `rope_kv_write_q4`, `kv4_read` and
+    `paged_attn_decode_q4`."""
+    if hd not in (64, 128) or block_size < 16 or block_size % 16:
+        raise ValueError("the 4-bit cache is built for head_dim 64 and 128 and block sizes that are multiples of 16")
+    if n_blocks * block_size > 2 ** 31 - 1:
+        raise ValueError("the cache's slots do not fit 32 bits")
+    return ref.kv4_cache(n_blocks, nkv, hd, block_size, device)
+
+
+def rope_kv_write_q4(qkv, positions, slots, cache, nq, nkv, hd, block_size, theta, bias=None, out=None):
+    """`rope_kv_write` into a 4-bit cache: q and k heads rotated, k (rotated) and v rounded to bf16, quantised and stored at
+    `slots` (int32 [rows], = block * block_size + offset; a row whose slot is below 0 or behind the cache is not kept; no two rows may
+    name the same slot).  qkv: bf16 [rows, (nq + 2 nkv) * hd], rotated in place, or into `out` (which must not overlap qkv unless it is qkv); or
+    fp32 slabs [splits, rows, width] of the QKV linear, summed, `bias` added, into `out` or a new tensor.  Angles are computed in
+    64 bits.  slots and cache None: RoPE alone.  A group of 32 dims with an infinity or NaN is kept as NaN.  Returns the rotated rows."""
+    if qkv.is_cuda:
+        _count()
+        return _C().rope_kv_write_q4(qkv, positions, slots, cache, nq, nkv, hd, block_size, theta, bias, out)
+    _check_q4(qkv, positions, slots, cache, nq, nkv, hd, block_size)
+    x = qkv
+    if qkv.dim() == 3:
+        x = qkv.float().sum(0) + bias.float() if bias is not None else qkv.float().sum(0)
+        x = x.to(bias.dtype if bias is not None else torch.bfloat16)
+        out = torch.empty_like(x) if out is None else out
+    elif bias is not None:
+        # (the model's CPU path hands the bias along with whole rows, as it does to rope_kv_write)
+        x = (x.float() + bias.float()).to(x.dtype)
+    return ref.rope_kv_write_q4(x, positions, slots, cache, nq, nkv, hd, block_size, theta, qkv if out is None else out)
+
+
+def _check_q4(qkv, positions, slots, cache, nq, nkv, hd, block_size):
+    if hd not in (64, 128) or block_size < 16 or block_size % 16:
+        raise ValueError("the 4-bit cache is built for head_dim 64 and 128 and block sizes that are multiples of 16")
+    if qkv.shape[-1] != (nq + 2 * nkv) * hd or positions.numel() != qkv.shape[-2]:
+        raise ValueError("qkv must be [rows, (nq + 2 nkv) * hd] and positions [rows]")
+    if (slots is None) != (cache is None):
+        raise ValueError("slots and the cache go together")
+    if cache is not None and (cache.dtype != torch.uint8 or tuple(cache.shape[1:]) != (nkv, block_size // 16, 20 * hd)
+                              or slots.numel() != qkv.shape[-2]):
+        raise ValueError("the 4-bit cache is uint8 [blocks, nkv, block_size / 16, tile bytes] as kv4_cache makes it, slots [rows]")
+
+
+def kv4_read(cache, slots, hd, block_size=16):
+    """(k, v) bf16 [rows, nkv, hd]: what the 4-bit cache holds at `slots` (int32 [rows]); zeros for a slot below 0 or behind the
+    cache.  For dense attention over a cached prefix, and for moving requests elsewhere."""
+    if cache.is_cuda:
+        _count()
+        return _C().kv4_read(cache, slots, hd, block_size)
+    return tuple(ref.kv4_read(cache, slots, hd, block_size))
+
+
+def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, out=None):
+    """`paged_attn_decode` over a 4-bit cache: q bf16 [batch, >= nq * hd] (the first nq * hd columns; rows start on 16-byte boundaries),
+    block_tables int32 [batch, max_blocks], ctx_lens int32 [batch].  At most 16 query heads per KV head.  A table entry that names no
+    block leaves its tokens out; a request without tokens gets zeros.  Returns bf16 [batch, nq * hd]."""
+    if q.is_cuda:
+        _count()
+        return _C().paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, out)
+    y = ref.paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale)
+    if out is not None:
+        out.copy_(y)
+        return out
+    return y
+
+
+# ---------------------------------------------------------------- serving steps
+class PagedLayout(NamedTuple):
+    """Where a step's tokens go, see `paged_layout`."""
+    cu: torch.Tensor          # int32 [batch + 1]: a request's rows are cu[b] .. cu[b + 1]
+    positions: torch.Tensor   # int32 [tokens]; 0 behind the last row
+    slots: torch.Tensor       # int32 [tokens]; -1 behind the last row, and where a token has no block
+    ctx_lens: torch.Tensor    # int32 [batch]
+    free_range: torch.Tensor  # int32 [3]: first free entry, free entries, blocks that were missing
+
+
+def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size=16, into=None):
+    """Block tables, row offsets, positions and slots of a step, from the requests' lengths, on the GPU and in one launch.
+
+    new_lens int32 [batch]: tokens that a request gets now (0 too); below 0: it has ended, and the blocks in its table go back to
+    the free ones.  past_lens int32 [batch]: tokens in the cache before.  block_tables int32 [batch, max_blocks]: the entries of new pages
+    are written (in place), all others stay.  free_list int32 [blocks]: a ring of block ids, of which free_range (int32 [3]:
+    first, count, ignored) are free; blocks are taken from the front in the order of requests and pages, and given back behind the
+    last; those given back are free from the next call on.  tokens: rows of `positions` and `slots`, at least the sum of
+    new_lens (a token beyond them gets no row).  Where blocks run out, table entries and slots are -1 and free_range[2] counts
+    what was missing; pages beyond max_blocks get no block, their tokens slot -1.
+
+    into: a PagedLayout to write to; its ctx_lens may be past_lens, its free_range may be free_range (a step that is captured
+    in a graph and replayed).  1 to 8192 requests."""
+    if new_lens.is_cuda:
+        _count()
+        return PagedLayout(*_C().paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size,
+                                              None if into is None else list(into)))
+    r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size)
+    if into is None:
+        return PagedLayout(*r)
+    for t, v in zip(into, r):
+        t.copy_(v)
+    return into
+
+
+class LogitRules:
+    """Rules on the logits of a batch, one row each; any of them may be None.
+
+    penalties  fp32 [rows, 3]: repetition, presence, frequency (1, 0, 0: none).  A token that the row has seen has its logit
+               divided by the repetition penalty where it is above 0, multiplied elsewhere; one that the row has produced c times
+               loses frequency * c + presence.
+    counts     int32 [rows, vocab], seen int32 [rows, ceil(vocab / 32)] (a bit per token): what the penalties go by, kept by
+               `count_tokens`; a counted token is a seen one.
+    bias_ids   int32 [rows, entries] (below 0: no entry), bias fp32 [rows, entries]: added after the penalties; entries of the
+               same token add up, in their order.
+    mask       int32 [rows, >= ceil(vocab / 32)], bit t of word w: token 32 w + t may be chosen; all others become -inf.
+    """
+    __slots__ = ("penalties", "counts", "seen", "bias_ids", "bias", "mask", "vocab")
+
+    def __init__(self, penalties=None, counts=None, seen=None, bias_ids=None, bias=None, mask=None, vocab=None):
+        if penalties is not None and (counts is None or seen is None):
+            raise ValueError("penalties need the counts and seen tables")
+        if (bias_ids is None) != (bias is None):
+            raise ValueError("bias_ids and bias go together")
+        if vocab is None:
+            if counts is not None:
+                vocab = counts.shape[1]
+            elif mask is not None:
+                vocab = mask.shape[1] * 32
+            else:
+                vocab = 2 ** 31 - 1
+        self.penalties, self.counts, self.seen, self.vocab = penalties, counts, seen, vocab
+        self.bias_ids, self.bias, self.mask = bias_ids, bias, mask
+
+    @staticmethod
+    def empty(rows, vocab, device="cuda", bias_entries=0, masked=False):
+        """Tables of rules that change nothing yet, to be filled in place (a captured step reads them anew every time)."""
+        i32 = dict(dtype=torch.int32, device=device)
+        pen = torch.tensor([1.0, 0.0, 0.0], device=device).repeat(rows, 1)
+        words = -(-vocab // 32)
+        return LogitRules(pen, torch.zeros(rows, vocab, **i32), torch.zeros(rows, words, **i32),
+                          torch.full((rows, bias_entries), -1, **i32) if bias_entries else None,
+                          torch.zeros(rows, bias_entries, device=device) if bias_entries else None,
+                          torch.full((rows, words), -1, **i32) if masked else None, vocab)
+
+    def _args(self):
+        return self.penalties, self.counts, self.seen, self.bias_ids, self.bias, self.mask
+
+
+def count_tokens(rules, ids, cu=None, prompt_lens=None, reset=False):
+    """Adds tokens to the tables of `rules`: every one is seen, and one behind a row's first prompt_lens (int32 [rows]; None: 0) is
+    counted as produced.  ids int32 [rows]: one token per row; with cu int32 [rows + 1]: row b's are ids[cu[b]:cu[b + 1]].  Ids below 0
+    or beyond the vocabulary are passed over.  reset: the tables are emptied first."""
+    if rules.counts is None or rules.seen is None:
+        raise ValueError("count_tokens needs rules with the counts and seen tables")
+    if rules.counts.is_cuda:
+        _count()
+        _C().count_tokens(rules.counts, rules.seen, ids, cu, prompt_lens, reset)
+    else:
+        if cu is None and ids.numel() != rules.counts.shape[0]:
+            raise ValueError("ids must be one per row, or packed with their row offsets")
+        ref.count_tokens(rules.counts, rules.seen, ids, cu, prompt_lens, reset)
+
+
+def logits_process(logits, rules, offset=0, out=None):
+    """Logits [rows, n] (bf16 or fp32; column i is token i + offset) under `rules` (LogitRules), for a sampler behind: penalties, biases,
+    mask, each operation in fp32, rounded once to the logits' type.  out may be the logits.  Columns at or beyond the vocabulary are
+    -inf where there is a mask, else left as they are."""
+    if logits.is_cuda:
+        _count()
+        return _C().logit_rules(logits, 0, rules.vocab, offset, *rules._args(), out)[0]
+    y = ref.logit_rules(logits, rules.vocab, offset, *rules._args()).to(logits.dtype)
+    if out is not None:
+        out.copy_(y)
+        return out
+    return y
+
+
+def logits_argmax(logits, rules, offset=0):
+    """(token int32 [rows], value fp32 [rows]): the arg max of the logits under `rules`, taken before they are rounded and without
+    writing them.  The lowest token of equals; NaN is passed over; -1 where nothing above -inf is left."""
+    if logits.is_cuda:
+        _count(2)
+        return tuple(_C().logit_rules(logits, 1, rules.vocab, offset, *rules._args()))
+    return ref.pick(ref.logit_rules(logits, rules.vocab, offset, *rules._args()), offset)
+
+
 __all__ = [
     "linear", "linear_split", "k_splits", "TiledWeight", "tile_weight", "untile_weight", "rmsnorm", "rmsnorm_digits", "rope_kv_write", "rope", "silu_mul", "embedding", "argmax",
     "paged_attn_decode", "rope_attn_decode", "attention", "w8a16_linear", "w8a16_linear_split", "W8GroupScales", "prepare_w8_scales", "w4a16_linear", "w4a16_linear_split", "qknorm_rope", "layernorm_modulate", "gate_residual", "ref",
+    "kv4_cache", "rope_kv_write_q4", "kv4_read", "paged_attn_decode_q4", "PagedLayout", "paged_layout", "LogitRules", "count_tokens",
+    "logits_process", "logits_argmax",
 ]

@@ -6,6 +6,7 @@ compare against, and they are the CPU execution path that lets the models and
 the tensor-parallel plumbing run (and be tested over gloo) on a machine
 without a GPU.  Shapes and argument order match `barlink_sm86_b200.ops`.
 """
+import functools
 import math
 
 import torch
@@ -302,3 +303,202 @@ def w4_dequant(qweight, scales, qzeros, group_size=128):
 
 def w4a16_linear(x, qweight, scales, qzeros, group_size=128):
     return (x.float() @ w4_dequant(qweight, scales, qzeros, group_size).t()).to(x.dtype)
+
+
+# ---------------------------------------------------------------- the key/value cache in 4 bits
+# Layout (csrc/kv4.cuh): [blocks, nkv, block_size / 16, 20 * hd] bytes; a tile holds 16 tokens of a head.
+KV4_GROUP = 32
+
+
+@functools.lru_cache(maxsize=None)
+def _kv4_maps(hd):
+    """Byte and shift of every code of a tile, [16, hd] for keys and for values, and the bytes of the groups' step and low,
+    [16, hd / 32]."""
+    na = hd // KV4_GROUP
+    r, d = torch.arange(16)[:, None], torch.arange(hd)[None]
+    k = r * (hd // 2) + ((d // 8 % 4) * na + d // 32) * 4 + d % 8 // 2
+    v = 8 * hd + (r // 2) * hd + (d // 4 % 8 * na + d // 32) * 4 + (r % 2) * 2 + d % 4 // 2
+    a = torch.arange(na)[None]
+    kp, vp = (at * hd + r * na * 4 + a * 2 for at in (16, 18))
+    shift = (d % 2 * 4).expand(16, -1)
+    return {"k": (k, shift, kp, kp + 2 * na), "v": (v, shift, vp, vp + 2 * na)}
+
+
+def kv4_cache(n_blocks, nkv, hd, block_size, device):
+    return torch.zeros(n_blocks, nkv, block_size // 16, 20 * hd, dtype=torch.uint8, device=device)
+
+
+def kv4_quantise(x):
+    """[..., hd] -> codes [..., hd / 32, 32] (int64), low and step (bf16) [..., hd / 32].  A group whose range is no finite number: step 0,
+    low NaN."""
+    x = x.to(torch.bfloat16).float().unflatten(-1, (-1, KV4_GROUP))
+    low = x.amin(-1)
+    step = ((x.amax(-1) - low) / 15).to(torch.bfloat16)
+    fine = torch.isfinite(step.float()) & torch.isfinite(x).all(-1)
+    step, low = torch.where(fine, step, torch.zeros_like(step)), torch.where(fine, low, torch.full_like(low, math.nan))
+    codes = torch.where((step.float() > 0)[..., None], torch.round((x - low[..., None]) / step.float()[..., None]), torch.zeros_like(x))
+    return codes.clamp(0, 15).long(), low.to(torch.bfloat16), step
+
+
+def kv4_write(cache, slots, k, v, block_size):
+    """Rows k, v [rows, nkv, hd] into the cache at their slots (below 0 or behind the cache: not kept)."""
+    nkv, hd = k.shape[1:]
+    maps, tiles = _kv4_maps(hd), cache.view(-1, 20 * hd)
+    slots = slots.long()
+    ok = (slots >= 0) & (slots < cache.shape[0] * block_size)
+    slots, k, v = slots[ok], k[ok], v[ok]
+    inb = slots % block_size
+    tile = ((slots // block_size)[:, None] * nkv + torch.arange(nkv)) * (block_size // 16) + (inb // 16)[:, None]   # [rows, nkv]
+    r = inb % 16
+    for x, name in ((k, "k"), (v, "v")):
+        codes, low, step = kv4_quantise(x)
+        byte, shift, ps, pl = maps[name]
+        val = codes.flatten(-2) << shift[r][:, None]
+        rows = torch.zeros(*tile.shape, 20 * hd, dtype=torch.int64)
+        rows.scatter_add_(2, byte[r][:, None].expand(-1, nkv, -1), val)   # (two codes to a byte)
+        tiles[tile[:, :, None], byte[r][:, None]] = rows.gather(2, byte[r][:, None].expand(-1, nkv, -1)).to(torch.uint8)
+        for t, at in ((step, ps), (low, pl)):
+            b = t.contiguous().view(torch.uint8).view(*t.shape, 2)
+            for j in range(2):
+                tiles[tile[:, :, None], at[r][:, None] + j] = b[..., j]
+
+
+def kv4_values(cache, slots, hd, block_size):
+    """fp32 k, v [rows, nkv, hd] of the slots (all within the cache)."""
+    nkv = cache.shape[1]
+    maps, tiles = _kv4_maps(hd), cache.view(-1, 20 * hd)
+    slots = slots.long()
+    inb = slots % block_size
+    tile = ((slots // block_size)[:, None] * nkv + torch.arange(nkv)) * (block_size // 16) + (inb // 16)[:, None]
+    r, got = inb % 16, []
+    for name in ("k", "v"):
+        byte, shift, ps, pl = maps[name]
+        codes = (tiles[tile[:, :, None], byte[r][:, None]].long() >> shift[r][:, None]) & 15
+        par = []
+        for at in (ps, pl):
+            b = torch.stack([tiles[tile[:, :, None], at[r][:, None] + j] for j in range(2)], -1).contiguous()
+            par.append(b.view(torch.bfloat16)[..., 0].float().repeat_interleave(KV4_GROUP, -1))
+        got.append(par[1] + par[0] * codes.float())
+    return got
+
+
+def kv4_read(cache, slots, hd, block_size):
+    ok = (slots >= 0) & (slots.long() < cache.shape[0] * block_size)
+    k, v = kv4_values(cache, torch.where(ok, slots, torch.zeros_like(slots)), hd, block_size)
+    return [torch.where(ok[:, None, None], t, torch.zeros_like(t)).to(torch.bfloat16) for t in (k, v)]
+
+
+def rope_kv_write_q4(qkv, positions, slots, cache, nq, nkv, hd, block_size, theta, out):
+    """Rotates q and k of qkv [rows, (nq + 2 nkv) * hd] into out, angles in 64 bits; k and v into the cache."""
+    rows = qkv.shape[0]
+    x = qkv.float().view(rows, nq + 2 * nkv, hd).clone()
+    inv = theta ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)
+    ang = positions.double()[:, None] * inv
+    c, s = ang.cos().float()[:, None], ang.sin().float()[:, None]
+    a, b = x[:, :nq + nkv, :hd // 2].clone(), x[:, :nq + nkv, hd // 2:].clone()
+    x[:, :nq + nkv, :hd // 2], x[:, :nq + nkv, hd // 2:] = a * c - b * s, b * c + a * s
+    out.copy_(x.view(rows, -1).to(out.dtype))
+    if slots is not None:
+        o = out.view(rows, nq + 2 * nkv, hd)
+        kv4_write(cache, slots, o[:, nq:nq + nkv], o[:, nq + nkv:], block_size)
+    return out
+
+
+def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale):
+    """As paged_attn_decode, on the 4-bit cache; tokens of table entries that name no block are left out."""
+    bs, G = cache.shape[2] * 16, nq // nkv
+    out = torch.zeros(q.shape[0], nq * hd, dtype=q.dtype)
+    for b in range(q.shape[0]):
+        t = torch.arange(min(int(ctx_lens[b]), block_tables.shape[1] * bs))
+        blk = block_tables[b].long()[t // bs]
+        slots = (blk * bs + t % bs)[(blk >= 0) & (blk < cache.shape[0])]
+        if len(slots) == 0:
+            continue
+        k, v = kv4_values(cache, slots, hd, bs)
+        p = torch.softmax(torch.einsum("hgd,thd->hgt", q[b, :nq * hd].view(nkv, G, hd).float(), k) * scale, -1)
+        out[b] = torch.einsum("hgt,thd->hgd", p, v).reshape(-1).to(q.dtype)
+    return out
+
+
+# ---------------------------------------------------------------- serving steps
+def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size):
+    """See ops.paged_layout; block_tables and free_list are updated in place."""
+    width, cap = block_tables.shape[1], free_list.numel()
+    head, free, _ = (int(v) for v in free_range)
+    free = min(max(free, 0), cap)
+    cu, ctx, need, back = [0], [], 0, []
+    pos = torch.zeros(tokens, dtype=torch.int32)
+    slots = torch.full((tokens,), -1, dtype=torch.int32)
+    for b, (n, past) in enumerate(zip(new_lens.tolist(), past_lens.tolist())):
+        past = max(past, 0)
+        had = min(-(-past // block_size), width)
+        if n < 0:
+            back += [i for i in block_tables[b, :had].tolist() if i >= 0]
+            cu.append(cu[-1])
+            ctx.append(0)
+            continue
+        for page in range(had, min(-(-(past + n) // block_size), width)):
+            block_tables[b, page] = free_list[(head + need) % cap] if need < free else -1
+            need += 1
+        for i in range(n):
+            row, p = cu[-1] + i, past + i
+            if row >= tokens:
+                break
+            pos[row] = p
+            blk = int(block_tables[b, p // block_size]) if p // block_size < width else -1
+            slots[row] = blk * block_size + p % block_size if blk >= 0 else -1
+        cu.append(cu[-1] + n)
+        ctx.append(past + n)
+    taken, given = min(need, free), min(len(back), cap - free)
+    for i, blk in enumerate(back[:given]):
+        free_list[(head + free + i) % cap] = blk
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return [i32(cu), pos, slots, i32(ctx), i32([(head + taken) % cap, free - taken + given, max(need - free, 0)])]
+
+
+def count_tokens(counts, seen, ids, cu=None, prompt_lens=None, reset=False):
+    rows, vocab = counts.shape
+    if reset:
+        counts.zero_()
+        seen.zero_()
+    for r in range(rows):
+        lo, hi = (max(int(cu[r]), 0), min(int(cu[r + 1]), ids.numel())) if cu is not None else (r, r + 1)
+        h = ids[lo:hi].long()
+        ok = (h >= 0) & (h < vocab)
+        made = torch.arange(len(h)) >= (int(prompt_lens[r]) if prompt_lens is not None else 0)
+        counts[r].scatter_add_(0, h[ok & made], torch.ones(int((ok & made).sum()), dtype=torch.int32))
+        for i in set(h[ok].tolist()):
+            w = (int(seen[r, i // 32]) & 0xffffffff) | 1 << (i % 32)
+            seen[r, i // 32] = w - (1 << 32) if w >= 1 << 31 else w
+
+
+def _word_bits(words, ids):
+    return (words[:, ids // 32] >> (ids % 32).to(torch.int32)) & 1 != 0
+
+
+def logit_rules(logits, vocab, offset=0, penalties=None, counts=None, seen=None, bias_ids=None, bias=None, mask=None):
+    """fp32 logits [rows, n] under the rules; column i is token i + offset."""
+    x = logits.float().clone()
+    ids = torch.arange(x.shape[1]) + offset
+    known = ids < vocab
+    at = torch.where(known, ids, torch.zeros_like(ids))
+    if penalties is not None:
+        again, presence, frequency = (penalties[:, i:i + 1] for i in range(3))
+        hit = _word_bits(seen, at) & known
+        c = torch.where(hit, counts[:, at], torch.zeros_like(counts[:, at])).float()
+        x = torch.where(hit, torch.where(x > 0, x / again, x * again), x)
+        x = torch.where(c > 0, x - frequency * c - presence, x)
+    if bias_ids is not None:
+        for j in range(bias_ids.shape[1]):
+            x = torch.where((bias_ids[:, j:j + 1] == ids) & (bias_ids[:, j:j + 1] >= 0), x + bias[:, j:j + 1], x)
+    if mask is not None:
+        x = torch.where(_word_bits(mask, at) & known, x, torch.full_like(x, -math.inf))
+    return x
+
+
+def pick(x, offset=0):
+    """(token int32, value fp32) of every row's greatest (the first of equals, NaN passed over); token -1 where all are -inf."""
+    x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
+    val = x.amax(-1)
+    idx = (x == val[:, None]).int().argmax(-1) + offset
+    return torch.where(val == -math.inf, torch.full_like(idx, -1), idx).to(torch.int32), val
