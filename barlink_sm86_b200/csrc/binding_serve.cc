@@ -116,6 +116,14 @@ std::tuple<at::Tensor, at::Tensor> kv4_read(const at::Tensor& cache, const at::T
   return {k, v};
 }
 
+// 1: a kernel of this device gave up waiting for its copies
+int kv4_error_flag(int dev) {
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  unsigned v = 0;
+  BL_CHECK(bl_kv4_error(&v, err, errlen));
+  return int(v);
+}
+
 at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables, const at::Tensor& ctx_lens,
                                 int nq, int nkv, int hd, double scale, const OptTensor& out_opt) {
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 2 && q.stride(1) == 1 && q.stride(0) % 8 == 0 && aligned16(q),
@@ -137,10 +145,15 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
   TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == 2 && out.size(0) == batch &&
                   out.size(1) == int64_t(nq) * hd && aligned16(out),
               "barlink: out must be a contiguous, 16-byte aligned bfloat16 [batch, nq * hd]");
-  if (batch > 0)
+  if (batch > 0 && block_tables.size(1) == 0) {
+    out.zero_();
+  } else if (batch > 0) {
+    const size_t bytes = bl_paged_attn_decode_q4_ws(nq, nkv, hd);
+    at::Tensor ws = at::empty({int64_t(bytes)}, cache.options());
     BL_CHECK(bl_paged_attn_decode_q4(q.data_ptr(), int(q.stride(0)), cache.data_ptr(), bt, cl, out.data_ptr(), batch, nq, nkv, hd,
                                      block_size, small(cache.size(0), "blocks"), small(block_tables.size(1), "max_blocks"), float(scale),
-                                     nullptr, 0, stream_of(q), err, errlen));
+                                     ws.data_ptr(), bytes, stream_of(q), err, errlen));
+  }
   return out;
 }
 
@@ -279,6 +292,7 @@ void bind_serve(py::module_& m) {
   m.def("kv4_read", &kv4_read, py::arg("cache"), py::arg("slots"), py::arg("hd"), py::arg("block_size"));
   m.def("paged_attn_decode_q4", &paged_attn_decode_q4, py::arg("q"), py::arg("cache"), py::arg("block_tables"), py::arg("ctx_lens"),
         py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none());
+  m.def("kv4_error_flag", &kv4_error_flag, py::arg("device") = 0);
   m.def("paged_layout", &paged_layout, py::arg("new_lens"), py::arg("past_lens"), py::arg("block_tables"), py::arg("free_list"),
         py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("into") = py::none());
   m.def("count_tokens", &count_tokens, py::arg("counts"), py::arg("seen"), py::arg("ids"), py::arg("cu") = py::none(),

@@ -239,83 +239,527 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ ca
 // ---------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------
-// One block per (request, KV head); a warp takes every fourth token, a lane hd / 32 dims of it.
+// S = Q K^T and O = P V by mma.sync with the tokens (S) and the dims (O) on the 16-row side and up to eight query heads on the
+// 8-column side, so that a group of 4 to 8 heads wastes little of a product; the codes come from shared memory in the order in
+// which a lane needs them and become fp16 operands by one mask each: the 16 bits 0x000c are the subnormal number c * 2^-24,
+// 0x00c0 is 16 c * 2^-24, and the powers of two are taken out of Q and of the result.  step and low never touch the codes:
+//   s_t = sum over groups a of step_ta (sum q c) + low_ta (sum q)     -- one accumulator per group; the second sum is a product
+//                                                                        of k = (parts of sum q) x groups in bf16, exact parts
+//   o_d = sum over tokens of (p_t step_ta) c + p_t low_ta             -- p step rounded to fp16 (2^-11), the second sum in fp32
+// Queries go in as fp16 of a power of two per head (exact: 2^-27 of the head's largest element is still whole).  The reference of
+// the running softmax is the greatest of x_t + log2(largest step of t), so that p step stays within fp16 whatever the values'
+// size; it moves only when it is exceeded by 2^8, which one vote per tile finds out.
+//
+// Work: the tiles of all (request, KV head) pairs in one row, cut into equal runs, one for each block; a block's eight warps take
+// every eighth tile of the run, each with a ring of its own that the bulk copies fill across pairs.  Lengths are on the GPU only, so
+// every block adds them up by itself.  Pairs that were cut are joined by k_q4_merge.
 constexpr int kQ4MaxG = 16;
+constexpr int kQ4Warps = 8;
+constexpr float kQ4None = -3.402823466e38f;  // reference before the first token
+
+// (whole 16-byte vectors)
+__host__ __device__ constexpr size_t q4_part_floats(int G, int hd) { return size_t(G) * hd + (2 * G + 3) / 4 * 4; }
+
+// set by a wait that ran out; one word per device
+__device__ uint32_t g_kv4_err;
+
+struct Q4Attn {
+  const __nv_bfloat16* q;
+  const uint8_t* cache;
+  const int* tables;
+  const int* ctx_lens;
+  __nv_bfloat16* out;
+  float* part;   // [2 * grid] of G * hd sums, G times (reference, sum of p)
+  int4* meta;    // [grid]: pair that begins in this block's run and goes on behind it: request, head, number of runs, its slot
+  int q_stride, batch, nq, nkv, block_size, n_blocks, max_blocks, min_run;
+  float scale_log2;
+};
+
+__device__ __forceinline__ float q4_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void q4_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void q4_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t q4_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Where a flat tile index stands: its pair begins at `start` and has `tiles`.
+struct Q4At {
+  int b, h, start, tiles;
+};
+__device__ __forceinline__ int q4_tiles(const Q4Attn& a, int b) {
+  const int most = a.max_blocks * a.block_size, n = min(max(a.ctx_lens[b], 0), most);
+  return (n + kQ4Tokens - 1) / kQ4Tokens;
+}
+__device__ __forceinline__ void q4_advance(const Q4Attn& a, Q4At& p, int idx) {
+  while (idx >= p.start + p.tiles && p.b < a.batch) {
+    p.start += p.tiles;
+    if (++p.h == a.nkv) {
+      p.h = 0;
+      do {
+        ++p.b;
+      } while (p.b < a.batch && (p.tiles = q4_tiles(a, p.b)) == 0);
+    }
+  }
+}
+
+template <int HD, int NT, int STAGES>
+constexpr int q4_smem_bytes() {
+  return kQ4Warps * STAGES * q4_tile_bytes(HD) + kQ4Warps * 8 * HD * 4 + kQ4Warps * 8 * 2 * 4 + kQ4Warps * STAGES * 8;
+}
+
+template <int HD, int NT, int STAGES>
+__global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q4(const Q4Attn a) {
+  constexpr int NA = HD / kQ4Group, TB = q4_tile_bytes(HD);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int s_warp_sum[kQ4Warps], s_where[3];
+  __shared__ uint32_t s_abort;
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float* s_o = reinterpret_cast<float*>(smem + kQ4Warps * STAGES * TB);  // [warp][8 heads][HD]
+  float* s_ml = s_o + kQ4Warps * 8 * HD;                                 // [warp][8 heads] reference, sum
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_ml + kQ4Warps * 8 * 2) + warp * STAGES;
+  const uint32_t ring = smem_u32(smem) + warp * STAGES * TB;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
+    mbar_fence_init();
+  }
+  if (threadIdx.x == 0) s_abort = 0;
+  pdl_wait();
+
+  // ---- this block's run of tiles: [lo, hi) of all pairs' tiles ------------------------------------
+  const int G = a.nq / a.nkv;
+  int lo, hi, run;
+  Q4At seg;
+  {
+    const int per = (a.batch + kQ4Warps * 32 - 1) / (kQ4Warps * 32);
+    const int b0 = min(int(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += q4_tiles(a, b) * a.nkv;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    if (lane == 31) s_warp_sum[warp] = upto;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kQ4Warps; ++w) {
+      if (w < warp) upto += s_warp_sum[w];
+      total += s_warp_sum[w];
+    }
+    run = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_run);
+    run = (run + kQ4Warps - 1) / kQ4Warps * kQ4Warps;
+    lo = int(min(int64_t(blockIdx.x) * run, int64_t(total)));
+    hi = min(lo + run, total);
+    if (lo < hi && upto - mine <= lo && lo < upto) {  // one thread's requests hold the first tile
+      int at = upto - mine, b = b0, n = q4_tiles(a, b) * a.nkv;
+      while (lo >= at + n) {
+        at += n;
+        n = q4_tiles(a, ++b) * a.nkv;
+      }
+      s_where[0] = b;
+      s_where[1] = at;
+      s_where[2] = n / a.nkv;
+    }
+    __syncthreads();
+    if (lo < hi) {
+      seg.b = s_where[0];
+      seg.tiles = s_where[2];
+      seg.h = (lo - s_where[1]) / seg.tiles;
+      seg.start = s_where[1] + seg.h * seg.tiles;
+    }
+  }
+  // requests without tokens
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+    if (q4_tiles(a, b) == 0)
+      for (int i = threadIdx.x; i < a.nq * HD / 8; i += blockDim.x)
+        reinterpret_cast<uint4*>(a.out + size_t(b) * a.nq * HD)[i] = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (lo >= hi) return;
+
+  // ---- copies: lane l knows where the l-th of the next 32 tiles of this warp lies ------------------
+  const int count = hi > lo + warp ? (hi - lo - warp + kQ4Warps - 1) / kQ4Warps : 0;
+  Q4At ahead = seg;
+  int chunk = -1;
+  long long where = -1;
+  uint32_t absent = 0;  // bit s: the tile of stage s has no block
+  uint32_t pending = 0; // bit s: a copy into stage s has been asked for
+  const uint32_t leader = elect_leader();
+  auto issue = [&](int i, int stage) {
+    if ((i >> 5) != chunk) {
+      chunk = i >> 5;
+      const int mine = chunk * 32 + lane;
+      where = -1;
+      if (mine < count) {
+        const int idx = lo + warp + mine * kQ4Warps;
+        q4_advance(a, ahead, idx);
+        const int tok = (idx - ahead.start) * kQ4Tokens, page = tok / a.block_size;
+        const int blk = a.tables[size_t(ahead.b) * a.max_blocks + page];
+        if (blk >= 0 && blk < a.n_blocks)
+          where = (long long)(q4_tile_offset(blk, tok - page * a.block_size, ahead.h, a.nkv, a.block_size, HD));
+      }
+    }
+    const long long off = __shfl_sync(0xffffffffu, where, i & 31);
+    if (off < 0) {
+      absent |= 1u << stage;
+      return;
+    }
+    absent &= ~(1u << stage);
+    pending |= 1u << stage;
+    mbar_expect_tx_warp(leader, bars + stage, TB);
+    bulk_load_warp(leader, ring + stage * TB, a.cache + off, TB, smem_u32(bars + stage), kHintEvictFirst);
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    if (i < count) issue(i, i);
+
+  int k = 0, stage = 0;       // own tile, its stage
+  uint32_t parity = 0;        // bit s: parity that stage s's next copy completes
+  bool dead = false;
+  int pos = lo;
+  bool first_seg = true;
+  while (pos < hi) {
+    const int seg_end = min(hi, seg.start + seg.tiles);
+    const int ctx = min(max(a.ctx_lens[seg.b], 0), a.max_blocks * a.block_size);
+    // ---- queries of this pair: operands, factor, sums --------------------------------------------
+    uint32_t qb[NT][NA][4], qs[NT][2];
+    float f[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int head = 8 * n + g;
+      uint4 raw[NA];
+#pragma unroll
+      for (int ga = 0; ga < NA; ++ga)
+        raw[ga] = head < G ? *reinterpret_cast<const uint4*>(a.q + size_t(seg.b) * a.q_stride + (size_t(seg.h) * G + head) * HD + 32 * ga + 8 * t)
+                           : make_uint4(0, 0, 0, 0);
+      float big = 0.f;
+#pragma unroll
+      for (int ga = 0; ga < NA; ++ga) {
+        const uint32_t w[4] = {raw[ga].x, raw[ga].y, raw[ga].z, raw[ga].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(bf16_lo(w[j])), fabsf(bf16_hi(w[j]))));
+      }
+      big = quad_max(big);
+      const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -100), 127);
+      const float up = __uint_as_float(uint32_t(14 - ex + 127) << 23);  // the largest element comes to 2^14 .. 2^15
+      float sum[NA];
+#pragma unroll
+      for (int ga = 0; ga < NA; ++ga) {
+        const float e0 = bf16_lo(raw[ga].x) * up, e1 = bf16_hi(raw[ga].x) * up, e2 = bf16_lo(raw[ga].y) * up, e3 = bf16_hi(raw[ga].y) * up,
+                    e4 = bf16_lo(raw[ga].z) * up, e5 = bf16_hi(raw[ga].z) * up, e6 = bf16_lo(raw[ga].w) * up, e7 = bf16_hi(raw[ga].w) * up;
+        qb[n][ga][0] = pack_f16x2(e0, e4);
+        qb[n][ga][1] = pack_f16x2(e1 * 0.0625f, e5 * 0.0625f);
+        qb[n][ga][2] = pack_f16x2(e2, e6);
+        qb[n][ga][3] = pack_f16x2(e3 * 0.0625f, e7 * 0.0625f);
+        float v = ((e0 + e1) + (e2 + e3)) + ((e4 + e5) + (e6 + e7));
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        sum[ga] = v * 5.9604644775390625e-8f;  // 2^-24, as the codes have it
+      }
+      // three bf16 parts of every sum, along k = part * NA + group
+      const int part0 = NA == 4 ? t >> 1 : t;
+      float lo2[2], b1v[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float v = NA == 4 ? ((t & 1) ? sum[2 * (NA / 4) + j] : sum[j]) : sum[j];
+        const float p0 = __bfloat162float(__float2bfloat16(v)), p1 = __bfloat162float(__float2bfloat16(v - p0)), p2 = v - p0 - p1;
+        lo2[j] = part0 == 0 ? p0 : part0 == 1 ? p1 : part0 == 2 ? p2 : 0.f;
+        b1v[j] = NA == 4 && part0 == 0 ? p2 : 0.f;
+      }
+      qs[n][0] = pack_bf16x2(lo2[0], lo2[1]);
+      qs[n][1] = pack_bf16x2(b1v[0], b1v[1]);
+      const float fac = __uint_as_float(uint32_t(min(ex + 10, 127) + 127) << 23) * a.scale_log2;  // 2^24 * 2^(ex - 14)
+      f[n][0] = __shfl_sync(0xffffffffu, fac, 8 * t);
+      f[n][1] = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
+    }
+    float o[NT][2 * NA][4], vm[NT][NA][2], R[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2 * NA; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) vm[n][i][0] = vm[n][i][1] = 0.f;
+      R[n][0] = R[n][1] = kQ4None;
+      l[n][0] = l[n][1] = 0.f;
+    }
+
+    for (; lo + warp + k * kQ4Warps < seg_end; ++k) {
+      {
+        const int nxt = k + STAGES - 1;
+        int ns = stage + STAGES - 1;
+        if (ns >= STAGES) ns -= STAGES;
+        if (nxt < count && !dead) issue(nxt, ns);
+      }
+      const int st = stage;
+      if (++stage == STAGES) stage = 0;
+      if (dead || (absent >> st & 1)) continue;
+      if (!mbar_wait_bounded_warp(bars + st, parity >> st & 1, &s_abort)) {
+        dead = true;
+        continue;
+      }
+      parity ^= 1u << st;
+      pending &= ~(1u << st);
+      const uint32_t tile = ring + st * TB;
+      const int left = ctx - (lo + warp + k * kQ4Warps - seg.start) * kQ4Tokens;  // tokens of this tile
+
+      // ---- scores ----
+      float x[NT][4];
+      {
+        uint32_t w0[NA], w1[NA], sl0[NA], sl1[NA];
+        lds_words<NA>(tile + g * (HD / 2) + t * NA * 4, w0);
+        lds_words<NA>(tile + (g + 8) * (HD / 2) + t * NA * 4, w1);
+        lds_words<NA>(tile + q4_k_params(HD) + g * NA * 4, sl0);  // step[NA], low[NA]
+        lds_words<NA>(tile + q4_k_params(HD) + (g + 8) * NA * 4, sl1);
+        const uint32_t m0 = NA == 4 && (t & 1) ? sl0[NA - 1] : sl0[NA / 2], m1 = NA == 4 && (t & 1) ? sl1[NA - 1] : sl1[NA / 2];
+        float c[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+          q4_mma_bf16(c[n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
+        }
+#pragma unroll
+        for (int ga = 0; ga < NA; ++ga) {
+          const float s0 = ga & 1 ? bf16_hi(sl0[ga >> 1]) : bf16_lo(sl0[ga >> 1]), s1 = ga & 1 ? bf16_hi(sl1[ga >> 1]) : bf16_lo(sl1[ga >> 1]);
+          const uint32_t v0 = w0[ga] >> 8, v1 = w1[ga] >> 8;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            q4_mma_f16(d, w0[ga] & 0x000f000fu, w1[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00f000f0u, qb[n][ga][0], qb[n][ga][1]);
+            q4_mma_f16(d, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qb[n][ga][2], qb[n][ga][3]);
+            c[n][0] += s0 * d[0];
+            c[n][1] += s0 * d[1];
+            c[n][2] += s1 * d[2];
+            c[n][3] += s1 * d[3];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          x[n][0] = c[n][0] * f[n][0];
+          x[n][1] = c[n][1] * f[n][1];
+          x[n][2] = c[n][2] * f[n][0];
+          x[n][3] = c[n][3] * f[n][1];
+        }
+      }
+      uint32_t vs0[NA], vs1[NA];  // step[NA], low[NA] of the values of tokens g and g + 8
+      lds_words<NA>(tile + q4_v_params(HD) + g * NA * 4, vs0);
+      lds_words<NA>(tile + q4_v_params(HD) + (g + 8) * NA * 4, vs1);
+      if (left < kQ4Tokens) {
+        // behind the last token: whatever the cache holds there (NaN too) stays out
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (g + 8 * j >= left) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[n][2 * j] = x[n][2 * j + 1] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NA; ++i) (j ? vs1 : vs0)[i] = 0;
+          }
+      }
+      // ---- the softmax's reference ----
+      float e0, e1;  // log2 of the largest step of either token, rounded down
+      {
+        uint32_t b0 = vs0[0], b1 = vs1[0];
+        if constexpr (NA == 4) {
+          b0 = __vmaxu2(b0, vs0[1]);
+          b1 = __vmaxu2(b1, vs1[1]);
+        }
+        b0 = max(b0 & 0xffffu, b0 >> 16) >> 7;
+        b1 = max(b1 & 0xffffu, b1 >> 16) >> 7;
+        e0 = float(min(max(int(b0) - 127, -90), 110));
+        e1 = float(min(max(int(b1) - 127, -90), 110));
+      }
+      bool over = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) over |= fmaxf(x[n][j] + e0, x[n][2 + j] + e1) > R[n][j] + 8.f;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float z = fmaxf(x[n][j] + e0, x[n][2 + j] + e1);
+            z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 4));
+            z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 8));
+            z = fmaxf(fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 16)), R[n][j]);
+            const float al = q4_ex2(R[n][j] - z);
+            R[n][j] = z;
+            l[n][j] *= al;
+#pragma unroll
+            for (int i = 0; i < NA; ++i) vm[n][i][j] *= al;
+#pragma unroll
+            for (int i = 0; i < 2 * NA; ++i) {
+              o[n][i][j] *= al;
+              o[n][i][2 + j] *= al;
+            }
+          }
+      }
+      // ---- probabilities, times step, as the columns' operand ----
+      uint32_t pb[NT][NA][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float p0 = q4_ex2(x[n][0] - R[n][0]), p1 = q4_ex2(x[n][1] - R[n][1]), p2 = q4_ex2(x[n][2] - R[n][0]),
+                    p3 = q4_ex2(x[n][3] - R[n][1]);
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+#pragma unroll
+        for (int ga = 0; ga < NA; ++ga) {
+          const float s0 = ga & 1 ? bf16_hi(vs0[ga >> 1]) : bf16_lo(vs0[ga >> 1]), s1 = ga & 1 ? bf16_hi(vs1[ga >> 1]) : bf16_lo(vs1[ga >> 1]);
+          const uint32_t lw0 = vs0[NA / 2 + (ga >> 1)], lw1 = vs1[NA / 2 + (ga >> 1)];
+          const float m0 = ga & 1 ? bf16_hi(lw0) : bf16_lo(lw0), m1 = ga & 1 ? bf16_hi(lw1) : bf16_lo(lw1);
+          pb[n][ga][0] = q4_transpose(pack_f16x2(p0 * s0, p1 * s0));
+          pb[n][ga][1] = q4_transpose(pack_f16x2(p2 * s1, p3 * s1));
+          vm[n][ga][0] += p0 * m0 + p2 * m1;
+          vm[n][ga][1] += p1 * m0 + p3 * m1;
+        }
+      }
+      // ---- values ----
+      {
+        uint32_t w0[NA], w1[NA];
+        lds_words<NA>(tile + q4_v_codes(HD) + t * HD + g * NA * 4, w0);
+        lds_words<NA>(tile + q4_v_codes(HD) + (t + 4) * HD + g * NA * 4, w1);
+#pragma unroll
+        for (int ga = 0; ga < NA; ++ga) {
+          const uint32_t v0 = w0[ga] >> 8, v1 = w1[ga] >> 8;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x000f000fu, w1[ga] & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
+            q4_mma_f16(o[n][2 * ga + 1], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
+          }
+        }
+      }
+      __syncwarp();  // all lanes have read the stage that the next copy fills
+    }
+
+    // ---- join the warps ----------------------------------------------------------------------------
+    const bool whole = pos == seg.start && seg_end == seg.start + seg.tiles;
+    const int slot = 2 * blockIdx.x + (first_seg ? 0 : 1);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (8 * n >= G) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], d);
+#pragma unroll
+          for (int i = 0; i < NA; ++i) vm[n][i][j] += __shfl_xor_sync(0xffffffffu, vm[n][i][j], d);
+        }
+        const int head = 2 * t + j;
+#pragma unroll
+        for (int i = 0; i < NA; ++i)  // 2^24, and the 16 of the odd dims
+          *reinterpret_cast<float4*>(s_o + (warp * 8 + head) * HD + 4 * (8 * i + g)) =
+              make_float4(o[n][2 * i][j] * 16777216.f + vm[n][i][j], o[n][2 * i][2 + j] * 1048576.f + vm[n][i][j],
+                          o[n][2 * i + 1][j] * 16777216.f + vm[n][i][j], o[n][2 * i + 1][2 + j] * 1048576.f + vm[n][i][j]);
+        if (g == 0) {
+          s_ml[(warp * 8 + head) * 2] = R[n][j];
+          s_ml[(warp * 8 + head) * 2 + 1] = l[n][j];
+        }
+      }
+      __syncthreads();
+      const int heads = min(8, G - 8 * n);
+      for (int e = threadIdx.x; e < heads * (HD / 4); e += blockDim.x) {
+        const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+        float M = kQ4None, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kQ4Warps; ++w) M = fmaxf(M, s_ml[(w * 8 + r) * 2]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kQ4Warps; ++w) {
+          const float m = s_ml[(w * 8 + r) * 2], sc = m == kQ4None ? 0.f : exp2f(m - M);
+          const float4 v = *reinterpret_cast<const float4*>(s_o + (w * 8 + r) * HD + d);
+          L += s_ml[(w * 8 + r) * 2 + 1] * sc;
+          acc.x += v.x * sc;
+          acc.y += v.y * sc;
+          acc.z += v.z * sc;
+          acc.w += v.w * sc;
+        }
+        const int head = 8 * n + r;
+        if (whole) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          *reinterpret_cast<uint2*>(a.out + (size_t(seg.b) * a.nq + size_t(seg.h) * G + head) * HD + d) =
+              make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        } else {
+          float* p = a.part + size_t(slot) * q4_part_floats(G, HD);
+          *reinterpret_cast<float4*>(p + head * HD + d) = acc;
+          if (d == 0) {
+            p[G * HD + 2 * head] = M;
+            p[G * HD + 2 * head + 1] = L;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!whole && pos == seg.start && threadIdx.x == 0)  // the pair begins here and goes on
+      a.meta[blockIdx.x] = make_int4(seg.b, seg.h, (seg.start + seg.tiles - 1) / run - int(blockIdx.x) + 1, slot);
+    pos = seg_end;
+    first_seg = false;
+    if (pos < hi) q4_advance(a, seg, pos);
+  }
+  if (dead) {
+    // a copy did not arrive in time: say so, and leave with none in flight
+    if (lane == 0) g_kv4_err = 1;
+    for (int s = 0; s < STAGES; ++s)
+      if (pending >> s & 1) mbar_wait_bounded_warp(bars + s, parity >> s & 1, &s_abort);
+  }
+}
+
+// The runs that a pair was cut into: block (c, head) joins those of the pair that begins in run c.
 template <int HD>
-__global__ void __launch_bounds__(128) k_paged_attn_q4(const __nv_bfloat16* __restrict__ q, int q_stride,
-                                                       const uint8_t* __restrict__ cache, const int* __restrict__ tables,
-                                                       const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, int nq,
-                                                       int nkv, int block_size, int n_blocks, int max_blocks, float scale_log2) {
-  constexpr int NA = HD / kQ4Group, D = HD / 32;  // a lane's dims are D * lane ..
+__global__ void __launch_bounds__(HD) k_q4_merge(const Q4Attn a, int G) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float s_o[4][HD];
-  __shared__ float s_m[4], s_l[4];
-  const int h = blockIdx.x, b = blockIdx.y, G = nq / nkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ctx = min(ctx_lens[b], max_blocks * block_size);
-  float m[kQ4MaxG], l[kQ4MaxG], o[kQ4MaxG][D];
-#pragma unroll
-  for (int g = 0; g < kQ4MaxG; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D; ++j) o[g][j] = 0.f;
+  const int4 m = a.meta[blockIdx.x];
+  if (m.z == 0) return;
+  const int head = blockIdx.y, d = threadIdx.x;
+  const size_t pitch = q4_part_floats(G, HD);
+  auto at = [&](int i) { return a.part + size_t(i == 0 ? m.w : 2 * (int(blockIdx.x) + i)) * pitch; };
+  float M = kQ4None;
+  for (int i = threadIdx.x & 31; i < m.z; i += 32) M = fmaxf(M, at(i)[G * HD + 2 * head]);
+  M = warp_max(M);
+  float L = 0.f, acc = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < m.z; ++i) {
+    const float* p = at(i);
+    const float r = p[G * HD + 2 * head], sc = r == kQ4None ? 0.f : exp2f(r - M);
+    L += p[G * HD + 2 * head + 1] * sc;
+    acc += p[head * HD + d] * sc;
   }
-  const __nv_bfloat16* qb = q + size_t(b) * q_stride + size_t(h) * G * HD + D * lane;
-  const int d0 = D * lane, ga = d0 / kQ4Group;
-  for (int tok = warp; tok < ctx; tok += 4) {
-    const int blk = tables[size_t(b) * max_blocks + tok / block_size];
-    if (blk < 0 || blk >= n_blocks) continue;
-    const int in_block = tok % block_size, r = in_block % kQ4Tokens;
-    const uint8_t* tile = cache + q4_tile_offset(blk, in_block, h, nkv, block_size, HD);
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(tile + r * (HD / 2) + (((d0 >> 3) & 3) * NA + ga) * 4) >> (4 * (d0 & 7));
-    const uint32_t vw = *reinterpret_cast<const uint16_t*>(tile + q4_v_codes(HD) + (r >> 1) * HD + (r & 1) * 2 +
-                                                           (((d0 >> 2) & 7) * NA + ga) * 4) >> (4 * (d0 & 3));
-    const __nv_bfloat16* kp = reinterpret_cast<const __nv_bfloat16*>(tile + q4_k_params(HD) + r * NA * 4);
-    const __nv_bfloat16* vp = reinterpret_cast<const __nv_bfloat16*>(tile + q4_v_params(HD) + r * NA * 4);
-    float k[D], v[D];
-#pragma unroll
-    for (int j = 0; j < D; ++j) {
-      k[j] = __bfloat162float(kp[NA + ga]) + __bfloat162float(kp[ga]) * float((kw >> (4 * j)) & 15);
-      v[j] = __bfloat162float(vp[NA + ga]) + __bfloat162float(vp[ga]) * float((vw >> (4 * j)) & 15);
-    }
-#pragma unroll
-    for (int g = 0; g < kQ4MaxG; ++g) {
-      if (g >= G) break;
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < D; ++j) s += __bfloat162float(qb[g * HD + j]) * k[j];
-      s = warp_sum(s) * scale_log2;
-      const float n = fmaxf(m[g], s);
-      const float al = exp2f(m[g] - n), p = exp2f(s - n);
-      m[g] = n;
-      l[g] = l[g] * al + p;
-#pragma unroll
-      for (int j = 0; j < D; ++j) o[g][j] = o[g][j] * al + p * v[j];
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < kQ4MaxG; ++g) {
-    if (g >= G) break;
-    __syncthreads();
-    if (lane == 0) {
-      s_m[warp] = m[g];
-      s_l[warp] = l[g];
-    }
-#pragma unroll
-    for (int j = 0; j < D; ++j) s_o[warp][d0 + j] = o[g][j];
-    __syncthreads();
-    if (threadIdx.x < HD) {
-      const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-      float L = 0.f, acc = 0.f;
-      for (int w = 0; w < 4; ++w) {
-        const float f = s_m[w] == -INFINITY ? 0.f : exp2f(s_m[w] - M);
-        L += s_l[w] * f;
-        acc += s_o[w][threadIdx.x] * f;
-      }
-      out[(size_t(b) * nq + h * G + g) * HD + threadIdx.x] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
-    }
-  }
+  a.out[(size_t(m.x) * a.nq + size_t(m.y) * G + head) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
 }
 
 }  // namespace bl
@@ -374,6 +818,17 @@ extern "C" int bl_kv4_read(const void* cache, const int* slots, void* k, void* v
   return 0;
 }
 
+extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
+  const cudaError_t e = cudaMemcpyFromSymbol(out, g_kv4_err, sizeof(*out));
+  if (e != cudaSuccess) set_err(err, errlen, "barlink: kv4_error: %s", cudaGetErrorString(e));
+  return e == cudaSuccess ? 0 : -1;
+}
+
+extern "C" size_t bl_paged_attn_decode_q4_ws(int nq, int nkv, int hd) {
+  const size_t G = nq / nkv, grid = size_t(sm_count()) * (G > 8 ? 1 : 2);
+  return grid * (sizeof(int4) + 2 * q4_part_floats(int(G), hd) * sizeof(float));
+}
+
 extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, const int* block_tables, const int* ctx_lens,
                                        void* out, int batch, int nq, int nkv, int hd, int block_size, int n_blocks, int max_blocks,
                                        float scale, void* ws, size_t ws_bytes, void* stream, char* err, size_t errlen) {
@@ -382,16 +837,49 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs nq %% nkv == 0 and at most %d query heads per KV head", kQ4MaxG);
     return -1;
   }
-  if (int64_t(max_blocks) * block_size > 0x7fffffffLL || batch > 65535) {
-    set_err(err, errlen, "barlink: attention over the 4-bit cache: contexts must fit 32 bits, and at most 65535 requests");
+  // (runs are counted in 32 bits, one of them beyond the last tile)
+  if (int64_t(max_blocks) * block_size > 0x7fffffffLL - 16 || int64_t(max_blocks) * (block_size / kQ4Tokens) * batch * nkv > 0x3fffffffLL) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache: the tables' tokens, times KV heads, must not exceed 2^34");
     return -1;
   }
   if (batch == 0) return 0;
-  (void)ws; (void)ws_bytes;
-  const float scale_log2 = scale * 1.4426950408889634f;
-  launch_k(hd == 64 ? k_paged_attn_q4<64> : k_paged_attn_q4<128>, dim3(nkv, batch), dim3(128), 0, static_cast<cudaStream_t>(stream),
-           static_cast<const __nv_bfloat16*>(q), q_stride, static_cast<const uint8_t*>(cache), block_tables, ctx_lens,
-           static_cast<__nv_bfloat16*>(out), nq, nkv, block_size, n_blocks, max_blocks, scale_log2);
+  if (max_blocks < 1) return -1;
+  const int G = nq / nkv, nt = G > 8 ? 2 : 1, grid = sm_count() * (nt == 1 ? 2 : 1);
+  if (!ws || ws_bytes < bl_paged_attn_decode_q4_ws(nq, nkv, hd)) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache needs %zu bytes of workspace", bl_paged_attn_decode_q4_ws(nq, nkv, hd));
+    return -1;
+  }
+  Q4Attn a;
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.tables = block_tables;
+  a.ctx_lens = ctx_lens;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.meta = static_cast<int4*>(ws);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + size_t(grid) * sizeof(int4));
+  a.q_stride = q_stride; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks;
+  a.max_blocks = max_blocks;
+  a.min_run = 2 * kQ4Warps;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  static bool attr[4][64] = {};
+  auto go = [&](auto* kernel, auto* merge, int smem, bool (&done)[64]) {
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem, done);
+    if (e != cudaSuccess) return e;
+    launch_k(kernel, dim3(grid), dim3(kQ4Warps * 32), smem, st, a);
+    return launch_k(merge, dim3(grid, G), dim3(hd), 0, st, a, G);
+  };
+  cudaError_t e;
+  if (hd == 128)
+    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 1, 4>(), attr[0])
+                : go(k_paged_attn_q4<128, 2, 6>, k_q4_merge<128>, q4_smem_bytes<128, 2, 6>(), attr[1]);
+  else
+    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 5>, k_q4_merge<64>, q4_smem_bytes<64, 1, 5>(), attr[2])
+                : go(k_paged_attn_q4<64, 2, 8>, k_q4_merge<64>, q4_smem_bytes<64, 2, 8>(), attr[3]);
+  if (e != cudaSuccess) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache could not be launched: %s", cudaGetErrorString(e));
+    return -1;
+  }
   KV4_LAUNCH_CHECK("paged_attn_decode_q4");
   return 0;
 }
