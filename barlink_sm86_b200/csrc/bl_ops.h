@@ -447,10 +447,10 @@ int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nsplit, size_t s
 int bl_kv4_read(const void* cache, const int* slots, void* k, void* v, int rows, int nkv, int hd, int block_size, int n_blocks,
                 void* stream, char* err, size_t errlen);
 /* One query token per request against the cache; q rows q_stride elements apart.  A block-table entry that names no
- * block leaves its tokens out; a request without tokens gets zeros.  ws: bl_paged_attn_decode_q4_ws bytes of this call's own, 16-byte
+ * block leaves its tokens out; a request without tokens gets zeros.  scale > 0.  ws: bl_paged_attn_decode_q4_ws bytes of this call's own, 16-byte
  * aligned.  A wait that runs out (a copy within the kernel that does not arrive) sets the current device's bl_kv4_error to 1. */
 int bl_kv4_error(unsigned* out, char* err, size_t errlen);
-size_t bl_paged_attn_decode_q4_ws(int nq, int nkv, int hd);
+size_t bl_paged_attn_decode_q4_ws(int batch, int nq, int nkv, int hd);
 int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, const int* block_tables, const int* ctx_lens, void* out,
                             int batch, int nq, int nkv, int hd, int block_size, int n_blocks, int max_blocks, float scale, void* ws,
                             size_t ws_bytes, void* stream, char* err, size_t errlen);

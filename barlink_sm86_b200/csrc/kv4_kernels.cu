@@ -250,11 +250,11 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ ca
 // the running softmax is the greatest of x_t + log2(largest step of t), so that p step stays within fp16 whatever the values'
 // size; it moves only when it is exceeded by 2^8, which one vote per tile finds out.
 //
-// Work: the tiles of all (request, KV head) pairs in one row, cut into equal runs, one for each block; a block's eight warps take
-// every eighth tile of the run, each with a ring of its own that the bulk copies fill across pairs.  Lengths are on the GPU only, so
-// every block adds them up by itself.  Pairs that were cut are joined by k_q4_merge.
+// Work: the tiles of all (request, KV head) pairs in one row, cut into equal runs, one for each warp; a warp has a ring of its own
+// that the bulk copies fill across pairs, and shares nothing with others.  Lengths are on the GPU only, so every warp adds
+// them up by itself.  Pairs that were cut are joined by k_q4_merge.
 constexpr int kQ4MaxG = 16;
-constexpr int kQ4Warps = 8;
+constexpr int kQ4Warps = 4;
 constexpr float kQ4None = -3.402823466e38f;  // reference before the first token
 
 // (whole 16-byte vectors)
@@ -269,8 +269,8 @@ struct Q4Attn {
   const int* tables;
   const int* ctx_lens;
   __nv_bfloat16* out;
-  float* part;   // [2 * grid] of G * hd sums, G times (reference, sum of p)
-  int4* meta;    // [grid]: pair that begins in this block's run and goes on behind it: request, head, number of runs, its slot
+  float* part;   // [2 * runs]: a run's first piece of a pair and its last; G * hd sums, G times (reference, sum of p)
+  int2* meta;    // [batch * nkv]: a pair's first piece, and the number of its pieces (0: done); the others are the first of their runs
   int q_stride, batch, nq, nkv, block_size, n_blocks, max_blocks, min_run;
   float scale_log2;
 };
@@ -286,11 +286,18 @@ __device__ __forceinline__ void q4_mma_f16(float (&d)[4], uint32_t a0, uint32_t 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void q4_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// (the same with nothing to add to)
+__device__ __forceinline__ void q4_mma_f16_0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void q4_mma_bf16_0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t q4_transpose(uint32_t v) {
   uint32_t r;
@@ -334,99 +341,83 @@ __device__ __forceinline__ void q4_advance(const Q4Attn& a, Q4At& p, int idx) {
   }
 }
 
-template <int HD, int NT, int STAGES>
+template <int HD, int STAGES>
 constexpr int q4_smem_bytes() {
-  return kQ4Warps * STAGES * q4_tile_bytes(HD) + kQ4Warps * 8 * HD * 4 + kQ4Warps * 8 * 2 * 4 + kQ4Warps * STAGES * 8;
+  return kQ4Warps * STAGES * (q4_tile_bytes(HD) + 8);
 }
 
 template <int HD, int NT, int STAGES>
-__global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q4(const Q4Attn a) {
+__global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q4(const Q4Attn a) {
   constexpr int NA = HD / kQ4Group, TB = q4_tile_bytes(HD);
+  constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_warp_sum[kQ4Warps], s_where[3];
-  __shared__ uint32_t s_abort;
+  __shared__ uint32_t s_abort[kQ4Warps];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float* s_o = reinterpret_cast<float*>(smem + kQ4Warps * STAGES * TB);  // [warp][8 heads][HD]
-  float* s_ml = s_o + kQ4Warps * 8 * HD;                                 // [warp][8 heads] reference, sum
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_ml + kQ4Warps * 8 * 2) + warp * STAGES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kQ4Warps * STAGES * TB) + warp * STAGES;
   const uint32_t ring = smem_u32(smem) + warp * STAGES * TB;
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
     mbar_fence_init();
+    s_abort[warp] = 0;
   }
-  if (threadIdx.x == 0) s_abort = 0;
+  __syncwarp();
   pdl_wait();
 
-  // ---- this block's run of tiles: [lo, hi) of all pairs' tiles ------------------------------------
-  const int G = a.nq / a.nkv;
+  // ---- this warp's run of tiles: [lo, hi) of all pairs' tiles (neighbouring runs on different SMs) ---------------
+  const int G = a.nq / a.nkv, me = warp * gridDim.x + blockIdx.x, runs = gridDim.x * kQ4Warps;
   int lo, hi, run;
   Q4At seg;
   {
-    const int per = (a.batch + kQ4Warps * 32 - 1) / (kQ4Warps * 32);
-    const int b0 = min(int(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
+    const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += q4_tiles(a, b) * a.nkv;
+    for (int b = b0; b < b1; ++b) mine += q4_tiles(a, b);
+    mine *= a.nkv;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      const int u = __shfl_up_sync(kAll, upto, o);
       if (lane >= o) upto += u;
     }
-    if (lane == 31) s_warp_sum[warp] = upto;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kQ4Warps; ++w) {
-      if (w < warp) upto += s_warp_sum[w];
-      total += s_warp_sum[w];
-    }
-    run = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_run);
-    run = (run + kQ4Warps - 1) / kQ4Warps * kQ4Warps;
-    lo = int(min(int64_t(blockIdx.x) * run, int64_t(total)));
+    const int total = __shfl_sync(kAll, upto, 31);
+    run = max((total + runs - 1) / runs, a.min_run);
+    lo = int(min(int64_t(me) * run, int64_t(total)));
     hi = min(lo + run, total);
-    if (lo < hi && upto - mine <= lo && lo < upto) {  // one thread's requests hold the first tile
-      int at = upto - mine, b = b0, n = q4_tiles(a, b) * a.nkv;
-      while (lo >= at + n) {
-        at += n;
-        n = q4_tiles(a, ++b) * a.nkv;
-      }
-      s_where[0] = b;
-      s_where[1] = at;
-      s_where[2] = n / a.nkv;
-    }
-    __syncthreads();
-    if (lo < hi) {
-      seg.b = s_where[0];
-      seg.tiles = s_where[2];
-      seg.h = (lo - s_where[1]) / seg.tiles;
-      seg.start = s_where[1] + seg.h * seg.tiles;
-    }
+    int b = b0, at = upto - mine, n = 0;
+    const bool holds = at <= lo && lo < upto;  // one lane's requests hold the first tile
+    if (holds)
+      for (n = q4_tiles(a, b) * a.nkv; lo >= at + n; n = q4_tiles(a, ++b) * a.nkv) at += n;
+    const uint32_t who = __ballot_sync(kAll, holds);
+    const int src = who ? __ffs(who) - 1 : 0;
+    seg.b = __shfl_sync(kAll, b, src);
+    at = __shfl_sync(kAll, at, src);
+    seg.tiles = max(__shfl_sync(kAll, n, src) / a.nkv, 1);
+    seg.h = (lo - at) / seg.tiles;
+    seg.start = at + seg.h * seg.tiles;
   }
   // requests without tokens
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (q4_tiles(a, b) == 0)
-      for (int i = threadIdx.x; i < a.nq * HD / 8; i += blockDim.x)
-        reinterpret_cast<uint4*>(a.out + size_t(b) * a.nq * HD)[i] = make_uint4(0, 0, 0, 0);
-  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  for (int b = me; b < a.batch; b += runs)
+    if (q4_tiles(a, b) == 0) {
+      for (int i = lane; i < a.nq * HD / 8; i += 32) reinterpret_cast<uint4*>(a.out + size_t(b) * a.nq * HD)[i] = make_uint4(0, 0, 0, 0);
+      for (int h = lane; h < a.nkv; h += 32) a.meta[size_t(b) * a.nkv + h] = make_int2(0, 0);
+    }
   if (lo >= hi) return;
 
-  // ---- copies: lane l knows where the l-th of the next 32 tiles of this warp lies ------------------
-  const int count = hi > lo + warp ? (hi - lo - warp + kQ4Warps - 1) / kQ4Warps : 0;
+  // ---- copies: lane l knows where the l-th of the next 32 tiles lies -------------------------------------------
+  const int count = hi - lo;
   Q4At ahead = seg;
   int chunk = -1;
   long long where = -1;
-  uint32_t absent = 0;  // bit s: the tile of stage s has no block
-  uint32_t pending = 0; // bit s: a copy into stage s has been asked for
+  uint32_t absent = 0;   // bit s: the tile of stage s has no block
+  uint32_t pending = 0;  // bit s: a copy into stage s is on its way
   const uint32_t leader = elect_leader();
   auto issue = [&](int i, int stage) {
     if ((i >> 5) != chunk) {
       chunk = i >> 5;
-      const int mine = chunk * 32 + lane;
+      const int idx = lo + chunk * 32 + lane;
       where = -1;
-      if (mine < count) {
-        const int idx = lo + warp + mine * kQ4Warps;
+      if (idx < hi) {
         q4_advance(a, ahead, idx);
         const int tok = (idx - ahead.start) * kQ4Tokens, page = tok / a.block_size;
         const int blk = a.tables[size_t(ahead.b) * a.max_blocks + page];
@@ -434,7 +425,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
           where = (long long)(q4_tile_offset(blk, tok - page * a.block_size, ahead.h, a.nkv, a.block_size, HD));
       }
     }
-    const long long off = __shfl_sync(0xffffffffu, where, i & 31);
+    const long long off = __shfl_sync(kAll, where, i & 31);
     if (off < 0) {
       absent |= 1u << stage;
       return;
@@ -444,17 +435,17 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
     mbar_expect_tx_warp(leader, bars + stage, TB);
     bulk_load_warp(leader, ring + stage * TB, a.cache + off, TB, smem_u32(bars + stage), kHintEvictFirst);
   };
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < STAGES - 1; ++i)
     if (i < count) issue(i, i);
 
-  int k = 0, stage = 0;       // own tile, its stage
-  uint32_t parity = 0;        // bit s: parity that stage s's next copy completes
+  int k = 0, stage = 0;  // tile of the run, its stage
+  uint32_t parity = 0;   // bit s: parity that stage s's next copy completes
   bool dead = false;
-  int pos = lo;
-  bool first_seg = true;
-  while (pos < hi) {
-    const int seg_end = min(hi, seg.start + seg.tiles);
+  while (k < count) {
+    const int seg_end = min(hi, seg.start + seg.tiles) - lo;
+    const bool begins = lo + k == seg.start, whole = begins && lo + seg_end == seg.start + seg.tiles;
+    const int piece = 2 * me + (k == 0 ? 0 : 1);
     const int ctx = min(max(a.ctx_lens[seg.b], 0), a.max_blocks * a.block_size);
     // ---- queries of this pair: operands, factor, sums --------------------------------------------
     uint32_t qb[NT][NA][4], qs[NT][2];
@@ -467,15 +458,14 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
       for (int ga = 0; ga < NA; ++ga)
         raw[ga] = head < G ? *reinterpret_cast<const uint4*>(a.q + size_t(seg.b) * a.q_stride + (size_t(seg.h) * G + head) * HD + 32 * ga + 8 * t)
                            : make_uint4(0, 0, 0, 0);
-      float big = 0.f;
+      uint32_t top = 0;  // the largest element's bits: magnitudes of bf16 compare as integers
 #pragma unroll
-      for (int ga = 0; ga < NA; ++ga) {
-        const uint32_t w[4] = {raw[ga].x, raw[ga].y, raw[ga].z, raw[ga].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(bf16_lo(w[j])), fabsf(bf16_hi(w[j]))));
-      }
-      big = quad_max(big);
-      const int ex = min(max(int(__float_as_uint(big) >> 23) - 127, -100), 127);
+      for (int ga = 0; ga < NA; ++ga)
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(raw[ga].x & 0x7fff7fffu, raw[ga].y & 0x7fff7fffu), __vmaxu2(raw[ga].z & 0x7fff7fffu, raw[ga].w & 0x7fff7fffu)));
+      top = max(top & 0xffffu, top >> 16);
+      top = max(top, __shfl_xor_sync(kAll, top, 1));
+      top = max(top, __shfl_xor_sync(kAll, top, 2));
+      const int ex = min(max(int(top >> 7) - 127, -100), 127);
       const float up = __uint_as_float(uint32_t(14 - ex + 127) << 23);  // the largest element comes to 2^14 .. 2^15
       float sum[NA];
 #pragma unroll
@@ -487,25 +477,26 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
         qb[n][ga][2] = pack_f16x2(e2, e6);
         qb[n][ga][3] = pack_f16x2(e3 * 0.0625f, e7 * 0.0625f);
         float v = ((e0 + e1) + (e2 + e3)) + ((e4 + e5) + (e6 + e7));
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        v += __shfl_xor_sync(0xffffffffu, v, 2);
+        v += __shfl_xor_sync(kAll, v, 1);
+        v += __shfl_xor_sync(kAll, v, 2);
         sum[ga] = v * 5.9604644775390625e-8f;  // 2^-24, as the codes have it
       }
       // three bf16 parts of every sum, along k = part * NA + group
       const int part0 = NA == 4 ? t >> 1 : t;
-      float lo2[2], b1v[2];
+      float first[2], second[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float v = NA == 4 ? ((t & 1) ? sum[2 * (NA / 4) + j] : sum[j]) : sum[j];
+        const float v = NA == 4 && (t & 1) ? sum[2 * (NA / 4) + j] : sum[j];
         const float p0 = __bfloat162float(__float2bfloat16(v)), p1 = __bfloat162float(__float2bfloat16(v - p0)), p2 = v - p0 - p1;
-        lo2[j] = part0 == 0 ? p0 : part0 == 1 ? p1 : part0 == 2 ? p2 : 0.f;
-        b1v[j] = NA == 4 && part0 == 0 ? p2 : 0.f;
+        first[j] = part0 == 0 ? p0 : part0 == 1 ? p1 : part0 == 2 ? p2 : 0.f;
+        second[j] = NA == 4 && part0 == 0 ? p2 : 0.f;
       }
-      qs[n][0] = pack_bf16x2(lo2[0], lo2[1]);
-      qs[n][1] = pack_bf16x2(b1v[0], b1v[1]);
-      const float fac = __uint_as_float(uint32_t(min(ex + 10, 127) + 127) << 23) * a.scale_log2;  // 2^24 * 2^(ex - 14)
-      f[n][0] = __shfl_sync(0xffffffffu, fac, 8 * t);
-      f[n][1] = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
+      qs[n][0] = pack_bf16x2(first[0], first[1]);
+      qs[n][1] = pack_bf16x2(second[0], second[1]);
+      // 2^24 * 2^(ex - 14); never 0, for it meets the infinity that stands for "behind the last token"
+      const float fac = fmaxf(__uint_as_float(uint32_t(min(ex + 10, 127) + 127) << 23) * a.scale_log2, 1.17549435e-38f);
+      f[n][0] = __shfl_sync(kAll, fac, 8 * t);
+      f[n][1] = __shfl_sync(kAll, fac, 8 * t + 4);
     }
     float o[NT][2 * NA][4], vm[NT][NA][2], R[NT][2], l[NT][2];
 #pragma unroll
@@ -518,27 +509,27 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
       l[n][0] = l[n][1] = 0.f;
     }
 
-    for (; lo + warp + k * kQ4Warps < seg_end; ++k) {
+#pragma unroll 1
+    for (; k < seg_end; ++k) {
       {
-        const int nxt = k + STAGES - 1;
         int ns = stage + STAGES - 1;
         if (ns >= STAGES) ns -= STAGES;
-        if (nxt < count && !dead) issue(nxt, ns);
+        if (k + STAGES - 1 < count && !dead) issue(k + STAGES - 1, ns);
       }
       const int st = stage;
       if (++stage == STAGES) stage = 0;
       if (dead || (absent >> st & 1)) continue;
-      if (!mbar_wait_bounded_warp(bars + st, parity >> st & 1, &s_abort)) {
+      if (!mbar_wait_bounded_warp(bars + st, parity >> st & 1, &s_abort[warp])) {
         dead = true;
         continue;
       }
       parity ^= 1u << st;
       pending &= ~(1u << st);
       const uint32_t tile = ring + st * TB;
-      const int left = ctx - (lo + warp + k * kQ4Warps - seg.start) * kQ4Tokens;  // tokens of this tile
+      const int left = ctx - (lo + k - seg.start) * kQ4Tokens;  // tokens of this tile
 
-      // ---- scores ----
-      float x[NT][4];
+      // ---- scores, over the factor f: tokens g (c[0], c[1]) and g + 8, heads 2 t and 2 t + 1 ----
+      float c[NT][4];
       {
         uint32_t w0[NA], w1[NA], sl0[NA], sl1[NA];
         lds_words<NA>(tile + g * (HD / 2) + t * NA * 4, w0);
@@ -546,33 +537,22 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
         lds_words<NA>(tile + q4_k_params(HD) + g * NA * 4, sl0);  // step[NA], low[NA]
         lds_words<NA>(tile + q4_k_params(HD) + (g + 8) * NA * 4, sl1);
         const uint32_t m0 = NA == 4 && (t & 1) ? sl0[NA - 1] : sl0[NA / 2], m1 = NA == 4 && (t & 1) ? sl1[NA - 1] : sl1[NA / 2];
-        float c[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-          q4_mma_bf16(c[n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
-        }
+        for (int n = 0; n < NT; ++n) q4_mma_bf16_0(c[n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
 #pragma unroll
         for (int ga = 0; ga < NA; ++ga) {
           const float s0 = ga & 1 ? bf16_hi(sl0[ga >> 1]) : bf16_lo(sl0[ga >> 1]), s1 = ga & 1 ? bf16_hi(sl1[ga >> 1]) : bf16_lo(sl1[ga >> 1]);
           const uint32_t v0 = w0[ga] >> 8, v1 = w1[ga] >> 8;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            q4_mma_f16(d, w0[ga] & 0x000f000fu, w1[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00f000f0u, qb[n][ga][0], qb[n][ga][1]);
+            float d[4];
+            q4_mma_f16_0(d, w0[ga] & 0x000f000fu, w1[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00f000f0u, qb[n][ga][0], qb[n][ga][1]);
             q4_mma_f16(d, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qb[n][ga][2], qb[n][ga][3]);
             c[n][0] += s0 * d[0];
             c[n][1] += s0 * d[1];
             c[n][2] += s1 * d[2];
             c[n][3] += s1 * d[3];
           }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          x[n][0] = c[n][0] * f[n][0];
-          x[n][1] = c[n][1] * f[n][1];
-          x[n][2] = c[n][2] * f[n][0];
-          x[n][3] = c[n][3] * f[n][1];
         }
       }
       uint32_t vs0[NA], vs1[NA];  // step[NA], low[NA] of the values of tokens g and g + 8
@@ -584,38 +564,42 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
         for (int j = 0; j < 2; ++j)
           if (g + 8 * j >= left) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x[n][2 * j] = x[n][2 * j + 1] = -INFINITY;
+            for (int n = 0; n < NT; ++n) c[n][2 * j] = c[n][2 * j + 1] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NA; ++i) (j ? vs1 : vs0)[i] = 0;
           }
       }
-      // ---- the softmax's reference ----
-      float e0, e1;  // log2 of the largest step of either token, rounded down
-      {
-        uint32_t b0 = vs0[0], b1 = vs1[0];
-        if constexpr (NA == 4) {
-          b0 = __vmaxu2(b0, vs0[1]);
-          b1 = __vmaxu2(b1, vs1[1]);
-        }
-        b0 = max(b0 & 0xffffu, b0 >> 16) >> 7;
-        b1 = max(b1 & 0xffffu, b1 >> 16) >> 7;
-        e0 = float(min(max(int(b0) - 127, -90), 110));
-        e1 = float(min(max(int(b1) - 127, -90), 110));
+      float s0[NA], s1[NA], top0 = 8.0779356694631609e-28f, top1 = top0;  // the larger of the steps and 2^-90
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        s0[i] = i & 1 ? bf16_hi(vs0[i >> 1]) : bf16_lo(vs0[i >> 1]);
+        s1[i] = i & 1 ? bf16_hi(vs1[i >> 1]) : bf16_lo(vs1[i >> 1]);
+        top0 = fmaxf(top0, s0[i]);
+        top1 = fmaxf(top1, s1[i]);
       }
-      bool over = false;
+      // ---- probabilities; where one times step leaves fp16's range, a new reference first ----
+      float p[NT][4];
+      auto weigh = [&] {
+        float most = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) over |= fmaxf(x[n][j] + e0, x[n][2 + j] + e1) > R[n][j] + 8.f;
-      if (__any_sync(0xffffffffu, over)) {
+          for (int j = 0; j < 4; ++j) {
+            p[n][j] = q4_ex2(fmaf(c[n][j], f[n][j & 1], -R[n][j & 1]));
+            most = fmaxf(most, p[n][j] * (j < 2 ? top0 : top1));  // (a NaN leaves the reference alone)
+          }
+        return most;
+      };
+      if (__any_sync(kAll, weigh() > 512.f)) {
+        const float e0 = fminf(float(int(__float_as_uint(top0) >> 23) - 127), 110.f), e1 = fminf(float(int(__float_as_uint(top1) >> 23) - 127), 110.f);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float z = fmaxf(x[n][j] + e0, x[n][2 + j] + e1);
-            z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 4));
-            z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 8));
-            z = fmaxf(fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 16)), R[n][j]);
+            float z = fmaxf(fmaf(c[n][j], f[n][j], e0), fmaf(c[n][2 + j], f[n][j], e1));
+            z = fmaxf(z, __shfl_xor_sync(kAll, z, 4));
+            z = fmaxf(z, __shfl_xor_sync(kAll, z, 8));
+            z = fmaxf(fmaxf(z, __shfl_xor_sync(kAll, z, 16)), R[n][j]);
             const float al = q4_ex2(R[n][j] - z);
             R[n][j] = z;
             l[n][j] *= al;
@@ -627,139 +611,132 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 2 : 1) k_paged_attn_q
               o[n][i][2 + j] *= al;
             }
           }
+        weigh();
       }
-      // ---- probabilities, times step, as the columns' operand ----
-      uint32_t pb[NT][NA][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float p0 = q4_ex2(x[n][0] - R[n][0]), p1 = q4_ex2(x[n][1] - R[n][1]), p2 = q4_ex2(x[n][2] - R[n][0]),
-                    p3 = q4_ex2(x[n][3] - R[n][1]);
-        l[n][0] += p0 + p2;
-        l[n][1] += p1 + p3;
-#pragma unroll
-        for (int ga = 0; ga < NA; ++ga) {
-          const float s0 = ga & 1 ? bf16_hi(vs0[ga >> 1]) : bf16_lo(vs0[ga >> 1]), s1 = ga & 1 ? bf16_hi(vs1[ga >> 1]) : bf16_lo(vs1[ga >> 1]);
-          const uint32_t lw0 = vs0[NA / 2 + (ga >> 1)], lw1 = vs1[NA / 2 + (ga >> 1)];
-          const float m0 = ga & 1 ? bf16_hi(lw0) : bf16_lo(lw0), m1 = ga & 1 ? bf16_hi(lw1) : bf16_lo(lw1);
-          pb[n][ga][0] = q4_transpose(pack_f16x2(p0 * s0, p1 * s0));
-          pb[n][ga][1] = q4_transpose(pack_f16x2(p2 * s1, p3 * s1));
-          vm[n][ga][0] += p0 * m0 + p2 * m1;
-          vm[n][ga][1] += p1 * m0 + p3 * m1;
-        }
-      }
-      // ---- values ----
+      // ---- values: p times step as the columns' operand, p times low beside it ----
       {
         uint32_t w0[NA], w1[NA];
         lds_words<NA>(tile + q4_v_codes(HD) + t * HD + g * NA * 4, w0);
         lds_words<NA>(tile + q4_v_codes(HD) + (t + 4) * HD + g * NA * 4, w1);
 #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          l[n][0] += p[n][0] + p[n][2];
+          l[n][1] += p[n][1] + p[n][3];
+        }
+#pragma unroll
         for (int ga = 0; ga < NA; ++ga) {
+          const uint32_t lw0 = vs0[NA / 2 + (ga >> 1)], lw1 = vs1[NA / 2 + (ga >> 1)];
+          const float m0 = ga & 1 ? bf16_hi(lw0) : bf16_lo(lw0), m1 = ga & 1 ? bf16_hi(lw1) : bf16_lo(lw1);
           const uint32_t v0 = w0[ga] >> 8, v1 = w1[ga] >> 8;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x000f000fu, w1[ga] & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
-            q4_mma_f16(o[n][2 * ga + 1], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
+            const uint32_t pb0 = q4_transpose(pack_f16x2(p[n][0] * s0[ga], p[n][1] * s0[ga]));
+            const uint32_t pb1 = q4_transpose(pack_f16x2(p[n][2] * s1[ga], p[n][3] * s1[ga]));
+            vm[n][ga][0] = fmaf(p[n][0], m0, fmaf(p[n][2], m1, vm[n][ga][0]));
+            vm[n][ga][1] = fmaf(p[n][1], m0, fmaf(p[n][3], m1, vm[n][ga][1]));
+            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x000f000fu, w1[ga] & 0x00f000f0u, pb0, pb1);
+            q4_mma_f16(o[n][2 * ga + 1], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, pb0, pb1);
           }
         }
       }
       __syncwarp();  // all lanes have read the stage that the next copy fills
     }
 
-    // ---- join the warps ----------------------------------------------------------------------------
-    const bool whole = pos == seg.start && seg_end == seg.start + seg.tiles;
-    const int slot = 2 * blockIdx.x + (first_seg ? 0 : 1);
+    // ---- out: the whole pair, or a piece of it ---------------------------------------------------------
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (8 * n >= G) break;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
-          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], d);
+          l[n][j] += __shfl_xor_sync(kAll, l[n][j], d);
 #pragma unroll
-          for (int i = 0; i < NA; ++i) vm[n][i][j] += __shfl_xor_sync(0xffffffffu, vm[n][i][j], d);
+          for (int i = 0; i < NA; ++i) vm[n][i][j] += __shfl_xor_sync(kAll, vm[n][i][j], d);
         }
-        const int head = 2 * t + j;
+        const int head = 8 * n + 2 * t + j;
+        if (head >= G) continue;
+        const float inv = !whole ? 1.f : l[n][j] == 0.f ? 0.f : 1.f / l[n][j];
+        float* part = a.part + size_t(piece) * q4_part_floats(G, HD);
 #pragma unroll
-        for (int i = 0; i < NA; ++i)  // 2^24, and the 16 of the odd dims
-          *reinterpret_cast<float4*>(s_o + (warp * 8 + head) * HD + 4 * (8 * i + g)) =
-              make_float4(o[n][2 * i][j] * 16777216.f + vm[n][i][j], o[n][2 * i][2 + j] * 1048576.f + vm[n][i][j],
-                          o[n][2 * i + 1][j] * 16777216.f + vm[n][i][j], o[n][2 * i + 1][2 + j] * 1048576.f + vm[n][i][j]);
-        if (g == 0) {
-          s_ml[(warp * 8 + head) * 2] = R[n][j];
-          s_ml[(warp * 8 + head) * 2 + 1] = l[n][j];
+        for (int i = 0; i < NA; ++i) {  // 2^24, and the 16 of the odd dims
+          const float v0 = fmaf(o[n][2 * i][j], 16777216.f, vm[n][i][j]) * inv, v1 = fmaf(o[n][2 * i][2 + j], 1048576.f, vm[n][i][j]) * inv,
+                      v2 = fmaf(o[n][2 * i + 1][j], 16777216.f, vm[n][i][j]) * inv, v3 = fmaf(o[n][2 * i + 1][2 + j], 1048576.f, vm[n][i][j]) * inv;
+          const int d = 4 * (8 * i + g);
+          if (whole)
+            *reinterpret_cast<uint2*>(a.out + (size_t(seg.b) * a.nq + size_t(seg.h) * G + head) * HD + d) =
+                make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+          else
+            *reinterpret_cast<float4*>(part + head * HD + d) = make_float4(v0, v1, v2, v3);
         }
+        if (!whole && g == 0) *reinterpret_cast<float2*>(part + G * HD + 2 * head) = make_float2(R[n][j], l[n][j]);
       }
-      __syncthreads();
-      const int heads = min(8, G - 8 * n);
-      for (int e = threadIdx.x; e < heads * (HD / 4); e += blockDim.x) {
-        const int r = e / (HD / 4), d = e % (HD / 4) * 4;
-        float M = kQ4None, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < kQ4Warps; ++w) M = fmaxf(M, s_ml[(w * 8 + r) * 2]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kQ4Warps; ++w) {
-          const float m = s_ml[(w * 8 + r) * 2], sc = m == kQ4None ? 0.f : exp2f(m - M);
-          const float4 v = *reinterpret_cast<const float4*>(s_o + (w * 8 + r) * HD + d);
-          L += s_ml[(w * 8 + r) * 2 + 1] * sc;
-          acc.x += v.x * sc;
-          acc.y += v.y * sc;
-          acc.z += v.z * sc;
-          acc.w += v.w * sc;
-        }
-        const int head = 8 * n + r;
-        if (whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          *reinterpret_cast<uint2*>(a.out + (size_t(seg.b) * a.nq + size_t(seg.h) * G + head) * HD + d) =
-              make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        } else {
-          float* p = a.part + size_t(slot) * q4_part_floats(G, HD);
-          *reinterpret_cast<float4*>(p + head * HD + d) = acc;
-          if (d == 0) {
-            p[G * HD + 2 * head] = M;
-            p[G * HD + 2 * head + 1] = L;
-          }
-        }
-      }
-      __syncthreads();
-    }
-    if (!whole && pos == seg.start && threadIdx.x == 0)  // the pair begins here and goes on
-      a.meta[blockIdx.x] = make_int4(seg.b, seg.h, (seg.start + seg.tiles - 1) / run - int(blockIdx.x) + 1, slot);
-    pos = seg_end;
-    first_seg = false;
-    if (pos < hi) q4_advance(a, seg, pos);
+    if (begins && lane == 0)
+      a.meta[size_t(seg.b) * a.nkv + seg.h] = make_int2(piece, whole ? 0 : (seg.start + seg.tiles - 1) / run - me + 1);
+    if (k < count) q4_advance(a, seg, lo + k);
   }
   if (dead) {
     // a copy did not arrive in time: say so, and leave with none in flight
     if (lane == 0) g_kv4_err = 1;
     for (int s = 0; s < STAGES; ++s)
-      if (pending >> s & 1) mbar_wait_bounded_warp(bars + s, parity >> s & 1, &s_abort);
+      if (pending >> s & 1) mbar_wait_bounded_warp(bars + s, parity >> s & 1, &s_abort[warp]);
   }
 }
 
-// The runs that a pair was cut into: block (c, head) joins those of the pair that begins in run c.
+// The pieces of a pair that was cut: block (pair, head), a warp takes every kQ4MergeWarps-th piece, a lane HD / 32 dims of it.
+constexpr int kQ4MergeWarps = 8;
 template <int HD>
-__global__ void __launch_bounds__(HD) k_q4_merge(const Q4Attn a, int G) {
+__global__ void __launch_bounds__(kQ4MergeWarps * 32) k_q4_merge(const Q4Attn a, int G) {
+  constexpr int D = HD / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const int4 m = a.meta[blockIdx.x];
-  if (m.z == 0) return;
-  const int head = blockIdx.y, d = threadIdx.x;
+  __shared__ float s_o[kQ4MergeWarps][HD], s_m[kQ4MergeWarps], s_l[kQ4MergeWarps];
+  const int2 m = a.meta[blockIdx.x];
+  if (m.y == 0) return;
+  const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t pitch = q4_part_floats(G, HD);
-  auto at = [&](int i) { return a.part + size_t(i == 0 ? m.w : 2 * (int(blockIdx.x) + i)) * pitch; };
-  float M = kQ4None;
-  for (int i = threadIdx.x & 31; i < m.z; i += 32) M = fmaxf(M, at(i)[G * HD + 2 * head]);
-  M = warp_max(M);
-  float L = 0.f, acc = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < m.z; ++i) {
+  auto at = [&](int i) { return a.part + size_t(i == 0 ? m.x : 2 * ((m.x >> 1) + i)) * pitch; };
+  float M = kQ4None, L = 0.f, acc[D];
+#pragma unroll
+  for (int j = 0; j < D; ++j) acc[j] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < m.y; i += kQ4MergeWarps) {
     const float* p = at(i);
-    const float r = p[G * HD + 2 * head], sc = r == kQ4None ? 0.f : exp2f(r - M);
-    L += p[G * HD + 2 * head + 1] * sc;
-    acc += p[head * HD + d] * sc;
+    const float2 rl = *reinterpret_cast<const float2*>(p + G * HD + 2 * head);
+    float v[D];
+    if constexpr (D == 4) {
+      const float4 u = *reinterpret_cast<const float4*>(p + head * HD + 4 * lane);
+      v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    } else {
+      const float2 u = *reinterpret_cast<const float2*>(p + head * HD + 2 * lane);
+      v[0] = u.x; v[1] = u.y;
+    }
+    const float n = fmaxf(M, rl.x), s0 = q4_ex2(M - n), s1 = q4_ex2(rl.x - n);
+    M = n;
+    L = L * s0 + rl.y * s1;
+#pragma unroll
+    for (int j = 0; j < D; ++j) acc[j] = acc[j] * s0 + v[j] * s1;
   }
-  a.out[(size_t(m.x) * a.nq + size_t(m.y) * G + head) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
+#pragma unroll
+  for (int j = 0; j < D; ++j) s_o[warp][D * lane + j] = acc[j];
+  if (lane == 0) {
+    s_m[warp] = M;
+    s_l[warp] = L;
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= HD) return;
+  M = kQ4None;
+#pragma unroll
+  for (int w = 0; w < kQ4MergeWarps; ++w) M = fmaxf(M, s_m[w]);
+  L = 0.f;
+  float o = 0.f;
+#pragma unroll
+  for (int w = 0; w < kQ4MergeWarps; ++w) {
+    const float sc = q4_ex2(s_m[w] - M);
+    L += s_l[w] * sc;
+    o += s_o[w][d] * sc;
+  }
+  a.out[(size_t(blockIdx.x) * G + head) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : o / L);
 }
 
 }  // namespace bl
@@ -824,9 +801,12 @@ extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
   return e == cudaSuccess ? 0 : -1;
 }
 
-extern "C" size_t bl_paged_attn_decode_q4_ws(int nq, int nkv, int hd) {
-  const size_t G = nq / nkv, grid = size_t(sm_count()) * (G > 8 ? 1 : 2);
-  return grid * (sizeof(int4) + 2 * q4_part_floats(int(G), hd) * sizeof(float));
+// blocks of attention: as many as are resident at once
+static int q4_grid(int G) { return sm_count() * (G > 8 ? 2 : 4); }
+
+extern "C" size_t bl_paged_attn_decode_q4_ws(int batch, int nq, int nkv, int hd) {
+  const int G = nq / nkv;
+  return 2 * size_t(q4_grid(G)) * kQ4Warps * q4_part_floats(G, hd) * sizeof(float) + size_t(batch) * nkv * sizeof(int2);
 }
 
 extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, const int* block_tables, const int* ctx_lens,
@@ -844,9 +824,14 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   }
   if (batch == 0) return 0;
   if (max_blocks < 1) return -1;
-  const int G = nq / nkv, nt = G > 8 ? 2 : 1, grid = sm_count() * (nt == 1 ? 2 : 1);
-  if (!ws || ws_bytes < bl_paged_attn_decode_q4_ws(nq, nkv, hd)) {
-    set_err(err, errlen, "barlink: attention over the 4-bit cache needs %zu bytes of workspace", bl_paged_attn_decode_q4_ws(nq, nkv, hd));
+  if (!(scale > 0.f) || scale > 3e38f) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache needs a positive scale");
+    return -1;
+  }
+  const int G = nq / nkv, nt = G > 8 ? 2 : 1, grid = q4_grid(G);
+  if (!ws || ws_bytes < bl_paged_attn_decode_q4_ws(batch, nq, nkv, hd)) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache needs %zu bytes of workspace",
+            bl_paged_attn_decode_q4_ws(batch, nq, nkv, hd));
     return -1;
   }
   Q4Attn a;
@@ -855,11 +840,11 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   a.tables = block_tables;
   a.ctx_lens = ctx_lens;
   a.out = static_cast<__nv_bfloat16*>(out);
-  a.meta = static_cast<int4*>(ws);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + size_t(grid) * sizeof(int4));
+  a.part = static_cast<float*>(ws);
+  a.meta = reinterpret_cast<int2*>(a.part + 2 * size_t(grid) * kQ4Warps * q4_part_floats(G, hd));
   a.q_stride = q_stride; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks;
   a.max_blocks = max_blocks;
-  a.min_run = 2 * kQ4Warps;
+  a.min_run = 2;
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   static bool attr[4][64] = {};
@@ -867,15 +852,15 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
     const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return e;
     launch_k(kernel, dim3(grid), dim3(kQ4Warps * 32), smem, st, a);
-    return launch_k(merge, dim3(grid, G), dim3(hd), 0, st, a, G);
+    return launch_k(merge, dim3(batch * nkv, G), dim3(kQ4MergeWarps * 32), 0, st, a, G);
   };
   cudaError_t e;
   if (hd == 128)
-    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 1, 4>(), attr[0])
-                : go(k_paged_attn_q4<128, 2, 6>, k_q4_merge<128>, q4_smem_bytes<128, 2, 6>(), attr[1]);
+    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[0])
+                : go(k_paged_attn_q4<128, 2, 8>, k_q4_merge<128>, q4_smem_bytes<128, 8>(), attr[1]);
   else
-    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 5>, k_q4_merge<64>, q4_smem_bytes<64, 1, 5>(), attr[2])
-                : go(k_paged_attn_q4<64, 2, 8>, k_q4_merge<64>, q4_smem_bytes<64, 2, 8>(), attr[3]);
+    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 8>, k_q4_merge<64>, q4_smem_bytes<64, 8>(), attr[2])
+                : go(k_paged_attn_q4<64, 2, 8>, k_q4_merge<64>, q4_smem_bytes<64, 8>(), attr[3]);
   if (e != cudaSuccess) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache could not be launched: %s", cudaGetErrorString(e));
     return -1;

@@ -442,7 +442,9 @@ def kv4_read(cache, slots, hd, block_size=16):
 def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, out=None):
     """`paged_attn_decode` over a 4-bit cache: q bf16 [batch, >= nq * hd] (the first nq * hd columns; rows start on 16-byte boundaries),
     block_tables int32 [batch, max_blocks], ctx_lens int32 [batch].  At most 16 query heads per KV head.  A table entry that names no
-    block leaves its tokens out; a request without tokens gets zeros.  Returns bf16 [batch, nq * hd]."""
+    block leaves its tokens out; a request without tokens gets zeros.  scale > 0.  Returns bf16 [batch, nq * hd]."""
+    if not scale > 0:
+        raise ValueError("attention over the 4-bit cache needs a positive scale")
     if q.is_cuda:
         _count()
         return _C().paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, out)

@@ -343,6 +343,9 @@ def test_refusals():
                 dict(block_tables=table.long()), dict(ctx_lens=ctx[:1]), dict(ctx_lens=ctx.cpu()), dict(out=q.float())):
         with pytest.raises((RuntimeError, TypeError)):
             ops.paged_attn_decode_q4(**{**ok, **bad})
+    for scale in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError):
+            ops.paged_attn_decode_q4(**{**ok, "scale": scale})
     x = _randn(2, 2, 12 * 128).bfloat16()
     w = dict(qkv=x, positions=ctx, slots=ctx, cache=cache, nq=8, nkv=2, hd=128, block_size=16, theta=1e6)
     for bad in (dict(hd=64), dict(nq=7), dict(block_size=32), dict(block_size=8), dict(positions=ctx[:1]), dict(slots=ctx.long()), dict(slots=None),
