@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ ca
 // the running softmax is the greatest of x_t + log2(largest step of t), so that p step stays within fp16 whatever the values'
 // size; it moves only when it is exceeded by 2^8, which one vote per tile finds out.
 //
-// Work: the tiles of all (request, KV head) pairs in one row, cut into equal runs, one for each warp; a warp has a ring of its own
-// that the bulk copies fill across pairs, and shares nothing with others.  Lengths are on the GPU only, so every warp adds
+// Work: the units (two tiles) of all (request, KV head) pairs in one row, cut into equal runs, one for each warp; a warp has a
+// ring of its own that the bulk copies fill across pairs, and shares nothing with others.  Lengths are on the GPU only, so every warp adds
 // them up by itself.  Pairs that were cut are joined by k_q4_merge.
 constexpr int kQ4MaxG = 16;
 constexpr int kQ4Warps = 4;
@@ -321,29 +321,28 @@ __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// Where a flat tile index stands: its pair begins at `start` and has `tiles`.
+// Where a flat unit index stands: its pair begins at `start` and has `units`.
+constexpr int kQ4Unit = 2 * kQ4Tokens;
 struct Q4At {
-  int b, h, start, tiles;
+  int b, h, start, units;
 };
-__device__ __forceinline__ int q4_tiles(const Q4Attn& a, int b) {
-  const int most = a.max_blocks * a.block_size, n = min(max(a.ctx_lens[b], 0), most);
-  return (n + kQ4Tokens - 1) / kQ4Tokens;
-}
+__device__ __forceinline__ int q4_context(const Q4Attn& a, int b) { return min(max(a.ctx_lens[b], 0), a.max_blocks * a.block_size); }
+__device__ __forceinline__ int q4_units(const Q4Attn& a, int b) { return (q4_context(a, b) + kQ4Unit - 1) / kQ4Unit; }
 __device__ __forceinline__ void q4_advance(const Q4Attn& a, Q4At& p, int idx) {
-  while (idx >= p.start + p.tiles && p.b < a.batch) {
-    p.start += p.tiles;
+  while (idx >= p.start + p.units && p.b < a.batch) {
+    p.start += p.units;
     if (++p.h == a.nkv) {
       p.h = 0;
       do {
         ++p.b;
-      } while (p.b < a.batch && (p.tiles = q4_tiles(a, p.b)) == 0);
+      } while (p.b < a.batch && (p.units = q4_units(a, p.b)) == 0);
     }
   }
 }
 
 template <int HD, int STAGES>
 constexpr int q4_smem_bytes() {
-  return kQ4Warps * STAGES * (q4_tile_bytes(HD) + 8);
+  return kQ4Warps * STAGES * (2 * q4_tile_bytes(HD) + 8);
 }
 
 template <int HD, int NT, int STAGES>
@@ -354,8 +353,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
   __shared__ uint32_t s_abort[kQ4Warps];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kQ4Warps * STAGES * TB) + warp * STAGES;
-  const uint32_t ring = smem_u32(smem) + warp * STAGES * TB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kQ4Warps * STAGES * 2 * TB) + warp * STAGES;
+  const uint32_t ring = smem_u32(smem) + warp * STAGES * 2 * TB;
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
@@ -365,14 +364,14 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
   __syncwarp();
   pdl_wait();
 
-  // ---- this warp's run of tiles: [lo, hi) of all pairs' tiles (neighbouring runs on different SMs) ---------------
+  // ---- this warp's run of units: [lo, hi) of all pairs' units (neighbouring runs on different SMs) ---------------
   const int G = a.nq / a.nkv, me = warp * gridDim.x + blockIdx.x, runs = gridDim.x * kQ4Warps;
   int lo, hi, run;
   Q4At seg;
   {
     const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += q4_tiles(a, b);
+    for (int b = b0; b < b1; ++b) mine += q4_units(a, b);
     mine *= a.nkv;
     int upto = mine;
 #pragma unroll
@@ -385,68 +384,67 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
     lo = int(min(int64_t(me) * run, int64_t(total)));
     hi = min(lo + run, total);
     int b = b0, at = upto - mine, n = 0;
-    const bool holds = at <= lo && lo < upto;  // one lane's requests hold the first tile
+    const bool holds = at <= lo && lo < upto;  // one lane's requests hold the first unit
     if (holds)
-      for (n = q4_tiles(a, b) * a.nkv; lo >= at + n; n = q4_tiles(a, ++b) * a.nkv) at += n;
+      for (n = q4_units(a, b) * a.nkv; lo >= at + n; n = q4_units(a, ++b) * a.nkv) at += n;
     const uint32_t who = __ballot_sync(kAll, holds);
     const int src = who ? __ffs(who) - 1 : 0;
     seg.b = __shfl_sync(kAll, b, src);
     at = __shfl_sync(kAll, at, src);
-    seg.tiles = max(__shfl_sync(kAll, n, src) / a.nkv, 1);
-    seg.h = (lo - at) / seg.tiles;
-    seg.start = at + seg.h * seg.tiles;
+    seg.units = max(__shfl_sync(kAll, n, src) / a.nkv, 1);
+    seg.h = (lo - at) / seg.units;
+    seg.start = at + seg.h * seg.units;
   }
   // requests without tokens
   for (int b = me; b < a.batch; b += runs)
-    if (q4_tiles(a, b) == 0) {
+    if (q4_units(a, b) == 0) {
       for (int i = lane; i < a.nq * HD / 8; i += 32) reinterpret_cast<uint4*>(a.out + size_t(b) * a.nq * HD)[i] = make_uint4(0, 0, 0, 0);
       for (int h = lane; h < a.nkv; h += 32) a.meta[size_t(b) * a.nkv + h] = make_int2(0, 0);
     }
   if (lo >= hi) return;
 
-  // ---- copies: lane l knows where the l-th of the next 32 tiles lies -------------------------------------------
+  // ---- copies: lane l knows where tile l of the next 16 units lies ---------------------------------------------
   const int count = hi - lo;
   Q4At ahead = seg;
   int chunk = -1;
   long long where = -1;
-  uint32_t absent = 0;   // bit s: the tile of stage s has no block
-  uint32_t pending = 0;  // bit s: a copy into stage s is on its way
+  uint32_t there = 0;  // bits 2 s, 2 s + 1: the tiles of stage s have a block
   const uint32_t leader = elect_leader();
   auto issue = [&](int i, int stage) {
-    if ((i >> 5) != chunk) {
-      chunk = i >> 5;
-      const int idx = lo + chunk * 32 + lane;
+    if ((i >> 4) != chunk) {
+      chunk = i >> 4;
+      const int idx = lo + chunk * 16 + (lane >> 1);
       where = -1;
       if (idx < hi) {
         q4_advance(a, ahead, idx);
-        const int tok = (idx - ahead.start) * kQ4Tokens, page = tok / a.block_size;
-        const int blk = a.tables[size_t(ahead.b) * a.max_blocks + page];
-        if (blk >= 0 && blk < a.n_blocks)
-          where = (long long)(q4_tile_offset(blk, tok - page * a.block_size, ahead.h, a.nkv, a.block_size, HD));
+        const int tok = (idx - ahead.start) * kQ4Unit + (lane & 1) * kQ4Tokens;
+        if (tok < q4_context(a, ahead.b)) {
+          const int page = tok / a.block_size, blk = a.tables[size_t(ahead.b) * a.max_blocks + page];
+          if (blk >= 0 && blk < a.n_blocks)
+            where = (long long)(q4_tile_offset(blk, tok - page * a.block_size, ahead.h, a.nkv, a.block_size, HD));
+        }
       }
     }
-    const long long off = __shfl_sync(kAll, where, i & 31);
-    if (off < 0) {
-      absent |= 1u << stage;
-      return;
-    }
-    absent &= ~(1u << stage);
-    pending |= 1u << stage;
-    mbar_expect_tx_warp(leader, bars + stage, TB);
-    bulk_load_warp(leader, ring + stage * TB, a.cache + off, TB, smem_u32(bars + stage), kHintEvictFirst);
+    const int from = 2 * (i & 15);
+    const long long off0 = __shfl_sync(kAll, where, from), off1 = __shfl_sync(kAll, where, from + 1);
+    const uint32_t has = (off0 >= 0 ? 1u : 0u) | (off1 >= 0 ? 2u : 0u), dst = ring + stage * 2 * TB;
+    there = (there & ~(3u << (2 * stage))) | has << (2 * stage);
+    mbar_expect_tx_warp(leader, bars + stage, TB * __popc(has));
+    if (off0 >= 0) bulk_load_warp(leader, dst, a.cache + off0, TB, smem_u32(bars + stage), kHintEvictFirst);
+    if (off1 >= 0) bulk_load_warp(leader, dst + TB, a.cache + off1, TB, smem_u32(bars + stage), kHintEvictFirst);
   };
 #pragma unroll 1
-  for (int i = 0; i < STAGES - 1; ++i)
+  for (int i = 0; i < STAGES; ++i)
     if (i < count) issue(i, i);
 
-  int k = 0, stage = 0;  // tile of the run, its stage
-  uint32_t parity = 0;   // bit s: parity that stage s's next copy completes
+  int k = 0, stage = 0;  // unit of the run, its stage
+  uint32_t phase = 0;
   bool dead = false;
-  while (k < count) {
-    const int seg_end = min(hi, seg.start + seg.tiles) - lo;
-    const bool begins = lo + k == seg.start, whole = begins && lo + seg_end == seg.start + seg.tiles;
+  while (k < count && !dead) {
+    const int seg_end = min(hi, seg.start + seg.units) - lo;
+    const bool begins = lo + k == seg.start, whole = begins && lo + seg_end == seg.start + seg.units;
     const int piece = 2 * me + (k == 0 ? 0 : 1);
-    const int ctx = min(max(a.ctx_lens[seg.b], 0), a.max_blocks * a.block_size);
+    const int ctx = q4_context(a, seg.b);
     // ---- queries of this pair: operands, factor, sums --------------------------------------------
     uint32_t qb[NT][NA][4], qs[NT][2];
     float f[NT][2];
@@ -511,34 +509,25 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
 
 #pragma unroll 1
     for (; k < seg_end; ++k) {
-      {
-        int ns = stage + STAGES - 1;
-        if (ns >= STAGES) ns -= STAGES;
-        if (k + STAGES - 1 < count && !dead) issue(k + STAGES - 1, ns);
-      }
-      const int st = stage;
-      if (++stage == STAGES) stage = 0;
-      if (dead || (absent >> st & 1)) continue;
-      if (!mbar_wait_bounded_warp(bars + st, parity >> st & 1, &s_abort[warp])) {
+      if (!mbar_wait_bounded_warp(bars + stage, phase, &s_abort[warp])) {
         dead = true;
-        continue;
+        break;
       }
-      parity ^= 1u << st;
-      pending &= ~(1u << st);
-      const uint32_t tile = ring + st * TB;
-      const int left = ctx - (lo + k - seg.start) * kQ4Tokens;  // tokens of this tile
+      const uint32_t tile = ring + stage * 2 * TB;
+      const int left = ctx - (lo + k - seg.start) * kQ4Unit;  // tokens of this unit
 
-      // ---- scores, over the factor f: tokens g (c[0], c[1]) and g + 8, heads 2 t and 2 t + 1 ----
-      float c[NT][4];
-      {
+      // ---- scores, over the factor f: tokens g (c[.][.][0], [1]) and g + 8 of either tile, heads 2 t and 2 t + 1 ----
+      float c[2][NT][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
         uint32_t w0[NA], w1[NA], sl0[NA], sl1[NA];
-        lds_words<NA>(tile + g * (HD / 2) + t * NA * 4, w0);
-        lds_words<NA>(tile + (g + 8) * (HD / 2) + t * NA * 4, w1);
-        lds_words<NA>(tile + q4_k_params(HD) + g * NA * 4, sl0);  // step[NA], low[NA]
-        lds_words<NA>(tile + q4_k_params(HD) + (g + 8) * NA * 4, sl1);
+        lds_words<NA>(tile + u * TB + g * (HD / 2) + t * NA * 4, w0);
+        lds_words<NA>(tile + u * TB + (g + 8) * (HD / 2) + t * NA * 4, w1);
+        lds_words<NA>(tile + u * TB + q4_k_params(HD) + g * NA * 4, sl0);  // step[NA], low[NA]
+        lds_words<NA>(tile + u * TB + q4_k_params(HD) + (g + 8) * NA * 4, sl1);
         const uint32_t m0 = NA == 4 && (t & 1) ? sl0[NA - 1] : sl0[NA / 2], m1 = NA == 4 && (t & 1) ? sl1[NA - 1] : sl1[NA / 2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) q4_mma_bf16_0(c[n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
+        for (int n = 0; n < NT; ++n) q4_mma_bf16_0(c[u][n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
 #pragma unroll
         for (int ga = 0; ga < NA; ++ga) {
           const float s0 = ga & 1 ? bf16_hi(sl0[ga >> 1]) : bf16_lo(sl0[ga >> 1]), s1 = ga & 1 ? bf16_hi(sl1[ga >> 1]) : bf16_lo(sl1[ga >> 1]);
@@ -548,55 +537,70 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
             float d[4];
             q4_mma_f16_0(d, w0[ga] & 0x000f000fu, w1[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00f000f0u, qb[n][ga][0], qb[n][ga][1]);
             q4_mma_f16(d, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qb[n][ga][2], qb[n][ga][3]);
-            c[n][0] += s0 * d[0];
-            c[n][1] += s0 * d[1];
-            c[n][2] += s1 * d[2];
-            c[n][3] += s1 * d[3];
+            c[u][n][0] += s0 * d[0];
+            c[u][n][1] += s0 * d[1];
+            c[u][n][2] += s1 * d[2];
+            c[u][n][3] += s1 * d[3];
           }
         }
       }
-      uint32_t vs0[NA], vs1[NA];  // step[NA], low[NA] of the values of tokens g and g + 8
-      lds_words<NA>(tile + q4_v_params(HD) + g * NA * 4, vs0);
-      lds_words<NA>(tile + q4_v_params(HD) + (g + 8) * NA * 4, vs1);
-      if (left < kQ4Tokens) {
-        // behind the last token: whatever the cache holds there (NaN too) stays out
+      uint32_t vs0[2][NA], vs1[2][NA];  // step[NA], low[NA] of the values of tokens g and g + 8
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (g + 8 * j >= left) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) c[n][2 * j] = c[n][2 * j + 1] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < NA; ++i) (j ? vs1 : vs0)[i] = 0;
-          }
+      for (int u = 0; u < 2; ++u) {
+        lds_words<NA>(tile + u * TB + q4_v_params(HD) + g * NA * 4, vs0[u]);
+        lds_words<NA>(tile + u * TB + q4_v_params(HD) + (g + 8) * NA * 4, vs1[u]);
       }
-      float s0[NA], s1[NA], top0 = 8.0779356694631609e-28f, top1 = top0;  // the larger of the steps and 2^-90
+      const uint32_t has = there >> (2 * stage) & 3;
+      if (left < kQ4Unit || has != 3) {
+        // behind the last token, and where there is no block: whatever stands there (NaN too) stays out
 #pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        s0[i] = i & 1 ? bf16_hi(vs0[i >> 1]) : bf16_lo(vs0[i >> 1]);
-        s1[i] = i & 1 ? bf16_hi(vs1[i >> 1]) : bf16_lo(vs1[i >> 1]);
-        top0 = fmaxf(top0, s0[i]);
-        top1 = fmaxf(top1, s1[i]);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (16 * u + 8 * j + g >= left || !(has >> u & 1)) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) c[u][n][2 * j] = c[u][n][2 * j + 1] = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < NA; ++i) (j ? vs1[u] : vs0[u])[i] = 0;
+            }
+      }
+      float top[2][2];  // the larger of a token's steps and 2^-90
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        top[u][0] = top[u][1] = 8.0779356694631609e-28f;
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+          top[u][0] = fmaxf(top[u][0], i & 1 ? bf16_hi(vs0[u][i >> 1]) : bf16_lo(vs0[u][i >> 1]));
+          top[u][1] = fmaxf(top[u][1], i & 1 ? bf16_hi(vs1[u][i >> 1]) : bf16_lo(vs1[u][i >> 1]));
+        }
       }
       // ---- probabilities; where one times step leaves fp16's range, a new reference first ----
-      float p[NT][4];
+      float p[2][NT][4];
       auto weigh = [&] {
         float most = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            p[n][j] = q4_ex2(fmaf(c[n][j], f[n][j & 1], -R[n][j & 1]));
-            most = fmaxf(most, p[n][j] * (j < 2 ? top0 : top1));  // (a NaN leaves the reference alone)
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              p[u][n][j] = q4_ex2(fmaf(c[u][n][j], f[n][j & 1], -R[n][j & 1]));
+              most = fmaxf(most, p[u][n][j] * top[u][j >> 1]);  // (a NaN leaves the reference alone)
+            }
         return most;
       };
       if (__any_sync(kAll, weigh() > 512.f)) {
-        const float e0 = fminf(float(int(__float_as_uint(top0) >> 23) - 127), 110.f), e1 = fminf(float(int(__float_as_uint(top1) >> 23) - 127), 110.f);
+        float e[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) e[u][j] = fminf(float(int(__float_as_uint(top[u][j]) >> 23) - 127), 110.f);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float z = fmaxf(fmaf(c[n][j], f[n][j], e0), fmaf(c[n][2 + j], f[n][j], e1));
+            float z = fmaxf(fmaxf(fmaf(c[0][n][j], f[n][j], e[0][0]), fmaf(c[0][n][2 + j], f[n][j], e[0][1])),
+                            fmaxf(fmaf(c[1][n][j], f[n][j], e[1][0]), fmaf(c[1][n][2 + j], f[n][j], e[1][1])));
             z = fmaxf(z, __shfl_xor_sync(kAll, z, 4));
             z = fmaxf(z, __shfl_xor_sync(kAll, z, 8));
             z = fmaxf(fmaxf(z, __shfl_xor_sync(kAll, z, 16)), R[n][j]);
@@ -613,34 +617,43 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
           }
         weigh();
       }
-      // ---- values: p times step as the columns' operand, p times low beside it ----
-      {
+      // ---- values: p times step as the columns' operand, p times low beside it.  The rows g of a product take a byte's two codes together,
+      // low + 16 high, the rows g + 8 the high one: one instruction less for a word, and the difference is taken at the end ----
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
         uint32_t w0[NA], w1[NA];
-        lds_words<NA>(tile + q4_v_codes(HD) + t * HD + g * NA * 4, w0);
-        lds_words<NA>(tile + q4_v_codes(HD) + (t + 4) * HD + g * NA * 4, w1);
+        lds_words<NA>(tile + u * TB + q4_v_codes(HD) + t * HD + g * NA * 4, w0);
+        lds_words<NA>(tile + u * TB + q4_v_codes(HD) + (t + 4) * HD + g * NA * 4, w1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          l[n][0] += p[n][0] + p[n][2];
-          l[n][1] += p[n][1] + p[n][3];
+          l[n][0] += p[u][n][0] + p[u][n][2];
+          l[n][1] += p[u][n][1] + p[u][n][3];
         }
 #pragma unroll
         for (int ga = 0; ga < NA; ++ga) {
-          const uint32_t lw0 = vs0[NA / 2 + (ga >> 1)], lw1 = vs1[NA / 2 + (ga >> 1)];
+          const float s0 = ga & 1 ? bf16_hi(vs0[u][ga >> 1]) : bf16_lo(vs0[u][ga >> 1]), s1 = ga & 1 ? bf16_hi(vs1[u][ga >> 1]) : bf16_lo(vs1[u][ga >> 1]);
+          const uint32_t lw0 = vs0[u][NA / 2 + (ga >> 1)], lw1 = vs1[u][NA / 2 + (ga >> 1)];
           const float m0 = ga & 1 ? bf16_hi(lw0) : bf16_lo(lw0), m1 = ga & 1 ? bf16_hi(lw1) : bf16_lo(lw1);
-          const uint32_t v0 = w0[ga] >> 8, v1 = w1[ga] >> 8;
+          const uint32_t v0 = __byte_perm(w0[ga], 0, 0x4341), v1 = __byte_perm(w1[ga], 0, 0x4341);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint32_t pb0 = q4_transpose(pack_f16x2(p[n][0] * s0[ga], p[n][1] * s0[ga]));
-            const uint32_t pb1 = q4_transpose(pack_f16x2(p[n][2] * s1[ga], p[n][3] * s1[ga]));
-            vm[n][ga][0] = fmaf(p[n][0], m0, fmaf(p[n][2], m1, vm[n][ga][0]));
-            vm[n][ga][1] = fmaf(p[n][1], m0, fmaf(p[n][3], m1, vm[n][ga][1]));
-            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x000f000fu, w1[ga] & 0x00f000f0u, pb0, pb1);
-            q4_mma_f16(o[n][2 * ga + 1], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu, v1 & 0x00f000f0u, pb0, pb1);
+            const float *q = p[u][n];
+            const uint32_t pb0 = q4_transpose(pack_f16x2(q[0] * s0, q[1] * s0)), pb1 = q4_transpose(pack_f16x2(q[2] * s1, q[3] * s1));
+            vm[n][ga][0] = fmaf(q[0], m0, fmaf(q[2], m1, vm[n][ga][0]));
+            vm[n][ga][1] = fmaf(q[1], m0, fmaf(q[3], m1, vm[n][ga][1]));
+            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x00ff00ffu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00ff00ffu, w1[ga] & 0x00f000f0u, pb0, pb1);
+            q4_mma_f16(o[n][2 * ga + 1], v0, v0 & 0x00f000f0u, v1, v1 & 0x00f000f0u, pb0, pb1);
           }
         }
       }
-      __syncwarp();  // all lanes have read the stage that the next copy fills
+      __syncwarp();  // all lanes have read the stage that the next copies fill
+      if (k + STAGES < count) issue(k + STAGES, stage);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
+    if (dead) break;
 
     // ---- out: the whole pair, or a piece of it ---------------------------------------------------------
 #pragma unroll
@@ -659,8 +672,9 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
         float* part = a.part + size_t(piece) * q4_part_floats(G, HD);
 #pragma unroll
         for (int i = 0; i < NA; ++i) {  // 2^24, and the 16 of the odd dims
-          const float v0 = fmaf(o[n][2 * i][j], 16777216.f, vm[n][i][j]) * inv, v1 = fmaf(o[n][2 * i][2 + j], 1048576.f, vm[n][i][j]) * inv,
-                      v2 = fmaf(o[n][2 * i + 1][j], 16777216.f, vm[n][i][j]) * inv, v3 = fmaf(o[n][2 * i + 1][2 + j], 1048576.f, vm[n][i][j]) * inv;
+          const float *o0 = o[n][2 * i], *o1 = o[n][2 * i + 1], add = vm[n][i][j];
+          const float v0 = fmaf(o0[j] - o0[2 + j], 16777216.f, add) * inv, v1 = fmaf(o0[2 + j], 1048576.f, add) * inv,
+                      v2 = fmaf(o1[j] - o1[2 + j], 16777216.f, add) * inv, v3 = fmaf(o1[2 + j], 1048576.f, add) * inv;
           const int d = 4 * (8 * i + g);
           if (whole)
             *reinterpret_cast<uint2*>(a.out + (size_t(seg.b) * a.nq + size_t(seg.h) * G + head) * HD + d) =
@@ -671,14 +685,19 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q
         if (!whole && g == 0) *reinterpret_cast<float2*>(part + G * HD + 2 * head) = make_float2(R[n][j], l[n][j]);
       }
     if (begins && lane == 0)
-      a.meta[size_t(seg.b) * a.nkv + seg.h] = make_int2(piece, whole ? 0 : (seg.start + seg.tiles - 1) / run - me + 1);
+      a.meta[size_t(seg.b) * a.nkv + seg.h] = make_int2(piece, whole ? 0 : (seg.start + seg.units - 1) / run - me + 1);
     if (k < count) q4_advance(a, seg, lo + k);
   }
   if (dead) {
     // a copy did not arrive in time: say so, and leave with none in flight
     if (lane == 0) g_kv4_err = 1;
-    for (int s = 0; s < STAGES; ++s)
-      if (pending >> s & 1) mbar_wait_bounded_warp(bars + s, parity >> s & 1, &s_abort[warp]);
+    for (int i = k; i < min(k + STAGES, count); ++i) {
+      mbar_wait_bounded_warp(bars + stage, phase, &s_abort[warp]);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
   }
 }
 
@@ -844,7 +863,7 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   a.meta = reinterpret_cast<int2*>(a.part + 2 * size_t(grid) * kQ4Warps * q4_part_floats(G, hd));
   a.q_stride = q_stride; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks;
   a.max_blocks = max_blocks;
-  a.min_run = 2;
+  a.min_run = 1;
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   static bool attr[4][64] = {};
@@ -856,11 +875,11 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   };
   cudaError_t e;
   if (hd == 128)
-    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[0])
-                : go(k_paged_attn_q4<128, 2, 8>, k_q4_merge<128>, q4_smem_bytes<128, 8>(), attr[1]);
+    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 2>, k_q4_merge<128>, q4_smem_bytes<128, 2>(), attr[0])
+                : go(k_paged_attn_q4<128, 2, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[1]);
   else
-    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 8>, k_q4_merge<64>, q4_smem_bytes<64, 8>(), attr[2])
-                : go(k_paged_attn_q4<64, 2, 8>, k_q4_merge<64>, q4_smem_bytes<64, 8>(), attr[3]);
+    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 4>, k_q4_merge<64>, q4_smem_bytes<64, 4>(), attr[2])
+                : go(k_paged_attn_q4<64, 2, 4>, k_q4_merge<64>, q4_smem_bytes<64, 4>(), attr[3]);
   if (e != cudaSuccess) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache could not be launched: %s", cudaGetErrorString(e));
     return -1;
