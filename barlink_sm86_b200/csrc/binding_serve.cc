@@ -208,8 +208,8 @@ void count_tokens(const at::Tensor& counts, const at::Tensor& seen, const at::Te
                              stream_of(counts), err, errlen));
 }
 
-// what = 0: the logits under the rules (into out, or a new tensor); 1: (token, value) of the arg max; 2: (value, token
-// bits) pairs of the slices of every row, float32 [slices, rows, 2], as argmax_merge takes them
+// what = 0: the logits under the rules (into out, or a new tensor); 1: (token, value) of the arg max; 2: the
+// same as (value, token bits) pairs, float32 [1, rows, 2], of which argmax_merge takes those of all ranks
 std::vector<at::Tensor> logit_rules(const at::Tensor& logits, int what, int64_t vocab, int offset, const OptTensor& penalties,
                                     const OptTensor& counts, const OptTensor& seen, const OptTensor& bias_ids, const OptTensor& bias,
                                     const OptTensor& mask, const OptTensor& out_opt) {
@@ -258,7 +258,6 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, int what, int64_t 
   }
   c10::cuda::CUDAGuard guard(logits.device());
   std::vector<at::Tensor> r;
-  at::Tensor part;
   if (what == 0) {
     at::Tensor out = out_opt ? *out_opt : at::empty({a.rows, a.n}, logits.options());
     check_on(out, logits, "out");
@@ -269,10 +268,9 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, int what, int64_t 
     a.ld_out = size_t(out.stride(0));
     r = {out};
   } else {
-    part = at::empty({bl_rules_chunks(a.rows, a.n), a.rows, 2}, logits.options().dtype(at::kFloat));
-    a.part = part.data_ptr();
     if (what == 2) {
-      r = {part};
+      r = {at::empty({1, a.rows, 2}, logits.options().dtype(at::kFloat))};
+      a.part = r[0].data_ptr();
     } else {
       r = {at::empty({a.rows}, logits.options().dtype(at::kInt)), at::empty({a.rows}, logits.options().dtype(at::kFloat))};
       a.idx = r[0].data_ptr();

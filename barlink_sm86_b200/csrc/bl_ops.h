@@ -466,8 +466,8 @@ int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables
 int bl_count_tokens(const int* ids, const int* cu, const int* prompt_lens, int* counts, void* seen, int rows, int n_ids, int vocab,
                     int reset, void* stream, char* err, size_t errlen);
 /* Rules on logits [rows][n] (bf16, or fp32): token id = column + offset.  seen: x / r or x * r; counted: - f * count - p; biases;
- * mask bits (1: allowed).  out: the result in the logits' type (may be logits); part: bl_rules_chunks(rows, n) x rows (value, token)
- * pairs, as bl_argmax_merge takes them; idx, val: arg max (lowest token; -1 where nothing is left). */
+ * mask bits (1: allowed).  out: the result in the logits' type (may be logits); part: (value, token) pairs of the rows, as
+ * bl_argmax_merge takes those of several ranks; idx, val: arg max (lowest token; -1 where nothing is left). */
 typedef struct blRulesArgs {
   const void* logits;
   size_t ld;
@@ -488,7 +488,6 @@ typedef struct blRulesArgs {
   int mask_words;
   size_t ld_mask;
 } blRulesArgs;
-int bl_rules_chunks(int rows, int n);
 int bl_logit_rules(const blRulesArgs* a, void* stream, char* err, size_t errlen);
 
 #ifdef __cplusplus

@@ -138,39 +138,45 @@ __device__ __forceinline__ void q4_store8(uint8_t* tile, int r, int hd, bool val
   }
 }
 
-// One block per row.  A thread takes an octet of a head's lower half and its rotation partner; the angles of the row are
-// computed once, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01 radians), and the products are
-// rounded one by one: the rotated elements are the formula's to the bit.
-__global__ void __launch_bounds__(256) k_rope_kv_write_q4(const Q4Write a) {
+// A block takes kQ4Rows neighbouring rows.  A thread turns an octet of a head's lower half and its rotation partner; the angles of
+// the block's rows are computed once, one or two to a thread, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01
+// radians), and the products are rounded one by one: the rotated elements are the formula's to the bit.
+template <int ROWS, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_rope_kv_write_q4(const Q4Write a) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float2 s_rot[128];
-  const int row = blockIdx.x, half = a.hd >> 1, width = (a.nq + 2 * a.nkv) * a.hd;
-  for (int i = threadIdx.x; i < half; i += blockDim.x) {
-    const double turn = double(a.positions[row]) * exp2(-a.log2_theta * (double(2 * i) / a.hd)) * 0.15915494309189533577;
+  __shared__ float2 s_rot[ROWS][64];
+  __shared__ int s_slot[ROWS];
+  const int row0 = blockIdx.x * ROWS, rows = min(ROWS, a.rows - row0), half = a.hd >> 1, width = (a.nq + 2 * a.nkv) * a.hd;
+  // (THREADS is a multiple of 64: a thread has the same pair in every row that it visits)
+  const double inv = exp2(-a.log2_theta * (double(2 * (int(threadIdx.x) & (half - 1))) / a.hd)) * 0.15915494309189533577;
+  for (int e = threadIdx.x; e < rows * half; e += THREADS) {
+    const int r = e / half;
+    const double turn = double(a.positions[row0 + r]) * inv;
     double sn, cs;
     sincospi(2.0 * (turn - rint(turn)), &sn, &cs);
-    s_rot[i] = make_float2(float(cs), float(sn));
+    s_rot[r][e & (half - 1)] = make_float2(float(cs), float(sn));
+  }
+  if (threadIdx.x < rows) {
+    const int slot = a.slots ? a.slots[row0 + threadIdx.x] : -1;
+    s_slot[threadIdx.x] = slot >= 0 && slot / a.block_size < a.n_blocks ? slot : -1;  // (no such block: not kept)
   }
   __syncthreads();
-  int slot = a.slots ? a.slots[row] : -1;
-  const int blk = slot >= 0 ? slot / a.block_size : 0, in_block = slot >= 0 ? slot % a.block_size : 0;
-  if (blk >= a.n_blocks) slot = -1;  // no such block: not kept
-  const int oph = a.hd >> 4;  // octets of half a head
+  const int oph = a.hd >> 4;  // octets of half a head: 4 or 8, so that quads are whole
   const int units = (a.nq + 2 * a.nkv) * oph;
-  for (int u0 = 0; u0 < units; u0 += blockDim.x) {
+  for (int u0 = 0; u0 < rows * units; u0 += THREADS) {
     const int u = u0 + threadIdx.x;
-    const bool there = u < units;  // (whole quads: oph is a multiple of 4)
-    const int h = there ? u / oph : 0, o = there ? u % oph : 0, col = h * a.hd + 8 * o;
+    const bool there = u < rows * units;
+    const int r = there ? u / units : 0, v = there ? u - r * units : 0, h = v / oph, o = v & (oph - 1), col = h * a.hd + 8 * o;
     float x[8] = {}, y[8] = {};
     if (there) {
-      q4_load8(a, row, width, col, x);
-      q4_load8(a, row, width, col + half, y);
+      q4_load8(a, row0 + r, width, col, x);
+      q4_load8(a, row0 + r, width, col + half, y);
       uint32_t ox[4], oy[4];
       if (h < a.nq + a.nkv) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float2 cs = s_rot[8 * o + j];
+          const float2 cs = s_rot[r][8 * o + j];
           const float p = __fsub_rn(__fmul_rn(x[j], cs.x), __fmul_rn(y[j], cs.y));
           const float q = __fadd_rn(__fmul_rn(y[j], cs.x), __fmul_rn(x[j], cs.y));
           x[j] = __bfloat162float(__float2bfloat16(p));
@@ -182,20 +188,22 @@ __global__ void __launch_bounds__(256) k_rope_kv_write_q4(const Q4Write a) {
         ox[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
         oy[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
       }
-      __nv_bfloat16* p = a.out + size_t(row) * width + col;
+      __nv_bfloat16* p = a.out + size_t(row0 + r) * width + col;
       *reinterpret_cast<uint4*>(p) = make_uint4(ox[0], ox[1], ox[2], ox[3]);
       *reinterpret_cast<uint4*>(p + half) = make_uint4(oy[0], oy[1], oy[2], oy[3]);
     }
+    const int slot = s_slot[r];
     const bool keep = there && h >= a.nq && slot >= 0;
     if (!__any_sync(0xffffffffu, keep)) continue;
     uint16_t s0, l0, s1, l1;
     const uint32_t w0 = q4_quantise8(x, s0, l0), w1 = q4_quantise8(y, s1, l1);
     if (keep) {
       const bool value = h >= a.nq + a.nkv;
+      const int blk = slot / a.block_size, in_block = slot - blk * a.block_size;
       uint8_t* tile = a.cache + q4_tile_offset(blk, in_block, h - a.nq - (value ? a.nkv : 0), a.nkv, a.block_size, a.hd);
-      const int r = in_block % kQ4Tokens;
-      q4_store8(tile, r, a.hd, value, o >> 2, o & 3, w0, s0, l0);
-      q4_store8(tile, r, a.hd, value, (o + oph) >> 2, o & 3, w1, s1, l1);
+      const int tr = in_block % kQ4Tokens;
+      q4_store8(tile, tr, a.hd, value, o >> 2, o & 3, w0, s0, l0);
+      q4_store8(tile, tr, a.hd, value, (o + oph) >> 2, o & 3, w1, s1, l1);
     }
   }
 }
@@ -346,7 +354,7 @@ constexpr int q4_smem_bytes() {
 }
 
 template <int HD, int NT, int STAGES>
-__global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 4 : 2) k_paged_attn_q4(const Q4Attn a) {
+__global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q4(const Q4Attn a) {
   constexpr int NA = HD / kQ4Group, TB = q4_tile_bytes(HD);
   constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -797,7 +805,10 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
   a.cache = static_cast<uint8_t*>(cache);
   a.rows = rows; a.nq = nq; a.nkv = nkv; a.hd = hd; a.block_size = block_size; a.n_blocks = n_blocks;
   a.log2_theta = log2(theta);
-  launch_k(k_rope_kv_write_q4, dim3(rows), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Many rows: four to a block share the threads' angles; few rows (a decode step): one each, all loads in one go.
+  if (rows > 4 * sm_count()) launch_k(k_rope_kv_write_q4<4, 256>, dim3((rows + 3) / 4), dim3(256), 0, st, a);
+  else launch_k(k_rope_kv_write_q4<1, 320>, dim3(rows), dim3(320), 0, st, a);
   KV4_LAUNCH_CHECK("rope_kv_write_q4");
   return 0;
 }
@@ -821,7 +832,7 @@ extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
 }
 
 // blocks of attention: as many as are resident at once
-static int q4_grid(int G) { return sm_count() * (G > 8 ? 2 : 4); }
+static int q4_grid(int G) { return sm_count() * (G > 8 ? 2 : 3); }
 
 extern "C" size_t bl_paged_attn_decode_q4_ws(int batch, int nq, int nkv, int hd) {
   const int G = nq / nkv;
@@ -875,7 +886,7 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   };
   cudaError_t e;
   if (hd == 128)
-    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 2>, k_q4_merge<128>, q4_smem_bytes<128, 2>(), attr[0])
+    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 3>, k_q4_merge<128>, q4_smem_bytes<128, 3>(), attr[0])
                 : go(k_paged_attn_q4<128, 2, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[1]);
   else
     e = nt == 1 ? go(k_paged_attn_q4<64, 1, 4>, k_q4_merge<64>, q4_smem_bytes<64, 4>(), attr[2])

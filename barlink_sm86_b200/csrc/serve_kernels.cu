@@ -26,6 +26,7 @@ namespace bl {
 // ---------------------------------------------------------------------------
 constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutMaxBatch = 8192;
+constexpr int kLayoutAlone = 2048;  // rows up to which the one block writes them itself
 
 struct RequestLayout {
   const int* new_lens;  // tokens that a request gets now; below 0: it has ended
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
     const int b = owner_of(s_fresh, B, j);
     a.tables[size_t(b) * a.width + s_had[b] + j - s_fresh[b]] = j < free_n ? a.ring[ring_at(j)] : -1;
   }
+  if (a.tokens > kLayoutAlone) return;  // k_layout_rows does the rest
   for (int row = tid; row < a.tokens; row += kLayoutThreads) {
     int pos = 0, slot = -1;
     if (row < tot[0]) {
@@ -183,22 +185,79 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
   }
 }
 
+// The rows of many tokens, behind k_paged_layout: four rows a thread, the first by bisection, the others by going on.
+__global__ void __launch_bounds__(256) k_layout_rows(const RequestLayout a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row0 = (blockIdx.x * 256 + threadIdx.x) * 4, bs = a.block_size;
+  if (row0 >= a.tokens) return;
+  int pos[4] = {0, 0, 0, 0}, slot[4] = {-1, -1, -1, -1};
+  if (row0 < a.cu[a.batch]) {
+    int b = owner_of(a.cu, a.batch, row0), next = a.cu[b + 1];
+    int base = a.ctx_lens[b] - next;  // position = base + row
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + i;
+      while (row >= next && ++b < a.batch) {
+        next = a.cu[b + 1];
+        base = a.ctx_lens[b] - next;
+      }
+      if (b >= a.batch) break;
+      pos[i] = base + row;
+      const int page = pos[i] / bs;
+      if (pos[i] >= 0 && page < a.width) {
+        const int id = a.tables[size_t(b) * a.width + page];
+        if (id >= 0) slot[i] = id * bs + pos[i] % bs;
+      }
+    }
+  }
+  if (row0 + 4 <= a.tokens && ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots)) & 15) == 0) {
+    *reinterpret_cast<int4*>(a.positions + row0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    *reinterpret_cast<int4*>(a.slots + row0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+  } else {
+    for (int i = 0; i < 4 && row0 + i < a.tokens; ++i) {
+      a.positions[row0 + i] = pos[i];
+      a.slots[row0 + i] = slot[i];
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // token histories to count tables
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) k_count_tokens(const int* __restrict__ ids, const int* __restrict__ cu,
-                                                      const int* __restrict__ prompt, int* __restrict__ counts,
-                                                      uint32_t* __restrict__ seen, int n_ids, int vocab, int words) {
+// A cluster of blocks owns a row: empties its tables, if asked to, and counts its tokens behind the cluster's barrier.
+constexpr int kCountThreads = 512;
+__device__ __forceinline__ void zero_words(uint32_t* p, size_t n, int who, int of) {
+  const size_t skip = min(n, size_t(-(reinterpret_cast<uintptr_t>(p) >> 2) & 3));  // to the next 16 bytes
+  if (size_t(who) < skip) p[who] = 0;
+  uint4* v = reinterpret_cast<uint4*>(p + skip);
+  const size_t nv = (n - skip) / 4;
+  for (size_t i = who; i < nv; i += of) v[i] = make_uint4(0, 0, 0, 0);
+  const size_t at = skip + nv * 4 + who;
+  if (at < n) p[at] = 0;
+}
+__global__ void __launch_bounds__(kCountThreads) k_count_tokens(const int* __restrict__ ids, const int* __restrict__ cu,
+                                                                const int* __restrict__ prompt, int* __restrict__ counts,
+                                                                uint32_t* __restrict__ seen, int n_ids, int vocab, int words, int reset) {
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x;
+  const int row = blockIdx.x / cluster_nctarank(), who = cluster_ctarank() * kCountThreads + threadIdx.x, of = cluster_nctarank() * kCountThreads;
+  counts += size_t(row) * vocab;
+  seen += size_t(row) * words;
+  if (reset) {
+    zero_words(reinterpret_cast<uint32_t*>(counts), vocab, who, of);
+    zero_words(seen, words, who, of);
+    __threadfence();
+    __syncwarp();
+    cluster_sync_all();
+  }
   const int lo = cu ? max(cu[row], 0) : row, hi = cu ? min(cu[row + 1], n_ids) : row + 1;
   const int p = prompt ? prompt[row] : 0;
-  for (int i = lo + blockIdx.y * blockDim.x + threadIdx.x; i < hi; i += gridDim.y * blockDim.x) {
+  for (int i = lo + who; i < hi; i += of) {
     const int id = ids[i];
     if (id < 0 || id >= vocab) continue;
-    atomicOr(seen + size_t(row) * words + (id >> 5), 1u << (id & 31));
-    if (i - lo >= p) atomicAdd(counts + size_t(row) * vocab + id, 1);
+    atomicOr(seen + (id >> 5), 1u << (id & 31));
+    if (i - lo >= p) atomicAdd(counts + id, 1);
   }
 }
 
@@ -208,7 +267,9 @@ __global__ void __launch_bounds__(256) k_count_tokens(const int* __restrict__ id
 struct Rules {
   const void* logits;
   void* out;     // same type, or null
-  float2* part;  // [chunks][rows] (value, token), or null
+  float2* part;  // [rows] (value, token), or null
+  int* idx;      // [rows], with val; or null
+  float* val;
   const float* penalties;  // [rows][3]: repetition, presence, frequency; or null
   const int* counts;
   const uint32_t* seen;
@@ -230,82 +291,178 @@ __device__ __forceinline__ T from_float(float v) {
   else return v;
 }
 
-// grid (rows, chunks).  Each operation is rounded by itself (no fused multiply-add): the values are the formula's to the bit.
+// bits [at, at + 8) of a row of `total` bits; those behind it are 0
+__device__ __forceinline__ uint32_t bits8(const uint32_t* words, int at, int total) {
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(words) + (at >> 3);
+  const int left = total - at, sh = at & 7;
+  if (left <= 0) return 0;
+  uint32_t v = p[0] >> sh;
+  if (sh && left > 8 - sh) v |= uint32_t(p[1]) << (8 - sh);
+  return left >= 8 ? v & 0xffu : v & ((1u << left) - 1);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) k_logit_rules(const Rules a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ float s_v[8];
-  __shared__ int s_i[8];
-  const int row = blockIdx.x, chunk = blockIdx.y, chunks = gridDim.y;
-  const T* p = static_cast<const T*>(a.logits) + size_t(row) * a.ld;
-  const int per = (a.n + chunks - 1) / chunks, lo = min(chunk * per, a.n), hi = min(lo + per, a.n);
-  const bool pen = a.penalties != nullptr;
-  const float again = pen ? a.penalties[row * 3] : 1.f, presence = pen ? a.penalties[row * 3 + 1] : 0.f,
-              frequency = pen ? a.penalties[row * 3 + 2] : 0.f;
-  float best = -INFINITY;
-  int bi = 0x7fffffff;
-  for (int i = lo + threadIdx.x; i < hi; i += blockDim.x) {
-    const int id = i + a.offset;
-    float x = to_float<T>(p[i]);
-    const bool known = id >= 0 && id < a.vocab;
-    if (pen && known && (a.seen[size_t(row) * a.words + (id >> 5)] >> (id & 31) & 1)) {
-      x = x > 0.f ? __fdiv_rn(x, again) : __fmul_rn(x, again);
-      const int c = a.counts[size_t(row) * a.vocab + id];
-      if (c > 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(frequency, float(c))), presence);
+__device__ __forceinline__ void load8(const T* p, int m, bool vec, float (&x)[8]) {
+  if (vec && m == 8) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
+      x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
-    for (int j = 0; j < a.n_bias; ++j)
-      if (a.bias_ids[row * a.n_bias + j] == id) x = __fadd_rn(x, a.bias[row * a.n_bias + j]);
-    if (a.mask && !(known && (a.mask[size_t(row) * a.ld_mask + (id >> 5)] >> (id & 31) & 1))) x = -INFINITY;
-    if (a.out) static_cast<T*>(a.out)[size_t(row) * a.ld_out + i] = from_float<T>(x);
-    if (x > best) {
-      best = x;
-      bi = id;
-    }
-  }
-  if (!a.part) return;
+  } else {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-    if (ov > best || (ov == best && oi < bi)) {
-      best = ov;
-      bi = oi;
+    for (int j = 0; j < 8; ++j) x[j] = j < m ? to_float<T>(p[j]) : -INFINITY;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int m, bool vec, const float (&x)[8]) {
+  if (vec && m == 8) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    } else {
+      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < m) p[j] = from_float<T>(x[j]);
   }
-  if ((threadIdx.x & 31) == 0) {
-    s_v[threadIdx.x >> 5] = best;
-    s_i[threadIdx.x >> 5] = bi;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w)
-      if (s_v[w] > best || (s_v[w] == best && s_i[w] < bi)) {
-        best = s_v[w];
-        bi = s_i[w];
-      }
-    a.part[size_t(chunk) * a.rows + row] = make_float2(best, __int_as_float(bi));
+}
+__device__ __forceinline__ void better(float& best, int& bi, float v, int i) {
+  if (v > best || (v == best && i < bi)) {
+    best = v;
+    bi = i;
   }
 }
 
-// (value, token) of a row's chunks -> the first of the greatest; -1 where nothing is left
-__global__ void k_rules_pick(const float2* __restrict__ part, int chunks, int rows, int* __restrict__ idx, float* __restrict__ val) {
+// A cluster of blocks shares a row, a thread takes eight neighbouring logits (16 bytes of bf16) with a byte of each bit table; only where a
+// byte says so are counts and biases read.  Two such vectors are on their way at a time.  Each operation is rounded by itself
+// (no fused multiply-add): the values are the formula's to the bit.  The blocks' maxima meet in the first block's shared memory.
+constexpr int kRulesThreads = 512;
+constexpr int kRulesShare = 8;  // blocks of a row at most
+template <typename T>
+__global__ void __launch_bounds__(kRulesThreads) k_logit_rules(const Rules a) {
+  extern __shared__ uint32_t s_biased[];  // a bit per logit of this block's slice: some bias entry names it
+  __shared__ float s_v[kRulesThreads / 32];
+  __shared__ int s_i[kRulesThreads / 32];
+  __shared__ uint32_t s_all[kRulesShare][2];
   pdl_launch_dependents();
+  const int share = cluster_nctarank(), rank = cluster_ctarank(), row = blockIdx.x / share, tid = threadIdx.x;
+  const int per = ((a.n + share - 1) / share + 7) & ~7, lo = min(rank * per, a.n), hi = min(lo + per, a.n);
+  const bool pick = a.part || a.idx;
+  if (pick) cluster_sync_all();  // the first block runs: its shared memory may be written
+  if (a.n_bias) {
+    for (int i = tid; i < (per + 31) / 32; i += kRulesThreads) s_biased[i] = 0;
+    __syncthreads();
+  }
   pdl_wait();
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= rows) return;
+  if (a.n_bias) {
+    for (int j = tid; j < a.n_bias; j += kRulesThreads) {
+      const int id = a.bias_ids[size_t(row) * a.n_bias + j], at = id - a.offset - lo;
+      if (id >= 0 && at >= 0 && at < hi - lo) atomicOr(s_biased + (at >> 5), 1u << (at & 31));
+    }
+    __syncthreads();
+  }
+  const T* in = static_cast<const T*>(a.logits) + size_t(row) * a.ld;
+  T* out = a.out ? static_cast<T*>(a.out) + size_t(row) * a.ld_out : nullptr;
+  const bool vin = (reinterpret_cast<uintptr_t>(in) & 15) == 0, vout = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool pen = a.penalties != nullptr;
+  const float again = pen ? a.penalties[row * 3] : 1.f, presence = pen ? a.penalties[row * 3 + 1] : 0.f,
+              frequency = pen ? a.penalties[row * 3 + 2] : 0.f;
+  const uint32_t* seen = a.seen + size_t(row) * a.words;
+  const uint32_t* mask = a.mask + size_t(row) * a.ld_mask;
+  const int* counts = a.counts + size_t(row) * a.vocab + a.offset;
   float best = -INFINITY;
   int bi = 0x7fffffff;
-  for (int c = 0; c < chunks; ++c) {
-    const float2 p = part[size_t(c) * rows + r];
-    const int i = __float_as_int(p.y);
-    if (p.x > best || (p.x == best && i < bi)) {
-      best = p.x;
-      bi = i;
+  constexpr int U = 2;
+  for (int i0 = lo + tid * 8; i0 < hi; i0 += U * kRulesThreads * 8) {
+    float x[U][8];
+    uint32_t ok[U], sb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kRulesThreads * 8, m = min(8, hi - i);
+      ok[u] = sb[u] = 0;
+      if (m <= 0) continue;
+      load8<T>(in + i, m, vin, x[u]);
+      ok[u] = a.mask ? bits8(mask, i + a.offset, a.vocab) : 0xffu;
+      if (pen) sb[u] = bits8(seen, i + a.offset, a.vocab);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kRulesThreads * 8, m = min(8, hi - i);
+      if (m <= 0) continue;
+      if (sb[u]) {
+        int c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = sb[u] >> j & (j < m) ? counts[i + j] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (sb[u] >> j & 1) {
+            float v = x[u][j];
+            v = v > 0.f ? __fdiv_rn(v, again) : __fmul_rn(v, again);
+            if (c[j] > 0) v = __fsub_rn(__fsub_rn(v, __fmul_rn(frequency, float(c[j]))), presence);
+            x[u][j] = v;
+          }
+      }
+      if (a.n_bias) {
+        const uint32_t named = s_biased[(i - lo) >> 5] >> ((i - lo) & 31) & 0xffu;  // (whole bytes: i - lo is a multiple of 8)
+        if (named) {
+          for (int e = 0; e < a.n_bias; ++e) {
+            const int id = a.bias_ids[size_t(row) * a.n_bias + e], at = id - a.offset - i;
+            if (id < 0 || at < 0 || at >= 8) continue;
+            const float v = a.bias[size_t(row) * a.n_bias + e];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j == at) x[u][j] = __fadd_rn(x[u][j], v);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (!(ok[u] >> j & 1)) x[u][j] = -INFINITY;
+        if (j < m && x[u][j] > best) {  // (ascending: the first of equals)
+          best = x[u][j];
+          bi = i + j + a.offset;
+        }
+      }
+      if (out) store8<T>(out + i, m, vout, x[u]);
     }
   }
-  idx[r] = bi == 0x7fffffff ? -1 : bi;
-  val[r] = best;
+  if (!pick) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) better(best, bi, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, bi, o));
+  if ((tid & 31) == 0) {
+    s_v[tid >> 5] = best;
+    s_i[tid >> 5] = bi;
+  }
+  __syncthreads();
+  if (tid < 32) {
+    best = tid < kRulesThreads / 32 ? s_v[tid] : -INFINITY;
+    bi = tid < kRulesThreads / 32 ? s_i[tid] : 0x7fffffff;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) better(best, bi, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, bi, o));
+    if (tid == 0) {
+      const uint32_t to = map_to_cta(smem_u32(&s_all[rank][0]), 0);
+      st_cluster_u32(to, __float_as_uint(best));
+      st_cluster_u32(to + 4, uint32_t(bi));
+    }
+    __syncwarp();
+  }
+  cluster_sync_all();
+  if (rank == 0 && tid == 0) {
+    best = -INFINITY;
+    bi = 0x7fffffff;
+    for (int r = 0; r < share; ++r) better(best, bi, __uint_as_float(s_all[r][0]), int(s_all[r][1]));
+    if (a.part) a.part[row] = make_float2(best, __int_as_float(bi));
+    if (a.idx) {
+      a.idx[row] = bi == 0x7fffffff ? -1 : bi;
+      a.val[row] = best;
+    }
+  }
 }
 
 }  // namespace bl
@@ -334,8 +491,13 @@ extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* b
     set_err(err, errlen, "barlink: paged_layout shared memory opt-in failed: %s", cudaGetErrorString(e));
     return -1;
   }
-  launch_k(k_paged_layout, dim3(1), dim3(kLayoutThreads), smem, static_cast<cudaStream_t>(stream), a);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  launch_k(k_paged_layout, dim3(1), dim3(kLayoutThreads), smem, st, a);
   SERVE_LAUNCH_CHECK("paged_layout");
+  if (tokens > kLayoutAlone) {
+    launch_k(k_layout_rows, dim3((tokens + 1023) / 1024), dim3(256), 0, st, a);
+    SERVE_LAUNCH_CHECK("layout_rows");
+  }
   return 0;
 }
 
@@ -347,21 +509,20 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int words = (vocab + 31) / 32;
-  if (reset) {
-    cudaMemsetAsync(counts, 0, size_t(rows) * vocab * 4, st);
-    cudaMemsetAsync(seen, 0, size_t(rows) * words * 4, st);
+  // Eight blocks a row while the GPU holds them all at once; one where a step adds a token per row.
+  const int share = !cu && !reset ? 1 : rows <= 2 * sm_count() / 4 ? 8 : rows <= 2 * sm_count() ? 2 : 1;
+  const cudaError_t e = launch_cluster(k_count_tokens, dim3(unsigned(rows) * share), dim3(kCountThreads), 0, share, st, ids, cu, prompt_lens,
+                                       counts, static_cast<uint32_t*>(seen), n_ids, vocab, words, reset);
+  if (e != cudaSuccess) {
+    set_err(err, errlen, "barlink: count_tokens launch failed: %s", cudaGetErrorString(e));
+    return -1;
   }
-  const int y = cu ? (n_ids / rows + 1023) / 1024 : 1;
-  launch_k(k_count_tokens, dim3(rows, y < 1 ? 1 : y > 64 ? 64 : y), dim3(256), 0, st, ids, cu, prompt_lens, counts,
-           static_cast<uint32_t*>(seen), n_ids, vocab, words);
   SERVE_LAUNCH_CHECK("count_tokens");
   return 0;
 }
 
-extern "C" int bl_rules_chunks(int rows, int n) { (void)rows; (void)n; return 16; }
-
 extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, size_t errlen) {
-  if (r->rows < 1 || r->n < 1 || (!r->out && !r->part) || (r->penalties && (!r->counts || !r->seen)) ||
+  if (r->rows < 1 || r->n < 1 || (!r->out && !r->part && !r->idx) || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
       (r->n_bias > 0 && (!r->bias_ids || !r->bias)) || r->vocab < 0 ||
       (r->mask && int64_t(r->mask_words) * 32 < r->vocab)) {
     set_err(err, errlen, "barlink: logit rules need logits, an output, and the tables of the rules that are set");
@@ -375,14 +536,25 @@ extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, siz
   a.rows = r->rows; a.n = r->n; a.vocab = r->vocab; a.offset = r->offset; a.n_bias = r->n_bias;
   a.words = (r->vocab + 31) / 32;
   a.ld = r->ld; a.ld_out = r->ld_out; a.ld_mask = r->ld_mask;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(r->rows, bl_rules_chunks(r->rows, r->n));
-  launch_k(r->fp32 ? k_logit_rules<float> : k_logit_rules<__nv_bfloat16>, grid, dim3(256), 0, st, a);
-  SERVE_LAUNCH_CHECK("logit_rules");
-  if (r->part && r->idx) {
-    launch_k(k_rules_pick, dim3((r->rows + 127) / 128), dim3(128), 0, st, static_cast<const float2*>(r->part), int(grid.y), r->rows,
-             static_cast<int*>(r->idx), static_cast<float*>(r->val));
-    SERVE_LAUNCH_CHECK("rules_pick");
+  a.idx = static_cast<int*>(r->idx); a.val = static_cast<float*>(r->val);
+  // Blocks of a row: as many as leave all of them resident at once (four to an SM), none with less than 2048 logits.
+  const int slots = 4 * sm_count();
+  int share = 1;
+  while (share < kRulesShare && r->rows * int64_t(2 * share) <= slots && r->n >= 2048 * 2 * share) share *= 2;
+  const int per = (r->n + share - 1) / share + 8, smem = r->n_bias ? (per + 31) / 32 * 4 : 0;
+  if (smem > 200 * 1024) {
+    set_err(err, errlen, "barlink: logit rules: biases on rows of at most 1600000 logits");
+    return -1;
   }
+  const auto kernel = r->fp32 ? k_logit_rules<float> : k_logit_rules<__nv_bfloat16>;
+  static bool attr[2][64] = {};
+  cudaError_t e = smem > 40 * 1024 ? allow_smem(reinterpret_cast<const void*>(kernel), 200 * 1024, attr[r->fp32 ? 1 : 0]) : cudaSuccess;
+  if (e == cudaSuccess)
+    e = launch_cluster(kernel, dim3(unsigned(r->rows) * share), dim3(kRulesThreads), smem, share, static_cast<cudaStream_t>(stream), a);
+  if (e != cudaSuccess) {
+    set_err(err, errlen, "barlink: logit_rules launch failed: %s", cudaGetErrorString(e));
+    return -1;
+  }
+  SERVE_LAUNCH_CHECK("logit_rules");
   return 0;
 }

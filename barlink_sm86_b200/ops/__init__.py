@@ -446,7 +446,7 @@ def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, o
     if not scale > 0:
         raise ValueError("attention over the 4-bit cache needs a positive scale")
     if q.is_cuda:
-        _count()
+        _count(2)
         return _C().paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, out)
     y = ref.paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale)
     if out is not None:
@@ -479,7 +479,7 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
     into: a PagedLayout to write to; its ctx_lens may be past_lens, its free_range may be free_range (a step that is captured
     in a graph and replayed).  1 to 8192 requests."""
     if new_lens.is_cuda:
-        _count()
+        _count(2 if tokens > 2048 else 1)
         return PagedLayout(*_C().paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size,
                                               None if into is None else list(into)))
     r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size)
@@ -567,7 +567,7 @@ def logits_argmax(logits, rules, offset=0):
     """(token int32 [rows], value fp32 [rows]): the arg max of the logits under `rules`, taken before they are rounded and without
     writing them.  The lowest token of equals; NaN is passed over; -1 where nothing above -inf is left."""
     if logits.is_cuda:
-        _count(2)
+        _count()
         return tuple(_C().logit_rules(logits, 1, rules.vocab, offset, *rules._args()))
     return ref.pick(ref.logit_rules(logits, rules.vocab, offset, *rules._args()), offset)
 
