@@ -466,7 +466,7 @@ int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables
 int bl_count_tokens(const int* ids, const int* cu, const int* prompt_lens, int* counts, void* seen, int rows, int n_ids, int vocab,
                     int reset, void* stream, char* err, size_t errlen);
 /* Rules on logits [rows][n] (bf16, or fp32): token id = column + offset.  seen: x / r or x * r; counted: - f * count - p; biases;
- * mask bits (1: allowed).  out: the result in the logits' type (may be logits); part: (value, token) pairs of the rows, as
+ * mask bits (1: allowed).  out: the result in the logits' type (may be logits); or, instead of it, part: (value, token) pairs of the rows, as
  * bl_argmax_merge takes those of several ranks; idx, val: arg max (lowest token; -1 where nothing is left). */
 typedef struct blRulesArgs {
   const void* logits;

@@ -42,13 +42,15 @@ struct Q4Write {
   double log2_theta;
 };
 
-// eight elements of a row from column `col`: the bf16 buffer, or the slabs added in split order, then the bias,
+// eight elements of a row from column `col`: the bf16 buffer (as it lies), or the slabs added in split order, then the bias,
 // rounded to bf16 (as k_rope_kv_write does)
-__device__ __forceinline__ void q4_load8(const Q4Write& a, int row, int width, int col, float (&f)[8]) {
-  if (a.slabs) {
-    const float* p = a.slabs + size_t(row) * width + col;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+template <bool SLABS>
+__device__ __forceinline__ uint4 q4_load8(const Q4Write& a, size_t row, int width, int col) {
+  if constexpr (!SLABS) {
+    return *reinterpret_cast<const uint4*>(a.qkv + row * width + col);
+  } else {
+    const float* p = a.slabs + row * width + col;
+    float f[8] = {};
     for (int s = 0; s < a.nsplit; ++s) {
       const float4 u = __ldcg(reinterpret_cast<const float4*>(p + s * a.slab));
       const float4 w = __ldcg(reinterpret_cast<const float4*>(p + s * a.slab) + 1);
@@ -65,17 +67,15 @@ __device__ __forceinline__ void q4_load8(const Q4Write& a, int row, int width, i
         f[2 * j + 1] += v.y;
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = __bfloat162float(__float2bfloat16(f[j]));
-    return;
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
   }
-  const uint4 b = *reinterpret_cast<const uint4*>(a.qkv + size_t(row) * width + col);
-  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+}
+__device__ __forceinline__ void q4_unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 v = unpack_bf16x2(w[j]);
-    f[2 * j] = v.x;
-    f[2 * j + 1] = v.y;
+    f[2 * j] = __uint_as_float(w[j] << 16);
+    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
   }
 }
 
@@ -89,15 +89,15 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 
 // Eight of a group's 32 elements, the rest with the other lanes of the quad -> codes (nibble e = element e), and the
-// group's step and low as bf16 bits.  (x - low) / step is divided, not multiplied by a reciprocal: the codes are
-// those of the formula to the bit.
+// group's step and low as bf16 bits.  The codes are those of the formula to the bit: (x - low) * (1 / step) is within 10^-5 of the
+// quotient, so that it rounds the same way unless it lies that near to the middle of two codes; then it is divided.
 __device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t& step_bits, uint16_t& low_bits) {
   float lo = x[0], hi = x[0], nan = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     lo = fminf(lo, x[e]);
     hi = fmaxf(hi, x[e]);
-    nan += x[e] * 0.f;  // NaN where an element is no finite number (minimum and maximum pass over NaN)
+    nan = fmaf(x[e], 0.f, nan);  // NaN where an element is no finite number (minimum and maximum pass over NaN)
   }
   lo = quad_min(lo);
   hi = quad_max(hi);
@@ -109,10 +109,18 @@ __device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t& 
   if (!fine) step = 0.f;
   uint32_t w = 0;
   if (step > 0.f) {
+    const float inv = __fdividef(1.f, step);
+    bool near = step < 1e-30f;  // (1 / step must be a finite number)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float c = fminf(rintf(__fdiv_rn(x[e] - lo, step)), 15.f);
-      w |= uint32_t(c) << (4 * e);
+      const float v = (x[e] - lo) * inv, r = v + 12582912.f;  // 3 * 2^22: the sum's last bits are the rounded quotient
+      near |= fabsf(v - (r - 12582912.f)) > 0.49999f;
+      w |= (min(__float_as_uint(r) & 31u, 15u)) << (4 * e);
+    }
+    if (near) {
+      w = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w |= uint32_t(fminf(rintf(__fdiv_rn(x[e] - lo, step)), 15.f)) << (4 * e);
     }
   }
   step_bits = fine ? __bfloat16_as_ushort(st) : 0;
@@ -138,72 +146,85 @@ __device__ __forceinline__ void q4_store8(uint8_t* tile, int r, int hd, bool val
   }
 }
 
-// A block takes kQ4Rows neighbouring rows.  A thread turns an octet of a head's lower half and its rotation partner; the angles of
-// the block's rows are computed once, one or two to a thread, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01
-// radians), and the products are rounded one by one: the rotated elements are the formula's to the bit.
-template <int ROWS, int THREADS>
+// A block takes ROWS neighbouring rows, PER = THREADS / ROWS threads each.  A thread keeps one octet of the heads' lower halves and its
+// rotation partner, with their eight angles, and goes through the heads, BATCH of them requested at a time.  The angles of
+// the block's rows are computed once, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01 radians), and the products are
+// rounded one by one: the rotated elements are the formula's to the bit.
+template <int HD, bool SLABS, int ROWS, int THREADS, int BATCH>
 __global__ void __launch_bounds__(THREADS) k_rope_kv_write_q4(const Q4Write a) {
+  constexpr int HALF = HD / 2, OPH = HD / 16, PER = THREADS / ROWS, STEP = PER / OPH;  // octets of half a head; heads of a pass
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float2 s_rot[ROWS][64];
-  __shared__ int s_slot[ROWS];
-  const int row0 = blockIdx.x * ROWS, rows = min(ROWS, a.rows - row0), half = a.hd >> 1, width = (a.nq + 2 * a.nkv) * a.hd;
-  // (THREADS is a multiple of 64: a thread has the same pair in every row that it visits)
-  const double inv = exp2(-a.log2_theta * (double(2 * (int(threadIdx.x) & (half - 1))) / a.hd)) * 0.15915494309189533577;
-  for (int e = threadIdx.x; e < rows * half; e += THREADS) {
-    const int r = e / half;
-    const double turn = double(a.positions[row0 + r]) * inv;
-    double sn, cs;
-    sincospi(2.0 * (turn - rint(turn)), &sn, &cs);
-    s_rot[r][e & (half - 1)] = make_float2(float(cs), float(sn));
+  __shared__ __align__(16) float2 s_rot[ROWS][HALF];
+  const int row0 = blockIdx.x * ROWS, rows = min(ROWS, a.rows - row0), heads = a.nq + 2 * a.nkv, width = heads * HD;
+  {
+    // (THREADS is a multiple of HALF: a thread has the same pair in every row that it visits)
+    const int i = threadIdx.x % HALF;
+    const double inv = exp2(-a.log2_theta * (double(2 * i) / HD)) * 0.15915494309189533577;
+    for (int r = threadIdx.x / HALF; r < rows; r += THREADS / HALF) {
+      const double turn = double(a.positions[row0 + r]) * inv;
+      double sn, cs;
+      sincospi(2.0 * (turn - rint(turn)), &sn, &cs);
+      s_rot[r][i] = make_float2(float(cs), float(sn));
+    }
   }
-  if (threadIdx.x < rows) {
-    const int slot = a.slots ? a.slots[row0 + threadIdx.x] : -1;
-    s_slot[threadIdx.x] = slot >= 0 && slot / a.block_size < a.n_blocks ? slot : -1;  // (no such block: not kept)
-  }
+  const int r = threadIdx.x / PER, o = threadIdx.x % OPH, h0 = threadIdx.x % PER / OPH;
+  const bool row_there = r < rows;  // (whole warps: PER is a multiple of 32)
+  const size_t row = row0 + (row_there ? r : 0);
+  const int slot = a.slots ? a.slots[row] : -1;
   __syncthreads();
-  const int oph = a.hd >> 4;  // octets of half a head: 4 or 8, so that quads are whole
-  const int units = (a.nq + 2 * a.nkv) * oph;
-  for (int u0 = 0; u0 < rows * units; u0 += THREADS) {
-    const int u = u0 + threadIdx.x;
-    const bool there = u < rows * units;
-    const int r = there ? u / units : 0, v = there ? u - r * units : 0, h = v / oph, o = v & (oph - 1), col = h * a.hd + 8 * o;
-    float x[8] = {}, y[8] = {};
-    if (there) {
-      q4_load8(a, row0 + r, width, col, x);
-      q4_load8(a, row0 + r, width, col + half, y);
-      uint32_t ox[4], oy[4];
-      if (h < a.nq + a.nkv) {
+  if (!row_there) return;
+  const int blk = slot >= 0 ? slot / a.block_size : -1, in_block = slot >= 0 ? slot - blk * a.block_size : 0;
+  const bool kept = blk >= 0 && blk < a.n_blocks;  // (no such block: not kept)
+  for (int hb = h0; hb - h0 < heads; hb += STEP * BATCH) {
+    uint4 lo[BATCH], hi[BATCH];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 cs = s_rot[r][8 * o + j];
-          const float p = __fsub_rn(__fmul_rn(x[j], cs.x), __fmul_rn(y[j], cs.y));
-          const float q = __fadd_rn(__fmul_rn(y[j], cs.x), __fmul_rn(x[j], cs.y));
-          x[j] = __bfloat162float(__float2bfloat16(p));
-          y[j] = __bfloat162float(__float2bfloat16(q));
+    for (int c = 0; c < BATCH; ++c) {
+      const int h = hb + c * STEP;
+      lo[c] = hi[c] = make_uint4(0, 0, 0, 0);
+      if (h < heads) {
+        lo[c] = q4_load8<SLABS>(a, row, width, h * HD + 8 * o);
+        hi[c] = q4_load8<SLABS>(a, row, width, h * HD + 8 * o + HALF);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < BATCH; ++c) {
+      const int h = hb + c * STEP;
+      const bool there = h < heads;
+      if (!__any_sync(0xffffffffu, there)) break;
+      if (there && h < a.nq + a.nkv) {
+        float x[8], y[8];
+        q4_unpack8(lo[c], x);
+        q4_unpack8(hi[c], y);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float4 cs = *reinterpret_cast<const float4*>(&s_rot[r][8 * o + j]);
+          const float p0 = __fsub_rn(__fmul_rn(x[j], cs.x), __fmul_rn(y[j], cs.y)), q0 = __fadd_rn(__fmul_rn(y[j], cs.x), __fmul_rn(x[j], cs.y));
+          const float p1 = __fsub_rn(__fmul_rn(x[j + 1], cs.z), __fmul_rn(y[j + 1], cs.w)),
+                      q1 = __fadd_rn(__fmul_rn(y[j + 1], cs.z), __fmul_rn(x[j + 1], cs.w));
+          (&lo[c].x)[j / 2] = pack_bf16x2(p0, p1);
+          (&hi[c].x)[j / 2] = pack_bf16x2(q0, q1);
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ox[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
-        oy[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
+      if (there) {
+        __nv_bfloat16* p = a.out + row * width + h * HD + 8 * o;
+        *reinterpret_cast<uint4*>(p) = lo[c];
+        *reinterpret_cast<uint4*>(p + HALF) = hi[c];
       }
-      __nv_bfloat16* p = a.out + size_t(row0 + r) * width + col;
-      *reinterpret_cast<uint4*>(p) = make_uint4(ox[0], ox[1], ox[2], ox[3]);
-      *reinterpret_cast<uint4*>(p + half) = make_uint4(oy[0], oy[1], oy[2], oy[3]);
-    }
-    const int slot = s_slot[r];
-    const bool keep = there && h >= a.nq && slot >= 0;
-    if (!__any_sync(0xffffffffu, keep)) continue;
-    uint16_t s0, l0, s1, l1;
-    const uint32_t w0 = q4_quantise8(x, s0, l0), w1 = q4_quantise8(y, s1, l1);
-    if (keep) {
-      const bool value = h >= a.nq + a.nkv;
-      const int blk = slot / a.block_size, in_block = slot - blk * a.block_size;
-      uint8_t* tile = a.cache + q4_tile_offset(blk, in_block, h - a.nq - (value ? a.nkv : 0), a.nkv, a.block_size, a.hd);
-      const int tr = in_block % kQ4Tokens;
-      q4_store8(tile, tr, a.hd, value, o >> 2, o & 3, w0, s0, l0);
-      q4_store8(tile, tr, a.hd, value, (o + oph) >> 2, o & 3, w1, s1, l1);
+      const bool keep = there && h >= a.nq && kept;
+      if (!__any_sync(0xffffffffu, keep)) continue;
+      float x[8], y[8];
+      q4_unpack8(lo[c], x);
+      q4_unpack8(hi[c], y);
+      uint16_t s0, l0, s1, l1;
+      const uint32_t w0 = q4_quantise8(x, s0, l0), w1 = q4_quantise8(y, s1, l1);
+      if (keep) {
+        const bool value = h >= a.nq + a.nkv;
+        uint8_t* tile = a.cache + q4_tile_offset(blk, in_block, h - a.nq - (value ? a.nkv : 0), a.nkv, a.block_size, HD);
+        const int tr = in_block % kQ4Tokens;
+        q4_store8(tile, tr, HD, value, o >> 2, o & 3, w0, s0, l0);
+        q4_store8(tile, tr, HD, value, (o + OPH) >> 2, o & 3, w1, s1, l1);
+      }
     }
   }
 }
@@ -806,9 +827,17 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
   a.rows = rows; a.nq = nq; a.nkv = nkv; a.hd = hd; a.block_size = block_size; a.n_blocks = n_blocks;
   a.log2_theta = log2(theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Many rows: four to a block share the threads' angles; few rows (a decode step): one each, all loads in one go.
-  if (rows > 4 * sm_count()) launch_k(k_rope_kv_write_q4<4, 256>, dim3((rows + 3) / 4), dim3(256), 0, st, a);
-  else launch_k(k_rope_kv_write_q4<1, 320>, dim3(rows), dim3(320), 0, st, a);
+  // Many rows: four to a block, with few threads each that go through the heads; few rows (a decode step): a block each whose
+  // threads have about a head's octet at once.
+  const bool many = rows > 4 * sm_count();
+  const dim3 grid(many ? (rows + 3) / 4 : rows), block(256);
+  if (hd == 128) {
+    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<128, true, 4, 256, 1> : k_rope_kv_write_q4<128, true, 1, 256, 2>, grid, block, 0, st, a);
+    else launch_k(many ? k_rope_kv_write_q4<128, false, 4, 256, 3> : k_rope_kv_write_q4<128, false, 1, 256, 2>, grid, block, 0, st, a);
+  } else {
+    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<64, true, 4, 256, 1> : k_rope_kv_write_q4<64, true, 1, 256, 2>, grid, block, 0, st, a);
+    else launch_k(many ? k_rope_kv_write_q4<64, false, 4, 256, 3> : k_rope_kv_write_q4<64, false, 1, 256, 2>, grid, block, 0, st, a);
+  }
   KV4_LAUNCH_CHECK("rope_kv_write_q4");
   return 0;
 }

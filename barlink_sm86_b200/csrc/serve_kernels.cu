@@ -291,47 +291,69 @@ __device__ __forceinline__ T from_float(float v) {
   else return v;
 }
 
-// bits [at, at + 8) of a row of `total` bits; those behind it are 0
-__device__ __forceinline__ uint32_t bits8(const uint32_t* words, int at, int total) {
-  const uint8_t* p = reinterpret_cast<const uint8_t*>(words) + (at >> 3);
-  const int left = total - at, sh = at & 7;
-  if (left <= 0) return 0;
-  uint32_t v = p[0] >> sh;
-  if (sh && left > 8 - sh) v |= uint32_t(p[1]) << (8 - sh);
-  return left >= 8 ? v & 0xffu : v & ((1u << left) - 1);
+// the top bits of bytes `s & 7` of v, each spread over a byte (a selector of 8 + byte)
+__device__ __forceinline__ uint32_t spread_signs(uint32_t v, uint32_t s) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(v), "r"(s));
+  return r;
 }
-
+// eight neighbouring logits as they lie, 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int m, bool vec, float (&x)[8]) {
-  if (vec && m == 8) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
-      x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
-    } else {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < m ? to_float<T>(p[j]) : -INFINITY;
+struct Eight;
+template <>
+struct Eight<__nv_bfloat16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int m, bool vec, const float (&x)[8]) {
-  if (vec && m == 8) {
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-    } else {
-      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+  __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
+  // -inf where the bit is 0: four bits become the top bits of four bytes, which a byte permutation spreads over the halves
+  __device__ __forceinline__ void keep(uint32_t bits) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t top = ((bits >> (4 * q) & 15u) * 0x10204080u) & 0x80808080u;
+      const uint32_t m0 = spread_signs(top, 0x9988), m1 = spread_signs(top, 0xbbaa);
+      w[2 * q] = (w[2 * q] & m0) | (~m0 & 0xff80ff80u);
+      w[2 * q + 1] = (w[2 * q + 1] & m1) | (~m1 & 0xff80ff80u);
     }
-  } else {
+  }
+  __device__ __forceinline__ float top() const {  // (a NaN is passed over)
+    auto h = [](uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); };
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(h(w[0]), h(w[1])), __hmax2(h(w[2]), h(w[3]))));
+    return fmaxf(m.x, m.y);
+  }
+};
+template <>
+struct Eight<float> {
+  float x[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  }
+  __device__ __forceinline__ float get(int j) const { return x[j]; }
+  __device__ __forceinline__ void keep(uint32_t bits) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < m) p[j] = from_float<T>(x[j]);
+      if (!(bits >> j & 1)) x[j] = -INFINITY;
   }
+  __device__ __forceinline__ float top() const {
+    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+  }
+};
+// the bytes that hold bits [at, at + 8)
+__device__ __forceinline__ uint32_t two_bytes(const uint32_t* words, int at, bool both) {
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(words) + (at >> 3);
+  uint32_t v = p[0];
+  if (both) v |= uint32_t(p[1]) << 8;
+  return v;
 }
+
 __device__ __forceinline__ void better(float& best, int& bi, float v, int i) {
   if (v > best || (v == best && i < bi)) {
     best = v;
@@ -339,103 +361,176 @@ __device__ __forceinline__ void better(float& best, int& bi, float v, int i) {
   }
 }
 
-// A cluster of blocks shares a row, a thread takes eight neighbouring logits (16 bytes of bf16) with a byte of each bit table; only where a
-// byte says so are counts and biases read.  Two such vectors are on their way at a time.  Each operation is rounded by itself
-// (no fused multiply-add): the values are the formula's to the bit.  The blocks' maxima meet in the first block's shared memory.
+// A cluster of blocks shares a row.  Most tokens carry no rule but the mask, and those that do lie close together (frequent tokens
+// have low ids), so there are two passes: the first takes eight neighbouring logits to a thread, 16 bytes of bf16, several such
+// vectors on their way at a time, with a byte of each bit table; it lists the vectors in which a token was seen, and leaves those
+// tokens and the ones with a bias aside.  The second gives a listed vector to a thread.  The bias entries come last, one to a thread.  Of the maximum the
+// first pass keeps the vector, and looks for the place in it at the end.  Each operation is rounded by itself (no fused multiply-add):
+// the values are the formula's to the bit.  The blocks' maxima meet in the first block's shared memory.  Measured, 64 x 152064,
+// us: one pass that branches into the penalties for every vector with a seen token 30; the seen words dealt out to warps 20.
 constexpr int kRulesThreads = 512;
-constexpr int kRulesShare = 8;  // blocks of a row at most
-template <typename T>
-__global__ void __launch_bounds__(kRulesThreads) k_logit_rules(const Rules a) {
-  extern __shared__ uint32_t s_biased[];  // a bit per logit of this block's slice: some bias entry names it
+constexpr int kRulesShare = 8;    // blocks of a row at most
+constexpr int kRulesLap = 5;      // vectors that a thread takes at a time
+template <typename T, bool PICK>  // the arg max, or the logits under the rules
+__global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a) {
+  extern __shared__ uint32_t s_rules[];  // with biases: a bit per column that an entry names; the entries' columns and values
   __shared__ float s_v[kRulesThreads / 32];
   __shared__ int s_i[kRulesThreads / 32];
   __shared__ uint32_t s_all[kRulesShare][2];
+  __shared__ int2 s_list[kRulesLap * kRulesThreads];  // first column, bits of the tokens
+  __shared__ int s_listed;
   pdl_launch_dependents();
-  const int share = cluster_nctarank(), rank = cluster_ctarank(), row = blockIdx.x / share, tid = threadIdx.x;
-  const int per = ((a.n + share - 1) / share + 7) & ~7, lo = min(rank * per, a.n), hi = min(lo + per, a.n);
-  const bool pick = a.part || a.idx;
-  if (pick) cluster_sync_all();  // the first block runs: its shared memory may be written
-  if (a.n_bias) {
-    for (int i = tid; i < (per + 31) / 32; i += kRulesThreads) s_biased[i] = 0;
-    __syncthreads();
-  }
+  const int share = cluster_nctarank(), rank = cluster_ctarank(), row = blockIdx.x / share, tid = threadIdx.x, lane = tid & 31;
+  const bool pen = a.penalties != nullptr;
+  if (PICK) cluster_sync_all();  // the first block runs: its shared memory may be written
+  uint32_t* s_named = s_rules;
+  int* s_col = reinterpret_cast<int*>(s_rules + (a.n + 31) / 32);
+  float* s_add = reinterpret_cast<float*>(s_col + a.n_bias);
+  if (tid == 0) s_listed = 0;
+  if (a.n_bias)
+    for (int i = tid; i < (a.n + 31) / 32; i += kRulesThreads) s_named[i] = 0;
+  __syncthreads();
   pdl_wait();
   if (a.n_bias) {
     for (int j = tid; j < a.n_bias; j += kRulesThreads) {
-      const int id = a.bias_ids[size_t(row) * a.n_bias + j], at = id - a.offset - lo;
-      if (id >= 0 && at >= 0 && at < hi - lo) atomicOr(s_biased + (at >> 5), 1u << (at & 31));
+      const int id = a.bias_ids[size_t(row) * a.n_bias + j], at = id >= a.offset && id - a.offset < a.n ? id - a.offset : -1;
+      s_col[j] = at;  // (below 0: none of this slice)
+      s_add[j] = a.bias[size_t(row) * a.n_bias + j];
+      if (at >= 0) atomicOr(s_named + (at >> 5), 1u << (at & 31));
     }
     __syncthreads();
   }
   const T* in = static_cast<const T*>(a.logits) + size_t(row) * a.ld;
-  T* out = a.out ? static_cast<T*>(a.out) + size_t(row) * a.ld_out : nullptr;
-  const bool vin = (reinterpret_cast<uintptr_t>(in) & 15) == 0, vout = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const bool pen = a.penalties != nullptr;
-  const float again = pen ? a.penalties[row * 3] : 1.f, presence = pen ? a.penalties[row * 3 + 1] : 0.f,
-              frequency = pen ? a.penalties[row * 3 + 2] : 0.f;
+  T* out = PICK ? nullptr : static_cast<T*>(a.out) + size_t(row) * a.ld_out;
   const uint32_t* seen = a.seen + size_t(row) * a.words;
   const uint32_t* mask = a.mask + size_t(row) * a.ld_mask;
   const int* counts = a.counts + size_t(row) * a.vocab + a.offset;
+  const float again = pen ? a.penalties[row * 3] : 1.f, presence = pen ? a.penalties[row * 3 + 1] : 0.f,
+              frequency = pen ? a.penalties[row * 3 + 2] : 0.f;
+  auto penalised = [&](float x, int c) {
+    x = x > 0.f ? __fdiv_rn(x, again) : __fmul_rn(x, again);
+    return c > 0 ? __fsub_rn(__fsub_rn(x, __fmul_rn(frequency, float(c))), presence) : x;
+  };
   float best = -INFINITY;
   int bi = 0x7fffffff;
-  constexpr int U = 2;
-  for (int i0 = lo + tid * 8; i0 < hi; i0 += U * kRulesThreads * 8) {
-    float x[U][8];
-    uint32_t ok[U], sb[U];
+  auto seen_tokens = [&](int i, uint32_t bits) {
+    float x[8];
+    int c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = bits >> j & 1 ? to_float<T>(in[i + j]) : 0.f;
+      c[j] = bits >> j & 1 ? counts[i + j] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (bits >> j & 1) {
+        x[j] = penalised(x[j], c[j]);
+        if (PICK) better(best, bi, x[j], i + j + a.offset);
+        else out[i + j] = from_float<T>(x[j]);
+      }
+  };
+  // vectors from the row's first 16-byte boundary on, as far as the vocabulary goes; the few columns around them one by one
+  const int known = int(max(min(int64_t(a.n), int64_t(a.vocab) - a.offset), int64_t(0)));
+  const int skip = min(int((16 - (reinterpret_cast<uintptr_t>(in) & 15)) % 16 / sizeof(T)), known), nvec = (known - skip) / 8;
+  const bool vout = (reinterpret_cast<uintptr_t>(out + skip) & 15) == 0;
+  const int sh = (a.offset + skip) & 7, lap = share * kRulesThreads;
+  constexpr int U = sizeof(T) == 2 ? kRulesLap : 3;
+  Eight<T> kept;  // the vector of the first pass's maximum
+  float kept_top = -INFINITY;
+  int kept_at = -1;
+  // (a warp's 32 vectors in turn with the other blocks': frequent tokens lie together)
+  for (int lap0 = 0; lap0 < nvec; lap0 += U * lap) {
+    const int v0 = min(lap0 + ((tid >> 5) * share + rank) * 32 + lane, nvec - 1), mine0 = lap0 + ((tid >> 5) * share + rank) * 32 + lane;
+    Eight<T> x[U];
+    uint32_t okb[U], sb[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kRulesThreads * 8, m = min(8, hi - i);
-      ok[u] = sb[u] = 0;
-      if (m <= 0) continue;
-      load8<T>(in + i, m, vin, x[u]);
-      ok[u] = a.mask ? bits8(mask, i + a.offset, a.vocab) : 0xffu;
-      if (pen) sb[u] = bits8(seen, i + a.offset, a.vocab);
+      const int v = mine0 + u * lap, i = skip + 8 * (v < nvec ? v : v0);
+      x[u].load(in + i);
+      okb[u] = a.mask ? two_bytes(mask, i + a.offset, sh != 0) : 0xffffu;
+      sb[u] = pen ? two_bytes(seen, i + a.offset, sh != 0) : 0u;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kRulesThreads * 8, m = min(8, hi - i);
-      if (m <= 0) continue;
-      if (sb[u]) {
-        int c[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = sb[u] >> j & (j < m) ? counts[i + j] : 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (sb[u] >> j & 1) {
-            float v = x[u][j];
-            v = v > 0.f ? __fdiv_rn(v, again) : __fmul_rn(v, again);
-            if (c[j] > 0) v = __fsub_rn(__fsub_rn(v, __fmul_rn(frequency, float(c[j]))), presence);
-            x[u][j] = v;
-          }
-      }
+      const int v = mine0 + u * lap, i = skip + 8 * v;
+      if (v >= nvec) break;
+      const uint32_t ok = okb[u] >> sh & 0xffu;
+      uint32_t aside = sb[u] >> sh & 0xffu, mine = aside & ok;
       if (a.n_bias) {
-        const uint32_t named = s_biased[(i - lo) >> 5] >> ((i - lo) & 31) & 0xffu;  // (whole bytes: i - lo is a multiple of 8)
-        if (named) {
-          for (int e = 0; e < a.n_bias; ++e) {
-            const int id = a.bias_ids[size_t(row) * a.n_bias + e], at = id - a.offset - i;
-            if (id < 0 || at < 0 || at >= 8) continue;
-            const float v = a.bias[size_t(row) * a.n_bias + e];
+        const uint32_t named = __funnelshift_r(s_named[i >> 5], s_named[min((i >> 5) + 1, (a.n - 1) >> 5)], i & 31);
+        mine &= ~named;
+        aside |= named;
+      }
+      if (mine) s_list[atomicAdd(&s_listed, 1)] = make_int2(i, int(mine));
+      x[u].keep(PICK ? ok & ~aside : ok);
+      if (!PICK) {
+        if (vout) x[u].store(out + i);
+        else
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j == at) x[u][j] = __fadd_rn(x[u][j], v);
-          }
+          for (int j = 0; j < 8; ++j) out[i + j] = from_float<T>(x[u].get(j));
+      }
+      if (PICK) {
+        const float m = x[u].top();
+        if (m > kept_top) {  // (ascending: the first of equals)
+          kept_top = m;
+          kept = x[u];
+          kept_at = i;
         }
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (!(ok[u] >> j & 1)) x[u][j] = -INFINITY;
-        if (j < m && x[u][j] > best) {  // (ascending: the first of equals)
-          best = x[u][j];
-          bi = i + j + a.offset;
-        }
-      }
-      if (out) store8<T>(out + i, m, vout, x[u]);
+    }
+    if (pen) {
+      __syncthreads();
+      for (int e = tid; e < s_listed; e += kRulesThreads) seen_tokens(s_list[e].x, uint32_t(s_list[e].y));
+      __syncthreads();
+      if (tid == 0) s_listed = 0;
+      if (lap0 + U * lap < nvec) __syncthreads();
     }
   }
-  if (!pick) return;
+  if (kept_at >= 0) {
+    int at = 0;
+#pragma unroll
+    for (int j = 7; j >= 0; --j)
+      if (kept.get(j) == kept_top) at = j;
+    better(best, bi, kept_top, kept_at + at + a.offset);
+  }
+  const int tail = skip + 8 * nvec;
+  for (int e = rank * kRulesThreads + tid; e < skip + a.n - tail; e += lap) {
+    const int i = e < skip ? e : tail + e - skip, id = i + a.offset;
+    const bool in_vocab = i < known;
+    const bool ok = !a.mask || (in_vocab && (mask[id >> 5] >> (id & 31) & 1));
+    const bool named = a.n_bias && (s_named[i >> 5] >> (i & 31) & 1);
+    float x = ok ? to_float<T>(in[i]) : -INFINITY;
+    if (ok && !named && pen && in_vocab && (seen[id >> 5] >> (id & 31) & 1)) x = penalised(x, counts[i]);
+    if (!PICK) out[i] = from_float<T>(x);
+    else if (!named) better(best, bi, x, id);
+  }
+  if (!PICK && a.n_bias) {
+    // the bias entries overwrite what the first pass has copied, in whichever block
+    __threadfence();
+    __syncwarp();
+    cluster_sync_all();
+  }
+  for (int j = rank * kRulesThreads + tid; j < a.n_bias; j += lap) {
+    const int col = s_col[j], id = col + a.offset;
+    bool go = col >= 0;
+    for (int e = 0; go && e < j; ++e) go = s_col[e] != col;  // the first entry of a token adds them all
+    if (!go) continue;
+    const bool in_vocab = col < known;
+    const uint32_t mw = a.mask && in_vocab ? mask[id >> 5] : a.mask ? 0u : ~0u, sw = pen && in_vocab ? seen[id >> 5] : 0u;
+    const int c = pen && in_vocab ? counts[col] : 0;
+    float x = to_float<T>(in[col]);
+    if (!(mw >> (id & 31) & 1)) continue;
+    if (sw >> (id & 31) & 1) x = penalised(x, c);
+    for (int e = j; e < a.n_bias; ++e)
+      if (s_col[e] == col) x = __fadd_rn(x, s_add[e]);
+    if (PICK) better(best, bi, x, id);
+    else out[col] = from_float<T>(x);
+  }
+  if (!PICK) return;
+  __syncwarp();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) better(best, bi, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, bi, o));
-  if ((tid & 31) == 0) {
+  if (lane == 0) {
     s_v[tid >> 5] = best;
     s_i[tid >> 5] = bi;
   }
@@ -457,6 +552,7 @@ __global__ void __launch_bounds__(kRulesThreads) k_logit_rules(const Rules a) {
     best = -INFINITY;
     bi = 0x7fffffff;
     for (int r = 0; r < share; ++r) better(best, bi, __uint_as_float(s_all[r][0]), int(s_all[r][1]));
+    if (best == -INFINITY) bi = 0x7fffffff;
     if (a.part) a.part[row] = make_float2(best, __int_as_float(bi));
     if (a.idx) {
       a.idx[row] = bi == 0x7fffffff ? -1 : bi;
@@ -522,7 +618,7 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
 }
 
 extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, size_t errlen) {
-  if (r->rows < 1 || r->n < 1 || (!r->out && !r->part && !r->idx) || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
+  if (r->rows < 1 || r->n < 1 || !r->out == !(r->part || r->idx) || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
       (r->n_bias > 0 && (!r->bias_ids || !r->bias)) || r->vocab < 0 ||
       (r->mask && int64_t(r->mask_words) * 32 < r->vocab)) {
     set_err(err, errlen, "barlink: logit rules need logits, an output, and the tables of the rules that are set");
@@ -537,18 +633,21 @@ extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, siz
   a.words = (r->vocab + 31) / 32;
   a.ld = r->ld; a.ld_out = r->ld_out; a.ld_mask = r->ld_mask;
   a.idx = static_cast<int*>(r->idx); a.val = static_cast<float*>(r->val);
-  // Blocks of a row: as many as leave all of them resident at once (four to an SM), none with less than 2048 logits.
-  const int slots = 4 * sm_count();
+  // Blocks of a row: as many as leave all of them resident at once (two to an SM), none with less than 2048 logits.
+  const int slots = 2 * sm_count();
   int share = 1;
   while (share < kRulesShare && r->rows * int64_t(2 * share) <= slots && r->n >= 2048 * 2 * share) share *= 2;
-  const int per = (r->n + share - 1) / share + 8, smem = r->n_bias ? (per + 31) / 32 * 4 : 0;
-  if (smem > 200 * 1024) {
-    set_err(err, errlen, "barlink: logit rules: biases on rows of at most 1600000 logits");
+  const int64_t need = r->n_bias ? (int64_t(r->n) + 31) / 32 * 4 + int64_t(r->n_bias) * 8 : 0;
+  if (need > 180 * 1024) {
+    set_err(err, errlen, "barlink: logit rules: too many bias entries, or logits in a row with biases (n / 8 + 8 entries <= 184320)");
     return -1;
   }
-  const auto kernel = r->fp32 ? k_logit_rules<float> : k_logit_rules<__nv_bfloat16>;
-  static bool attr[2][64] = {};
-  cudaError_t e = smem > 40 * 1024 ? allow_smem(reinterpret_cast<const void*>(kernel), 200 * 1024, attr[r->fp32 ? 1 : 0]) : cudaSuccess;
+  const int smem = int(need);
+  const bool pick = !r->out;
+  const auto kernel = r->fp32 ? pick ? k_logit_rules<float, true> : k_logit_rules<float, false>
+                              : pick ? k_logit_rules<__nv_bfloat16, true> : k_logit_rules<__nv_bfloat16, false>;
+  static bool attr[4][64] = {};
+  cudaError_t e = smem > 24 * 1024 ? allow_smem(reinterpret_cast<const void*>(kernel), 180 * 1024, attr[2 * (r->fp32 ? 1 : 0) + pick]) : cudaSuccess;
   if (e == cudaSuccess)
     e = launch_cluster(kernel, dim3(unsigned(r->rows) * share), dim3(kRulesThreads), smem, share, static_cast<cudaStream_t>(stream), a);
   if (e != cudaSuccess) {
