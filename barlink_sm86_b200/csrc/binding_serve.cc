@@ -159,7 +159,7 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
 
 // [cu, positions, slots, ctx_lens, free_range]; `into`: the same five to write to
 std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tensor& past_lens, const at::Tensor& block_tables,
-                                     const at::Tensor& free_list, const at::Tensor& free_range, int64_t tokens, int block_size,
+                                     const at::Tensor& free_list, const at::Tensor& free_range, int64_t tokens, int block_size, int rows_per_request,
                                      const c10::optional<std::vector<at::Tensor>>& into) {
   TORCH_CHECK(new_lens.is_cuda() && new_lens.dim() == 1, "barlink: new_lens must be a 1-D CUDA tensor");
   const int batch = small(new_lens.numel(), "batch"), rows = small(tokens, "tokens");
@@ -169,7 +169,7 @@ std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tenso
   i32(block_tables, new_lens, -1, "block_tables");
   i32(free_list, new_lens, -1, "free_list");
   const int* fr = i32(free_range, new_lens, 3, "free_range");
-  TORCH_CHECK(block_size >= 1, "barlink: block_size must be positive");
+  TORCH_CHECK(block_size >= 1 && rows_per_request >= 0, "barlink: block_size must be positive, rows_per_request not below 0");
   c10::cuda::CUDAGuard guard(new_lens.device());
   auto o = new_lens.options();
   std::vector<at::Tensor> r;
@@ -186,7 +186,7 @@ std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tenso
   i32(r[4], new_lens, 3, "free_range");
   BL_CHECK(bl_paged_layout(nl, pl, block_tables.data_ptr<int>(), free_list.data_ptr<int>(), fr, r[0].data_ptr<int>(),
                            r[1].data_ptr<int>(), r[2].data_ptr<int>(), r[3].data_ptr<int>(), r[4].data_ptr<int>(), batch,
-                           small(block_tables.size(1), "max_blocks"), small(free_list.numel(), "free_list"), rows, block_size,
+                           small(block_tables.size(1), "max_blocks"), small(free_list.numel(), "free_list"), rows, block_size, rows_per_request,
                            stream_of(new_lens), err, errlen));
   return r;
 }
@@ -208,9 +208,8 @@ void count_tokens(const at::Tensor& counts, const at::Tensor& seen, const at::Te
                              stream_of(counts), err, errlen));
 }
 
-// what = 0: the logits under the rules (into out, or a new tensor); 1: (token, value) of the arg max; 2: the
-// same as (value, token bits) pairs, float32 [1, rows, 2], of which argmax_merge takes those of all ranks
-std::vector<at::Tensor> logit_rules(const at::Tensor& logits, int what, int64_t vocab, int offset, const OptTensor& penalties,
+// pick: (token, value) of the arg max; else the logits under the rules (into out, or a new tensor)
+std::vector<at::Tensor> logit_rules(const at::Tensor& logits, bool pick, int64_t vocab, int offset, const OptTensor& penalties,
                                     const OptTensor& counts, const OptTensor& seen, const OptTensor& bias_ids, const OptTensor& bias,
                                     const OptTensor& mask, const OptTensor& out_opt) {
   const bool fp32 = logits.scalar_type() == at::kFloat;
@@ -258,7 +257,7 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, int what, int64_t 
   }
   c10::cuda::CUDAGuard guard(logits.device());
   std::vector<at::Tensor> r;
-  if (what == 0) {
+  if (!pick) {
     at::Tensor out = out_opt ? *out_opt : at::empty({a.rows, a.n}, logits.options());
     check_on(out, logits, "out");
     TORCH_CHECK(out.scalar_type() == logits.scalar_type() && out.dim() == 2 && out.size(0) == a.rows && out.size(1) == a.n && out.stride(1) == 1 &&
@@ -268,14 +267,9 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, int what, int64_t 
     a.ld_out = size_t(out.stride(0));
     r = {out};
   } else {
-    if (what == 2) {
-      r = {at::empty({1, a.rows, 2}, logits.options().dtype(at::kFloat))};
-      a.part = r[0].data_ptr();
-    } else {
-      r = {at::empty({a.rows}, logits.options().dtype(at::kInt)), at::empty({a.rows}, logits.options().dtype(at::kFloat))};
-      a.idx = r[0].data_ptr();
-      a.val = r[1].data_ptr();
-    }
+    r = {at::empty({a.rows}, logits.options().dtype(at::kInt)), at::empty({a.rows}, logits.options().dtype(at::kFloat))};
+    a.idx = r[0].data_ptr();
+    a.val = r[1].data_ptr();
   }
   if (a.rows > 0) BL_CHECK(bl_logit_rules(&a, stream_of(logits), err, errlen));
   return r;
@@ -292,10 +286,10 @@ void bind_serve(py::module_& m) {
         py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none());
   m.def("kv4_error_flag", &kv4_error_flag, py::arg("device") = 0);
   m.def("paged_layout", &paged_layout, py::arg("new_lens"), py::arg("past_lens"), py::arg("block_tables"), py::arg("free_list"),
-        py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("into") = py::none());
+        py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("rows_per_request") = 0, py::arg("into") = py::none());
   m.def("count_tokens", &count_tokens, py::arg("counts"), py::arg("seen"), py::arg("ids"), py::arg("cu") = py::none(),
         py::arg("prompt_lens") = py::none(), py::arg("reset") = false);
-  m.def("logit_rules", &logit_rules, py::arg("logits"), py::arg("what"), py::arg("vocab"), py::arg("offset") = 0,
+  m.def("logit_rules", &logit_rules, py::arg("logits"), py::arg("pick"), py::arg("vocab"), py::arg("offset") = 0,
         py::arg("penalties") = py::none(), py::arg("counts") = py::none(), py::arg("seen") = py::none(), py::arg("bias_ids") = py::none(),
         py::arg("bias") = py::none(), py::arg("mask") = py::none(), py::arg("out") = py::none());
 }

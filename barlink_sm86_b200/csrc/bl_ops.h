@@ -458,16 +458,17 @@ int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, cons
 /* ---- serving steps (serve_kernels.cu) ---------------------------------------------------------------
  * Request lengths to row offsets cu [batch + 1], positions and slots [tokens], context lengths and block tables.  new_lens:
  * tokens that a request gets now, below 0: it has ended and its blocks go back.  free_list: ring of n_free entries, free_range
- * (first, count, missing); free_range_out may be free_range, ctx_lens may be past_lens. */
+ * (first, count, missing); free_range_out may be free_range, ctx_lens may be past_lens.
+ * rows_per_request > 0: request b's rows are b * rows_per_request ..; 0: packed. */
 int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range, int* cu,
                     int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks, int n_free, int tokens,
-                    int block_size, void* stream, char* err, size_t errlen);
+                    int block_size, int rows_per_request, void* stream, char* err, size_t errlen);
 /* counts int32 [rows][vocab] += 1 for every id behind a row's first prompt_lens ids; seen (bits) |= every id */
 int bl_count_tokens(const int* ids, const int* cu, const int* prompt_lens, int* counts, void* seen, int rows, int n_ids, int vocab,
                     int reset, void* stream, char* err, size_t errlen);
 /* Rules on logits [rows][n] (bf16, or fp32): token id = column + offset.  seen: x / r or x * r; counted: - f * count - p; biases;
- * mask bits (1: allowed).  out: the result in the logits' type (may be logits); or, instead of it, part: (value, token) pairs of the rows, as
- * bl_argmax_merge takes those of several ranks; idx, val: arg max (lowest token; -1 where nothing is left). */
+ * mask bits (1: allowed); columns behind the vocabulary are -inf.  out: the result in the logits' type (may be logits); or, instead of it, idx, val: arg max (lowest token; -1 where
+ * nothing is left). */
 typedef struct blRulesArgs {
   const void* logits;
   size_t ld;
@@ -475,7 +476,6 @@ typedef struct blRulesArgs {
   int vocab, offset;
   void* out;
   size_t ld_out;
-  void* part;
   void* idx; /* int32 [rows], with val fp32 [rows]; or null */
   void* val;
   const void* penalties; /* fp32 [rows][3]: repetition, presence, frequency; or null (then counts and seen are not read) */

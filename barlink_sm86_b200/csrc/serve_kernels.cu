@@ -36,6 +36,7 @@ struct RequestLayout {
   const int* range;
   int *cu, *positions, *slots, *ctx_lens, *range_out;
   int batch, width, cap, tokens, block_size;
+  int per;  // rows of a request where every request has as many (those behind its tokens are empty); 0: packed
 };
 
 // exclusive block-wide scan of three ints per thread; total in tot
@@ -169,10 +170,17 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
   }
   if (a.tokens > kLayoutAlone) return;  // k_layout_rows does the rest
   for (int row = tid; row < a.tokens; row += kLayoutThreads) {
-    int pos = 0, slot = -1;
-    if (row < tot[0]) {
-      const int b = owner_of(s_cu, B, row);
-      pos = s_past[b] + row - s_cu[b];
+    int pos = 0, slot = -1, b = -1, i = 0;  // the i-th token of request b
+    if (a.per > 0) {
+      b = row / a.per;
+      i = row - b * a.per;
+      if (b >= B || i >= s_cu[b + 1] - s_cu[b]) b = -1;
+    } else if (row < tot[0]) {
+      b = owner_of(s_cu, B, row);
+      i = row - s_cu[b];
+    }
+    if (b >= 0) {
+      pos = s_past[b] + i;
       const int page = pos / bs;
       if (pos >= 0 && page < a.width) {
         const int j = s_fresh[b] + page - s_had[b];
@@ -192,22 +200,23 @@ __global__ void __launch_bounds__(256) k_layout_rows(const RequestLayout a) {
   const int row0 = (blockIdx.x * 256 + threadIdx.x) * 4, bs = a.block_size;
   if (row0 >= a.tokens) return;
   int pos[4] = {0, 0, 0, 0}, slot[4] = {-1, -1, -1, -1};
-  if (row0 < a.cu[a.batch]) {
-    int b = owner_of(a.cu, a.batch, row0), next = a.cu[b + 1];
-    int base = a.ctx_lens[b] - next;  // position = base + row
+  const int total = a.cu[a.batch];
+  if (a.per > 0 || row0 < total) {
+    int b = a.per > 0 ? row0 / a.per : owner_of(a.cu, a.batch, row0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + i;
-      while (row >= next && ++b < a.batch) {
-        next = a.cu[b + 1];
-        base = a.ctx_lens[b] - next;
-      }
+    for (int k = 0; k < 4; ++k) {
+      const int row = row0 + k;
+      if (a.per > 0) b = row / a.per;
+      else
+        while (b < a.batch && row >= a.cu[b + 1]) ++b;
       if (b >= a.batch) break;
-      pos[i] = base + row;
-      const int page = pos[i] / bs;
-      if (pos[i] >= 0 && page < a.width) {
+      const int first = a.cu[b], n = a.cu[b + 1] - first, i = row - (a.per > 0 ? b * a.per : first);
+      if (i >= n) continue;
+      pos[k] = a.ctx_lens[b] - n + i;
+      const int page = pos[k] / bs;
+      if (pos[k] >= 0 && page < a.width) {
         const int id = a.tables[size_t(b) * a.width + page];
-        if (id >= 0) slot[i] = id * bs + pos[i] % bs;
+        if (id >= 0) slot[k] = id * bs + pos[k] % bs;
       }
     }
   }
@@ -267,7 +276,6 @@ __global__ void __launch_bounds__(kCountThreads) k_count_tokens(const int* __res
 struct Rules {
   const void* logits;
   void* out;     // same type, or null
-  float2* part;  // [rows] (value, token), or null
   int* idx;      // [rows], with val; or null
   float* val;
   const float* penalties;  // [rows][3]: repetition, presence, frequency; or null
@@ -497,10 +505,10 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
   for (int e = rank * kRulesThreads + tid; e < skip + a.n - tail; e += lap) {
     const int i = e < skip ? e : tail + e - skip, id = i + a.offset;
     const bool in_vocab = i < known;
-    const bool ok = !a.mask || (in_vocab && (mask[id >> 5] >> (id & 31) & 1));
+    const bool ok = in_vocab && (!a.mask || (mask[id >> 5] >> (id & 31) & 1));
     const bool named = a.n_bias && (s_named[i >> 5] >> (i & 31) & 1);
     float x = ok ? to_float<T>(in[i]) : -INFINITY;
-    if (ok && !named && pen && in_vocab && (seen[id >> 5] >> (id & 31) & 1)) x = penalised(x, counts[i]);
+    if (ok && !named && pen && (seen[id >> 5] >> (id & 31) & 1)) x = penalised(x, counts[i]);
     if (!PICK) out[i] = from_float<T>(x);
     else if (!named) better(best, bi, x, id);
   }
@@ -516,7 +524,7 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
     for (int e = 0; go && e < j; ++e) go = s_col[e] != col;  // the first entry of a token adds them all
     if (!go) continue;
     const bool in_vocab = col < known;
-    const uint32_t mw = a.mask && in_vocab ? mask[id >> 5] : a.mask ? 0u : ~0u, sw = pen && in_vocab ? seen[id >> 5] : 0u;
+    const uint32_t mw = !in_vocab ? 0u : a.mask ? mask[id >> 5] : ~0u, sw = pen && in_vocab ? seen[id >> 5] : 0u;
     const int c = pen && in_vocab ? counts[col] : 0;
     float x = to_float<T>(in[col]);
     if (!(mw >> (id & 31) & 1)) continue;
@@ -553,11 +561,8 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
     bi = 0x7fffffff;
     for (int r = 0; r < share; ++r) better(best, bi, __uint_as_float(s_all[r][0]), int(s_all[r][1]));
     if (best == -INFINITY) bi = 0x7fffffff;
-    if (a.part) a.part[row] = make_float2(best, __int_as_float(bi));
-    if (a.idx) {
-      a.idx[row] = bi == 0x7fffffff ? -1 : bi;
-      a.val[row] = best;
-    }
+    a.idx[row] = bi == 0x7fffffff ? -1 : bi;
+    a.val[row] = best;
   }
 }
 
@@ -567,8 +572,9 @@ using namespace bl;
 
 extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range,
                                int* cu, int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks,
-                               int n_free, int tokens, int block_size, void* stream, char* err, size_t errlen) {
-  if (batch < 1 || batch > kLayoutMaxBatch || max_blocks < 1 || n_free < 1 || tokens < 0 || block_size < 1) {
+                               int n_free, int tokens, int block_size, int rows_per_request, void* stream, char* err, size_t errlen) {
+  if (batch < 1 || batch > kLayoutMaxBatch || max_blocks < 1 || n_free < 1 || tokens < 0 || block_size < 1 ||
+      rows_per_request < 0) {
     set_err(err, errlen, "barlink: paged_layout takes 1 to %d requests, a table and a list of free blocks", kLayoutMaxBatch);
     return -1;
   }
@@ -579,7 +585,7 @@ extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* b
   RequestLayout a;
   a.new_lens = new_lens; a.past_lens = past_lens; a.tables = block_tables; a.ring = free_list; a.range = free_range;
   a.cu = cu; a.positions = positions; a.slots = slots; a.ctx_lens = ctx_lens; a.range_out = free_range_out;
-  a.batch = batch; a.width = max_blocks; a.cap = n_free; a.tokens = tokens; a.block_size = block_size;
+  a.batch = batch; a.width = max_blocks; a.cap = n_free; a.tokens = tokens; a.block_size = block_size; a.per = rows_per_request;
   const int smem = int((size_t(batch) * 6 + 2) * sizeof(int));
   static bool attr[64] = {};
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k_paged_layout), (kLayoutMaxBatch * 6 + 2) * int(sizeof(int)), attr);
@@ -618,14 +624,14 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
 }
 
 extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, size_t errlen) {
-  if (r->rows < 1 || r->n < 1 || !r->out == !(r->part || r->idx) || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
+  if (r->rows < 1 || r->n < 1 || !r->out == !r->idx || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
       (r->n_bias > 0 && (!r->bias_ids || !r->bias)) || r->vocab < 0 ||
       (r->mask && int64_t(r->mask_words) * 32 < r->vocab)) {
     set_err(err, errlen, "barlink: logit rules need logits, an output, and the tables of the rules that are set");
     return -1;
   }
   Rules a;
-  a.logits = r->logits; a.out = r->out; a.part = static_cast<float2*>(r->part); a.penalties = static_cast<const float*>(r->penalties);
+  a.logits = r->logits; a.out = r->out; a.penalties = static_cast<const float*>(r->penalties);
   a.counts = static_cast<const int*>(r->counts); a.seen = static_cast<const uint32_t*>(r->seen);
   a.bias_ids = static_cast<const int*>(r->bias_ids); a.bias = static_cast<const float*>(r->bias);
   a.mask = static_cast<const uint32_t*>(r->mask);

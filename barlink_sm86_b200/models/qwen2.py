@@ -271,6 +271,24 @@ class PagedKV:
         return (blk * self.block_size + positions_2d % self.block_size).to(torch.int32).reshape(-1)
 
 
+class PagedKV4:
+    """Key/value cache in 4 bits (`ops.kv4_cache` per layer) whose blocks are dealt out on the GPU: block_tables [batch, max_blocks]
+    are filled by `ops.paged_layout` from the ring of free blocks.  n_blocks: blocks in all (default: enough for max_len tokens of
+    every request)."""
+
+    def __init__(self, n_layers, batch, max_len, nkv, hd, device, block_size=16, n_blocks=None):
+        self.block_size = block_size
+        width = -(-max_len // block_size)
+        self.n_blocks = batch * width if n_blocks is None else n_blocks
+        self.kv = [ops.kv4_cache(self.n_blocks, nkv, hd, block_size, device) for _ in range(n_layers)]
+        self.block_tables = torch.full((batch, width), -1, dtype=torch.int32, device=device)
+        self.free_list = torch.arange(self.n_blocks, dtype=torch.int32, device=device)
+        self.free_range = torch.tensor([0, self.n_blocks, 0], dtype=torch.int32, device=device)
+
+    def nbytes(self):
+        return sum(t.numel() for t in self.kv)
+
+
 class Qwen2Model:
     def __init__(self, cfg: Qwen2Config, comm: Optional[TPComm] = None, device="cpu",
                  dtype=torch.float32, seed=0, layers=None, quant="none", shard_of=None, source=None):
@@ -357,6 +375,14 @@ class Qwen2Model:
             normed, res = ops.rmsnorm(h, w.ln_f, cfg.eps, res)
         return normed
 
+    def _rope_write(self, cache, li, qkv, positions, slots, bias=None):
+        """RoPE on the step's rows, their keys and values into layer li of either kind of cache (None: RoPE alone)."""
+        nq, nkv, hd, theta = self.nq, self.nkv, self.hd, self.cfg.theta
+        if isinstance(cache, PagedKV4):
+            return ops.rope_kv_write_q4(qkv, positions, slots, cache.kv[li], nq, nkv, hd, cache.block_size, theta, bias)
+        kc, vc, bs = (None, None, 16) if cache is None else (cache.k[li], cache.v[li], cache.block_size)
+        return ops.rope_kv_write(qkv, positions, slots, kc, vc, nq, nkv, hd, bs, theta, bias)
+
     # ---- prefill: dense causal attention, optional KV write ----------------
     def prefill(self, ids_2d, cache: Optional[PagedKV] = None, seq_offset: int = 0):
         """ids [batch, seq] -> final normed hidden [batch*seq, hidden]; with a
@@ -367,23 +393,25 @@ class Qwen2Model:
         positions = pos2d.reshape(-1)
         slots = cache.slots(pos2d, seq_offset) if cache is not None else None
         cu = torch.arange(0, (batch + 1) * seq, seq, device=dev, dtype=torch.int32)
+        return self.prefill_packed(ids_2d.reshape(-1), positions, slots, cu, seq, cache)
+
+    def prefill_packed(self, ids, positions, slots, cu, max_len, cache=None):
+        """Prompts of different lengths, packed: ids, positions, slots int32 [tokens], cu int32 [batch + 1] (request b's rows are
+        cu[b] .. cu[b + 1]), max_len no less than the longest -> final normed hidden [tokens, hidden].  Keys and values go to
+        `cache` (PagedKV or PagedKV4) at `slots`; attention is over the prompts themselves."""
         nq, nkv, hd = self.nq, self.nkv, self.hd
 
         def attn_factory(li):
             def attn(qkv, bias=None):
-                kc = cache.k[li] if cache is not None else None
-                vc = cache.v[li] if cache is not None else None
-                qkv = ops.rope_kv_write(qkv, positions, slots, kc, vc, nq, nkv, hd,
-                                        cache.block_size if cache is not None else 16, self.cfg.theta,
-                                        bias)
+                qkv = self._rope_write(cache, li, qkv, positions, slots, bias)
                 T = qkv.shape[0]
                 v3 = qkv.view(T, nq + 2 * nkv, hd)
-                o = ops.attention(v3[:, :nq], v3[:, nq:nq + nkv], v3[:, nq + nkv:], cu, cu, seq,
-                                  self.scale, True, max_k=seq)
+                o = ops.attention(v3[:, :nq], v3[:, nq:nq + nkv], v3[:, nq + nkv:], cu, cu, max_len,
+                                  self.scale, True, max_k=max_len)
                 return o.reshape(T, nq * hd)
             return attn
 
-        return self._run_layers(ids_2d.reshape(-1).to(torch.int32), positions, attn_factory)
+        return self._run_layers(ids.to(torch.int32), positions, attn_factory)
 
     # ---- decode: one token per sequence against the paged cache ------------
     def decode_hidden(self, ids, positions, slots, ctx_lens, cache: PagedKV, splits=0):
@@ -394,6 +422,9 @@ class Qwen2Model:
 
         def attn_factory(li):
             def attn(qkv, bias=None):
+                if isinstance(cache, PagedKV4):
+                    qkv = self._rope_write(cache, li, qkv, positions, slots, bias)
+                    return ops.paged_attn_decode_q4(qkv, cache.kv[li], cache.block_tables, ctx_lens, nq, nkv, hd, self.scale)
                 if fuse:
                     # opt-in: RoPE, the KV write and the attention in one launch
                     return ops.rope_attn_decode(qkv, bias, positions, slots, cache.k[li], cache.v[li],
@@ -567,8 +598,8 @@ class Qwen2Model:
         full = self.comm.all_gather_cols(self.logits_local(hidden))
         return full[:, : self.cfg.vocab]
 
-    def next_tokens(self, hidden, out=None, dlin=False):
-        """Greedy next token per row (local arg max + a few bytes per row exchanged).
+    def next_tokens(self, hidden, out=None, dlin=False, rules=None):
+        """Greedy next token per row (local arg max + a few bytes per row exchanged), under `rules` (ops.LogitRules) if given.
         dlin: the head may run on the decode-linear kernel; it does when its row tiles fit the GPU
         at once (a vocabulary shard of 149 tiles takes the persistent GEMM two laps of its 148 CTAs)."""
         head = self.w.lm_head
@@ -579,7 +610,7 @@ class Qwen2Model:
             logits = load_extension().dlin(hidden, head, epi="store")
         else:
             logits = self.logits_local(hidden)
-        return self.comm.argmax_vocab_parallel(logits, self.w.vocab_local, out)
+        return self.comm.argmax_vocab_parallel(logits, self.w.vocab_local, out, rules)
 
 
 class DecodeEngine:
@@ -592,14 +623,30 @@ class DecodeEngine:
     and the collectives are replay-safe (their expectations are device
     counters).  `step_host` is the end-to-end form: token ids arrive in pinned
     host memory and the result is read back to the host every step.
+
+    kv_bits=4 holds the cache in 4 bits and deals its blocks out on the GPU: requests then have lengths of their own
+    (`start`), come and go while the others run (`start`, `finish`), and the captured step takes the blocks that it
+    needs (n_blocks of block_size tokens in all; `blocks_missing`).  rules (ops.LogitRules, one row per request): the greedy token is
+    that of the logits under them, and their counts follow the tokens that are produced.
     """
 
     def __init__(self, model: Qwen2Model, batch: int, max_len: int, use_graph: bool = True,
-                 attn_splits: int = 0):
+                 attn_splits: int = 0, kv_bits: int = 16, rules: Optional[ops.LogitRules] = None, block_size: int = 16,
+                 n_blocks: Optional[int] = None):
         self.m = model
         self.batch, self.max_len = batch, max_len
         dev, dt = model.device, model.dtype
-        self.cache = PagedKV(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, dt)
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 4 or 16")
+        if kv_bits == 16 and (block_size != 16 or n_blocks is not None):
+            raise ValueError("block_size and n_blocks are for the 4-bit cache")
+        self.kv_bits, self.rules = kv_bits, rules
+        if kv_bits == 4:
+            self.cache = PagedKV4(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, block_size, n_blocks)
+            self.new_lens = torch.zeros(batch, dtype=torch.int32, device=dev)  # 1: the request takes part in steps
+            self.running = [False] * batch
+        else:
+            self.cache = PagedKV(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, dt)
         self.ids = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.positions = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.ctx_lens = torch.zeros(batch, dtype=torch.int32, device=dev)
@@ -609,12 +656,98 @@ class DecodeEngine:
         self.graph = None
         self.attn_splits = attn_splits
         self.launches_per_step = 0
+        if kv_bits == 4:
+            # what a step's layout is written to, in place
+            cu = torch.zeros(batch + 1, dtype=torch.int32, device=dev)
+            self.layout = ops.PagedLayout(cu, self.positions, self.slots, self.ctx_lens, self.cache.free_range)
         if dev.type == "cuda":
             self.h_in = torch.zeros(batch, dtype=torch.int32).pin_memory()
             self.h_out = torch.zeros(batch, dtype=torch.int32).pin_memory()
 
+    def _lay_out(self, new_lens, tokens=0):
+        """Blocks for (or from) the requests outside a step: the layout of `tokens` packed rows, the state in place."""
+        c = self.cache
+        i32 = dict(dtype=torch.int32, device=new_lens.device)
+        into = ops.PagedLayout(torch.empty(self.batch + 1, **i32), torch.empty(tokens, **i32), torch.empty(tokens, **i32),
+                               self.ctx_lens, c.free_range)
+        return ops.paged_layout(new_lens, self.ctx_lens, c.block_tables, c.free_list, c.free_range, tokens, c.block_size, into)
+
+    def blocks_missing(self):
+        """Blocks that the last step or `start` could not have (4-bit cache; waits for the GPU): their tokens are not kept."""
+        return int(self.cache.free_range[2])
+
+    def finish(self, rows):
+        """Requests `rows` have ended: their blocks are free again, and they rest until `start` gives them a new prompt."""
+        if self.kv_bits != 4:
+            raise ValueError("requests end one by one with the 4-bit cache only")
+        rows = sorted(set(int(r) for r in rows))
+        if any(r < 0 or r >= self.batch for r in rows):
+            raise ValueError("no such request")
+        gone = torch.zeros(self.batch, dtype=torch.int32)
+        gone[rows] = -1
+        gone = gone.to(self.new_lens.device)
+        self._lay_out(gone)
+        self.new_lens.masked_fill_(gone < 0, 0)
+        for r in rows:
+            self.running[r] = False
+
+    def start(self, ids, lens, max_tokens: int = 8192):
+        """New prompts, packed: ids int32 [tokens]; lens (one per request, 0: none) of requests that rest.  Runs them through the model, at
+        most `max_tokens` tokens (and at least one request) per pass, writes their keys and values to the cache, and returns the first token
+        of every request (int32 [batch]; the current input of those that got no prompt).  The next `step` consumes these once they are
+        in `ids`."""
+        if self.kv_bits != 4:
+            raise ValueError("prompts of different lengths need the 4-bit cache")
+        lens = [int(n) for n in lens]
+        if len(lens) != self.batch or any(n < 0 or n > self.max_len for n in lens) or sum(lens) != ids.numel():
+            raise ValueError("lens must be one length per request, up to max_len, and add up to the ids")
+        if any(n and r for n, r in zip(lens, self.running)):
+            raise ValueError("a request that runs gets no new prompt: finish it first")
+        out = self.ids.clone()
+        if not ids.numel():
+            return out
+        dev = self.positions.device
+        new = torch.tensor(lens, dtype=torch.int32).to(dev)
+        lay = self._lay_out(new, ids.numel())
+        ids = ids.to(device=dev, dtype=torch.int32)
+        if self.rules is not None:
+            fresh = new > 0
+            self.rules.counts.masked_fill_(fresh[:, None], 0)
+            self.rules.seen.masked_fill_(fresh[:, None], 0)
+            ops.count_tokens(self.rules, ids, lay.cu, new)
+        lasts, rows, b0, t0 = [], [b for b in range(self.batch) if lens[b]], 0, 0
+        while b0 < len(rows):
+            b1, n = b0 + 1, lens[rows[b0]]
+            while b1 < len(rows) and n + lens[rows[b1]] <= max_tokens:
+                n += lens[rows[b1]]
+                b1 += 1
+            part = [lens[r] for r in rows[b0:b1]]
+            cu = torch.tensor([0] + part, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+            hidden = self.m.prefill_packed(ids[t0:t0 + n].contiguous(), lay.positions[t0:t0 + n].contiguous(), lay.slots[t0:t0 + n].contiguous(),
+                                           cu, max(part), self.cache)
+            lasts.append(hidden[cu[1:].long() - 1])
+            b0, t0 = b1, t0 + n
+        # (rules have a row per request: all requests' logits, of which those with a prompt count)
+        at = torch.tensor(rows).to(dev)
+        last = torch.zeros(self.batch, lasts[0].shape[1], dtype=lasts[0].dtype, device=dev)
+        last[at] = torch.cat(lasts, 0)
+        nxt = self.m.next_tokens(last, rules=self.rules)
+        out[at] = nxt[at]
+        if self.rules is not None:
+            ops.count_tokens(self.rules, torch.where(new > 0, nxt, -1))
+        self.new_lens.masked_fill_(new > 0, 1)
+        for r in rows:
+            self.running[r] = True
+        return out
+
     def set_context(self, length: int):
         """Declare that every sequence already has `length` tokens in the cache."""
+        if self.kv_bits == 4:
+            self.finish(range(self.batch))
+            self._lay_out(torch.full_like(self.new_lens, length))
+            self.new_lens.fill_(1)
+            self.running = [True] * self.batch
+            return
         self.positions.fill_(length)
         self._refresh()
 
@@ -629,6 +762,9 @@ class DecodeEngine:
         """Run the prompts through the model (a few sequences at a time, at most
         `max_tokens` tokens per pass) and return the first generated token."""
         seq = ids_2d.shape[1]
+        if self.kv_bits == 4:
+            self.finish(range(self.batch))
+            return self.start(ids_2d.reshape(-1), [seq] * self.batch, max_tokens)
         per = max(1, max_tokens // seq)
         lasts = []
         for b0 in range(0, self.batch, per):
@@ -636,12 +772,34 @@ class DecodeEngine:
             hidden = self.m.prefill(part, self.cache, seq_offset=b0)
             lasts.append(hidden.view(part.shape[0], seq, -1)[:, -1])
         last = torch.cat(lasts, 0).contiguous()
-        nxt = self.m.next_tokens(last)
+        if self.rules is not None:
+            cu = torch.arange(0, (self.batch + 1) * seq, seq, device=ids_2d.device, dtype=torch.int32)
+            ops.count_tokens(self.rules, ids_2d.reshape(-1).to(torch.int32), cu, torch.full_like(cu[1:], seq), reset=True)
+        nxt = self.m.next_tokens(last, rules=self.rules)
+        if self.rules is not None:
+            ops.count_tokens(self.rules, nxt)
         self.set_context(seq)
         return nxt
 
+    def _step_ruled(self):
+        """A step on the 4-bit cache, or under rules: the plain decode path."""
+        c = self.cache
+        if self.kv_bits == 4:
+            ops.paged_layout(self.new_lens, self.ctx_lens, c.block_tables, c.free_list, c.free_range, self.batch, c.block_size,
+                             self.layout, rows_per_request=1)
+        hidden = self.m.decode_hidden(self.ids, self.positions, self.slots, self.ctx_lens, c, self.attn_splits)
+        self.m.next_tokens(hidden, self.out_ids, rules=self.rules)
+        if self.rules is not None:
+            ops.count_tokens(self.rules, self.out_ids if self.kv_bits != 4 else torch.where(self.new_lens > 0, self.out_ids, -1))
+
     def _step_body(self):
-        if self.m.dlin_ok(self.batch):
+        if self.kv_bits == 4 or self.rules is not None:
+            self._step_ruled()
+            nxt = self.out_ids
+            if self.kv_bits == 4:
+                self.ids.copy_(nxt)  # replays feed themselves unless the caller overwrites ids
+                return
+        elif self.m.dlin_ok(self.batch):
             hidden = self.m.decode_hidden_dlin(self.ids, self.positions, self.slots, self.ctx_lens,
                                                self.cache, self.attn_splits)
             nxt = self.m.next_tokens(hidden, self.out_ids, dlin=True)
@@ -672,7 +830,19 @@ class DecodeEngine:
         """Warm up (allocator, lazy attributes) and capture the step."""
         if not self.use_graph:
             return
-        saved = (self.positions.clone(), self.ids.clone())
+        state = [self.positions, self.ids]
+        if self.kv_bits == 4:
+            state += [self.slots, self.ctx_lens, self.cache.block_tables, self.cache.free_list, self.cache.free_range]
+        if self.rules is not None:
+            state += [self.rules.counts, self.rules.seen]
+        saved = [t.clone() for t in state]
+
+        def restore():
+            for t, v in zip(state, saved):
+                t.copy_(v)
+            if self.kv_bits != 4:
+                self._refresh()
+
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -680,17 +850,14 @@ class DecodeEngine:
                 self._step_body()
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
-        self.positions.copy_(saved[0])
-        self._refresh()
+        restore()
         before = ops.launch_count
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self._step_body()
         self.launches_per_step = ops.launch_count - before
         # the captured run did not execute; state is as before the capture
-        self.positions.copy_(saved[0])
-        self.ids.copy_(saved[1])
-        self._refresh()
+        restore()
         torch.cuda.synchronize()
 
     def step(self, ids=None):

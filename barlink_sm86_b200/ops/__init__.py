@@ -465,7 +465,7 @@ class PagedLayout(NamedTuple):
     free_range: torch.Tensor  # int32 [3]: first free entry, free entries, blocks that were missing
 
 
-def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size=16, into=None):
+def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size=16, into=None, rows_per_request=0):
     """Block tables, row offsets, positions and slots of a step, from the requests' lengths, on the GPU and in one launch.
 
     new_lens int32 [batch]: tokens that a request gets now (0 too); below 0: it has ended, and the blocks in its table go back to
@@ -476,13 +476,16 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
     new_lens (a token beyond them gets no row).  Where blocks run out, table entries and slots are -1 and free_range[2] counts
     what was missing; pages beyond max_blocks get no block, their tokens slot -1.
 
+    rows_per_request: 0, or the number of rows that every request has: request b's tokens are rows b * rows_per_request .. then, and
+    the rows behind them are empty (a decode step in which some requests rest: 1).
+
     into: a PagedLayout to write to; its ctx_lens may be past_lens, its free_range may be free_range (a step that is captured
     in a graph and replayed).  1 to 8192 requests."""
     if new_lens.is_cuda:
         _count(2 if tokens > 2048 else 1)
         return PagedLayout(*_C().paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size,
-                                              None if into is None else list(into)))
-    r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size)
+                                              rows_per_request, None if into is None else list(into)))
+    r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request)
     if into is None:
         return PagedLayout(*r)
     for t, v in zip(into, r):
@@ -501,6 +504,8 @@ class LogitRules:
     bias_ids   int32 [rows, entries] (below 0: no entry), bias fp32 [rows, entries]: added after the penalties; entries of the
                same token add up, in their order.
     mask       int32 [rows, >= ceil(vocab / 32)], bit t of word w: token 32 w + t may be chosen; all others become -inf.
+    vocab      tokens in all: columns behind them (the padding of a sharded head) become -inf.  By default that of counts, else of the
+               mask's words, else no limit.
     """
     __slots__ = ("penalties", "counts", "seen", "bias_ids", "bias", "mask", "vocab")
 
@@ -552,10 +557,10 @@ def count_tokens(rules, ids, cu=None, prompt_lens=None, reset=False):
 def logits_process(logits, rules, offset=0, out=None):
     """Logits [rows, n] (bf16 or fp32; column i is token i + offset) under `rules` (LogitRules), for a sampler behind: penalties, biases,
     mask, each operation in fp32, rounded once to the logits' type.  out may be the logits.  Columns at or beyond the vocabulary are
-    -inf where there is a mask, else left as they are."""
+    -inf."""
     if logits.is_cuda:
         _count()
-        return _C().logit_rules(logits, 0, rules.vocab, offset, *rules._args(), out)[0]
+        return _C().logit_rules(logits, False, rules.vocab, offset, *rules._args(), out)[0]
     y = ref.logit_rules(logits, rules.vocab, offset, *rules._args()).to(logits.dtype)
     if out is not None:
         out.copy_(y)
@@ -568,7 +573,7 @@ def logits_argmax(logits, rules, offset=0):
     writing them.  The lowest token of equals; NaN is passed over; -1 where nothing above -inf is left."""
     if logits.is_cuda:
         _count()
-        return tuple(_C().logit_rules(logits, 1, rules.vocab, offset, *rules._args()))
+        return tuple(_C().logit_rules(logits, True, rules.vocab, offset, *rules._args()))
     return ref.pick(ref.logit_rules(logits, rules.vocab, offset, *rules._args()), offset)
 
 

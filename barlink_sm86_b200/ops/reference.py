@@ -421,7 +421,7 @@ def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale):
 
 
 # ---------------------------------------------------------------- serving steps
-def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size):
+def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request=0):
     """See ops.paged_layout; block_tables and free_list are updated in place."""
     width, cap = block_tables.shape[1], free_list.numel()
     head, free, _ = (int(v) for v in free_range)
@@ -440,8 +440,8 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
         for page in range(had, min(-(-(past + n) // block_size), width)):
             block_tables[b, page] = free_list[(head + need) % cap] if need < free else -1
             need += 1
-        for i in range(n):
-            row, p = cu[-1] + i, past + i
+        for i in range(min(n, rows_per_request) if rows_per_request else n):
+            row, p = (b * rows_per_request if rows_per_request else cu[-1]) + i, past + i
             if row >= tokens:
                 break
             pos[row] = p
@@ -491,9 +491,8 @@ def logit_rules(logits, vocab, offset=0, penalties=None, counts=None, seen=None,
     if bias_ids is not None:
         for j in range(bias_ids.shape[1]):
             x = torch.where((bias_ids[:, j:j + 1] == ids) & (bias_ids[:, j:j + 1] >= 0), x + bias[:, j:j + 1], x)
-    if mask is not None:
-        x = torch.where(_word_bits(mask, at) & known, x, torch.full_like(x, -math.inf))
-    return x
+    ok = known if mask is None else _word_bits(mask, at) & known
+    return torch.where(ok, x, torch.full_like(x, -math.inf))
 
 
 def pick(x, offset=0):

@@ -197,12 +197,13 @@ class TPComm:
             return normed, x
         return _ops.rmsnorm(x, gamma, eps, residual)
 
-    def argmax_vocab_parallel(self, logits_local, vocab_per_rank, out=None):
+    def argmax_vocab_parallel(self, logits_local, vocab_per_rank, out=None, rules=None):
         """Global arg max over vocab-parallel logits [rows, vocab_per_rank] (int32 [rows], written
         to `out` when given).  On the link: the arg max kernel leaves (value, index) pairs per slice
         of a row in the layout the merge kernel reads, the pairs of all ranks are all-gathered as
-        they are, and one merge kernel picks -- three launches, no repacking in between."""
-        if logits_local.is_cuda and self.use_link and self.world > 1 and not self.no_comm:
+        they are, and one merge kernel picks -- three launches, no repacking in between.  rules: the arg max is that
+        of the logits under these `ops.LogitRules` (over the whole vocabulary, the same on every rank; -1: nothing is left)."""
+        if rules is None and logits_local.is_cuda and self.use_link and self.world > 1 and not self.no_comm:
             C = load_extension()
             parts = C.argmax_parts(logits_local, self.rank * vocab_per_rank)       # [chunks, rows, 2]
             if parts.numel() * 4 % 16 == 0:
@@ -211,7 +212,10 @@ class TPComm:
                 _ops._count(3)
                 C.allgather_into(allp.view(-1), parts.view(-1))
                 return C.argmax_merge(allp, out)
-        idx, val = _ops.argmax(logits_local, self.rank * vocab_per_rank)
+        if rules is None:
+            idx, val = _ops.argmax(logits_local, self.rank * vocab_per_rank)
+        else:
+            idx, val = _ops.logits_argmax(logits_local, rules, self.rank * vocab_per_rank)
         if self.world == 1 or self.no_comm:
             if out is not None:
                 out.copy_(idx)

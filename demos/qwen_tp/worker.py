@@ -50,6 +50,10 @@ def main():
                     help="after the timed region, run STEPS eager steps on the all-reduce path (one collective "
                          "kernel per row-parallel linear) with CUDA events around every collective and report "
                          "their device time per step")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[4, 16],
+                    help="key/value cache: bf16, or 4 bits in groups of 32 dims (3.2 times smaller)")
+    ap.add_argument("--repetition-penalty", type=float, default=1.0,
+                    help="divides the logits of tokens that a sequence has seen (multiplies those below 0)")
     ap.add_argument("--layers", type=int, default=0, help="debug: fewer layers")
     ap.add_argument("--seed", type=int, default=1234)
     ap.add_argument("--tag", default=None)
@@ -98,7 +102,11 @@ def main():
     g = torch.Generator().manual_seed(a.seed)
     prompts = torch.randint(0, cfg.vocab, (a.batch, a.prompt_len), generator=g, dtype=torch.int32).to(dev)
     total = a.prompt_len + a.warmup + a.gen + 2
-    eng = DecodeEngine(model, a.batch, total, use_graph=not a.no_graph)
+    rules = None
+    if a.repetition_penalty != 1.0:
+        rules = ops.LogitRules.empty(a.batch, cfg.vocab, dev)
+        rules.penalties[:, 0] = a.repetition_penalty
+    eng = DecodeEngine(model, a.batch, total, use_graph=not a.no_graph, kv_bits=a.kv_bits, rules=rules)
 
     def sync():
         if not cpu:
@@ -145,7 +153,7 @@ def main():
 
     # device time of the collectives themselves, call by call (eager, unfused path)
     coll = {"calls_per_step": 0, "device_ms_per_step": 0.0, "steps": 0}
-    if a.time_collectives > 0 and world > 1 and not cpu and not a.no_comm:
+    if a.time_collectives > 0 and world > 1 and not cpu and not a.no_comm and a.kv_bits == 16:
         saved = os.environ.get("BL_DLIN")
         os.environ["BL_DLIN"] = "0"
         eng2 = DecodeEngine(model, a.batch, total, use_graph=False)
@@ -178,12 +186,12 @@ def main():
         torch.save(logits0, os.path.join(a.out, "logits_%s.pt" % tag))
         with open(os.path.join(a.out, "stats_%s.json" % tag), "w") as f:
             json.dump({"tp": world, "backend": a.backend if world > 1 else None, "no_comm": a.no_comm,
-                       "model": cfg.name, "quant": a.quant, "batch": a.batch, "prompt_len": a.prompt_len,
+                       "model": cfg.name, "quant": a.quant, "kv_bits": a.kv_bits, "batch": a.batch, "prompt_len": a.prompt_len,
                        "gen": a.gen, "warmup": a.warmup, "graph": eng.graph is not None, "load_s": load_s,
                        "prefill_ms": prefill_ms, "decode_ms_per_token": ms_tok, "tokens_per_s": tps,
                        "kernels_per_step": eng.launches_per_step,
                        "allreduce_calls_timed": comm.ar_calls - ar0, "peak_mem_gib": mem,
-                       "decode_path": ("folded" if model.dlin_ok(a.batch) else "fused_rs_ag" if model.fused_ok(a.batch)
+                       "decode_path": ("allreduce" if a.kv_bits == 4 or rules is not None else "folded" if model.dlin_ok(a.batch) else "fused_rs_ag" if model.fused_ok(a.batch)
                                        else "allreduce"),
                        "collectives_eager": coll,
                        "weight_gib": model.w.nbytes() / (1 << 30), "link": link_stats()}, f, indent=2)

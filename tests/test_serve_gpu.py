@@ -60,6 +60,20 @@ def test_layout(batch, new, past, bs, spare):
         _layout_both(args, tokens, bs)
 
 
+@pytest.mark.parametrize("batch,per,tokens", [(1, 1, 1), (5, 1, 5), (64, 1, 64), (7, 4, 28), (7, 4, 25), (3, 2, 9), (700, 5, 3500), (2000, 3, 6000)])
+def test_layout_with_equal_rows(batch, per, tokens):
+    """Requests that rest or have ended keep their rows, empty; more tokens than rows: the first ones."""
+    args = _layout_case(batch + per, batch, per + 1, 60, 16, None, ended=0.2)
+    cpu, gpu = [t.clone() for t in args], [t.cuda() for t in args]
+    want = ops.paged_layout(*cpu, tokens, 16, rows_per_request=per)
+    got = ops.paged_layout(*gpu, tokens, 16, rows_per_request=per)
+    for name, a, b in zip(want._fields, want, got):
+        assert torch.equal(a, b.cpu()), name
+    for b in range(min(batch, tokens // per)):
+        n = max(int(args[0][b]), 0)
+        assert got.positions[b * per:(b + 1) * per].tolist() == [int(args[1][b]) + i if i < n else 0 for i in range(per)]
+
+
 def test_layout_edges():
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     # nothing new at all; all requests ended; a table too narrow; entries of a shortage before are not given back
@@ -228,7 +242,7 @@ def test_refusals():
     ok = dict(new_lens=i(2), past_lens=i(2), block_tables=i(2, 3), free_list=i(4), free_range=i(3), tokens=2, block_size=16)
     ops.paged_layout(**ok)
     for bad in (dict(new_lens=i(2).long()), dict(past_lens=i(3)), dict(block_tables=i(3, 3)), dict(block_tables=i(2, 0)), dict(free_list=i(0)),
-                dict(free_range=i(2)), dict(tokens=-1), dict(block_size=0), dict(block_size=2 ** 30), dict(free_list=i(4).cpu()),
+                dict(free_range=i(2)), dict(tokens=-1), dict(rows_per_request=-1), dict(block_size=0), dict(block_size=2 ** 30), dict(free_list=i(4).cpu()),
                 dict(new_lens=i(0), past_lens=i(0), block_tables=i(0, 3)), dict(new_lens=i(8193), past_lens=i(8193), block_tables=i(8193, 1)),
                 dict(into=ops.PagedLayout(i(2), i(2), i(2), i(2), i(3)))):
         with pytest.raises((RuntimeError, TypeError)):
