@@ -3,6 +3,7 @@
 // Third part of the `_C` binding: the 4-bit key/value cache, request layouts, rules on logits.  Workspaces are
 // allocated by each call from the caching allocator, so that calls on several streams and captured graphs share none.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
@@ -32,6 +33,18 @@ void* stream_of(const at::Tensor& t) {
   return at::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
 using OptTensor = c10::optional<at::Tensor>;
+
+// Small calls are bound by the host: a tensor costs half as much from the allocator directly, and parts of one buffer a tenth.
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(size, type, like.device(), c10::nullopt));
+}
+at::Tensor part_of(const at::Tensor& buf, at::ScalarType type, int64_t byte_offset, at::IntArrayRef size) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(byte_offset / int64_t(c10::elementSize(type)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+  return t;
+}
+int64_t to16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 void check_on(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "barlink: ", name, " must be on the same GPU as the other tensors");
@@ -89,7 +102,7 @@ at::Tensor rope_kv_write_q4(const at::Tensor& qkv, const at::Tensor& positions, 
     block_size = 16;
   }
   c10::cuda::CUDAGuard guard(qkv.device());
-  at::Tensor out = out_opt ? *out_opt : slabs ? at::empty({rows, width}, qkv.options().dtype(at::kBFloat16)) : qkv;
+  at::Tensor out = out_opt ? *out_opt : slabs ? fresh({rows, width}, at::kBFloat16, qkv) : qkv;
   check_on(out, qkv, "out");
   TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == 2 && out.size(0) == rows && out.size(1) == width &&
                   aligned16(out),
@@ -108,8 +121,9 @@ std::tuple<at::Tensor, at::Tensor> kv4_read(const at::Tensor& cache, const at::T
   const int rows = small(slots.numel(), "rows");
   const int* sl = i32(slots, cache, -1, "slots");
   c10::cuda::CUDAGuard guard(cache.device());
-  auto o = cache.options().dtype(at::kBFloat16);
-  at::Tensor k = at::empty({rows, nkv, hd}, o), v = at::empty({rows, nkv, hd}, o);
+  const int64_t half = int64_t(rows) * nkv * hd * 2;  // (hd: a multiple of 16 bytes)
+  at::Tensor both = fresh({2 * half}, at::kByte, cache);
+  at::Tensor k = part_of(both, at::kBFloat16, 0, {rows, nkv, hd}), v = part_of(both, at::kBFloat16, half, {rows, nkv, hd});
   if (rows > 0)
     BL_CHECK(bl_kv4_read(cache.data_ptr(), sl, k.data_ptr(), v.data_ptr(), rows, nkv, hd, block_size, small(cache.size(0), "blocks"),
                          stream_of(cache), err, errlen));
@@ -140,7 +154,7 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
   const int* bt = i32(block_tables, q, -1, "block_tables");
   const int* cl = i32(ctx_lens, q, batch, "ctx_lens");
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = out_opt ? *out_opt : at::empty({batch, int64_t(nq) * hd}, q.options());
+  at::Tensor out = out_opt ? *out_opt : fresh({batch, int64_t(nq) * hd}, at::kBFloat16, q);
   check_on(out, q, "out");
   TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == 2 && out.size(0) == batch &&
                   out.size(1) == int64_t(nq) * hd && aligned16(out),
@@ -149,7 +163,7 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
     out.zero_();
   } else if (batch > 0) {
     const size_t bytes = bl_paged_attn_decode_q4_ws(batch, nq, nkv, hd);
-    at::Tensor ws = at::empty({int64_t(bytes)}, cache.options());
+    at::Tensor ws = fresh({int64_t(bytes)}, at::kByte, cache);
     BL_CHECK(bl_paged_attn_decode_q4(q.data_ptr(), int(q.stride(0)), cache.data_ptr(), bt, cl, out.data_ptr(), batch, nq, nkv, hd,
                                      block_size, small(cache.size(0), "blocks"), small(block_tables.size(1), "max_blocks"), float(scale),
                                      ws.data_ptr(), bytes, stream_of(q), err, errlen));
@@ -171,13 +185,16 @@ std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tenso
   const int* fr = i32(free_range, new_lens, 3, "free_range");
   TORCH_CHECK(block_size >= 1 && rows_per_request >= 0, "barlink: block_size must be positive, rows_per_request not below 0");
   c10::cuda::CUDAGuard guard(new_lens.device());
-  auto o = new_lens.options();
   std::vector<at::Tensor> r;
   if (into) {
     r = *into;
     TORCH_CHECK(r.size() == 5, "barlink: paged_layout writes cu, positions, slots, ctx_lens and free_range");
   } else {
-    r = {at::empty({batch + 1}, o), at::empty({rows}, o), at::empty({rows}, o), at::empty({batch}, o), at::empty({3}, o)};
+    const int64_t n[5] = {int64_t(batch) + 1, rows, rows, batch, 3};
+    int64_t at[6] = {0};
+    for (int i = 0; i < 5; ++i) at[i + 1] = at[i] + to16(4 * n[i]);
+    const at::Tensor all = fresh({at[5]}, at::kByte, new_lens);
+    for (int i = 0; i < 5; ++i) r.push_back(part_of(all, at::kInt, at[i], {n[i]}));
   }
   i32(r[0], new_lens, batch + 1, "cu");
   i32(r[1], new_lens, rows, "positions");
@@ -258,7 +275,7 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, bool pick, int64_t
   c10::cuda::CUDAGuard guard(logits.device());
   std::vector<at::Tensor> r;
   if (!pick) {
-    at::Tensor out = out_opt ? *out_opt : at::empty({a.rows, a.n}, logits.options());
+    at::Tensor out = out_opt ? *out_opt : fresh({a.rows, a.n}, logits.scalar_type(), logits);
     check_on(out, logits, "out");
     TORCH_CHECK(out.scalar_type() == logits.scalar_type() && out.dim() == 2 && out.size(0) == a.rows && out.size(1) == a.n && out.stride(1) == 1 &&
                     (a.rows < 2 || out.stride(0) >= a.n),
@@ -267,7 +284,8 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, bool pick, int64_t
     a.ld_out = size_t(out.stride(0));
     r = {out};
   } else {
-    r = {at::empty({a.rows}, logits.options().dtype(at::kInt)), at::empty({a.rows}, logits.options().dtype(at::kFloat))};
+    const at::Tensor both = fresh({2 * to16(4 * int64_t(a.rows))}, at::kByte, logits);
+    r = {part_of(both, at::kInt, 0, {a.rows}), part_of(both, at::kFloat, to16(4 * int64_t(a.rows)), {a.rows})};
     a.idx = r[0].data_ptr();
     a.val = r[1].data_ptr();
   }
