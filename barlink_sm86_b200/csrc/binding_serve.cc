@@ -162,10 +162,11 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
   if (batch > 0 && block_tables.size(1) == 0) {
     out.zero_();
   } else if (batch > 0) {
+    const int max_blocks = small(block_tables.size(1), "max_blocks");
     const size_t bytes = bl_paged_attn_decode_q4_ws(batch, nq, nkv, hd);
     at::Tensor ws = fresh({int64_t(bytes)}, at::kByte, cache);
     BL_CHECK(bl_paged_attn_decode_q4(q.data_ptr(), int(q.stride(0)), cache.data_ptr(), bt, cl, out.data_ptr(), batch, nq, nkv, hd,
-                                     block_size, small(cache.size(0), "blocks"), small(block_tables.size(1), "max_blocks"), float(scale),
+                                     block_size, small(cache.size(0), "blocks"), max_blocks, float(scale),
                                      ws.data_ptr(), bytes, stream_of(q), err, errlen));
   }
   return out;

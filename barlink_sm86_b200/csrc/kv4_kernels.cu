@@ -280,8 +280,9 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ ca
 // size; it moves only when it is exceeded by 2^8, which one vote per tile finds out.
 //
 // Work: the units (two tiles) of all (request, KV head) pairs in one row, cut into equal runs, one for each warp; a warp has a
-// ring of its own that the bulk copies fill across pairs, and shares nothing with others.  Lengths are on the GPU only, so every warp adds
-// them up by itself.  Pairs that were cut are joined by k_q4_merge.
+// ring of its own that the bulk copies fill across pairs, and shares nothing with others.  Lengths are on the GPU only, so every warp
+// adds them up by itself.  Pairs that were cut are joined by k_q4_merge.  (A cluster of blocks for each pair, joined through distributed
+// shared memory without a second kernel: one request of 333 tokens 5.9 us and 6.0 so, 64 of up to 1100 16.8 and 13.7.)
 constexpr int kQ4MaxG = 16;
 constexpr int kQ4Warps = 4;
 constexpr float kQ4None = -3.402823466e38f;  // reference before the first token
@@ -300,7 +301,7 @@ struct Q4Attn {
   __nv_bfloat16* out;
   float* part;   // [2 * runs]: a run's first piece of a pair and its last; G * hd sums, G times (reference, sum of p)
   int2* meta;    // [batch * nkv]: a pair's first piece, and the number of its pieces (0: done); the others are the first of their runs
-  int q_stride, batch, nq, nkv, block_size, n_blocks, max_blocks, min_run;
+  int q_stride, batch, nq, nkv, block_size, n_blocks, max_blocks;
   float scale_log2;
 };
 
@@ -375,7 +376,7 @@ constexpr int q4_smem_bytes() {
 }
 
 template <int HD, int NT, int STAGES>
-__global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q4(const Q4Attn a) {
+__global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn a) {
   constexpr int NA = HD / kQ4Group, TB = q4_tile_bytes(HD);
   constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
       if (lane >= o) upto += u;
     }
     const int total = __shfl_sync(kAll, upto, 31);
-    run = max((total + runs - 1) / runs, a.min_run);
+    run = (total + runs - 1) / runs;
     lo = int(min(int64_t(me) * run, int64_t(total)));
     hi = min(lo + run, total);
     int b = b0, at = upto - mine, n = 0;
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
   const int count = hi - lo;
   Q4At ahead = seg;
   int chunk = -1;
-  long long where = -1;
+  int where = -1;      // its number in the cache, below 0: none
   uint32_t there = 0;  // bits 2 s, 2 s + 1: the tiles of stage s have a block
   const uint32_t leader = elect_leader();
   auto issue = [&](int i, int stage) {
@@ -450,18 +451,29 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
         if (tok < q4_context(a, ahead.b)) {
           const int page = tok / a.block_size, blk = a.tables[size_t(ahead.b) * a.max_blocks + page];
           if (blk >= 0 && blk < a.n_blocks)
-            where = (long long)(q4_tile_offset(blk, tok - page * a.block_size, ahead.h, a.nkv, a.block_size, HD));
+            where = (blk * a.nkv + ahead.h) * (a.block_size / kQ4Tokens) + (tok - page * a.block_size) / kQ4Tokens;
         }
       }
     }
     const int from = 2 * (i & 15);
-    const long long off0 = __shfl_sync(kAll, where, from), off1 = __shfl_sync(kAll, where, from + 1);
-    const uint32_t has = (off0 >= 0 ? 1u : 0u) | (off1 >= 0 ? 2u : 0u), dst = ring + stage * 2 * TB;
+    const int t0 = __shfl_sync(kAll, where, from), t1 = __shfl_sync(kAll, where, from + 1);
+    const uint32_t has = (t0 >= 0 ? 1u : 0u) | (t1 >= 0 ? 2u : 0u), dst = ring + stage * 2 * TB;
     there = (there & ~(3u << (2 * stage))) | has << (2 * stage);
     mbar_expect_tx_warp(leader, bars + stage, TB * __popc(has));
-    if (off0 >= 0) bulk_load_warp(leader, dst, a.cache + off0, TB, smem_u32(bars + stage), kHintEvictFirst);
-    if (off1 >= 0) bulk_load_warp(leader, dst + TB, a.cache + off1, TB, smem_u32(bars + stage), kHintEvictFirst);
+    if (t0 >= 0) bulk_load_warp(leader, dst, a.cache + size_t(t0) * TB, TB, smem_u32(bars + stage), kHintEvictFirst);
+    if (t1 >= 0) bulk_load_warp(leader, dst + TB, a.cache + size_t(t1) * TB, TB, smem_u32(bars + stage), kHintEvictFirst);
   };
+  // (the queries first: behind the copies they would wait for what may be the whole cache)
+  uint4 raw[NT][NA];
+  auto ask_queries = [&] {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int ga = 0; ga < NA; ++ga)
+        raw[n][ga] = 8 * n + g < G ? *reinterpret_cast<const uint4*>(a.q + size_t(seg.b) * a.q_stride + (size_t(seg.h) * G + 8 * n + g) * HD + 32 * ga + 8 * t)
+                                   : make_uint4(0, 0, 0, 0);
+  };
+  ask_queries();
 #pragma unroll 1
   for (int i = 0; i < STAGES; ++i)
     if (i < count) issue(i, i);
@@ -479,16 +491,10 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
     float f[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int head = 8 * n + g;
-      uint4 raw[NA];
-#pragma unroll
-      for (int ga = 0; ga < NA; ++ga)
-        raw[ga] = head < G ? *reinterpret_cast<const uint4*>(a.q + size_t(seg.b) * a.q_stride + (size_t(seg.h) * G + head) * HD + 32 * ga + 8 * t)
-                           : make_uint4(0, 0, 0, 0);
       uint32_t top = 0;  // the largest element's bits: magnitudes of bf16 compare as integers
 #pragma unroll
       for (int ga = 0; ga < NA; ++ga)
-        top = __vmaxu2(top, __vmaxu2(__vmaxu2(raw[ga].x & 0x7fff7fffu, raw[ga].y & 0x7fff7fffu), __vmaxu2(raw[ga].z & 0x7fff7fffu, raw[ga].w & 0x7fff7fffu)));
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(raw[n][ga].x & 0x7fff7fffu, raw[n][ga].y & 0x7fff7fffu), __vmaxu2(raw[n][ga].z & 0x7fff7fffu, raw[n][ga].w & 0x7fff7fffu)));
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(kAll, top, 1));
       top = max(top, __shfl_xor_sync(kAll, top, 2));
@@ -497,8 +503,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
       float sum[NA];
 #pragma unroll
       for (int ga = 0; ga < NA; ++ga) {
-        const float e0 = bf16_lo(raw[ga].x) * up, e1 = bf16_hi(raw[ga].x) * up, e2 = bf16_lo(raw[ga].y) * up, e3 = bf16_hi(raw[ga].y) * up,
-                    e4 = bf16_lo(raw[ga].z) * up, e5 = bf16_hi(raw[ga].z) * up, e6 = bf16_lo(raw[ga].w) * up, e7 = bf16_hi(raw[ga].w) * up;
+        const float e0 = bf16_lo(raw[n][ga].x) * up, e1 = bf16_hi(raw[n][ga].x) * up, e2 = bf16_lo(raw[n][ga].y) * up, e3 = bf16_hi(raw[n][ga].y) * up,
+                    e4 = bf16_lo(raw[n][ga].z) * up, e5 = bf16_hi(raw[n][ga].z) * up, e6 = bf16_lo(raw[n][ga].w) * up, e7 = bf16_hi(raw[n][ga].w) * up;
         qb[n][ga][0] = pack_f16x2(e0, e4);
         qb[n][ga][1] = pack_f16x2(e1 * 0.0625f, e5 * 0.0625f);
         qb[n][ga][2] = pack_f16x2(e2, e6);
@@ -546,31 +552,56 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
       const int left = ctx - (lo + k - seg.start) * kQ4Unit;  // tokens of this unit
 
       // ---- scores, over the factor f: tokens g (c[.][.][0], [1]) and g + 8 of either tile, heads 2 t and 2 t + 1 ----
+      // (the asm statements keep their order: products that wait for one another stand four apart)
       float c[2][NT][4];
+      {
+        uint32_t w0[2][NA], w1[2][NA], sl0[2][NA], sl1[2][NA];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t w0[NA], w1[NA], sl0[NA], sl1[NA];
-        lds_words<NA>(tile + u * TB + g * (HD / 2) + t * NA * 4, w0);
-        lds_words<NA>(tile + u * TB + (g + 8) * (HD / 2) + t * NA * 4, w1);
-        lds_words<NA>(tile + u * TB + q4_k_params(HD) + g * NA * 4, sl0);  // step[NA], low[NA]
-        lds_words<NA>(tile + u * TB + q4_k_params(HD) + (g + 8) * NA * 4, sl1);
-        const uint32_t m0 = NA == 4 && (t & 1) ? sl0[NA - 1] : sl0[NA / 2], m1 = NA == 4 && (t & 1) ? sl1[NA - 1] : sl1[NA / 2];
+        for (int u = 0; u < 2; ++u) {
+          lds_words<NA>(tile + u * TB + q4_k_params(HD) + g * NA * 4, sl0[u]);  // step[NA], low[NA]
+          lds_words<NA>(tile + u * TB + q4_k_params(HD) + (g + 8) * NA * 4, sl1[u]);
+          lds_words<NA>(tile + u * TB + g * (HD / 2) + t * NA * 4, w0[u]);
+          lds_words<NA>(tile + u * TB + (g + 8) * (HD / 2) + t * NA * 4, w1[u]);
+        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) q4_mma_bf16_0(c[u][n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t m0 = NA == 4 && (t & 1) ? sl0[u][NA - 1] : sl0[u][NA / 2], m1 = NA == 4 && (t & 1) ? sl1[u][NA - 1] : sl1[u][NA / 2];
 #pragma unroll
-        for (int ga = 0; ga < NA; ++ga) {
-          const float s0 = ga & 1 ? bf16_hi(sl0[ga >> 1]) : bf16_lo(sl0[ga >> 1]), s1 = ga & 1 ? bf16_hi(sl1[ga >> 1]) : bf16_lo(sl1[ga >> 1]);
-          const uint32_t v0 = w0[ga] >> 8, v1 = w1[ga] >> 8;
+          for (int n = 0; n < NT; ++n) q4_mma_bf16_0(c[u][n], m0, m1, m0, m1, qs[n][0], qs[n][1]);
+        }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float d[4];
-            q4_mma_f16_0(d, w0[ga] & 0x000f000fu, w1[ga] & 0x000f000fu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00f000f0u, qb[n][ga][0], qb[n][ga][1]);
-            q4_mma_f16(d, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qb[n][ga][2], qb[n][ga][3]);
-            c[u][n][0] += s0 * d[0];
-            c[u][n][1] += s0 * d[1];
-            c[u][n][2] += s1 * d[2];
-            c[u][n][3] += s1 * d[3];
-          }
+        for (int gp = 0; gp < NA; gp += 2) {
+          float d[2][2][NT][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                q4_mma_f16_0(d[i][u][n], w0[u][gp + i] & 0x000f000fu, w1[u][gp + i] & 0x000f000fu, w0[u][gp + i] & 0x00f000f0u, w1[u][gp + i] & 0x00f000f0u,
+                             qb[n][gp + i][0], qb[n][gp + i][1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t v0 = w0[u][gp + i] >> 8, v1 = w1[u][gp + i] >> 8;
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                q4_mma_f16(d[i][u][n], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qb[n][gp + i][2], qb[n][gp + i][3]);
+            }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float s0 = i ? bf16_hi(sl0[u][gp >> 1]) : bf16_lo(sl0[u][gp >> 1]), s1 = i ? bf16_hi(sl1[u][gp >> 1]) : bf16_lo(sl1[u][gp >> 1]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                c[u][n][0] += s0 * d[i][u][n][0];
+                c[u][n][1] += s0 * d[i][u][n][1];
+                c[u][n][2] += s1 * d[i][u][n][2];
+                c[u][n][3] += s1 * d[i][u][n][3];
+              }
+            }
         }
       }
       uint32_t vs0[2][NA], vs1[2][NA];  // step[NA], low[NA] of the values of tokens g and g + 8
@@ -593,17 +624,16 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
               for (int i = 0; i < NA; ++i) (j ? vs1[u] : vs0[u])[i] = 0;
             }
       }
-      float top[2][2];  // the larger of a token's steps and 2^-90
+      // ---- probabilities; where one times step may leave fp16's range, a new reference first ----
+      float top;  // the larger of all the steps here and 2^-90 (bf16 above 0 compare as integers)
+      {
+        uint32_t m = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        top[u][0] = top[u][1] = 8.0779356694631609e-28f;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-          top[u][0] = fmaxf(top[u][0], i & 1 ? bf16_hi(vs0[u][i >> 1]) : bf16_lo(vs0[u][i >> 1]));
-          top[u][1] = fmaxf(top[u][1], i & 1 ? bf16_hi(vs1[u][i >> 1]) : bf16_lo(vs1[u][i >> 1]));
-        }
+          for (int i = 0; i < NA / 2; ++i) m = __vmaxu2(m, __vmaxu2(vs0[u][i], vs1[u][i]));
+        top = fmaxf(fmaxf(bf16_lo(m), bf16_hi(m)), 8.0779356694631609e-28f);
       }
-      // ---- probabilities; where one times step leaves fp16's range, a new reference first ----
       float p[2][NT][4];
       auto weigh = [&] {
         float most = 0.f;
@@ -614,16 +644,20 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               p[u][n][j] = q4_ex2(fmaf(c[u][n][j], f[n][j & 1], -R[n][j & 1]));
-              most = fmaxf(most, p[u][n][j] * top[u][j >> 1]);  // (a NaN leaves the reference alone)
+              most += p[u][n][j];  // (no less than the greatest; a NaN leaves the reference alone)
             }
         return most;
       };
-      if (__any_sync(kAll, weigh() > 512.f)) {
-        float e[2][2];
+      if (__any_sync(kAll, weigh() * top > 512.f)) {
+        float e[2][2];  // log2 of a token's largest step, rounded down
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) e[u][j] = fminf(float(int(__float_as_uint(top[u][j]) >> 23) - 127), 110.f);
+          for (int j = 0; j < 2; ++j) {
+            uint32_t m = (j ? vs1[u] : vs0[u])[0];
+            if constexpr (NA == 4) m = __vmaxu2(m, (j ? vs1[u] : vs0[u])[1]);
+            e[u][j] = float(min(max(int(max(m & 0xffffu, m >> 16) >> 7) - 127, -90), 110));
+          }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -650,28 +684,32 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
       // low + 16 high, the rows g + 8 the high one: one instruction less for a word, and the difference is taken at the end ----
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        uint32_t w0[NA], w1[NA];
+        uint32_t w0[NA], w1[NA], pb[NT][NA][2];
         lds_words<NA>(tile + u * TB + q4_v_codes(HD) + t * HD + g * NA * 4, w0);
         lds_words<NA>(tile + u * TB + q4_v_codes(HD) + (t + 4) * HD + g * NA * 4, w1);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          l[n][0] += p[u][n][0] + p[u][n][2];
-          l[n][1] += p[u][n][1] + p[u][n][3];
+          const float* q = p[u][n];
+          l[n][0] += q[0] + q[2];
+          l[n][1] += q[1] + q[3];
+#pragma unroll
+          for (int ga = 0; ga < NA; ++ga) {
+            const float s0 = ga & 1 ? bf16_hi(vs0[u][ga >> 1]) : bf16_lo(vs0[u][ga >> 1]), s1 = ga & 1 ? bf16_hi(vs1[u][ga >> 1]) : bf16_lo(vs1[u][ga >> 1]);
+            const uint32_t lw0 = vs0[u][NA / 2 + (ga >> 1)], lw1 = vs1[u][NA / 2 + (ga >> 1)];
+            const float m0 = ga & 1 ? bf16_hi(lw0) : bf16_lo(lw0), m1 = ga & 1 ? bf16_hi(lw1) : bf16_lo(lw1);
+            pb[n][ga][0] = q4_transpose(pack_f16x2(q[0] * s0, q[1] * s0));
+            pb[n][ga][1] = q4_transpose(pack_f16x2(q[2] * s1, q[3] * s1));
+            vm[n][ga][0] = fmaf(q[0], m0, fmaf(q[2], m1, vm[n][ga][0]));
+            vm[n][ga][1] = fmaf(q[1], m0, fmaf(q[3], m1, vm[n][ga][1]));
+          }
         }
 #pragma unroll
         for (int ga = 0; ga < NA; ++ga) {
-          const float s0 = ga & 1 ? bf16_hi(vs0[u][ga >> 1]) : bf16_lo(vs0[u][ga >> 1]), s1 = ga & 1 ? bf16_hi(vs1[u][ga >> 1]) : bf16_lo(vs1[u][ga >> 1]);
-          const uint32_t lw0 = vs0[u][NA / 2 + (ga >> 1)], lw1 = vs1[u][NA / 2 + (ga >> 1)];
-          const float m0 = ga & 1 ? bf16_hi(lw0) : bf16_lo(lw0), m1 = ga & 1 ? bf16_hi(lw1) : bf16_lo(lw1);
           const uint32_t v0 = __byte_perm(w0[ga], 0, 0x4341), v1 = __byte_perm(w1[ga], 0, 0x4341);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float *q = p[u][n];
-            const uint32_t pb0 = q4_transpose(pack_f16x2(q[0] * s0, q[1] * s0)), pb1 = q4_transpose(pack_f16x2(q[2] * s1, q[3] * s1));
-            vm[n][ga][0] = fmaf(q[0], m0, fmaf(q[2], m1, vm[n][ga][0]));
-            vm[n][ga][1] = fmaf(q[1], m0, fmaf(q[3], m1, vm[n][ga][1]));
-            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x00ff00ffu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00ff00ffu, w1[ga] & 0x00f000f0u, pb0, pb1);
-            q4_mma_f16(o[n][2 * ga + 1], v0, v0 & 0x00f000f0u, v1, v1 & 0x00f000f0u, pb0, pb1);
+            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x00ff00ffu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00ff00ffu, w1[ga] & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
+            q4_mma_f16(o[n][2 * ga + 1], v0, v0 & 0x00f000f0u, v1, v1 & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
           }
         }
       }
@@ -715,7 +753,10 @@ __global__ void __launch_bounds__(kQ4Warps * 32, NT == 1 ? 3 : 2) k_paged_attn_q
       }
     if (begins && lane == 0)
       a.meta[size_t(seg.b) * a.nkv + seg.h] = make_int2(piece, whole ? 0 : (seg.start + seg.units - 1) / run - me + 1);
-    if (k < count) q4_advance(a, seg, lo + k);
+    if (k < count) {
+      q4_advance(a, seg, lo + k);
+      ask_queries();
+    }
   }
   if (dead) {
     // a copy did not arrive in time: say so, and leave with none in flight
@@ -791,13 +832,13 @@ __global__ void __launch_bounds__(kQ4MergeWarps * 32) k_q4_merge(const Q4Attn a,
 
 using namespace bl;
 
-static int q4_shape(const char* what, int hd, int block_size, int n_blocks, char* err, size_t errlen) {
+static int q4_shape(const char* what, int hd, int nkv, int block_size, int n_blocks, char* err, size_t errlen) {
   if ((hd != 64 && hd != 128) || block_size < kQ4Tokens || block_size % kQ4Tokens) {
     set_err(err, errlen, "barlink: %s is built for head_dim 64 and 128 and block sizes that are multiples of %d", what, kQ4Tokens);
     return -1;
   }
-  if (n_blocks < 0 || int64_t(n_blocks) * block_size > 0x7fffffffLL) {
-    set_err(err, errlen, "barlink: %s: the cache's slots do not fit 32 bits", what);
+  if (n_blocks < 0 || int64_t(n_blocks) * block_size > 0x7fffffffLL || int64_t(n_blocks) * (block_size / kQ4Tokens) * nkv > 0x7fffffffLL) {
+    set_err(err, errlen, "barlink: %s: the cache's slots and tiles must fit 32 bits", what);
     return -1;
   }
   return 0;
@@ -808,7 +849,7 @@ extern "C" size_t bl_kv4_tile_bytes(int hd) { return q4_tile_bytes(hd); }
 extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nsplit, size_t slab, const void* bias, void* out,
                                    const int* positions, const int* slots, void* cache, int rows, int nq, int nkv, int hd,
                                    int block_size, int n_blocks, double theta, void* stream, char* err, size_t errlen) {
-  if (q4_shape("the 4-bit cache", hd, block_size, n_blocks, err, errlen)) return -1;
+  if (q4_shape("the 4-bit cache", hd, nkv, block_size, n_blocks, err, errlen)) return -1;
   if (rows < 0 || nq < 0 || nkv < 1 || (!qkv && (!slabs || nsplit < 1)) || !out || !positions || (slots && !cache) || !(theta > 0)) {
     set_err(err, errlen, "barlink: rope_kv_write_q4 needs the QKV rows or slabs, positions, an output and, with slots, a cache");
     return -1;
@@ -844,7 +885,7 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
 
 extern "C" int bl_kv4_read(const void* cache, const int* slots, void* k, void* v, int rows, int nkv, int hd, int block_size,
                            int n_blocks, void* stream, char* err, size_t errlen) {
-  if (q4_shape("the 4-bit cache", hd, block_size, n_blocks, err, errlen)) return -1;
+  if (q4_shape("the 4-bit cache", hd, nkv, block_size, n_blocks, err, errlen)) return -1;
   const size_t units = size_t(rows) * nkv * (hd / 8);
   if (units == 0) return 0;
   launch_k(k_kv4_read, dim3(unsigned((units + 255) / 256)), dim3(256), 0, static_cast<cudaStream_t>(stream),
@@ -860,18 +901,19 @@ extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
   return e == cudaSuccess ? 0 : -1;
 }
 
-// blocks of attention: as many as are resident at once
-static int q4_grid(int G) { return sm_count() * (G > 8 ? 2 : 3); }
+// Blocks of attention.  Two to an SM, with registers for two tiles at once: three and four of fewer registers (the last with spills) took
+// 34.5 and 37.9 us where two take 32.7 (4 requests of up to 32767 tokens), 14.9 and 17.0 against 13.7 (64 of up to 1100).
+static int q4_grid() { return sm_count() * 2; }
 
 extern "C" size_t bl_paged_attn_decode_q4_ws(int batch, int nq, int nkv, int hd) {
   const int G = nq / nkv;
-  return 2 * size_t(q4_grid(G)) * kQ4Warps * q4_part_floats(G, hd) * sizeof(float) + size_t(batch) * nkv * sizeof(int2);
+  return 2 * size_t(q4_grid()) * kQ4Warps * q4_part_floats(G, hd) * sizeof(float) + size_t(batch) * nkv * sizeof(int2);
 }
 
 extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, const int* block_tables, const int* ctx_lens,
                                        void* out, int batch, int nq, int nkv, int hd, int block_size, int n_blocks, int max_blocks,
                                        float scale, void* ws, size_t ws_bytes, void* stream, char* err, size_t errlen) {
-  if (q4_shape("attention over the 4-bit cache", hd, block_size, n_blocks, err, errlen)) return -1;
+  if (q4_shape("attention over the 4-bit cache", hd, nkv, block_size, n_blocks, err, errlen)) return -1;
   if (nkv < 1 || nq < 1 || nq % nkv || nq / nkv > kQ4MaxG) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs nq %% nkv == 0 and at most %d query heads per KV head", kQ4MaxG);
     return -1;
@@ -887,7 +929,7 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs a positive scale");
     return -1;
   }
-  const int G = nq / nkv, nt = G > 8 ? 2 : 1, grid = q4_grid(G);
+  const int G = nq / nkv, nt = G > 8 ? 2 : 1, grid = q4_grid();
   if (!ws || ws_bytes < bl_paged_attn_decode_q4_ws(batch, nq, nkv, hd)) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs %zu bytes of workspace",
             bl_paged_attn_decode_q4_ws(batch, nq, nkv, hd));
@@ -903,7 +945,6 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   a.meta = reinterpret_cast<int2*>(a.part + 2 * size_t(grid) * kQ4Warps * q4_part_floats(G, hd));
   a.q_stride = q_stride; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks;
   a.max_blocks = max_blocks;
-  a.min_run = 1;
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   static bool attr[4][64] = {};
@@ -915,7 +956,7 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   };
   cudaError_t e;
   if (hd == 128)
-    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 3>, k_q4_merge<128>, q4_smem_bytes<128, 3>(), attr[0])
+    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[0])
                 : go(k_paged_attn_q4<128, 2, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[1]);
   else
     e = nt == 1 ? go(k_paged_attn_q4<64, 1, 4>, k_q4_merge<64>, q4_smem_bytes<64, 4>(), attr[2])
