@@ -79,43 +79,36 @@ __device__ __forceinline__ void q4_unpack8(const uint4& v, float (&f)[8]) {
   }
 }
 
-__device__ __forceinline__ float quad_min(float v) {
-  v = fminf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fminf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-}
-
-// Eight of a group's 32 elements, the rest with the other lanes of the quad -> codes (nibble e = element e), and the
-// group's step and low as bf16 bits.  The codes are those of the formula to the bit: (x - low) * (1 / step) is within 10^-5 of the
-// quotient, so that it rounds the same way unless it lies that near to the middle of two codes; then it is divided.
-__device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t& step_bits, uint16_t& low_bits) {
-  float lo = x[0], hi = x[0], nan = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    nan = fmaf(x[e], 0.f, nan);  // NaN where an element is no finite number (minimum and maximum pass over NaN)
-  }
-  lo = quad_min(lo);
-  hi = quad_max(hi);
-  nan += __shfl_xor_sync(0xffffffffu, nan, 1);
-  nan += __shfl_xor_sync(0xffffffffu, nan, 2);
-  __nv_bfloat16 st = __float2bfloat16(__fdiv_rn(hi - lo, 15.f));
-  float step = __bfloat162float(st);
-  const bool fine = nan == 0.f && isfinite(step);
-  if (!fine) step = 0.f;
+// Eight of a group's 32 elements (bf16, as they lie), the rest with the other lanes of the quad -> codes (nibble e = element e), and
+// the group's step and low as bf16 bits.  Least and greatest are taken in pairs, the least as the greatest of the negatives, so that
+// one exchange carries both; a NaN or infinity comes out as a step that is no finite number.  The codes are those of the formula to the
+// bit: a product with 1 / 15 or 1 / step is within 10^-5 of the quotient (or a few units in the last place of a step), and where
+// that could round otherwise it is divided.
+__device__ __forceinline__ uint32_t q4_quantise8(const uint4& raw, uint16_t& step_bits, uint16_t& low_bits) {
+  auto h = [](uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); };
+  auto u = [](__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); };
+  const uint32_t hi2 = u(__hmax2_nan(__hmax2_nan(h(raw.x), h(raw.y)), __hmax2_nan(h(raw.z), h(raw.w))));
+  const uint32_t lo2 = u(__hmin2_nan(__hmin2_nan(h(raw.x), h(raw.y)), __hmin2_nan(h(raw.z), h(raw.w)))) ^ 0x80008000u;
+  uint32_t m = u(__hmax2_nan(h(__byte_perm(lo2, hi2, 0x5410)), h(__byte_perm(lo2, hi2, 0x7632))));  // (-low, greatest)
+  m = u(__hmax2_nan(h(m), h(__shfl_xor_sync(0xffffffffu, m, 1))));
+  m = u(__hmax2_nan(h(m), h(__shfl_xor_sync(0xffffffffu, m, 2))));
+  const float lo = -__uint_as_float(m << 16), range = __uint_as_float(m & 0xffff0000u) - lo;
+  float q = range * (1.f / 15.f);
+  if ((__float_as_uint(q) & 0xffffu) - 0x7ff8u < 16u) q = __fdiv_rn(range, 15.f);  // near the middle of two bf16 numbers
+  const __nv_bfloat16 st = __float2bfloat16(q);
+  const float step = __bfloat162float(st);
+  const bool fine = isfinite(step);
   uint32_t w = 0;
-  if (step > 0.f) {
+  if (fine && step > 0.f) {
+    float x[8];
+    q4_unpack8(raw, x);
     const float inv = __fdividef(1.f, step);
     bool near = step < 1e-30f;  // (1 / step must be a finite number)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float v = (x[e] - lo) * inv, r = v + 12582912.f;  // 3 * 2^22: the sum's last bits are the rounded quotient
       near |= fabsf(v - (r - 12582912.f)) > 0.49999f;
-      w |= (min(__float_as_uint(r) & 31u, 15u)) << (4 * e);
+      w |= (__float_as_uint(r) & 15u) << (4 * e);  // (at most 15: a step is no more than 2^-8 below a fifteenth of the range)
     }
     if (near) {
       w = 0;
@@ -124,7 +117,7 @@ __device__ __forceinline__ uint32_t q4_quantise8(const float (&x)[8], uint16_t& 
     }
   }
   step_bits = fine ? __bfloat16_as_ushort(st) : 0;
-  low_bits = fine ? __bfloat16_as_ushort(__float2bfloat16(lo)) : 0x7fc0;
+  low_bits = fine ? uint16_t((m & 0xffffu) ^ 0x8000u) : 0x7fc0;
   return w;
 }
 
@@ -151,7 +144,7 @@ __device__ __forceinline__ void q4_store8(uint8_t* tile, int r, int hd, bool val
 // the block's rows are computed once, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01 radians), and the products are
 // rounded one by one: the rotated elements are the formula's to the bit.
 template <int HD, bool SLABS, int ROWS, int THREADS, int BATCH>
-__global__ void __launch_bounds__(THREADS) k_rope_kv_write_q4(const Q4Write a) {
+__global__ void __launch_bounds__(THREADS, ROWS > 1 ? 1024 / THREADS : 1) k_rope_kv_write_q4(const Q4Write a) {
   constexpr int HALF = HD / 2, OPH = HD / 16, PER = THREADS / ROWS, STEP = PER / OPH;  // octets of half a head; heads of a pass
   pdl_launch_dependents();
   pdl_wait();
@@ -213,11 +206,8 @@ __global__ void __launch_bounds__(THREADS) k_rope_kv_write_q4(const Q4Write a) {
       }
       const bool keep = there && h >= a.nq && kept;
       if (!__any_sync(0xffffffffu, keep)) continue;
-      float x[8], y[8];
-      q4_unpack8(lo[c], x);
-      q4_unpack8(hi[c], y);
       uint16_t s0, l0, s1, l1;
-      const uint32_t w0 = q4_quantise8(x, s0, l0), w1 = q4_quantise8(y, s1, l1);
+      const uint32_t w0 = q4_quantise8(lo[c], s0, l0), w1 = q4_quantise8(hi[c], s1, l1);
       if (keep) {
         const bool value = h >= a.nq + a.nkv;
         uint8_t* tile = a.cache + q4_tile_offset(blk, in_block, h - a.nq - (value ? a.nkv : 0), a.nkv, a.block_size, HD);
@@ -229,40 +219,43 @@ __global__ void __launch_bounds__(THREADS) k_rope_kv_write_q4(const Q4Write a) {
   }
 }
 
-// Rows of the cache back as bf16 (zeros where a slot names none).  One octet of a key and of a value per thread.
-__global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ cache, const int* __restrict__ slots,
-                                                  __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v, size_t units, int nkv,
-                                                  int hd, int block_size, int n_blocks) {
+// Rows of the cache back as bf16 (zeros where a slot names none).  One octet of a key and of a value per thread; a block takes as many
+// rows as it has threads for, so that the numbers that are divided are small (with 64-bit ones: 8.7 us for 8191 rows of 4 heads).
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ cache, const int* __restrict__ slots, __nv_bfloat16* __restrict__ k,
+                                                  __nv_bfloat16* __restrict__ v, int rows, int block_rows, int nkv, int block_size, int n_blocks) {
+  constexpr int OH = HD / 8, NA = HD / kQ4Group;
   pdl_launch_dependents();
   pdl_wait();
-  const size_t u = size_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (u >= units) return;
-  const int oh = hd >> 3, o = int(u % oh), h = int(u / oh % nkv), na = hd / kQ4Group, ga = o >> 2, t = o & 3;
-  const size_t row = u / oh / nkv;
-  const int slot = slots[row];
-  uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
-  if (slot >= 0 && slot / block_size < n_blocks) {
-    const int in_block = slot % block_size, r = in_block % kQ4Tokens;
-    const uint8_t* tile = cache + q4_tile_offset(slot / block_size, in_block, h, nkv, block_size, hd);
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(tile + r * (hd / 2) + (t * na + ga) * 4);
-    const uint8_t* vp = tile + q4_v_codes(hd) + (r >> 1) * hd + (r & 1) * 2;
-    const uint32_t vw = *reinterpret_cast<const uint16_t*>(vp + ((2 * t) * na + ga) * 4) |
-                        uint32_t(*reinterpret_cast<const uint16_t*>(vp + ((2 * t + 1) * na + ga) * 4)) << 16;
-    const __nv_bfloat16* kp = reinterpret_cast<const __nv_bfloat16*>(tile + q4_k_params(hd) + r * na * 4);
-    const __nv_bfloat16* vq = reinterpret_cast<const __nv_bfloat16*>(tile + q4_v_params(hd) + r * na * 4);
-    const float ks = __bfloat162float(kp[ga]), kl = __bfloat162float(kp[na + ga]);
-    const float vs = __bfloat162float(vq[ga]), vl = __bfloat162float(vq[na + ga]);
-    uint32_t kk[4], vv[4];
+  const int row0 = blockIdx.x * block_rows, per = nkv * OH, count = min(block_rows, rows - row0) * per;
+  for (int u = threadIdx.x; u < count; u += 256) {
+    const int r0 = u / per, e = u - r0 * per, h = e / OH, o = e % OH, ga = o >> 2, t = o & 3;
+    const int slot = slots[row0 + r0], blk = slot / block_size;
+    uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
+    if (slot >= 0 && blk < n_blocks) {
+      const int in_block = slot - blk * block_size, r = in_block % kQ4Tokens;
+      const uint8_t* tile = cache + q4_tile_offset(blk, in_block, h, nkv, block_size, HD);
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(tile + r * (HD / 2) + (t * NA + ga) * 4);
+      const uint8_t* vp = tile + q4_v_codes(HD) + (r >> 1) * HD + (r & 1) * 2;
+      const uint32_t vw = *reinterpret_cast<const uint16_t*>(vp + ((2 * t) * NA + ga) * 4) |
+                          uint32_t(*reinterpret_cast<const uint16_t*>(vp + ((2 * t + 1) * NA + ga) * 4)) << 16;
+      const __nv_bfloat16* kp = reinterpret_cast<const __nv_bfloat16*>(tile + q4_k_params(HD) + r * NA * 4);
+      const __nv_bfloat16* vq = reinterpret_cast<const __nv_bfloat16*>(tile + q4_v_params(HD) + r * NA * 4);
+      const float ks = __bfloat162float(kp[ga]), kl = __bfloat162float(kp[NA + ga]);
+      const float vs = __bfloat162float(vq[ga]), vl = __bfloat162float(vq[NA + ga]);
+      uint32_t kk[4], vv[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      kk[j] = pack_bf16x2(kl + ks * float((kw >> (8 * j)) & 15), kl + ks * float((kw >> (8 * j + 4)) & 15));
-      vv[j] = pack_bf16x2(vl + vs * float((vw >> (8 * j)) & 15), vl + vs * float((vw >> (8 * j + 4)) & 15));
+      for (int j = 0; j < 4; ++j) {
+        kk[j] = pack_bf16x2(kl + ks * float((kw >> (8 * j)) & 15), kl + ks * float((kw >> (8 * j + 4)) & 15));
+        vv[j] = pack_bf16x2(vl + vs * float((vw >> (8 * j)) & 15), vl + vs * float((vw >> (8 * j + 4)) & 15));
+      }
+      ko = make_uint4(kk[0], kk[1], kk[2], kk[3]);
+      vo = make_uint4(vv[0], vv[1], vv[2], vv[3]);
     }
-    ko = make_uint4(kk[0], kk[1], kk[2], kk[3]);
-    vo = make_uint4(vv[0], vv[1], vv[2], vv[3]);
+    const size_t at = (size_t(row0) * per + u) * 8;
+    *reinterpret_cast<uint4*>(k + at) = ko;
+    *reinterpret_cast<uint4*>(v + at) = vo;
   }
-  *reinterpret_cast<uint4*>(k + u * 8) = ko;
-  *reinterpret_cast<uint4*>(v + u * 8) = vo;
 }
 
 // ---------------------------------------------------------------------------
@@ -868,16 +861,16 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
   a.rows = rows; a.nq = nq; a.nkv = nkv; a.hd = hd; a.block_size = block_size; a.n_blocks = n_blocks;
   a.log2_theta = log2(theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Many rows: four to a block, with few threads each that go through the heads; few rows (a decode step): a block each whose
-  // threads have about a head's octet at once.
+  // Many rows: four to a block, a warp each that goes through the heads (8191 rows of 36 heads: 35.7 us; two warps a row and three heads at
+  // a time 37 to 48, by registers); few rows (a decode step): a block each whose threads have about a head's octet at once.
   const bool many = rows > 4 * sm_count();
-  const dim3 grid(many ? (rows + 3) / 4 : rows), block(256);
+  const dim3 grid(many ? (rows + 3) / 4 : rows), block(many ? 128 : 256);
   if (hd == 128) {
-    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<128, true, 4, 256, 1> : k_rope_kv_write_q4<128, true, 1, 256, 2>, grid, block, 0, st, a);
-    else launch_k(many ? k_rope_kv_write_q4<128, false, 4, 256, 3> : k_rope_kv_write_q4<128, false, 1, 256, 2>, grid, block, 0, st, a);
+    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<128, true, 4, 128, 1> : k_rope_kv_write_q4<128, true, 1, 256, 2>, grid, block, 0, st, a);
+    else launch_k(many ? k_rope_kv_write_q4<128, false, 4, 128, 2> : k_rope_kv_write_q4<128, false, 1, 256, 2>, grid, block, 0, st, a);
   } else {
-    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<64, true, 4, 256, 1> : k_rope_kv_write_q4<64, true, 1, 256, 2>, grid, block, 0, st, a);
-    else launch_k(many ? k_rope_kv_write_q4<64, false, 4, 256, 3> : k_rope_kv_write_q4<64, false, 1, 256, 2>, grid, block, 0, st, a);
+    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<64, true, 4, 128, 1> : k_rope_kv_write_q4<64, true, 1, 256, 2>, grid, block, 0, st, a);
+    else launch_k(many ? k_rope_kv_write_q4<64, false, 4, 128, 2> : k_rope_kv_write_q4<64, false, 1, 256, 2>, grid, block, 0, st, a);
   }
   KV4_LAUNCH_CHECK("rope_kv_write_q4");
   return 0;
@@ -886,11 +879,15 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
 extern "C" int bl_kv4_read(const void* cache, const int* slots, void* k, void* v, int rows, int nkv, int hd, int block_size,
                            int n_blocks, void* stream, char* err, size_t errlen) {
   if (q4_shape("the 4-bit cache", hd, nkv, block_size, n_blocks, err, errlen)) return -1;
-  const size_t units = size_t(rows) * nkv * (hd / 8);
-  if (units == 0) return 0;
-  launch_k(k_kv4_read, dim3(unsigned((units + 255) / 256)), dim3(256), 0, static_cast<cudaStream_t>(stream),
-           static_cast<const uint8_t*>(cache), slots, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), units, nkv,
-           hd, block_size, n_blocks);
+  if (rows < 0 || nkv < 1 || nkv > 1 << 20) {
+    set_err(err, errlen, "barlink: kv4_read: rows and KV heads out of range");
+    return -1;
+  }
+  if (rows == 0) return 0;
+  const int per = nkv * (hd / 8), block_rows = per >= 256 ? 1 : 256 / per;
+  launch_k(hd == 64 ? k_kv4_read<64> : k_kv4_read<128>, dim3((rows + block_rows - 1) / block_rows), dim3(256), 0, static_cast<cudaStream_t>(stream),
+           static_cast<const uint8_t*>(cache), slots, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), rows, block_rows, nkv,
+           block_size, n_blocks);
   KV4_LAUNCH_CHECK("kv4_read");
   return 0;
 }
