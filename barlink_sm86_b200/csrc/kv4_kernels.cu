@@ -426,35 +426,34 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
     }
   if (lo >= hi) return;
 
-  // ---- copies: lane l knows where tile l of the next 16 units lies ---------------------------------------------
+  // ---- copies: lane l knows where tile l of the next 16 units lies, and asks for it when its turn comes ------------
   const int count = hi - lo;
   Q4At ahead = seg;
-  int chunk = -1;
-  int where = -1;      // its number in the cache, below 0: none
-  uint32_t there = 0;  // bits 2 s, 2 s + 1: the tiles of stage s have a block
+  const uint8_t* from = nullptr;
+  uint32_t have = 0;  // bit l: that tile has a block
+  uint32_t gone = 0;  // bits 2 s, 2 s + 1: the tiles of stage s have none
   const uint32_t leader = elect_leader();
-  auto issue = [&](int i, int stage) {
-    if ((i >> 4) != chunk) {
-      chunk = i >> 4;
-      const int idx = lo + chunk * 16 + (lane >> 1);
-      where = -1;
+  auto issue = [&](int i, int stage) {  // (units in turn)
+    if ((i & 15) == 0) {
+      const int idx = lo + i + (lane >> 1);
+      int tile = -1;
       if (idx < hi) {
         q4_advance(a, ahead, idx);
         const int tok = (idx - ahead.start) * kQ4Unit + (lane & 1) * kQ4Tokens;
         if (tok < q4_context(a, ahead.b)) {
           const int page = tok / a.block_size, blk = a.tables[size_t(ahead.b) * a.max_blocks + page];
           if (blk >= 0 && blk < a.n_blocks)
-            where = (blk * a.nkv + ahead.h) * (a.block_size / kQ4Tokens) + (tok - page * a.block_size) / kQ4Tokens;
+            tile = (blk * a.nkv + ahead.h) * (a.block_size / kQ4Tokens) + (tok - page * a.block_size) / kQ4Tokens;
         }
       }
+      from = a.cache + size_t(max(tile, 0)) * TB;
+      have = __ballot_sync(kAll, tile >= 0);
     }
-    const int from = 2 * (i & 15);
-    const int t0 = __shfl_sync(kAll, where, from), t1 = __shfl_sync(kAll, where, from + 1);
-    const uint32_t has = (t0 >= 0 ? 1u : 0u) | (t1 >= 0 ? 2u : 0u), dst = ring + stage * 2 * TB;
-    there = (there & ~(3u << (2 * stage))) | has << (2 * stage);
-    mbar_expect_tx_warp(leader, bars + stage, TB * __popc(has));
-    if (t0 >= 0) bulk_load_warp(leader, dst, a.cache + size_t(t0) * TB, TB, smem_u32(bars + stage), kHintEvictFirst);
-    if (t1 >= 0) bulk_load_warp(leader, dst + TB, a.cache + size_t(t1) * TB, TB, smem_u32(bars + stage), kHintEvictFirst);
+    const uint32_t has = have >> (2 * (i & 15)) & 3u;
+    if (has != 3 || gone) gone = (gone & ~(3u << (2 * stage))) | (has ^ 3u) << (2 * stage);
+    mbar_expect_tx_warp(leader, bars + stage, TB * ((has & 1) + (has >> 1)));
+    const uint32_t mine = (lane >> 1) == (i & 15) && (have >> lane & 1);
+    bulk_load_warp(mine, ring + (stage * 2 + (lane & 1)) * TB, from, TB, smem_u32(bars + stage), kHintEvictFirst);
   };
   // (the queries first: behind the copies they would wait for what may be the whole cache)
   uint4 raw[NT][NA];
@@ -603,14 +602,14 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
         lds_words<NA>(tile + u * TB + q4_v_params(HD) + g * NA * 4, vs0[u]);
         lds_words<NA>(tile + u * TB + q4_v_params(HD) + (g + 8) * NA * 4, vs1[u]);
       }
-      const uint32_t has = there >> (2 * stage) & 3;
-      if (left < kQ4Unit || has != 3) {
+      const uint32_t no_block = gone >> (2 * stage) & 3u;
+      if (left < kQ4Unit || no_block) {
         // behind the last token, and where there is no block: whatever stands there (NaN too) stays out
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (16 * u + 8 * j + g >= left || !(has >> u & 1)) {
+            if (16 * u + 8 * j + g >= left || (no_block >> u & 1)) {
 #pragma unroll
               for (int n = 0; n < NT; ++n) c[u][n][2 * j] = c[u][n][2 * j + 1] = -INFINITY;
 #pragma unroll
