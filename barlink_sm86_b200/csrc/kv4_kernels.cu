@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
   };
   // (the queries first: behind the copies they would wait for what may be the whole cache)
   uint4 raw[NT][NA];
-  auto ask_queries = [&] {
+  auto ask_queries = [&](const Q4At& seg) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
         raw[n][ga] = 8 * n + g < G ? *reinterpret_cast<const uint4*>(a.q + size_t(seg.b) * a.q_stride + (size_t(seg.h) * G + 8 * n + g) * HD + 32 * ga + 8 * t)
                                    : make_uint4(0, 0, 0, 0);
   };
-  ask_queries();
+  ask_queries(seg);
 #pragma unroll 1
   for (int i = 0; i < STAGES; ++i)
     if (i < count) issue(i, i);
@@ -522,6 +522,13 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
       const float fac = fmaxf(__uint_as_float(uint32_t(min(ex + 10, 127) + 127) << 23) * a.scale_log2, 1.17549435e-38f);
       f[n][0] = __shfl_sync(kAll, fac, 8 * t);
       f[n][1] = __shfl_sync(kAll, fac, 8 * t + 4);
+    }
+    // the next pair's queries, where there are registers for them: behind this pair's copies they take long
+    constexpr bool AHEAD = NT == 1;
+    Q4At next = seg;
+    if (AHEAD && seg_end < count) {
+      q4_advance(a, next, lo + seg_end);
+      ask_queries(next);
     }
     float o[NT][2 * NA][4], vm[NT][NA][2], R[NT][2], l[NT][2];
 #pragma unroll
@@ -745,9 +752,11 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
       }
     if (begins && lane == 0)
       a.meta[size_t(seg.b) * a.nkv + seg.h] = make_int2(piece, whole ? 0 : (seg.start + seg.units - 1) / run - me + 1);
-    if (k < count) {
+    if constexpr (AHEAD) {
+      seg = next;
+    } else if (k < count) {
       q4_advance(a, seg, lo + k);
-      ask_queries();
+      ask_queries(seg);
     }
   }
   if (dead) {
