@@ -855,6 +855,11 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
     set_err(err, errlen, "barlink: rope_kv_write_q4 needs the QKV rows or slabs, positions, an output and, with slots, a cache");
     return -1;
   }
+  if (((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(slabs) | reinterpret_cast<uintptr_t>(bias) |
+        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache)) & 15) || (slab & 3)) {
+    set_err(err, errlen, "barlink: rope_kv_write_q4 needs tensors on 16-byte boundaries");
+    return -1;
+  }
   if (rows == 0) return 0;
   Q4Write a;
   a.qkv = static_cast<const __nv_bfloat16*>(qkv);
@@ -887,7 +892,7 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
 extern "C" int bl_kv4_read(const void* cache, const int* slots, void* k, void* v, int rows, int nkv, int hd, int block_size,
                            int n_blocks, void* stream, char* err, size_t errlen) {
   if (q4_shape("the 4-bit cache", hd, nkv, block_size, n_blocks, err, errlen)) return -1;
-  if (rows < 0 || nkv < 1 || nkv > 1 << 20) {
+  if (rows < 0 || rows > 1 << 30 || nkv < 1 || nkv > 1 << 20) {
     set_err(err, errlen, "barlink: kv4_read: rows and KV heads out of range");
     return -1;
   }
@@ -929,7 +934,15 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
     return -1;
   }
   if (batch == 0) return 0;
-  if (max_blocks < 1) return -1;
+  if (max_blocks < 1) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache needs a table");
+    return -1;
+  }
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) |
+        reinterpret_cast<uintptr_t>(ws)) & 15) || q_stride % 8) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache needs tensors and rows on 16-byte boundaries");
+    return -1;
+  }
   if (!(scale > 0.f) || scale > 3e38f) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs a positive scale");
     return -1;

@@ -234,40 +234,61 @@ __global__ void __launch_bounds__(256) k_layout_rows(const RequestLayout a) {
 // ---------------------------------------------------------------------------
 // token histories to count tables
 // ---------------------------------------------------------------------------
-// A cluster of blocks owns a row: empties its tables, if asked to, and counts its tokens behind the cluster's barrier.
+// Tokens added to tables that stand.
 constexpr int kCountThreads = 512;
-__device__ __forceinline__ void zero_words(uint32_t* p, size_t n, int who, int of) {
-  const size_t skip = min(n, size_t(-(reinterpret_cast<uintptr_t>(p) >> 2) & 3));  // to the next 16 bytes
-  if (size_t(who) < skip) p[who] = 0;
-  uint4* v = reinterpret_cast<uint4*>(p + skip);
-  const size_t nv = (n - skip) / 4;
-  for (size_t i = who; i < nv; i += of) v[i] = make_uint4(0, 0, 0, 0);
-  const size_t at = skip + nv * 4 + who;
-  if (at < n) p[at] = 0;
-}
 __global__ void __launch_bounds__(kCountThreads) k_count_tokens(const int* __restrict__ ids, const int* __restrict__ cu,
                                                                 const int* __restrict__ prompt, int* __restrict__ counts,
-                                                                uint32_t* __restrict__ seen, int n_ids, int vocab, int words, int reset) {
+                                                                uint32_t* __restrict__ seen, int n_ids, int vocab, int words) {
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x / cluster_nctarank(), who = cluster_ctarank() * kCountThreads + threadIdx.x, of = cluster_nctarank() * kCountThreads;
-  counts += size_t(row) * vocab;
-  seen += size_t(row) * words;
-  if (reset) {
-    zero_words(reinterpret_cast<uint32_t*>(counts), vocab, who, of);
-    zero_words(seen, words, who, of);
-    __threadfence();
-    __syncwarp();
-    cluster_sync_all();
-  }
+  const int row = blockIdx.y;
   const int lo = cu ? max(cu[row], 0) : row, hi = cu ? min(cu[row + 1], n_ids) : row + 1;
   const int p = prompt ? prompt[row] : 0;
-  for (int i = lo + who; i < hi; i += of) {
+  for (int i = lo + blockIdx.x * kCountThreads + threadIdx.x; i < hi; i += gridDim.x * kCountThreads) {
     const int id = ids[i];
     if (id < 0 || id >= vocab) continue;
-    atomicOr(seen + (id >> 5), 1u << (id & 31));
-    if (i - lo >= p) atomicAdd(counts + id, 1);
+    atomicOr(seen + size_t(row) * words + (id >> 5), 1u << (id & 31));
+    if (i - lo >= p) atomicAdd(counts + size_t(row) * vocab + id, 1);
   }
+}
+// Tables made anew: block (slice, row) counts the row's tokens of its slice of the vocabulary in shared memory and writes the slice, so
+// that the tables are written once and nobody waits for zeros.  64 x 152064: 9.4 us; zeros, a fence, then counting in global memory
+// 11; a fill of the 40 MB alone 6.
+constexpr int kCountSlice = 19456;  // tokens, a multiple of 32
+__global__ void __launch_bounds__(kCountThreads) k_count_anew(const int* __restrict__ ids, const int* __restrict__ cu,
+                                                              const int* __restrict__ prompt, int* __restrict__ counts,
+                                                              uint32_t* __restrict__ seen, int n_ids, int vocab, int words, int slice) {
+  extern __shared__ __align__(16) int s_slice[];  // counts from `pad` on, so that their 16-byte vectors are the table's; the bits
+  pdl_launch_dependents();
+  const int row = blockIdx.y, first = blockIdx.x * slice, n = min(slice, vocab - first), tid = threadIdx.x;
+  int* to = counts + size_t(row) * vocab + first;
+  const int pad = int((reinterpret_cast<uintptr_t>(to) >> 2) & 3);
+  int* s_count = s_slice + pad;
+  uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_slice + slice + 4);
+  for (int i = tid; i < (slice + 4 + slice / 32) / 4; i += kCountThreads) reinterpret_cast<int4*>(s_slice)[i] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  pdl_wait();
+  const int lo = cu ? max(cu[row], 0) : row, hi = cu ? min(cu[row + 1], n_ids) : row + 1;
+  const int p = prompt ? prompt[row] : 0;
+  for (int64_t i0 = lo + tid; i0 < hi; i0 += 4 * kCountThreads) {
+    int id[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) id[j] = i0 + j * kCountThreads < hi ? ids[i0 + j * kCountThreads] : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = id[j] - first;
+      if (id[j] < 0 || at < 0 || at >= n) continue;
+      atomicOr(s_seen + (at >> 5), 1u << (at & 31));
+      if (i0 + j * kCountThreads - lo >= p) atomicAdd(s_count + at, 1);
+    }
+  }
+  __syncthreads();
+  const int skip = min((4 - pad) & 3, n), nv = (n - skip) / 4;
+  if (tid < skip) to[tid] = s_count[tid];
+  for (int i = tid; i < nv; i += kCountThreads)
+    reinterpret_cast<int4*>(to + skip)[i] = reinterpret_cast<const int4*>(s_count + skip)[i];
+  for (int i = skip + 4 * nv + tid; i < n; i += kCountThreads) to[i] = s_count[i];
+  for (int i = tid; i < (n + 31) / 32; i += kCountThreads) seen[size_t(row) * words + first / 32 + i] = s_seen[i];
 }
 
 // ---------------------------------------------------------------------------
@@ -379,13 +400,14 @@ __device__ __forceinline__ void better(float& best, int& bi, float v, int i) {
 constexpr int kRulesThreads = 512;
 constexpr int kRulesShare = 8;    // blocks of a row at most
 constexpr int kRulesLap = 5;      // vectors that a thread takes at a time
+constexpr int kRulesList = 2 * kRulesLap * kRulesThreads;
 template <typename T, bool PICK>  // the arg max, or the logits under the rules
 __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a) {
   extern __shared__ uint32_t s_rules[];  // with biases: a bit per column that an entry names; the entries' columns and values
   __shared__ float s_v[kRulesThreads / 32];
   __shared__ int s_i[kRulesThreads / 32];
   __shared__ uint32_t s_all[kRulesShare][2];
-  __shared__ int2 s_list[kRulesLap * kRulesThreads];  // first column, bits of the tokens
+  __shared__ int2 s_list[kRulesList];  // first column, bits of the tokens
   __shared__ int s_listed;
   pdl_launch_dependents();
   const int share = cluster_nctarank(), rank = cluster_ctarank(), row = blockIdx.x / share, tid = threadIdx.x, lane = tid & 31;
@@ -488,10 +510,16 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
     }
     if (pen) {
       __syncthreads();
-      for (int e = tid; e < s_listed; e += kRulesThreads) seen_tokens(s_list[e].x, uint32_t(s_list[e].y));
-      __syncthreads();
-      if (tid == 0) s_listed = 0;
-      if (lap0 + U * lap < nvec) __syncthreads();
+      const int listed = s_listed;
+      const bool more = lap0 + U * lap < nvec;
+      __syncthreads();  // (all have read it)
+      if (more && listed <= kRulesList - U * kRulesThreads) continue;  // room for another lap's
+      for (int e = tid; e < listed; e += kRulesThreads) seen_tokens(s_list[e].x, uint32_t(s_list[e].y));
+      if (more) {
+        __syncthreads();
+        if (tid == 0) s_listed = 0;
+        __syncthreads();
+      }
     }
   }
   if (kept_at >= 0) {
@@ -573,9 +601,9 @@ using namespace bl;
 extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range,
                                int* cu, int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks,
                                int n_free, int tokens, int block_size, int rows_per_request, void* stream, char* err, size_t errlen) {
-  if (batch < 1 || batch > kLayoutMaxBatch || max_blocks < 1 || n_free < 1 || tokens < 0 || block_size < 1 ||
+  if (batch < 1 || batch > kLayoutMaxBatch || max_blocks < 1 || n_free < 1 || tokens < 0 || tokens > 1 << 30 || block_size < 1 ||
       rows_per_request < 0) {
-    set_err(err, errlen, "barlink: paged_layout takes 1 to %d requests, a table and a list of free blocks", kLayoutMaxBatch);
+    set_err(err, errlen, "barlink: paged_layout takes 1 to %d requests, up to 2^30 tokens, a table and a list of free blocks", kLayoutMaxBatch);
     return -1;
   }
   if (int64_t(n_free) * block_size > 0x7fffffffLL || int64_t(batch) * max_blocks > 0x7fffffffLL) {
@@ -611,13 +639,28 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int words = (vocab + 31) / 32;
-  // Eight blocks a row while the GPU holds them all at once; one where a step adds a token per row.
-  const int share = !cu && !reset ? 1 : rows <= 2 * sm_count() / 4 ? 8 : rows <= 2 * sm_count() ? 2 : 1;
-  const cudaError_t e = launch_cluster(k_count_tokens, dim3(unsigned(rows) * share), dim3(kCountThreads), 0, share, st, ids, cu, prompt_lens,
-                                       counts, static_cast<uint32_t*>(seen), n_ids, vocab, words, reset);
-  if (e != cudaSuccess) {
-    set_err(err, errlen, "barlink: count_tokens launch failed: %s", cudaGetErrorString(e));
+  if (rows > 65535) {
+    set_err(err, errlen, "barlink: count_tokens takes at most 65535 rows");
     return -1;
+  }
+  if (reset) {
+    // Slices as large as let two blocks share an SM, smaller ones while there are fewer than four for an SM: one row of 152064 in
+    // 8 and 32 slices 3.0 and 2.0 us, 64 rows 9.4 and 12.5.
+    const int want = 4 * sm_count() / rows, most = want < 1 ? 1 : want > 32 ? 32 : want;
+    const int even = ((vocab + most - 1) / most + 127) / 128 * 128, slice = even < 1024 ? 1024 : even < kCountSlice ? even : kCountSlice;
+    const int smem = (slice + 4 + slice / 32) * 4;
+    static bool attr[64] = {};
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k_count_anew), (kCountSlice + 4 + kCountSlice / 32) * 4, attr);
+    if (e != cudaSuccess) {
+      set_err(err, errlen, "barlink: count_tokens shared memory opt-in failed: %s", cudaGetErrorString(e));
+      return -1;
+    }
+    launch_k(k_count_anew, dim3((vocab + slice - 1) / slice, rows), dim3(kCountThreads), smem, st, ids, cu, prompt_lens, counts,
+             static_cast<uint32_t*>(seen), n_ids, vocab, words, slice);
+  } else {
+    const int x = cu ? (n_ids / rows + kCountThreads - 1) / kCountThreads : 1;
+    launch_k(k_count_tokens, dim3(x < 1 ? 1 : x > 64 ? 64 : x, rows), dim3(kCountThreads), 0, st, ids, cu, prompt_lens, counts,
+             static_cast<uint32_t*>(seen), n_ids, vocab, words);
   }
   SERVE_LAUNCH_CHECK("count_tokens");
   return 0;
@@ -653,7 +696,7 @@ extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, siz
   const auto kernel = r->fp32 ? pick ? k_logit_rules<float, true> : k_logit_rules<float, false>
                               : pick ? k_logit_rules<__nv_bfloat16, true> : k_logit_rules<__nv_bfloat16, false>;
   static bool attr[4][64] = {};
-  cudaError_t e = smem > 24 * 1024 ? allow_smem(reinterpret_cast<const void*>(kernel), 180 * 1024, attr[2 * (r->fp32 ? 1 : 0) + pick]) : cudaSuccess;
+  cudaError_t e = smem > 4 * 1024 ? allow_smem(reinterpret_cast<const void*>(kernel), 180 * 1024, attr[2 * (r->fp32 ? 1 : 0) + pick]) : cudaSuccess;
   if (e == cudaSuccess)
     e = launch_cluster(kernel, dim3(unsigned(r->rows) * share), dim3(kRulesThreads), smem, share, static_cast<cudaStream_t>(stream), a);
   if (e != cudaSuccess) {

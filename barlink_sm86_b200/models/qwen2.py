@@ -640,7 +640,10 @@ class DecodeEngine:
             raise ValueError("kv_bits must be 4 or 16")
         if kv_bits == 16 and (block_size != 16 or n_blocks is not None):
             raise ValueError("block_size and n_blocks are for the 4-bit cache")
+        if rules is not None and any(t is not None and t.shape[0] != batch for t in rules._args()):
+            raise ValueError("rules must have one row per request")
         self.kv_bits, self.rules = kv_bits, rules
+        self.counted = rules is not None and rules.counts is not None  # (a mask or biases alone go by no counts)
         if kv_bits == 4:
             self.cache = PagedKV4(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, block_size, n_blocks)
             self.new_lens = torch.zeros(batch, dtype=torch.int32, device=dev)  # 1: the request takes part in steps
@@ -710,7 +713,7 @@ class DecodeEngine:
         new = torch.tensor(lens, dtype=torch.int32).to(dev)
         lay = self._lay_out(new, ids.numel())
         ids = ids.to(device=dev, dtype=torch.int32)
-        if self.rules is not None:
+        if self.counted:
             fresh = new > 0
             self.rules.counts.masked_fill_(fresh[:, None], 0)
             self.rules.seen.masked_fill_(fresh[:, None], 0)
@@ -733,7 +736,7 @@ class DecodeEngine:
         last[at] = torch.cat(lasts, 0)
         nxt = self.m.next_tokens(last, rules=self.rules)
         out[at] = nxt[at]
-        if self.rules is not None:
+        if self.counted:
             ops.count_tokens(self.rules, torch.where(new > 0, nxt, -1))
         self.new_lens.masked_fill_(new > 0, 1)
         for r in rows:
@@ -772,11 +775,11 @@ class DecodeEngine:
             hidden = self.m.prefill(part, self.cache, seq_offset=b0)
             lasts.append(hidden.view(part.shape[0], seq, -1)[:, -1])
         last = torch.cat(lasts, 0).contiguous()
-        if self.rules is not None:
+        if self.counted:
             cu = torch.arange(0, (self.batch + 1) * seq, seq, device=ids_2d.device, dtype=torch.int32)
             ops.count_tokens(self.rules, ids_2d.reshape(-1).to(torch.int32), cu, torch.full_like(cu[1:], seq), reset=True)
         nxt = self.m.next_tokens(last, rules=self.rules)
-        if self.rules is not None:
+        if self.counted:
             ops.count_tokens(self.rules, nxt)
         self.set_context(seq)
         return nxt
@@ -789,7 +792,7 @@ class DecodeEngine:
                              self.layout, rows_per_request=1)
         hidden = self.m.decode_hidden(self.ids, self.positions, self.slots, self.ctx_lens, c, self.attn_splits)
         self.m.next_tokens(hidden, self.out_ids, rules=self.rules)
-        if self.rules is not None:
+        if self.counted:
             ops.count_tokens(self.rules, self.out_ids if self.kv_bits != 4 else torch.where(self.new_lens > 0, self.out_ids, -1))
 
     def _step_body(self):
@@ -833,7 +836,7 @@ class DecodeEngine:
         state = [self.positions, self.ids]
         if self.kv_bits == 4:
             state += [self.slots, self.ctx_lens, self.cache.block_tables, self.cache.free_list, self.cache.free_range]
-        if self.rules is not None:
+        if self.counted:
             state += [self.rules.counts, self.rules.seen]
         saved = [t.clone() for t in state]
 

@@ -485,6 +485,9 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
         _count(2 if tokens > 2048 else 1)
         return PagedLayout(*_C().paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size,
                                               rows_per_request, None if into is None else list(into)))
+    if (block_tables.dim() != 2 or past_lens.shape != new_lens.shape or block_tables.shape[0] != new_lens.numel() or block_size < 1 or tokens < 0
+            or free_range.numel() != 3 or not free_list.numel() or rows_per_request < 0):
+        raise ValueError("paged_layout: one new and one past length and a row of the table per request, a list and a range of free blocks")
     r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request)
     if into is None:
         return PagedLayout(*r)

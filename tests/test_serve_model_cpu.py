@@ -109,6 +109,22 @@ def test_rules_in_a_run(kv_bits):
     assert int(rules.counts.sum()) == 2
 
 
+def test_rules_without_counts():
+    m = _model()
+    mask = torch.zeros(2, 16, dtype=torch.int32)
+    mask[:, 2] = 1 << 7
+    for kv_bits in (16, 4):
+        eng = DecodeEngine(m, 2, 60, kv_bits=kv_bits, rules=ops.LogitRules(mask=mask, vocab=500))
+        eng.ids.copy_(eng.prefill(torch.stack(_prompts([9, 9]))))
+        assert eng.step().tolist() == [71, 71]
+    # nothing allowed: no token, and the run goes on
+    eng = DecodeEngine(m, 2, 60, kv_bits=4, rules=ops.LogitRules(mask=torch.zeros_like(mask), vocab=500))
+    out = eng.prefill(torch.stack(_prompts([9, 9])))
+    assert out.tolist() == [-1, -1]
+    eng.ids.copy_(out)
+    assert eng.step().tolist() == [-1, -1]
+
+
 def test_blocks_run_out():
     m = _model()
     eng = DecodeEngine(m, 2, 64, kv_bits=4, n_blocks=3)
@@ -126,6 +142,11 @@ def test_refusals():
         DecodeEngine(m, 1, 32, kv_bits=8)
     with pytest.raises(ValueError):
         DecodeEngine(m, 1, 32, n_blocks=3)
+    with pytest.raises(ValueError):
+        DecodeEngine(m, 2, 32, rules=ops.LogitRules.empty(3, 500, "cpu"))
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.paged_layout(i, i[:1], i.view(2, 1), i, torch.zeros(3, dtype=torch.int32), 2)
     e16, e4 = DecodeEngine(m, 2, 32), DecodeEngine(m, 2, 32, kv_bits=4)
     p = _prompts([4])[0]
     for call in (lambda: e16.start(p, [4, 0]), lambda: e16.finish([0]), lambda: e4.finish([2]), lambda: e4.start(p, [4]),
