@@ -24,7 +24,6 @@ namespace bl {
 // ---------------------------------------------------------------------------
 // block tables, row offsets, positions and slots
 // ---------------------------------------------------------------------------
-constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutMaxBatch = 8192;
 constexpr int kLayoutAlone = 2048;  // rows up to which the one block writes them itself
 
@@ -40,6 +39,7 @@ struct RequestLayout {
 };
 
 // exclusive block-wide scan of three ints per thread; total in tot
+template <int T>
 __device__ __forceinline__ void block_scan3(int (&v)[3], int (&tot)[3], int (*s_warp)[3]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int in[3] = {v[0], v[1], v[2]};
@@ -56,7 +56,7 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&tot)[3], int (*s_
   __syncthreads();
 #pragma unroll
   for (int c = 0; c < 3; ++c) {
-    int w = lane < kLayoutThreads / 32 ? s_warp[lane][c] : 0;
+    int w = lane < T / 32 ? s_warp[lane][c] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, w, o);
@@ -87,11 +87,12 @@ __device__ __forceinline__ int pages_of(int64_t tokens, int block_size, int widt
 
 // One block.  Three running sums over the requests (tokens, fresh blocks, blocks given back) stay in shared memory;
 // every token and every fresh block then finds its request by bisection.
-__global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLayout a) {
+template <int T>
+__global__ void __launch_bounds__(T) k_paged_layout(const RequestLayout a) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ int s_dyn[];
-  __shared__ int s_warp[kLayoutThreads / 32][3];
+  __shared__ int s_warp[T / 32][3];
   __shared__ int s_ended;
   const int B = a.batch, bs = a.block_size, tid = threadIdx.x;
   int* s_cu = s_dyn;               // [B + 1]
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
   const int head = a.range[0], free_n = min(max(a.range[1], 0), a.cap);
   if (tid == 0) s_ended = 0;
   __syncthreads();
-  for (int b = tid; b < B; b += kLayoutThreads) {
+  for (int b = tid; b < B; b += T) {
     const int n = a.new_lens[b], past = max(a.past_lens[b], 0);
     const int had = pages_of(past, bs, a.width);
     s_cu[b] = max(n, 0);
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
   }
   __syncthreads();
   const int ended = s_ended, warp = tid >> 5, lane = tid & 31;
-  for (int e = warp; e < ended; e += kLayoutThreads / 32) {
+  for (int e = warp; e < ended; e += T / 32) {
     const int b = s_list[e];
     int n = 0;
     for (int p = lane; p < s_had[b]; p += 32) n += a.tables[size_t(b) * a.width + p] >= 0;
@@ -123,14 +124,14 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
     if (lane == 0) s_back[b] = n;
   }
   __syncthreads();
-  const int per = (B + kLayoutThreads - 1) / kLayoutThreads, b0 = min(tid * per, B), b1 = min(b0 + per, B);
+  const int per = (B + T - 1) / T, b0 = min(tid * per, B), b1 = min(b0 + per, B);
   int sum[3] = {0, 0, 0}, tot[3];
   for (int b = b0; b < b1; ++b) {
     sum[0] += s_cu[b];
     sum[1] += s_fresh[b];
     sum[2] += s_back[b];
   }
-  block_scan3(sum, tot, s_warp);
+  block_scan3<T>(sum, tot, s_warp);
   for (int b = b0; b < b1; ++b) {
     const int n0 = s_cu[b], n1 = s_fresh[b], n2 = s_back[b];
     a.cu[b] = s_cu[b] = sum[0];
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
   __syncthreads();
   auto ring_at = [&](int i) { return int((int64_t(head) + i) % a.cap); };
   // blocks that come back go behind the free ones, in the order of requests and pages
-  for (int e = warp; e < ended; e += kLayoutThreads / 32) {
+  for (int e = warp; e < ended; e += T / 32) {
     const int b = s_list[e];
     int at = free_n + s_back[b];
     for (int p0 = 0; p0 < s_had[b]; p0 += 32) {
@@ -164,12 +165,12 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
       at += __popc(m);
     }
   }
-  for (int j = tid; j < tot[1]; j += kLayoutThreads) {
+  for (int j = tid; j < tot[1]; j += T) {
     const int b = owner_of(s_fresh, B, j);
     a.tables[size_t(b) * a.width + s_had[b] + j - s_fresh[b]] = j < free_n ? a.ring[ring_at(j)] : -1;
   }
   if (a.tokens > kLayoutAlone) return;  // k_layout_rows does the rest
-  for (int row = tid; row < a.tokens; row += kLayoutThreads) {
+  for (int row = tid; row < a.tokens; row += T) {
     int pos = 0, slot = -1, b = -1, i = 0;  // the i-th token of request b
     if (a.per > 0) {
       b = row / a.per;
@@ -193,31 +194,34 @@ __global__ void __launch_bounds__(kLayoutThreads) k_paged_layout(const RequestLa
   }
 }
 
-// The rows of many tokens, behind k_paged_layout: four rows a thread, the first by bisection, the others by going on.
+// The rows of many tokens, behind k_paged_layout: four rows a thread, the first by bisection of the offsets in shared memory, the others by
+// going on.
 __global__ void __launch_bounds__(256) k_layout_rows(const RequestLayout a) {
+  extern __shared__ int s_dyn[];  // [batch + 1] row offsets, where the rows are packed
   pdl_launch_dependents();
   pdl_wait();
   const int row0 = (blockIdx.x * 256 + threadIdx.x) * 4, bs = a.block_size;
+  if (a.per == 0) {
+    for (int b = threadIdx.x; b <= a.batch; b += 256) s_dyn[b] = a.cu[b];
+    __syncthreads();
+  }
   if (row0 >= a.tokens) return;
   int pos[4] = {0, 0, 0, 0}, slot[4] = {-1, -1, -1, -1};
-  const int total = a.cu[a.batch];
-  if (a.per > 0 || row0 < total) {
-    int b = a.per > 0 ? row0 / a.per : owner_of(a.cu, a.batch, row0);
+  int b = a.per > 0 ? row0 / a.per : row0 < s_dyn[a.batch] ? owner_of(s_dyn, a.batch, row0) : a.batch;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = row0 + k;
-      if (a.per > 0) b = row / a.per;
-      else
-        while (b < a.batch && row >= a.cu[b + 1]) ++b;
-      if (b >= a.batch) break;
-      const int first = a.cu[b], n = a.cu[b + 1] - first, i = row - (a.per > 0 ? b * a.per : first);
-      if (i >= n) continue;
-      pos[k] = a.ctx_lens[b] - n + i;
-      const int page = pos[k] / bs;
-      if (pos[k] >= 0 && page < a.width) {
-        const int id = a.tables[size_t(b) * a.width + page];
-        if (id >= 0) slot[k] = id * bs + pos[k] % bs;
-      }
+  for (int k = 0; k < 4; ++k) {
+    const int row = row0 + k;
+    if (a.per > 0) b = row / a.per;
+    else
+      while (b < a.batch && row >= s_dyn[b + 1]) ++b;
+    if (b >= a.batch) break;
+    const int first = a.per > 0 ? a.cu[b] : s_dyn[b], n = (a.per > 0 ? a.cu[b + 1] : s_dyn[b + 1]) - first, i = row - (a.per > 0 ? b * a.per : first);
+    if (i >= n) continue;
+    pos[k] = a.ctx_lens[b] - n + i;
+    const int page = pos[k] / bs;
+    if (pos[k] >= 0 && page < a.width) {
+      const int id = a.tables[size_t(b) * a.width + page];
+      if (id >= 0) slot[k] = id * bs + pos[k] % bs;
     }
   }
   if (row0 + 4 <= a.tokens && ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots)) & 15) == 0) {
@@ -616,16 +620,18 @@ extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* b
   a.batch = batch; a.width = max_blocks; a.cap = n_free; a.tokens = tokens; a.block_size = block_size; a.per = rows_per_request;
   const int smem = int((size_t(batch) * 6 + 2) * sizeof(int));
   static bool attr[64] = {};
-  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k_paged_layout), (kLayoutMaxBatch * 6 + 2) * int(sizeof(int)), attr);
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k_paged_layout<1024>), (kLayoutMaxBatch * 6 + 2) * int(sizeof(int)), attr);
   if (e != cudaSuccess) {
     set_err(err, errlen, "barlink: paged_layout shared memory opt-in failed: %s", cudaGetErrorString(e));
     return -1;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  launch_k(k_paged_layout, dim3(1), dim3(kLayoutThreads), smem, st, a);
+  // (a decode step: a block whose barriers are cheap)
+  const bool few = batch <= 256 && tokens <= 512;
+  launch_k(few ? k_paged_layout<256> : k_paged_layout<1024>, dim3(1), dim3(few ? 256 : 1024), smem, st, a);
   SERVE_LAUNCH_CHECK("paged_layout");
   if (tokens > kLayoutAlone) {
-    launch_k(k_layout_rows, dim3((tokens + 1023) / 1024), dim3(256), 0, st, a);
+    launch_k(k_layout_rows, dim3((tokens + 1023) / 1024), dim3(256), rows_per_request > 0 ? 0 : size_t(batch + 1) * sizeof(int), st, a);
     SERVE_LAUNCH_CHECK("layout_rows");
   }
   return 0;
