@@ -394,24 +394,32 @@ __device__ __forceinline__ void better(float& best, int& bi, float v, int i) {
   }
 }
 
+// the same over a warp, as integers in the numbers' order (none of them NaN; -0 and 0 are equal)
+__device__ __forceinline__ void warp_best(float& best, int& bi) {
+  const uint32_t b = __float_as_uint(best + 0.f), key = b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+  const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+  bi = __reduce_min_sync(0xffffffffu, key == top ? bi : 0x7fffffff);
+  best = __uint_as_float(top ^ (top >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
 // A cluster of blocks shares a row.  Most tokens carry no rule but the mask, and those that do lie close together (frequent tokens
 // have low ids), so there are two passes: the first takes eight neighbouring logits to a thread, 16 bytes of bf16, several such
-// vectors on their way at a time, with a byte of each bit table; it lists the vectors in which a token was seen, and leaves those
-// tokens and the ones with a bias aside.  The second gives a listed vector to a thread.  The bias entries come last, one to a thread.  Of the maximum the
+// vectors on their way at a time, with a byte of each bit table; it lists the tokens that were seen, and leaves them
+// and the ones with a bias aside.  The second gives a listed token to a thread, and a bias entry.  Of the maximum the
 // first pass keeps the vector, and looks for the place in it at the end.  Each operation is rounded by itself (no fused multiply-add):
 // the values are the formula's to the bit.  The blocks' maxima meet in the first block's shared memory.  Measured, 64 x 152064,
 // us: one pass that branches into the penalties for every vector with a seen token 30; the seen words dealt out to warps 20.
 constexpr int kRulesThreads = 512;
 constexpr int kRulesShare = 8;    // blocks of a row at most
 constexpr int kRulesLap = 5;      // vectors that a thread takes at a time
-constexpr int kRulesList = 2 * kRulesLap * kRulesThreads;
+constexpr int kRulesList = 6144;  // seen tokens of a block that are put off; what is beyond is dealt with on the spot
 template <typename T, bool PICK>  // the arg max, or the logits under the rules
 __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a) {
   extern __shared__ uint32_t s_rules[];  // with biases: a bit per column that an entry names; the entries' columns and values
   __shared__ float s_v[kRulesThreads / 32];
   __shared__ int s_i[kRulesThreads / 32];
   __shared__ uint32_t s_all[kRulesShare][2];
-  __shared__ int2 s_list[kRulesList];  // first column, bits of the tokens
+  __shared__ int s_list[kRulesList];  // columns
   __shared__ int s_listed;
   pdl_launch_dependents();
   const int share = cluster_nctarank(), rank = cluster_ctarank(), row = blockIdx.x / share, tid = threadIdx.x, lane = tid & 31;
@@ -447,21 +455,10 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
   };
   float best = -INFINITY;
   int bi = 0x7fffffff;
-  auto seen_tokens = [&](int i, uint32_t bits) {
-    float x[8];
-    int c[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = bits >> j & 1 ? to_float<T>(in[i + j]) : 0.f;
-      c[j] = bits >> j & 1 ? counts[i + j] : 0;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (bits >> j & 1) {
-        x[j] = penalised(x[j], c[j]);
-        if (PICK) better(best, bi, x[j], i + j + a.offset);
-        else out[i + j] = from_float<T>(x[j]);
-      }
+  auto seen_token = [&](int i) {
+    const float x = penalised(to_float<T>(in[i]), counts[i]);
+    if (PICK) better(best, bi, x, i + a.offset);
+    else out[i] = from_float<T>(x);
   };
   // vectors from the row's first 16-byte boundary on, as far as the vocabulary goes; the few columns around them one by one
   const int known = int(max(min(int64_t(a.n), int64_t(a.vocab) - a.offset), int64_t(0)));
@@ -495,13 +492,20 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
         mine &= ~named;
         aside |= named;
       }
-      if (mine) s_list[atomicAdd(&s_listed, 1)] = make_int2(i, int(mine));
       x[u].keep(PICK ? ok & ~aside : ok);
       if (!PICK) {
         if (vout) x[u].store(out + i);
         else
 #pragma unroll
           for (int j = 0; j < 8; ++j) out[i + j] = from_float<T>(x[u].get(j));
+      }
+      if (mine) {  // (behind the store, which has the token as it was)
+        int at = atomicAdd(&s_listed, __popc(mine));
+#pragma unroll 1
+        for (; mine; mine &= mine - 1, ++at) {
+          if (at < kRulesList) s_list[at] = i + __ffs(mine) - 1;
+          else seen_token(i + __ffs(mine) - 1);
+        }
       }
       if (PICK) {
         const float m = x[u].top();
@@ -512,19 +516,6 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
         }
       }
     }
-    if (pen) {
-      __syncthreads();
-      const int listed = s_listed;
-      const bool more = lap0 + U * lap < nvec;
-      __syncthreads();  // (all have read it)
-      if (more && listed <= kRulesList - U * kRulesThreads) continue;  // room for another lap's
-      for (int e = tid; e < listed; e += kRulesThreads) seen_tokens(s_list[e].x, uint32_t(s_list[e].y));
-      if (more) {
-        __syncthreads();
-        if (tid == 0) s_listed = 0;
-        __syncthreads();
-      }
-    }
   }
   if (kept_at >= 0) {
     int at = 0;
@@ -533,6 +524,8 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
       if (kept.get(j) == kept_top) at = j;
     better(best, bi, kept_top, kept_at + at + a.offset);
   }
+  __syncthreads();
+  for (int e = tid, listed = min(s_listed, kRulesList); e < listed; e += kRulesThreads) seen_token(s_list[e]);
   const int tail = skip + 8 * nvec;
   for (int e = rank * kRulesThreads + tid; e < skip + a.n - tail; e += lap) {
     const int i = e < skip ? e : tail + e - skip, id = i + a.offset;
@@ -550,7 +543,8 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
     __syncwarp();
     cluster_sync_all();
   }
-  for (int j = rank * kRulesThreads + tid; j < a.n_bias; j += lap) {
+  // (from the last warp on: the first ones have the list)
+  for (int j = rank * kRulesThreads + kRulesThreads - 1 - tid; j < a.n_bias; j += lap) {
     const int col = s_col[j], id = col + a.offset;
     bool go = col >= 0;
     for (int e = 0; go && e < j; ++e) go = s_col[e] != col;  // the first entry of a token adds them all
@@ -568,8 +562,7 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
   }
   if (!PICK) return;
   __syncwarp();
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) better(best, bi, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, bi, o));
+  warp_best(best, bi);
   if (lane == 0) {
     s_v[tid >> 5] = best;
     s_i[tid >> 5] = bi;
@@ -578,8 +571,7 @@ __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a)
   if (tid < 32) {
     best = tid < kRulesThreads / 32 ? s_v[tid] : -INFINITY;
     bi = tid < kRulesThreads / 32 ? s_i[tid] : 0x7fffffff;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) better(best, bi, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, bi, o));
+    warp_best(best, bi);
     if (tid == 0) {
       const uint32_t to = map_to_cta(smem_u32(&s_all[rank][0]), 0);
       st_cluster_u32(to, __float_as_uint(best));

@@ -204,14 +204,35 @@ def test_rules_on_a_shard(offset, n):
     assert torch.equal(ops.logits_process(x, r, offset), ops.logits_process(xg, g, offset).cpu())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rules_where_all_is_seen(dtype):
+    """More seen tokens than a block puts off."""
+    rows, vocab = 300, 9001
+    r = _rules(40, rows, vocab, 2, True, hist=20)
+    r.seen.fill_(-1)
+    r.counts[:, ::3] = 2
+    x = (3 * torch.randn(rows, vocab, generator=_g(41))).to(dtype)
+    g, xg = _to_gpu(r), x.cuda()
+    want = ops.logits_process(x, r)
+    for a, b in zip(ops.logits_argmax(x, r), ops.logits_argmax(xg, g)):
+        assert torch.equal(a, b.cpu())
+    assert torch.equal(want, ops.logits_process(xg, g).cpu())
+    assert torch.equal(want, ops.logits_process(xg, g, out=xg).cpu())
+
+
 def test_ties_and_empty_rows():
     x = torch.zeros(3, 5000, dtype=torch.bfloat16, device="cuda")
     x[1, 4321] = x[1, 17] = 2.0
     x[2] = -math.inf
+    x[0, 5] = -0.0
     idx, val = ops.logits_argmax(x, ops.LogitRules())
     assert idx.tolist() == [0, 17, -1] and val.tolist() == [0.0, 2.0, -math.inf]
     x[2, 4999] = math.inf
     assert ops.logits_argmax(x, ops.LogitRules())[0].tolist() == [0, 17, 4999]
+    # -0 and 0 are equal, wherever they stand
+    y = torch.full((1, 152064), -1.0, device="cuda")
+    y[0, 100], y[0, 90000] = -0.0, 0.0
+    assert ops.logits_argmax(y, ops.LogitRules())[0].tolist() == [100]
     # one mask for all rows
     mask = torch.zeros(1, 157, dtype=torch.int32, device="cuda")
     mask[0, 135] = 1 << 1 | 1 << 2
