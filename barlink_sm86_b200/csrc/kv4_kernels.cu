@@ -363,9 +363,14 @@ __device__ __forceinline__ void q4_advance(const Q4Attn& a, Q4At& p, int idx) {
   }
 }
 
-template <int HD, int STAGES>
+// The tensor core cuts its sums off, toward 0, and they grow with every unit while a mean over many tokens is small: 4.2 million tokens,
+// 111 units a warp, were off by 1.0e-3 of the result's norm beside its rounding.  So they are put aside every kQ4Aside units, and
+// added there by rounded additions: two units of the last place of a sum, however long the run.
+constexpr int kQ4Aside = 32;
+
+template <int HD, int NT, int STAGES>
 constexpr int q4_smem_bytes() {
-  return kQ4Warps * STAGES * (2 * q4_tile_bytes(HD) + 8);
+  return kQ4Warps * (STAGES * (2 * q4_tile_bytes(HD) + 8) + NT * HD * 8 * 4);
 }
 
 template <int HD, int NT, int STAGES>
@@ -378,6 +383,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kQ4Warps * STAGES * 2 * TB) + warp * STAGES;
   const uint32_t ring = smem_u32(smem) + warp * STAGES * 2 * TB;
+  // [NT * 2 NA * 4][lane]
+  float* aside = reinterpret_cast<float*>(smem + kQ4Warps * STAGES * (2 * TB + 8)) + warp * (NT * HD * 8) + lane;
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
@@ -541,6 +548,16 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
       l[n][0] = l[n][1] = 0.f;
     }
 
+    int fresh = 0;         // units in o
+    bool put = false;      // sums stand aside
+    auto each_sum = [&](auto&& f) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2 * NA; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f(o[n][i][j], aside[((n * 2 * NA + i) * 4 + j) * 32]);
+    };
 #pragma unroll 1
     for (; k < seg_end; ++k) {
       if (!mbar_wait_bounded_warp(bars + stage, phase, &s_abort[warp])) {
@@ -676,11 +693,19 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
               o[n][i][j] *= al;
               o[n][i][2 + j] *= al;
             }
+            if (put) {
+#pragma unroll
+              for (int i = 0; i < 2 * NA; ++i) {
+                aside[((n * 2 * NA + i) * 4 + j) * 32] *= al;
+                aside[((n * 2 * NA + i) * 4 + 2 + j) * 32] *= al;
+              }
+            }
           }
         weigh();
       }
-      // ---- values: p times step as the columns' operand, p times low beside it.  The rows g of a product take a byte's two codes together,
-      // low + 16 high, the rows g + 8 the high one: one instruction less for a word, and the difference is taken at the end ----
+      // ---- values: p times step as the columns' operand, p times low beside it.  The rows g of a product take a byte's lower code, the
+      // rows g + 8 the two together, lower + 16 upper: one instruction less for a word, and the difference is taken at the end (of the
+      // two sums and not of the lower code's: what the tensor core cuts off its sums would come out sixteen times as large) ----
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t w0[NA], w1[NA], pb[NT][NA][2];
@@ -707,10 +732,18 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
           const uint32_t v0 = __byte_perm(w0[ga], 0, 0x4341), v1 = __byte_perm(w1[ga], 0, 0x4341);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x00ff00ffu, w0[ga] & 0x00f000f0u, w1[ga] & 0x00ff00ffu, w1[ga] & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
-            q4_mma_f16(o[n][2 * ga + 1], v0, v0 & 0x00f000f0u, v1, v1 & 0x00f000f0u, pb[n][ga][0], pb[n][ga][1]);
+            q4_mma_f16(o[n][2 * ga], w0[ga] & 0x000f000fu, w0[ga] & 0x00ff00ffu, w1[ga] & 0x000f000fu, w1[ga] & 0x00ff00ffu, pb[n][ga][0], pb[n][ga][1]);
+            q4_mma_f16(o[n][2 * ga + 1], v0 & 0x000f000fu, v0, v1 & 0x000f000fu, v1, pb[n][ga][0], pb[n][ga][1]);
           }
         }
+      }
+      if (++fresh == kQ4Aside) {
+        each_sum([&](float& sum, float& there) {
+          there = put ? there + sum : sum;
+          sum = 0.f;
+        });
+        fresh = 0;
+        put = true;
       }
       __syncwarp();  // all lanes have read the stage that the next copies fill
       if (k + STAGES < count) issue(k + STAGES, stage);
@@ -721,6 +754,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
     }
     if (dead) break;
 
+    if (put) each_sum([&](float& sum, float& there) { sum += there; });
     // ---- out: the whole pair, or a piece of it ---------------------------------------------------------
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -739,8 +773,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
 #pragma unroll
         for (int i = 0; i < NA; ++i) {  // 2^24, and the 16 of the odd dims
           const float *o0 = o[n][2 * i], *o1 = o[n][2 * i + 1], add = vm[n][i][j];
-          const float v0 = fmaf(o0[j] - o0[2 + j], 16777216.f, add) * inv, v1 = fmaf(o0[2 + j], 1048576.f, add) * inv,
-                      v2 = fmaf(o1[j] - o1[2 + j], 16777216.f, add) * inv, v3 = fmaf(o1[2 + j], 1048576.f, add) * inv;
+          const float v0 = fmaf(o0[j], 16777216.f, add) * inv, v1 = fmaf(o0[2 + j] - o0[j], 1048576.f, add) * inv,
+                      v2 = fmaf(o1[j], 16777216.f, add) * inv, v3 = fmaf(o1[2 + j] - o1[j], 1048576.f, add) * inv;
           const int d = 4 * (8 * i + g);
           if (whole)
             *reinterpret_cast<uint2*>(a.out + (size_t(seg.b) * a.nq + size_t(seg.h) * G + head) * HD + d) =
@@ -974,11 +1008,11 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   };
   cudaError_t e;
   if (hd == 128)
-    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[0])
-                : go(k_paged_attn_q4<128, 2, 4>, k_q4_merge<128>, q4_smem_bytes<128, 4>(), attr[1]);
+    e = nt == 1 ? go(k_paged_attn_q4<128, 1, 4>, k_q4_merge<128>, q4_smem_bytes<128, 1, 4>(), attr[0])
+                : go(k_paged_attn_q4<128, 2, 3>, k_q4_merge<128>, q4_smem_bytes<128, 2, 3>(), attr[1]);
   else
-    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 4>, k_q4_merge<64>, q4_smem_bytes<64, 4>(), attr[2])
-                : go(k_paged_attn_q4<64, 2, 4>, k_q4_merge<64>, q4_smem_bytes<64, 4>(), attr[3]);
+    e = nt == 1 ? go(k_paged_attn_q4<64, 1, 4>, k_q4_merge<64>, q4_smem_bytes<64, 1, 4>(), attr[2])
+                : go(k_paged_attn_q4<64, 2, 4>, k_q4_merge<64>, q4_smem_bytes<64, 2, 4>(), attr[3]);
   if (e != cudaSuccess) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache could not be launched: %s", cudaGetErrorString(e));
     return -1;

@@ -223,6 +223,27 @@ def test_attention_long_and_uneven(nq, nkv, hd, block, lens):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("repeat", [1, 500, 16384])
+@pytest.mark.parametrize("nq,hd", [(7, 128), (12, 64)])
+def test_attention_of_very_long_contexts(repeat, nq, hd):
+    """The same 1024 tokens over and over (the table names their blocks again): the result does not change, however long the sums.
+    Means over many tokens are small beside the values, so sums must not lose their last places: of the result's norm at most the
+    rounding to bf16 (2^-8 / sqrt 3 of a binade, 1.3 being the least root mean square in one: 1.74e-3), and p step in fp16 (2^-12 of terms
+    of twice a value's deviation, 1024 of them: 6e-4 of results of 0.02)."""
+    n = 1024
+    kv = _randn(95, n, 2, hd).bfloat16()
+    cache = ops.kv4_cache(n // 16, 1, hd)
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    ops.rope_kv_write_q4(kv.view(n, -1), torch.zeros_like(slots), slots, cache, 0, 1, hd, 16, 1e6)
+    k, v = (t[:, 0].double() for t in ref.kv4_values(cache.cpu(), slots.cpu(), hd, 16))
+    q = 0.1 * _randn(96, 1, nq * hd).bfloat16()
+    want = torch.softmax(q.double().cpu().view(nq, hd) @ k.T * 0.09, -1) @ v
+    table = torch.arange(n // 16, dtype=torch.int32, device="cuda").repeat(repeat)[None].contiguous()
+    ctx = torch.tensor([n * repeat], dtype=torch.int32, device="cuda")
+    got = ops.paged_attn_decode_q4(q, cache, table, ctx, nq, 1, hd, 0.09).double().cpu().view(nq, hd)
+    assert float((got - want).norm() / want.norm()) < math.hypot(1.74e-3, 6e-4) * 1.05
+
+
 @pytest.mark.parametrize("k_scale,v_scale", [(1.0, 1e-6), (1.0, 3e4), (1e-5, 1.0), (60.0, 1e-20), (1.0, 1e30)])
 def test_attention_sizes_of_values(k_scale, v_scale):
     """Steps far from 1: the products are held in types of narrow range inside."""
