@@ -51,11 +51,20 @@ __device__ __forceinline__ uint4 q4_load8(const Q4Write& a, size_t row, int widt
   } else {
     const float* p = a.slabs + row * width + col;
     float f[8] = {};
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float4 u = __ldcg(reinterpret_cast<const float4*>(p + s * a.slab));
-      const float4 w = __ldcg(reinterpret_cast<const float4*>(p + s * a.slab) + 1);
-      f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w;
-      f[4] += w.x; f[5] += w.y; f[6] += w.z; f[7] += w.w;
+    for (int s0 = 0; s0 < a.nsplit; s0 += 4) {  // (four on their way at a time, added in order)
+      float4 u[4], w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < a.nsplit) {
+          u[i] = __ldcg(reinterpret_cast<const float4*>(p + (s0 + i) * a.slab));
+          w[i] = __ldcg(reinterpret_cast<const float4*>(p + (s0 + i) * a.slab) + 1);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < a.nsplit) {
+          f[0] += u[i].x; f[1] += u[i].y; f[2] += u[i].z; f[3] += u[i].w;
+          f[4] += w[i].x; f[5] += w[i].y; f[6] += w[i].z; f[7] += w[i].w;
+        }
     }
     if (a.bias) {
       const uint4 b = *reinterpret_cast<const uint4*>(a.bias + col);
@@ -139,7 +148,7 @@ __device__ __forceinline__ void q4_store8(uint8_t* tile, int r, int hd, bool val
   }
 }
 
-// A block takes ROWS neighbouring rows, PER = THREADS / ROWS threads each.  A thread keeps one octet of the heads' lower halves and its
+// A block takes ROWS neighbouring rows, or for one row the blocks of grid.y share its heads; PER = THREADS / ROWS threads to a row.  A thread keeps one octet of the heads' lower halves and its
 // rotation partner, with their eight angles, and goes through the heads, BATCH of them requested at a time.  The angles of
 // the block's rows are computed once, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01 radians), and the products are
 // rounded one by one: the rotated elements are the formula's to the bit.
@@ -161,7 +170,8 @@ __global__ void __launch_bounds__(THREADS, ROWS > 1 ? 1024 / THREADS : 1) k_rope
       s_rot[r][i] = make_float2(float(cs), float(sn));
     }
   }
-  const int r = threadIdx.x / PER, o = threadIdx.x % OPH, h0 = threadIdx.x % PER / OPH;
+  const int r = threadIdx.x / PER, o = threadIdx.x % OPH, h0 = threadIdx.x % PER / OPH + (ROWS == 1 ? blockIdx.y * STEP : 0);
+  const int all = ROWS == 1 ? gridDim.y * STEP : STEP;  // heads of a pass, over the blocks of a row
   const bool row_there = r < rows;  // (whole warps: PER is a multiple of 32)
   const size_t row = row0 + (row_there ? r : 0);
   const int slot = a.slots ? a.slots[row] : -1;
@@ -169,11 +179,12 @@ __global__ void __launch_bounds__(THREADS, ROWS > 1 ? 1024 / THREADS : 1) k_rope
   if (!row_there) return;
   const int blk = slot >= 0 ? slot / a.block_size : -1, in_block = slot >= 0 ? slot - blk * a.block_size : 0;
   const bool kept = blk >= 0 && blk < a.n_blocks;  // (no such block: not kept)
-  for (int hb = h0; hb - h0 < heads; hb += STEP * BATCH) {
+  for (int pass = 0; pass < heads; pass += all * BATCH) {
+    const int hb = h0 + pass;
     uint4 lo[BATCH], hi[BATCH];
 #pragma unroll
     for (int c = 0; c < BATCH; ++c) {
-      const int h = hb + c * STEP;
+      const int h = hb + c * all;
       lo[c] = hi[c] = make_uint4(0, 0, 0, 0);
       if (h < heads) {
         lo[c] = q4_load8<SLABS>(a, row, width, h * HD + 8 * o);
@@ -182,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, ROWS > 1 ? 1024 / THREADS : 1) k_rope
     }
 #pragma unroll
     for (int c = 0; c < BATCH; ++c) {
-      const int h = hb + c * STEP;
+      const int h = hb + c * all;
       const bool there = h < heads;
       if (!__any_sync(0xffffffffu, there)) break;
       if (there && h < a.nq + a.nkv) {
@@ -908,16 +919,17 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
   a.rows = rows; a.nq = nq; a.nkv = nkv; a.hd = hd; a.block_size = block_size; a.n_blocks = n_blocks;
   a.log2_theta = log2(theta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Many rows: four to a block, a warp each that goes through the heads (8191 rows of 36 heads: 35.7 us; two warps a row and three heads at
-  // a time 37 to 48, by registers); few rows (a decode step): a block each whose threads have about a head's octet at once.
-  const bool many = rows > 4 * sm_count();
-  const dim3 grid(many ? (rows + 3) / 4 : rows), block(many ? 128 : 256);
+  // Many rows: four to a block, a warp each that goes through the heads (8191 rows of 36 heads: 35 us; two warps a row and three heads at
+  // a time 37 to 48, by registers); few rows (a decode step) and slabs: a row's heads dealt out to blocks, each thread with one octet.
+  const bool many = rows > 4 * sm_count() && !a.slabs;
+  const int heads = nq + 2 * nkv, step = 128 / (hd / 16);
+  const dim3 grid(many ? (rows + 3) / 4 : rows, many ? 1 : (heads + step - 1) / step), block(128);
   if (hd == 128) {
-    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<128, true, 4, 128, 1> : k_rope_kv_write_q4<128, true, 1, 256, 2>, grid, block, 0, st, a);
-    else launch_k(many ? k_rope_kv_write_q4<128, false, 4, 128, 2> : k_rope_kv_write_q4<128, false, 1, 256, 2>, grid, block, 0, st, a);
+    if (a.slabs) launch_k(k_rope_kv_write_q4<128, true, 1, 128, 1>, grid, block, 0, st, a);
+    else launch_k(many ? k_rope_kv_write_q4<128, false, 4, 128, 2> : k_rope_kv_write_q4<128, false, 1, 128, 1>, grid, block, 0, st, a);
   } else {
-    if (a.slabs) launch_k(many ? k_rope_kv_write_q4<64, true, 4, 128, 1> : k_rope_kv_write_q4<64, true, 1, 256, 2>, grid, block, 0, st, a);
-    else launch_k(many ? k_rope_kv_write_q4<64, false, 4, 128, 2> : k_rope_kv_write_q4<64, false, 1, 256, 2>, grid, block, 0, st, a);
+    if (a.slabs) launch_k(k_rope_kv_write_q4<64, true, 1, 128, 1>, grid, block, 0, st, a);
+    else launch_k(many ? k_rope_kv_write_q4<64, false, 4, 128, 2> : k_rope_kv_write_q4<64, false, 1, 128, 1>, grid, block, 0, st, a);
   }
   KV4_LAUNCH_CHECK("rope_kv_write_q4");
   return 0;

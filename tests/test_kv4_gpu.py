@@ -89,6 +89,24 @@ def test_write(nq, nkv, hd, rows, block, splits):
     assert torch.equal(k.cpu(), wk) and torch.equal(v.cpu(), wv)
 
 
+@pytest.mark.parametrize("splits", [0, 2])
+def test_write_of_many_rows(splits):
+    """Beyond the rows that get blocks of their own; not a multiple of the rows of a block."""
+    nq, nkv, hd, rows = 3, 2, 128, 700
+    x = _randn(6, max(splits, 1), rows, 7 * hd)
+    whole = (x[0] + x[1]).bfloat16() if splits else x[0].bfloat16()
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda") * 37
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    cache = _dirty_cache(44, nkv, hd, 16)
+    got = ops.rope_kv_write_q4(x if splits else whole.clone(), pos, slots, cache, nq, nkv, hd, 16, 1e6)
+    want, size = _rotated(whole, pos, nq, nkv, hd, 1e6)
+    assert bool(((got.double().cpu().view_as(want) - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -22 * torch.cat([size, size], -1)).all())
+    mine = torch.full_like(cache.cpu(), 0xFF)
+    rot = got.cpu().view(rows, -1, hd)
+    ref.kv4_write(mine, slots.cpu(), rot[:, nq:nq + nkv], rot[:, nq + nkv:], 16)
+    assert torch.equal(mine, cache.cpu())
+
+
 def test_rope_alone_and_no_rows():
     x = _randn(1, 9, 6 * 128).bfloat16()
     pos = torch.arange(9, dtype=torch.int32, device="cuda") * 1000
