@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(T) k_paged_layout(const RequestLayout a) {
   int* s_past = s_had + B;         // [B]
   int* s_back = s_past + B;        // [B] blocks given back, then their running sum
   int* s_list = s_back + B;        // [B] requests that have ended
-  const int head = a.range[0], free_n = min(max(a.range[1], 0), a.cap);
+  // (whatever stands there: an entry of the ring, and no more free blocks than it has)
+  const int first = a.range[0] % a.cap, head = first < 0 ? first + a.cap : first, free_n = min(max(a.range[1], 0), a.cap);
   if (tid == 0) s_ended = 0;
   __syncthreads();
   for (int b = tid; b < B; b += T) {

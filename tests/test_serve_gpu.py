@@ -86,6 +86,13 @@ def test_layout_edges():
     _layout_both((i32(2, 2), i32(-7, 3), i32(-1, 5).view(2, 1), i32(0, 1, 2), i32(1, 3, 0)), 4, 16)
 
 
+@pytest.mark.parametrize("head", [-1, -2 ** 31, 5, 2 ** 31 - 1])
+def test_layout_of_a_head_outside_the_ring(head):
+    """A head that names no entry is taken modulo the ring's length."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    _layout_both((i32(20, -1), i32(0, 16), i32(-1, -1, 3, -1).view(2, 2), i32(0, 1, 2), i32(head, 2, 0)), 20, 16)
+
+
 def test_layout_of_a_run_in_place():
     """Prompts, then steps captured in a graph, in place, while one request ends: no block has two holders, positions count on."""
     bs, batch, width, n = 16, 5, 8, 24
