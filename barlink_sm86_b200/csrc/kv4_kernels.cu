@@ -148,9 +148,9 @@ __device__ __forceinline__ void q4_store8(uint8_t* tile, int r, int hd, bool val
   }
 }
 
-// A block takes ROWS neighbouring rows, or for one row the blocks of grid.y share its heads; PER = THREADS / ROWS threads to a row.  A thread keeps one octet of the heads' lower halves and its
-// rotation partner, with their eight angles, and goes through the heads, BATCH of them requested at a time.  The angles of
-// the block's rows are computed once, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01 radians), and the products are
+// A block takes ROWS neighbouring rows, or, one row at a time, the blocks of grid.y share its heads; PER = THREADS / ROWS threads to a
+// row.  A thread keeps one octet of the heads' lower halves and its rotation partner, and goes through the heads, BATCH of them
+// requested at a time.  The angles of the block's rows are computed once, in 64 bits (a position of 10^5 leaves 32 bits no better than 0.01 radians), and the products are
 // rounded one by one: the rotated elements are the formula's to the bit.
 template <int HD, bool SLABS, int ROWS, int THREADS, int BATCH>
 __global__ void __launch_bounds__(THREADS, ROWS > 1 ? 1024 / THREADS : 1) k_rope_kv_write_q4(const Q4Write a) {
@@ -820,13 +820,15 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
 // The pieces of a pair that was cut: block (pair, head), a warp takes every kQ4MergeWarps-th piece, a lane HD / 32 dims of it.
 constexpr int kQ4MergeWarps = 8;
 template <int HD>
-__global__ void __launch_bounds__(kQ4MergeWarps * 32) k_q4_merge(const Q4Attn a, int G) {
+__global__ void __launch_bounds__(kQ4MergeWarps * 32) k_q4_merge(const Q4Attn a, int G, int runs) {
   constexpr int D = HD / 32;
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float s_o[kQ4MergeWarps][HD], s_m[kQ4MergeWarps], s_l[kQ4MergeWarps];
   const int2 m = a.meta[blockIdx.x];
   if (m.y == 0) return;
+  // (a run that gave up waiting leaves this word as the workspace had it: no piece there is followed)
+  if (m.y < 0 || m.x < 0 || m.x >= 2 * runs || m.y > runs - (m.x >> 1)) return;
   const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t pitch = q4_part_floats(G, HD);
   auto at = [&](int i) { return a.part + size_t(i == 0 ? m.x : 2 * ((m.x >> 1) + i)) * pitch; };
@@ -1016,7 +1018,7 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
     const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem, done);
     if (e != cudaSuccess) return e;
     launch_k(kernel, dim3(grid), dim3(kQ4Warps * 32), smem, st, a);
-    return launch_k(merge, dim3(batch * nkv, G), dim3(kQ4MergeWarps * 32), 0, st, a, G);
+    return launch_k(merge, dim3(batch * nkv, G), dim3(kQ4MergeWarps * 32), 0, st, a, G, grid * kQ4Warps);
   };
   cudaError_t e;
   if (hd == 128)
