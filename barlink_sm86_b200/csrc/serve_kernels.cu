@@ -257,8 +257,8 @@ __global__ void __launch_bounds__(kCountThreads) k_count_tokens(const int* __res
   }
 }
 // Tables made anew: block (slice, row) counts the row's tokens of its slice of the vocabulary in shared memory and writes the slice, so
-// that the tables are written once and nobody waits for zeros.  64 x 152064: 9.4 us; zeros, a fence, then counting in global memory
-// 11; a fill of the 40 MB alone 6.
+// that the tables are written once and nobody waits for zeros.  64 x 152064: 9.8 us; zeros, a fence, then counting in global memory
+// 11; a fill of the 40 MB alone 6.1.
 constexpr int kCountSlice = 19456;  // tokens, a multiple of 32
 __global__ void __launch_bounds__(kCountThreads) k_count_anew(const int* __restrict__ ids, const int* __restrict__ cu,
                                                               const int* __restrict__ prompt, int* __restrict__ counts,
