@@ -280,8 +280,12 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ ca
 //                                                                        of k = (parts of sum q) x groups in bf16, exact parts
 //   o_d = sum over tokens of (p_t step_ta) c + p_t low_ta             -- p step rounded to fp16 (2^-11), the second sum in fp32
 // Queries go in as fp16 of a power of two per head (exact: 2^-27 of the head's largest element is still whole).  The reference of
-// the running softmax is the greatest of x_t + log2(largest step of t), so that p step stays within fp16 whatever the values'
-// size; it moves only when it is exceeded by 2^8, which one vote per tile finds out.
+// the running softmax is the greatest of x_t + e_t, e_t = log2 of the token's largest step, so that p step stays within fp16 whatever the
+// values' size, or of its largest |low| over 2^95, if that is more: a group of one value has no step, and p low has to stay within
+// fp32.  It moves only when p step exceeds it by 2^8, when a lane's four tokens have (next to) no steps, or when there is a low of 2^65
+// or more, which one vote per unit finds out.  Between the votes p is at most 2^29 where a token has less than 2^65, so that p low
+// is below 2^97 and its sums are finite, whatever the context's length.  (What that costs: beside a low above 2^95, groups with steps below
+// 2^-14 of low / 2^95 lose places.)
 //
 // Work: the units (two tiles) of all (request, KV head) pairs in one row, cut into equal runs, one for each warp; a warp has a
 // ring of its own that the bulk copies fill across pairs, and shares nothing with others.  Lengths are on the GPU only, so every warp
@@ -652,14 +656,23 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
             }
       }
       // ---- probabilities; where one times step may leave fp16's range, a new reference first ----
-      float top;  // the larger of all the steps here and 2^-90 (bf16 above 0 compare as integers)
+      float top;  // the largest of the steps here (bf16 above 0 compare as integers); 2^39 where they do not bound p low
       {
         uint32_t m = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < NA / 2; ++i) m = __vmaxu2(m, __vmaxu2(vs0[u][i], vs1[u][i]));
-        top = fmaxf(fmaxf(bf16_lo(m), bf16_hi(m)), 8.0779356694631609e-28f);
+        top = fmaxf(bf16_lo(m), bf16_hi(m));
+        if (top < 9.5367431640625e-7f) top = 549755813888.f;  // (2^-20: p up to 2^-30 passes, tokens that are not there among them)
+      }
+      uint32_t vast;  // token `lane` of the unit has a low of 2^65 or more: the two highest bits of its exponent
+      {
+        uint32_t w[NA / 2];
+        lds_words<NA / 2>(tile + (lane >> 4) * TB + q4_v_params(HD) + (lane & 15) * NA * 4 + NA * 2, w);
+        vast = w[0] & w[0] << 1;
+        if constexpr (NA == 4) vast |= w[1] & w[1] << 1;
+        vast &= lane < left && !(no_block >> (lane >> 4) & 1) ? 0x40004000u : 0u;
       }
       float p[2][NT][4];
       auto weigh = [&] {
@@ -675,8 +688,9 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
             }
         return most;
       };
-      if (__any_sync(kAll, weigh() * top > 512.f)) {
-        float e[2][2];  // log2 of a token's largest step, rounded down
+      const float most = weigh();
+      if (__any_sync(kAll, most * top > 512.f || vast)) {
+        float e[2][2];  // log2 of a token's largest step, rounded down, or that of its largest low less 95
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -685,6 +699,20 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
             if constexpr (NA == 4) m = __vmaxu2(m, (j ? vs1[u] : vs0[u])[1]);
             e[u][j] = float(min(max(int(max(m & 0xffffu, m >> 16) >> 7) - 127, -90), 110));
           }
+        if (__any_sync(kAll, vast || (top >= 549755813888.f && most > 0.f))) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t m = 0;
+#pragma unroll
+              for (int i = NA / 2; i < NA; ++i) {
+                const uint32_t low = (j ? vs1[u] : vs0[u])[i] & 0x7fff7fffu;
+                m = __vmaxu2(m, low & __vcmpleu2(low, 0x7f7f7f7fu));  // (a group that is no number bounds nothing)
+              }
+              e[u][j] = fmaxf(e[u][j], float(int(max(m & 0xffffu, m >> 16) >> 7) - 127 - 95));
+            }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll

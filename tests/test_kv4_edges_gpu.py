@@ -1,0 +1,79 @@
+# SPDX-License-Identifier: MIT
+"""The 4-bit key/value cache on the GPU where its numbers leave the ordinary: values without steps.
+Tolerances and 64-bit statements are those of test_kv4_gpu.py."""
+import pytest
+import torch
+
+from barlink_sm86_b200 import ops
+from test_kv4_gpu import _attention_64, _check, _filled, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+def _rewrite(cache, table, request, kv, block=16, first=0):
+    """Keys and values kv [tokens, 2 nkv, hd] in place of a request's tokens from `first` on."""
+    n, heads, hd = kv.shape
+    t = torch.arange(first, first + n, device="cuda")
+    slots = (table[request].long()[t // block] * block + t % block).to(torch.int32)
+    ops.rope_kv_write_q4(kv.bfloat16().reshape(n, -1), torch.zeros_like(slots), slots, cache, 0, heads // 2, hd, block, 1e6)
+
+
+@pytest.mark.parametrize("level", [1e-25, 1.0, -1e10, 1e12, 1e30, -3e38])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (12, 1, 64)])
+def test_values_without_steps(level, nq, nkv, hd):
+    """Groups of one value each (step 0), whatever its size: the mean over tokens is one of numbers that fp32 holds."""
+    lens = [1, 40, 700]
+    cache, table, ctx = _filled(200, lens, nkv, hd, 16)
+    for i, n in enumerate(lens):
+        kv = _randn(201 + i, n, 2 * nkv, hd)
+        kv[:, nkv:] = level * (0.25 + 0.75 * torch.rand(n, nkv, 1, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda"))
+        _rewrite(cache, table, i, kv)
+    q = _randn(210, 3, nq * hd).bfloat16()
+    got = ops.paged_attn_decode_q4(q, cache, table, ctx, nq, nkv, hd, 0.1)
+    _check(got, *_attention_64(q, cache, table, ctx, nq, nkv, hd, 0.1))
+
+
+def _again(table, n, repeat, block=16):
+    """A table that names a request's n tokens (whole blocks) over and over, so that a warp's run holds many of them; the softmax's mean
+    does not change.  With its length."""
+    return table[:, :n // block].repeat(1, repeat).contiguous(), torch.tensor([n * repeat], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("repeat", [1, 512])
+@pytest.mark.parametrize("grows", [False, True])
+def test_values_without_steps_behind_zeros(grows, repeat):
+    """Zeros, then constants, then ordinary values, one group of them constant: the sums are in scale for each of them.  grows: the
+    scores rise along the way."""
+    n, nkv, hd, nq = 1600, 1, 128, 8
+    cache, table, ctx = _filled(220, [n], nkv, hd, 16)
+    kv = _randn(221, n, 2, hd)
+    if grows:
+        kv[:, 0] = torch.linspace(0, 1, n, device="cuda")[:, None]
+    kv[:400, 1] = 0
+    kv[400:800, 1] = 1e12
+    kv[800:1200, 1] *= 1e-12
+    kv[1200:, 1, 32:64] = -1e25
+    _rewrite(cache, table, 0, kv)
+    q = torch.full((1, nq * hd), 1.0, device="cuda").bfloat16() if grows else _randn(222, 1, nq * hd).bfloat16()
+    for m in (n, 800, 1200, 400):
+        t, c = _again(table, m, repeat)
+        ctx.fill_(m)
+        got = ops.paged_attn_decode_q4(q, cache, t, c, nq, nkv, hd, 0.1)
+        _check(got, *_attention_64(q, cache, table, ctx, nq, nkv, hd, 0.1))
+
+
+@pytest.mark.parametrize("repeat", [1, 512])
+def test_a_group_at_the_end_of_the_range(repeat):
+    """3e38 beside ordinary values, and behind them: its own dims."""
+    n, hd, nq = 912, 128, 4
+    cache, table, ctx = _filled(230, [n], 1, hd, 16)
+    kv = _randn(231, n, 2, hd)
+    kv[500:, 1, 64:96] = 3e38
+    _rewrite(cache, table, 0, kv)
+    q = _randn(232, 1, nq * hd).bfloat16()
+    t, c = _again(table, n, repeat)
+    got = ops.paged_attn_decode_q4(q, cache, t, c, nq, 1, hd, 0.1)
+    want, size = _attention_64(q, cache, table, ctx, nq, 1, hd, 0.1)
+    own = (torch.arange(nq * hd) % hd // 32 == 2)[None]
+    _check(got[:, own[0].cuda()], want[own][None], size[own][None])
+    assert bool(torch.isfinite(got).all())
