@@ -684,12 +684,12 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               p[u][n][j] = q4_ex2(fmaf(c[u][n][j], f[n][j & 1], -R[n][j & 1]));
-              most += p[u][n][j];  // (no less than the greatest; a NaN leaves the reference alone)
+              most += p[u][n][j];  // (no less than the greatest; NaN if one of them is)
             }
         return most;
       };
       const float most = weigh();
-      if (__any_sync(kAll, most * top > 512.f || vast)) {
+      if (__any_sync(kAll, !(most * top <= 512.f) || vast)) {  // (NaN too: it is of one head, and would hide what the lane's others ask for)
         float e[2][2];  // log2 of a token's largest step, rounded down, or that of its largest low less 95
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
             if constexpr (NA == 4) m = __vmaxu2(m, (j ? vs1[u] : vs0[u])[1]);
             e[u][j] = float(min(max(int(max(m & 0xffffu, m >> 16) >> 7) - 127, -90), 110));
           }
-        if (__any_sync(kAll, vast || (top >= 549755813888.f && most > 0.f))) {
+        if (__any_sync(kAll, vast || (top >= 549755813888.f && !(most <= 0.f)))) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll

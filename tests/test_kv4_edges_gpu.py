@@ -1,6 +1,8 @@
 # SPDX-License-Identifier: MIT
-"""The 4-bit key/value cache on the GPU where its numbers leave the ordinary: values without steps.
+"""The 4-bit key/value cache on the GPU where its numbers leave the ordinary: values without steps, queries that are no numbers.
 Tolerances and 64-bit statements are those of test_kv4_gpu.py."""
+import math
+
 import pytest
 import torch
 
@@ -77,3 +79,23 @@ def test_a_group_at_the_end_of_the_range(repeat):
     own = (torch.arange(nq * hd) % hd // 32 == 2)[None]
     _check(got[:, own[0].cuda()], want[own][None], size[own][None])
     assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("repeat", [1, 512])
+@pytest.mark.parametrize("nq,hd", [(8, 128), (16, 128), (3, 64), (12, 64)])
+def test_a_query_that_is_no_number_spoils_its_own_head(nq, hd, repeat):
+    """Head 0 is NaN; head 1's scores rise by 46 in log2 late in the context, where nothing else moves."""
+    n = 1024
+    cache, table, ctx = _filled(240, [n], 1, hd, 16)
+    kv = _randn(241, n, 2, hd)
+    kv[:, 0] *= 0.01
+    kv[993:, 0, :32] = 10.0
+    _rewrite(cache, table, 0, kv)
+    t, c = _again(table, n, repeat)
+    q = torch.zeros(1, nq, hd, device="cuda")
+    q[0, 1, :32] = 1.0
+    want, size = _attention_64(q.view(1, -1).bfloat16(), cache, table, ctx, nq, 1, hd, 0.1)
+    q[0, 0, 5] = math.nan
+    got = ops.paged_attn_decode_q4(q.view(1, -1).bfloat16(), cache, t, c, nq, 1, hd, 0.1)
+    assert bool(got[0, :hd].isnan().all())
+    _check(got[:, hd:], want[:, hd:], size[:, hd:])
