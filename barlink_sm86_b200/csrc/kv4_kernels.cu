@@ -833,9 +833,13 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
     }
   }
   if (dead) {
-    // a copy did not arrive in time: say so, and leave with none in flight
+    // A copy did not arrive in time: say so, and wait for all that are in flight, each as long as a wait may take: shared memory is another
+    // block's behind this one.
     if (lane == 0) g_kv4_err = 1;
     for (int i = k; i < min(k + STAGES, count); ++i) {
+      __syncwarp();
+      if (lane == 0) s_abort[warp] = 0;
+      __syncwarp();
       mbar_wait_bounded_warp(bars + stage, phase, &s_abort[warp]);
       if (++stage == STAGES) {
         stage = 0;
