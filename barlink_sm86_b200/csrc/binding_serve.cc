@@ -137,6 +137,10 @@ int kv4_error_flag(int dev) {
   BL_CHECK(bl_kv4_error(&v, err, errlen));
   return int(v);
 }
+void kv4_error_clear(int dev) {
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  BL_CHECK(bl_kv4_error_clear(err, errlen));
+}
 
 at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables, const at::Tensor& ctx_lens,
                                 int nq, int nkv, int hd, double scale, const OptTensor& out_opt) {
@@ -304,6 +308,8 @@ void bind_serve(py::module_& m) {
   m.def("paged_attn_decode_q4", &paged_attn_decode_q4, py::arg("q"), py::arg("cache"), py::arg("block_tables"), py::arg("ctx_lens"),
         py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none());
   m.def("kv4_error_flag", &kv4_error_flag, py::arg("device") = 0);
+  m.def("kv4_error_clear", &kv4_error_clear, py::arg("device") = 0);
+  m.def("kv4_wait_polls", &bl_kv4_wait_polls, py::arg("polls"));
   m.def("paged_layout", &paged_layout, py::arg("new_lens"), py::arg("past_lens"), py::arg("block_tables"), py::arg("free_list"),
         py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("rows_per_request") = 0, py::arg("into") = py::none());
   m.def("count_tokens", &count_tokens, py::arg("counts"), py::arg("seen"), py::arg("ids"), py::arg("cu") = py::none(),

@@ -8,6 +8,8 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "bl_ops.h"
 #include "heap.h"
 #include "kv4.cuh"
@@ -300,6 +302,9 @@ __host__ __device__ constexpr size_t q4_part_floats(int G, int hd) { return size
 
 // set by a wait that ran out; one word per device
 __device__ uint32_t g_kv4_err;
+// polls of a wait for copies before it gives up
+constexpr uint32_t kQ4Polls = 1u << 24;
+static std::atomic<uint32_t> g_kv4_polls{kQ4Polls};
 
 struct Q4Attn {
   const __nv_bfloat16* q;
@@ -311,6 +316,7 @@ struct Q4Attn {
   int2* meta;    // [batch * nkv]: a pair's first piece, and the number of its pieces (0: done); the others are the first of their runs
   int q_stride, batch, nq, nkv, block_size, n_blocks, max_blocks;
   float scale_log2;
+  uint32_t polls;
 };
 
 __device__ __forceinline__ float q4_ex2(float x) {
@@ -575,7 +581,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
     };
 #pragma unroll 1
     for (; k < seg_end; ++k) {
-      if (!mbar_wait_bounded_warp(bars + stage, phase, &s_abort[warp])) {
+      if (!mbar_wait_bounded_warp(bars + stage, phase, &s_abort[warp], a.polls)) {
         dead = true;
         break;
       }
@@ -833,8 +839,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
     }
   }
   if (dead) {
-    // A copy did not arrive in time: say so, and wait for all that are in flight, each as long as a wait may take: shared memory is another
-    // block's behind this one.
+    // A copy did not arrive in time: say so, wait for all that are in flight (each as long as a wait may take: shared memory is another
+    // block's behind this one), and leave NaN in place of this pair's result and of all that follow in this run.
     if (lane == 0) g_kv4_err = 1;
     for (int i = k; i < min(k + STAGES, count); ++i) {
       __syncwarp();
@@ -845,6 +851,21 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
         stage = 0;
         phase ^= 1;
       }
+    }
+    for (;;) {
+      const int seg_end = min(hi, seg.start + seg.units) - lo, piece = 2 * me + (seg.start > lo ? 1 : 0);
+      const bool begins = seg.start >= lo, whole = begins && lo + seg_end == seg.start + seg.units;
+      if (whole) {
+        uint4* to = reinterpret_cast<uint4*>(a.out + (size_t(seg.b) * a.nq + size_t(seg.h) * G) * HD);
+        for (int i = lane; i < G * HD / 8; i += 32) to[i] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+      } else {
+        float* part = a.part + size_t(piece) * q4_part_floats(G, HD);
+        for (int i = lane; i < G * HD; i += 32) part[i] = 0.f;
+        for (int i = lane; i < G; i += 32) *reinterpret_cast<float2*>(part + G * HD + 2 * i) = make_float2(0.f, NAN);
+      }
+      if (begins && lane == 0) a.meta[size_t(seg.b) * a.nkv + seg.h] = make_int2(piece, whole ? 0 : (seg.start + seg.units - 1) / run - me + 1);
+      if (seg_end >= count) break;
+      q4_advance(a, seg, lo + seg_end);
     }
   }
 }
@@ -859,7 +880,7 @@ __global__ void __launch_bounds__(kQ4MergeWarps * 32) k_q4_merge(const Q4Attn a,
   __shared__ float s_o[kQ4MergeWarps][HD], s_m[kQ4MergeWarps], s_l[kQ4MergeWarps];
   const int2 m = a.meta[blockIdx.x];
   if (m.y == 0) return;
-  // (a run that gave up waiting leaves this word as the workspace had it: no piece there is followed)
+  // (every run leaves its words; lengths that another stream changes meanwhile, which nobody may, could leave some out: nothing there is followed)
   if (m.y < 0 || m.x < 0 || m.x >= 2 * runs || m.y > runs - (m.x >> 1)) return;
   const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t pitch = q4_part_floats(G, HD);
@@ -985,11 +1006,18 @@ extern "C" int bl_kv4_read(const void* cache, const int* slots, void* k, void* v
   return 0;
 }
 
-extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
-  const cudaError_t e = cudaMemcpyFromSymbol(out, g_kv4_err, sizeof(*out));
+static int q4_error_rc(cudaError_t e, char* err, size_t errlen) {
   if (e != cudaSuccess) set_err(err, errlen, "barlink: kv4_error: %s", cudaGetErrorString(e));
   return e == cudaSuccess ? 0 : -1;
 }
+extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
+  return q4_error_rc(cudaMemcpyFromSymbol(out, g_kv4_err, sizeof(*out)), err, errlen);
+}
+extern "C" int bl_kv4_error_clear(char* err, size_t errlen) {
+  const unsigned none = 0;
+  return q4_error_rc(cudaMemcpyToSymbol(g_kv4_err, &none, sizeof(none)), err, errlen);
+}
+extern "C" unsigned bl_kv4_wait_polls(unsigned polls) { return g_kv4_polls.exchange(polls); }
 
 // Blocks of attention.  Two to an SM, with registers for two tiles at once: three and four of fewer registers (the last with spills) took
 // 34.5 and 37.9 us where two take 32.7 (4 requests of up to 32767 tokens), 14.9 and 17.0 against 13.7 (64 of up to 1100).
@@ -1044,6 +1072,7 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   a.q_stride = q_stride; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks;
   a.max_blocks = max_blocks;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.polls = g_kv4_polls.load();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   static bool attr[4][64] = {};
   auto go = [&](auto* kernel, auto* merge, int smem, bool (&done)[64]) {

@@ -184,8 +184,9 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 // The same for a converged warp, all lanes with the same answer.
-__device__ __forceinline__ bool mbar_wait_bounded_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+__device__ __forceinline__ bool mbar_wait_bounded_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                       uint32_t max_polls = 1u << 24) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, max_polls));
 }
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

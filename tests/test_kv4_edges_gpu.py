@@ -1,5 +1,5 @@
 # SPDX-License-Identifier: MIT
-"""The 4-bit key/value cache on the GPU where its numbers leave the ordinary: values without steps, queries that are no numbers.
+"""The 4-bit key/value cache on the GPU where its numbers leave the ordinary: values without steps, queries that are no numbers, waits that run out.
 Tolerances and 64-bit statements are those of test_kv4_gpu.py."""
 import math
 
@@ -99,3 +99,41 @@ def test_a_query_that_is_no_number_spoils_its_own_head(nq, hd, repeat):
     got = ops.paged_attn_decode_q4(q.view(1, -1).bfloat16(), cache, t, c, nq, 1, hd, 0.1)
     assert bool(got[0, :hd].isnan().all())
     _check(got[:, hd:], want[:, hd:], size[:, hd:])
+
+
+@pytest.fixture
+def polls(ext):
+    """Sets how often a wait looks; back to what it was afterwards, and the error word to 0."""
+    before = ext.kv4_wait_polls(0)
+    yield ext.kv4_wait_polls
+    ext.kv4_wait_polls(before)
+    torch.cuda.synchronize()
+    ext.kv4_error_clear(0)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,lens", [(14, 2, 128, [3000, 0, 1, 800]), (16, 1, 128, [90000]), (8, 8, 64, [700] * 300), (12, 1, 64, [40] * 9)])
+def test_a_wait_that_runs_out(ext, polls, nq, nkv, hd, lens):
+    """A run that gives up says so and leaves NaN, not what the workspace held; requests without tokens and later calls are as ever."""
+    polls(1 << 24)
+    cache, table, ctx = _filled(250, lens, nkv, hd, 16)
+    q = _randn(251, len(lens), nq * hd).bfloat16()
+    want = ops.paged_attn_decode_q4(q, cache, table, ctx, nq, nkv, hd, 0.1)
+    torch.cuda.synchronize()
+    assert ext.kv4_error_flag(0) == 0
+    polls(0)
+    got = ops.paged_attn_decode_q4(q, cache, table, ctx, nq, nkv, hd, 0.1)
+    assert ext.kv4_error_flag(0) == 1
+    for i, n in enumerate(lens):
+        assert bool(got[i].isnan().all()) if n else not bool(got[i].any())
+    ext.kv4_error_clear(0)
+    # some look once or twice, and may be in time: a head is right or NaN, and NaN only where the word says so
+    for n in (1, 2):
+        polls(n)
+        got = ops.paged_attn_decode_q4(q, cache, table, ctx, nq, nkv, hd, 0.1)
+        bad = got.view(-1, hd).isnan()
+        assert torch.equal(bad.all(1), bad.any(1)) and bool(bad.any()) == bool(ext.kv4_error_flag(0))
+        assert torch.equal(torch.where(bad, 0, got.view(-1, hd)), torch.where(bad, 0, want.view(-1, hd)))
+        ext.kv4_error_clear(0)
+    polls(1 << 24)
+    assert torch.equal(ops.paged_attn_decode_q4(q, cache, table, ctx, nq, nkv, hd, 0.1), want)
+    assert ext.kv4_error_flag(0) == 0
