@@ -141,6 +141,12 @@ void kv4_error_clear(int dev) {
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
   BL_CHECK(bl_kv4_error_clear(err, errlen));
 }
+// The same word, into a pinned int32 tensor on the current stream of a device: the caller reads it once the stream has come that far.
+void kv4_error_into(const at::Tensor& out, int dev) {
+  TORCH_CHECK(out.is_cpu() && out.is_pinned() && out.scalar_type() == at::kInt && out.numel() == 1, "barlink: kv4_error_into needs a pinned int32 element");
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  BL_CHECK(bl_kv4_error_async(static_cast<unsigned*>(out.data_ptr()), at::cuda::getCurrentCUDAStream(dev).stream(), err, errlen));
+}
 
 at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_tables, const at::Tensor& ctx_lens,
                                 int nq, int nkv, int hd, double scale, const OptTensor& out_opt) {
@@ -309,6 +315,7 @@ void bind_serve(py::module_& m) {
         py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none());
   m.def("kv4_error_flag", &kv4_error_flag, py::arg("device") = 0);
   m.def("kv4_error_clear", &kv4_error_clear, py::arg("device") = 0);
+  m.def("kv4_error_into", &kv4_error_into, py::arg("out"), py::arg("device") = 0);
   m.def("kv4_wait_polls", &bl_kv4_wait_polls, py::arg("polls"));
   m.def("paged_layout", &paged_layout, py::arg("new_lens"), py::arg("past_lens"), py::arg("block_tables"), py::arg("free_list"),
         py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("rows_per_request") = 0, py::arg("into") = py::none());

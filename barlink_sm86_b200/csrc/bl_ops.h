@@ -449,10 +449,11 @@ int bl_kv4_read(const void* cache, const int* slots, void* k, void* v, int rows,
 /* One query token per request against the cache; q rows q_stride elements apart.  A block-table entry that names no
  * block leaves its tokens out; a request without tokens gets zeros.  scale > 0.  ws: bl_paged_attn_decode_q4_ws bytes of this call's own, 16-byte
  * aligned.  A wait that runs out (a copy within the kernel that does not arrive) sets the current device's bl_kv4_error to 1 and leaves NaN in
- * place of the results concerned.  bl_kv4_error_clear sets it back to 0.
+ * place of the results concerned.  bl_kv4_error_async copies the word to `out` (pinned) on a stream, bl_kv4_error_clear sets it back to 0.
  * bl_kv4_wait_polls sets how often the waits of calls from now on look (2^24; 0: they give up at once, and show what a call leaves then) and
  * returns what it was. */
 int bl_kv4_error(unsigned* out, char* err, size_t errlen);
+int bl_kv4_error_async(unsigned* out, void* stream, char* err, size_t errlen);
 int bl_kv4_error_clear(char* err, size_t errlen);
 unsigned bl_kv4_wait_polls(unsigned polls);
 size_t bl_paged_attn_decode_q4_ws(int batch, int nq, int nkv, int hd);

@@ -1013,6 +1013,9 @@ static int q4_error_rc(cudaError_t e, char* err, size_t errlen) {
 extern "C" int bl_kv4_error(unsigned* out, char* err, size_t errlen) {
   return q4_error_rc(cudaMemcpyFromSymbol(out, g_kv4_err, sizeof(*out)), err, errlen);
 }
+extern "C" int bl_kv4_error_async(unsigned* out, void* stream, char* err, size_t errlen) {
+  return q4_error_rc(cudaMemcpyFromSymbolAsync(out, g_kv4_err, sizeof(*out), 0, cudaMemcpyDeviceToHost, static_cast<cudaStream_t>(stream)), err, errlen);
+}
 extern "C" int bl_kv4_error_clear(char* err, size_t errlen) {
   const unsigned none = 0;
   return q4_error_rc(cudaMemcpyToSymbol(g_kv4_err, &none, sizeof(none)), err, errlen);

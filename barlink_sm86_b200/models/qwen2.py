@@ -666,6 +666,7 @@ class DecodeEngine:
         if dev.type == "cuda":
             self.h_in = torch.zeros(batch, dtype=torch.int32).pin_memory()
             self.h_out = torch.zeros(batch, dtype=torch.int32).pin_memory()
+            self.h_err = torch.zeros(1, dtype=torch.int32).pin_memory()
 
     def _lay_out(self, new_lens, tokens=0):
         """Blocks for (or from) the requests outside a step: the layout of `tokens` packed rows, the state in place."""
@@ -879,5 +880,22 @@ class DecodeEngine:
         self.ids.copy_(ids_host, non_blocking=True)
         self.step()
         self.h_out.copy_(self.out_ids, non_blocking=True)
-        torch.cuda.current_stream().synchronize()
+        self.check()
         return self.h_out
+
+    def check(self):
+        """Waits for the steps so far.  RuntimeError if attention over the 4-bit cache gave up waiting for its copies in one of them: its
+        results are NaN there, and tokens from there on are none of the model's.  (The error is reported once.)"""
+        if self.m.device.type != "cuda":
+            return
+        stream = torch.cuda.current_stream(self.m.device)
+        if self.kv_bits != 4:
+            stream.synchronize()
+            return
+        from .. import load_extension
+        ext, dev = load_extension(), self.positions.device.index
+        ext.kv4_error_into(self.h_err, dev)
+        stream.synchronize()
+        if int(self.h_err):
+            ext.kv4_error_clear(dev)
+            raise RuntimeError("attention over the 4-bit cache gave up waiting for its copies: the steps since the last check are not to be used")

@@ -140,6 +140,7 @@ def main():
             toks.append(eng.step().clone())
         e.record()
         torch.cuda.synchronize()
+        eng.check()
         decode_ms = s.elapsed_time(e)
     decode_ms = max_over_ranks(decode_ms, device=dev)
     ms_tok = decode_ms / a.gen

@@ -7,6 +7,8 @@ import pytest
 import torch
 
 from barlink_sm86_b200 import ops
+from barlink_sm86_b200.models import DecodeEngine, Qwen2Config, Qwen2Model
+from barlink_sm86_b200.parallel import TPComm
 from test_kv4_gpu import _attention_64, _check, _filled, _randn
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +139,23 @@ def test_a_wait_that_runs_out(ext, polls, nq, nkv, hd, lens):
     polls(1 << 24)
     assert torch.equal(ops.paged_attn_decode_q4(q, cache, table, ctx, nq, nkv, hd, 0.1), want)
     assert ext.kv4_error_flag(0) == 0
+
+
+def test_the_engine_reports_a_wait_that_ran_out(ext, polls):
+    polls(1 << 24)
+    cfg = Qwen2Config(hidden=512, layers=2, n_heads=4, n_kv_heads=2, head_dim=128, intermediate=1024, vocab=1000, name="test")
+    model = Qwen2Model(cfg, TPComm.single(), "cuda:0", torch.bfloat16, seed=3)
+    eng = DecodeEngine(model, 2, 200, use_graph=False, kv_bits=4)
+    prompt = torch.arange(60, dtype=torch.int32, device="cuda")
+    first = eng.start(prompt, [40, 20]).cpu().pin_memory()
+    want = eng.step_host(first).clone()
+    eng.finish([0, 1])
+    eng.start(prompt, [40, 20])
+    polls(0)
+    with pytest.raises(RuntimeError, match="gave up"):
+        eng.step_host(first)
+    polls(1 << 24)
+    eng.check()  # (reported once)
+    eng.finish([0, 1])
+    eng.start(prompt, [40, 20])
+    assert torch.equal(eng.step_host(first), want)
