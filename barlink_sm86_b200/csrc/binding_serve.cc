@@ -185,7 +185,7 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
 // [cu, positions, slots, ctx_lens, free_range]; `into`: the same five to write to
 std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tensor& past_lens, const at::Tensor& block_tables,
                                      const at::Tensor& free_list, const at::Tensor& free_range, int64_t tokens, int block_size, int rows_per_request,
-                                     const c10::optional<std::vector<at::Tensor>>& into) {
+                                     const c10::optional<std::vector<at::Tensor>>& into, const OptTensor& lost) {
   TORCH_CHECK(new_lens.is_cuda() && new_lens.dim() == 1, "barlink: new_lens must be a 1-D CUDA tensor");
   const int batch = small(new_lens.numel(), "batch"), rows = small(tokens, "tokens");
   const int* nl = i32(new_lens, new_lens, -1, "new_lens");
@@ -212,10 +212,11 @@ std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tenso
   i32(r[2], new_lens, rows, "slots");
   i32(r[3], new_lens, batch, "ctx_lens");
   i32(r[4], new_lens, 3, "free_range");
-  BL_CHECK(bl_paged_layout(nl, pl, block_tables.data_ptr<int>(), free_list.data_ptr<int>(), fr, r[0].data_ptr<int>(),
+  if (lost) i32(*lost, new_lens, 1, "lost");
+  BL_CHECK(bl_paged_layout_counting(nl, pl, block_tables.data_ptr<int>(), free_list.data_ptr<int>(), fr, r[0].data_ptr<int>(),
                            r[1].data_ptr<int>(), r[2].data_ptr<int>(), r[3].data_ptr<int>(), r[4].data_ptr<int>(), batch,
                            small(block_tables.size(1), "max_blocks"), small(free_list.numel(), "free_list"), rows, block_size, rows_per_request,
-                           stream_of(new_lens), err, errlen));
+                           lost ? lost->data_ptr<int>() : nullptr, stream_of(new_lens), err, errlen));
   return r;
 }
 
@@ -318,7 +319,7 @@ void bind_serve(py::module_& m) {
   m.def("kv4_error_into", &kv4_error_into, py::arg("out"), py::arg("device") = 0);
   m.def("kv4_wait_polls", &bl_kv4_wait_polls, py::arg("polls"));
   m.def("paged_layout", &paged_layout, py::arg("new_lens"), py::arg("past_lens"), py::arg("block_tables"), py::arg("free_list"),
-        py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("rows_per_request") = 0, py::arg("into") = py::none());
+        py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("rows_per_request") = 0, py::arg("into") = py::none(), py::arg("lost") = py::none());
   m.def("count_tokens", &count_tokens, py::arg("counts"), py::arg("seen"), py::arg("ids"), py::arg("cu") = py::none(),
         py::arg("prompt_lens") = py::none(), py::arg("reset") = false);
   m.def("logit_rules", &logit_rules, py::arg("logits"), py::arg("pick"), py::arg("vocab"), py::arg("offset") = 0,

@@ -469,6 +469,10 @@ int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* cache, cons
 int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range, int* cu,
                     int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks, int n_free, int tokens,
                     int block_size, int rows_per_request, void* stream, char* err, size_t errlen);
+/* the same; lost (one int32, or null) += the tokens that have a row but no slot: no block was free for their page, or the table ends before it */
+int bl_paged_layout_counting(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range, int* cu,
+                             int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks, int n_free, int tokens,
+                             int block_size, int rows_per_request, int* lost, void* stream, char* err, size_t errlen);
 /* counts int32 [rows][vocab] += 1 for every id behind a row's first prompt_lens ids; seen (bits) |= every id */
 int bl_count_tokens(const int* ids, const int* cu, const int* prompt_lens, int* counts, void* seen, int rows, int n_ids, int vocab,
                     int reset, void* stream, char* err, size_t errlen);

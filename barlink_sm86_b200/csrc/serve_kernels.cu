@@ -36,6 +36,7 @@ struct RequestLayout {
   int *cu, *positions, *slots, *ctx_lens, *range_out;
   int batch, width, cap, tokens, block_size;
   int per;  // rows of a request where every request has as many (those behind its tokens are empty); 0: packed
+  int* lost;  // += tokens that have a row and no slot; or null
 };
 
 // exclusive block-wide scan of three ints per thread; total in tot
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(T) k_paged_layout(const RequestLayout a) {
     a.tables[size_t(b) * a.width + s_had[b] + j - s_fresh[b]] = j < free_n ? a.ring[ring_at(j)] : -1;
   }
   if (a.tokens > kLayoutAlone) return;  // k_layout_rows does the rest
+  int lost = 0;
   for (int row = tid; row < a.tokens; row += T) {
     int pos = 0, slot = -1, b = -1, i = 0;  // the i-th token of request b
     if (a.per > 0) {
@@ -189,10 +191,12 @@ __global__ void __launch_bounds__(T) k_paged_layout(const RequestLayout a) {
         const int id = page < s_had[b] ? a.tables[size_t(b) * a.width + page] : j < free_n ? a.ring[ring_at(j)] : -1;
         if (id >= 0) slot = id * bs + pos % bs;
       }
+      lost += slot < 0;
     }
     a.positions[row] = pos;
     a.slots[row] = slot;
   }
+  if (lost > 0 && a.lost) atomicAdd(a.lost, lost);
 }
 
 // The rows of many tokens, behind k_paged_layout: four rows a thread, the first by bisection of the offsets in shared memory, the others by
@@ -224,6 +228,7 @@ __global__ void __launch_bounds__(256) k_layout_rows(const RequestLayout a) {
       const int id = a.tables[size_t(b) * a.width + page];
       if (id >= 0) slot[k] = id * bs + pos[k] % bs;
     }
+    if (slot[k] < 0 && a.lost) atomicAdd(a.lost, 1);
   }
   if (row0 + 4 <= a.tokens && ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots)) & 15) == 0) {
     *reinterpret_cast<int4*>(a.positions + row0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
@@ -598,6 +603,14 @@ using namespace bl;
 extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range,
                                int* cu, int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks,
                                int n_free, int tokens, int block_size, int rows_per_request, void* stream, char* err, size_t errlen) {
+  return bl_paged_layout_counting(new_lens, past_lens, block_tables, free_list, free_range, cu, positions, slots, ctx_lens, free_range_out, batch,
+                                  max_blocks, n_free, tokens, block_size, rows_per_request, nullptr, stream, err, errlen);
+}
+
+extern "C" int bl_paged_layout_counting(const int* new_lens, const int* past_lens, int* block_tables, int* free_list, const int* free_range,
+                                        int* cu, int* positions, int* slots, int* ctx_lens, int* free_range_out, int batch, int max_blocks,
+                                        int n_free, int tokens, int block_size, int rows_per_request, int* lost, void* stream, char* err,
+                                        size_t errlen) {
   if (batch < 1 || batch > kLayoutMaxBatch || max_blocks < 1 || n_free < 1 || tokens < 0 || tokens > 1 << 30 || block_size < 1 ||
       rows_per_request < 0) {
     set_err(err, errlen, "barlink: paged_layout takes 1 to %d requests, up to 2^30 tokens, a table and a list of free blocks", kLayoutMaxBatch);
@@ -611,6 +624,7 @@ extern "C" int bl_paged_layout(const int* new_lens, const int* past_lens, int* b
   a.new_lens = new_lens; a.past_lens = past_lens; a.tables = block_tables; a.ring = free_list; a.range = free_range;
   a.cu = cu; a.positions = positions; a.slots = slots; a.ctx_lens = ctx_lens; a.range_out = free_range_out;
   a.batch = batch; a.width = max_blocks; a.cap = n_free; a.tokens = tokens; a.block_size = block_size; a.per = rows_per_request;
+  a.lost = lost;
   const int smem = int((size_t(batch) * 6 + 2) * sizeof(int));
   static bool attr[64] = {};
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k_paged_layout<1024>), (kLayoutMaxBatch * 6 + 2) * int(sizeof(int)), attr);

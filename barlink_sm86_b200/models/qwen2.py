@@ -626,7 +626,7 @@ class DecodeEngine:
 
     kv_bits=4 holds the cache in 4 bits and deals its blocks out on the GPU: requests then have lengths of their own
     (`start`), come and go while the others run (`start`, `finish`), and the captured step takes the blocks that it
-    needs (n_blocks of block_size tokens in all; `blocks_missing`).  rules (ops.LogitRules, one row per request): the greedy token is
+    needs (n_blocks of block_size tokens in all; `blocks_missing`, `tokens_lost`).  rules (ops.LogitRules, one row per request): the greedy token is
     that of the logits under them, and their counts follow the tokens that are produced.
     """
 
@@ -648,6 +648,7 @@ class DecodeEngine:
             self.cache = PagedKV4(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, block_size, n_blocks)
             self.new_lens = torch.zeros(batch, dtype=torch.int32, device=dev)  # 1: the request takes part in steps
             self.running = [False] * batch
+            self.lost = torch.zeros(1, dtype=torch.int32, device=dev)
         else:
             self.cache = PagedKV(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, dt)
         self.ids = torch.zeros(batch, dtype=torch.int32, device=dev)
@@ -674,11 +675,17 @@ class DecodeEngine:
         i32 = dict(dtype=torch.int32, device=new_lens.device)
         into = ops.PagedLayout(torch.empty(self.batch + 1, **i32), torch.empty(tokens, **i32), torch.empty(tokens, **i32),
                                self.ctx_lens, c.free_range)
-        return ops.paged_layout(new_lens, self.ctx_lens, c.block_tables, c.free_list, c.free_range, tokens, c.block_size, into)
+        return ops.paged_layout(new_lens, self.ctx_lens, c.block_tables, c.free_list, c.free_range, tokens, c.block_size, into,
+                                lost=self.lost)
 
     def blocks_missing(self):
-        """Blocks that the last step or `start` could not have (4-bit cache; waits for the GPU): their tokens are not kept."""
+        """Blocks that the last step or `start` could not have (4-bit cache; waits for the GPU).  A page asks once: see tokens_lost."""
         return int(self.cache.free_range[2])
+
+    def tokens_lost(self):
+        """Tokens, over all steps and `start`s of the engine so far, whose keys and values are not kept (4-bit cache; waits for the GPU): no
+        block was free for their page, or their request has grown beyond max_len.  Attention goes on without them."""
+        return int(self.lost)
 
     def finish(self, rows):
         """Requests `rows` have ended: their blocks are free again, and they rest until `start` gives them a new prompt."""
@@ -790,7 +797,7 @@ class DecodeEngine:
         c = self.cache
         if self.kv_bits == 4:
             ops.paged_layout(self.new_lens, self.ctx_lens, c.block_tables, c.free_list, c.free_range, self.batch, c.block_size,
-                             self.layout, rows_per_request=1)
+                             self.layout, rows_per_request=1, lost=self.lost)
         hidden = self.m.decode_hidden(self.ids, self.positions, self.slots, self.ctx_lens, c, self.attn_splits)
         self.m.next_tokens(hidden, self.out_ids, rules=self.rules)
         if self.counted:
@@ -836,7 +843,7 @@ class DecodeEngine:
             return
         state = [self.positions, self.ids]
         if self.kv_bits == 4:
-            state += [self.slots, self.ctx_lens, self.cache.block_tables, self.cache.free_list, self.cache.free_range]
+            state += [self.slots, self.ctx_lens, self.cache.block_tables, self.cache.free_list, self.cache.free_range, self.lost]
         if self.counted:
             state += [self.rules.counts, self.rules.seen]
         saved = [t.clone() for t in state]

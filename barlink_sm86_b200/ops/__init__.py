@@ -465,7 +465,8 @@ class PagedLayout(NamedTuple):
     free_range: torch.Tensor  # int32 [3]: first free entry, free entries, blocks that were missing
 
 
-def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size=16, into=None, rows_per_request=0):
+def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size=16, into=None, rows_per_request=0,
+                 lost=None):
     """Block tables, row offsets, positions and slots of a step, from the requests' lengths, on the GPU and in one launch.
 
     new_lens int32 [batch]: tokens that a request gets now (0 too); below 0: it has ended, and the blocks in its table go back to
@@ -474,7 +475,12 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
     first, count, ignored) are free; blocks are taken from the front in the order of requests and pages, and given back behind the
     last; those given back are free from the next call on.  tokens: rows of `positions` and `slots`, at least the sum of
     new_lens (a token beyond them gets no row).  Where blocks run out, table entries and slots are -1 and free_range[2] counts
-    what was missing; pages beyond max_blocks get no block, their tokens slot -1.
+    what was missing; pages beyond max_blocks get no block, their tokens slot -1.  A page asks for a block once, with its first token: the
+    later tokens of one that got none have slot -1 too, without being counted in free_range[2] again (a block that came now would hold
+    another request's tokens in their place).
+
+    lost: int32 [1], to which the tokens are added that have a row but no slot, whatever the reason; it tells a caller that looks
+    now and then what free_range[2] tells about the last call only.
 
     rows_per_request: 0, or the number of rows that every request has: request b's tokens are rows b * rows_per_request .. then, and
     the rows behind them are empty (a decode step in which some requests rest: 1).
@@ -484,11 +490,12 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
     if new_lens.is_cuda:
         _count(2 if tokens > 2048 else 1)
         return PagedLayout(*_C().paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size,
-                                              rows_per_request, None if into is None else list(into)))
+                                              rows_per_request, None if into is None else list(into), lost))
     if (block_tables.dim() != 2 or past_lens.shape != new_lens.shape or block_tables.shape[0] != new_lens.numel() or block_size < 1 or tokens < 0
-            or free_range.numel() != 3 or not free_list.numel() or rows_per_request < 0):
+            or free_range.numel() != 3 or not free_list.numel() or rows_per_request < 0
+            or (lost is not None and (lost.numel() != 1 or lost.dtype != torch.int32))):
         raise ValueError("paged_layout: one new and one past length and a row of the table per request, a list and a range of free blocks")
-    r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request)
+    r = ref.paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request, lost)
     if into is None:
         return PagedLayout(*r)
     for t, v in zip(into, r):

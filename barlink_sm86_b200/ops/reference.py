@@ -421,8 +421,8 @@ def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale):
 
 
 # ---------------------------------------------------------------- serving steps
-def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request=0):
-    """See ops.paged_layout; block_tables and free_list are updated in place."""
+def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request=0, lost=None):
+    """See ops.paged_layout; block_tables, free_list and lost are updated in place."""
     width, cap = block_tables.shape[1], free_list.numel()
     head, free, _ = (int(v) for v in free_range)
     free = min(max(free, 0), cap)
@@ -447,6 +447,8 @@ def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, token
             pos[row] = p
             blk = int(block_tables[b, p // block_size]) if p // block_size < width else -1
             slots[row] = blk * block_size + p % block_size if blk >= 0 else -1
+            if blk < 0 and lost is not None:
+                lost += 1
         cu.append(cu[-1] + n)
         ctx.append(past + n)
     taken, given = min(need, free), min(len(back), cap - free)
