@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kCountThreads) k_count_tokens(const int* __res
   const int row = blockIdx.y;
   const int lo = cu ? max(cu[row], 0) : row, hi = cu ? min(cu[row + 1], n_ids) : row + 1;
   const int p = prompt ? prompt[row] : 0;
-  for (int i = lo + blockIdx.x * kCountThreads + threadIdx.x; i < hi; i += gridDim.x * kCountThreads) {
+  for (int64_t i = int64_t(lo) + blockIdx.x * kCountThreads + threadIdx.x; i < hi; i += gridDim.x * kCountThreads) {
     const int id = ids[i];
     if (id < 0 || id >= vocab) continue;
     atomicOr(seen + size_t(row) * words + (id >> 5), 1u << (id & 31));
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kCountThreads) k_count_anew(const int* __restr
   pdl_wait();
   const int lo = cu ? max(cu[row], 0) : row, hi = cu ? min(cu[row + 1], n_ids) : row + 1;
   const int p = prompt ? prompt[row] : 0;
-  for (int64_t i0 = lo + tid; i0 < hi; i0 += 4 * kCountThreads) {
+  for (int64_t i0 = int64_t(lo) + tid; i0 < hi; i0 += 4 * kCountThreads) {
     int id[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) id[j] = i0 + j * kCountThreads < hi ? ids[i0 + j * kCountThreads] : -1;

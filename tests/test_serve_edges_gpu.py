@@ -46,3 +46,17 @@ def test_a_captured_step_counts_its_losses():
     for _ in range(5):
         eng.step()
     assert eng.tokens_lost() == 4 + 5 + 3
+
+
+def test_counts_at_the_end_of_32_bits():
+    """As many ids as an int32 offset can name: indexes behind the last one are not taken for negative ones."""
+    n = 2 ** 31 - 1
+    ids = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    last = torch.tensor([3, 99, 3, 40], dtype=torch.int32, device="cuda")
+    ids[-4:] = last
+    for lo, reset in ((0, False), (n - 600, False), (n - 600, True)):
+        r = ops.LogitRules.empty(1, 100)
+        ops.count_tokens(r, ids, torch.tensor([lo, n], dtype=torch.int32, device="cuda"), reset=reset)
+        want = ops.LogitRules.empty(1, 100, "cpu")
+        ops.count_tokens(want, last.cpu(), torch.tensor([0, 4], dtype=torch.int32))
+        assert torch.equal(r.counts.cpu(), want.counts) and torch.equal(r.seen.cpu(), want.seen)
