@@ -651,7 +651,7 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
     return -1;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int words = (vocab + 31) / 32;
+  const int words = int((int64_t(vocab) + 31) / 32);
   if (rows > 65535) {
     set_err(err, errlen, "barlink: count_tokens takes at most 65535 rows");
     return -1;
@@ -660,7 +660,8 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
     // Slices as large as let two blocks share an SM, smaller ones while there are fewer than four for an SM: one row of 152064 in
     // 8 and 32 slices 3.0 and 2.0 us, 64 rows 9.4 and 12.5.
     const int want = 4 * sm_count() / rows, most = want < 1 ? 1 : want > 32 ? 32 : want;
-    const int even = ((vocab + most - 1) / most + 127) / 128 * 128, slice = even < 1024 ? 1024 : even < kCountSlice ? even : kCountSlice;
+    const int64_t even = ((int64_t(vocab) + most - 1) / most + 127) / 128 * 128;
+    const int slice = even < 1024 ? 1024 : even < kCountSlice ? int(even) : kCountSlice;
     const int smem = (slice + 4 + slice / 32) * 4;
     static bool attr[64] = {};
     const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k_count_anew), (kCountSlice + 4 + kCountSlice / 32) * 4, attr);
@@ -668,7 +669,7 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
       set_err(err, errlen, "barlink: count_tokens shared memory opt-in failed: %s", cudaGetErrorString(e));
       return -1;
     }
-    launch_k(k_count_anew, dim3((vocab + slice - 1) / slice, rows), dim3(kCountThreads), smem, st, ids, cu, prompt_lens, counts,
+    launch_k(k_count_anew, dim3(unsigned((int64_t(vocab) + slice - 1) / slice), rows), dim3(kCountThreads), smem, st, ids, cu, prompt_lens, counts,
              static_cast<uint32_t*>(seen), n_ids, vocab, words, slice);
   } else {
     const int x = cu ? (n_ids / rows + kCountThreads - 1) / kCountThreads : 1;
@@ -692,7 +693,7 @@ extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, siz
   a.bias_ids = static_cast<const int*>(r->bias_ids); a.bias = static_cast<const float*>(r->bias);
   a.mask = static_cast<const uint32_t*>(r->mask);
   a.rows = r->rows; a.n = r->n; a.vocab = r->vocab; a.offset = r->offset; a.n_bias = r->n_bias;
-  a.words = (r->vocab + 31) / 32;
+  a.words = int((int64_t(r->vocab) + 31) / 32);
   a.ld = r->ld; a.ld_out = r->ld_out; a.ld_mask = r->ld_mask;
   a.idx = static_cast<int*>(r->idx); a.val = static_cast<float*>(r->val);
   // Blocks of a row: as many as leave all of them resident at once (two to an SM), none with less than 2048 logits.

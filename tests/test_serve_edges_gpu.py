@@ -60,3 +60,19 @@ def test_counts_at_the_end_of_32_bits():
         want = ops.LogitRules.empty(1, 100, "cpu")
         ops.count_tokens(want, last.cpu(), torch.tensor([0, 4], dtype=torch.int32))
         assert torch.equal(r.counts.cpu(), want.counts) and torch.equal(r.seen.cpu(), want.seen)
+
+
+def test_the_largest_vocabulary():
+    """2^31 - 1 tokens: numbers of words and slices are those of 64-bit arithmetic; the second row's tables begin behind the first's."""
+    vocab = 2 ** 31 - 1
+    r = ops.LogitRules.empty(2, vocab)
+    ids = torch.tensor([0, vocab - 1, vocab - 2, vocab - 2], dtype=torch.int32, device="cuda")
+    for reset in (True, False):
+        ops.count_tokens(r, ids, torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda"), reset=reset)
+    assert r.counts[:, -2:].tolist() == [[0, 2], [4, 0]] and int(r.counts[0, 0]) == 2 and int(r.counts[1, 0]) == 0
+    assert r.seen[:, -1].tolist() == [1 << 30, 1 << 29] and r.seen[:, 0].tolist() == [1, 0]
+    r.penalties[:, 2] = 1.0
+    x = torch.tensor([[5.0, 6.0, 7.0], [5.0, 9.0, 7.0]], device="cuda")
+    got = ops.logits_process(x, r, offset=vocab - 3)
+    assert got.tolist() == [[5.0, 6.0, 5.0], [5.0, 5.0, 7.0]]
+    assert ops.logits_argmax(x, r, offset=vocab - 3)[0].tolist() == [vocab - 2, vocab - 1]
