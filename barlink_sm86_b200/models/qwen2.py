@@ -643,7 +643,8 @@ class DecodeEngine:
         if rules is not None and any(t is not None and t.shape[0] != batch for t in rules._args()):
             raise ValueError("rules must have one row per request")
         self.kv_bits, self.rules = kv_bits, rules
-        self.counted = rules is not None and rules.counts is not None  # (a mask or biases alone go by no counts)
+        # (a mask or biases alone go by no counts)
+        self.counted = rules is not None and rules.counts is not None and rules.seen is not None
         if kv_bits == 4:
             self.cache = PagedKV4(len(model.w.layers), batch, max_len, model.nkv, model.hd, dev, block_size, n_blocks)
             self.new_lens = torch.zeros(batch, dtype=torch.int32, device=dev)  # 1: the request takes part in steps

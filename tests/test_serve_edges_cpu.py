@@ -49,3 +49,13 @@ def test_lost_refusals():
     for bad in (i, i[:1].long()):
         with pytest.raises(ValueError):
             ops.paged_layout(**call, lost=bad)
+
+
+@pytest.mark.parametrize("kv_bits", [4, 16])
+@pytest.mark.parametrize("table", ["counts", "seen"])
+def test_rules_with_one_of_the_two_tables(kv_bits, table):
+    """Without penalties nothing reads them: a run does without either."""
+    rules = ops.LogitRules(**{table: torch.zeros(2, 500 if table == "counts" else 16, dtype=torch.int32)}, vocab=500)
+    eng = DecodeEngine(_model(), 2, 64, kv_bits=kv_bits, rules=rules)
+    eng.ids.copy_(eng.prefill(_ids(20).view(2, 10)))
+    assert eng.step().shape == (2,)
