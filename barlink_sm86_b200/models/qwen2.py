@@ -755,6 +755,8 @@ class DecodeEngine:
     def set_context(self, length: int):
         """Declare that every sequence already has `length` tokens in the cache."""
         if self.kv_bits == 4:
+            if not 0 <= length <= self.max_len:
+                raise ValueError("a context has 0 to max_len tokens")
             self.finish(range(self.batch))
             self._lay_out(torch.full_like(self.new_lens, length))
             self.new_lens.fill_(1)

@@ -59,3 +59,13 @@ def test_rules_with_one_of_the_two_tables(kv_bits, table):
     eng = DecodeEngine(_model(), 2, 64, kv_bits=kv_bits, rules=rules)
     eng.ids.copy_(eng.prefill(_ids(20).view(2, 10)))
     assert eng.step().shape == (2,)
+
+
+def test_a_context_longer_than_the_table():
+    eng = DecodeEngine(_model(), 2, 64, kv_bits=4)
+    eng.set_context(64)
+    assert eng.ctx_lens.tolist() == [64, 64]
+    for length in (65, -1):
+        with pytest.raises(ValueError):
+            eng.set_context(length)
+    assert eng.ctx_lens.tolist() == [64, 64]
