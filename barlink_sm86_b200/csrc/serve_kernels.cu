@@ -672,7 +672,7 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
     launch_k(k_count_anew, dim3(unsigned((int64_t(vocab) + slice - 1) / slice), rows), dim3(kCountThreads), smem, st, ids, cu, prompt_lens, counts,
              static_cast<uint32_t*>(seen), n_ids, vocab, words, slice);
   } else {
-    const int x = cu ? (n_ids / rows + kCountThreads - 1) / kCountThreads : 1;
+    const int x = cu ? int((int64_t(n_ids) / rows + kCountThreads - 1) / kCountThreads) : 1;
     launch_k(k_count_tokens, dim3(x < 1 ? 1 : x > 64 ? 64 : x, rows), dim3(kCountThreads), 0, st, ids, cu, prompt_lens, counts,
              static_cast<uint32_t*>(seen), n_ids, vocab, words);
   }
