@@ -998,6 +998,10 @@ extern "C" int bl_kv4_read(const void* cache, const int* slots, void* k, void* v
     return -1;
   }
   if (rows == 0) return 0;
+  if ((!cache && n_blocks) || !slots || !k || !v || ((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) {
+    set_err(err, errlen, "barlink: kv4_read needs slots, and a cache and outputs on 16-byte boundaries");
+    return -1;
+  }
   const int per = nkv * (hd / 8), block_rows = per >= 256 ? 1 : 256 / per;
   launch_k(hd == 64 ? k_kv4_read<64> : k_kv4_read<128>, dim3((rows + block_rows - 1) / block_rows), dim3(256), 0, static_cast<cudaStream_t>(stream),
            static_cast<const uint8_t*>(cache), slots, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), rows, block_rows, nkv,
@@ -1027,6 +1031,7 @@ extern "C" unsigned bl_kv4_wait_polls(unsigned polls) { return g_kv4_polls.excha
 static int q4_grid() { return sm_count() * 2; }
 
 extern "C" size_t bl_paged_attn_decode_q4_ws(int batch, int nq, int nkv, int hd) {
+  if (batch < 1 || nkv < 1 || nq < 1) return 0;
   const int G = nq / nkv;
   return 2 * size_t(q4_grid()) * kQ4Warps * q4_part_floats(G, hd) * sizeof(float) + size_t(batch) * nkv * sizeof(int2);
 }
@@ -1039,6 +1044,10 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs nq %% nkv == 0 and at most %d query heads per KV head", kQ4MaxG);
     return -1;
   }
+  if (batch < 0) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache: a negative batch");
+    return -1;
+  }
   // (runs are counted in 32 bits, one of them beyond the last tile)
   if (int64_t(max_blocks) * block_size > 0x7fffffffLL - 16 || int64_t(max_blocks) * (block_size / kQ4Tokens) * batch * nkv > 0x3fffffffLL) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache: the tables' tokens, times KV heads, must not exceed 2^34");
@@ -1047,6 +1056,10 @@ extern "C" int bl_paged_attn_decode_q4(const void* q, int q_stride, const void* 
   if (batch == 0) return 0;
   if (max_blocks < 1) {
     set_err(err, errlen, "barlink: attention over the 4-bit cache needs a table");
+    return -1;
+  }
+  if (!q || (!cache && n_blocks) || !block_tables || !ctx_lens || !out) {
+    set_err(err, errlen, "barlink: attention over the 4-bit cache needs queries, a cache, block tables, context lengths and an output");
     return -1;
   }
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) |

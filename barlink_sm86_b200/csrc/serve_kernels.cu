@@ -620,6 +620,11 @@ extern "C" int bl_paged_layout_counting(const int* new_lens, const int* past_len
     set_err(err, errlen, "barlink: paged_layout: the cache's slots and the table's entries must fit 32 bits");
     return -1;
   }
+  if (!new_lens || !past_lens || !block_tables || !free_list || !free_range || !cu || !ctx_lens || !free_range_out ||
+      (tokens > 0 && (!positions || !slots))) {
+    set_err(err, errlen, "barlink: paged_layout needs its lengths, table, list and range of free blocks, and all outputs");
+    return -1;
+  }
   RequestLayout a;
   a.new_lens = new_lens; a.past_lens = past_lens; a.tables = block_tables; a.ring = free_list; a.range = free_range;
   a.cu = cu; a.positions = positions; a.slots = slots; a.ctx_lens = ctx_lens; a.range_out = free_range_out;
@@ -646,7 +651,11 @@ extern "C" int bl_paged_layout_counting(const int* new_lens, const int* past_len
 
 extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_lens, int* counts, void* seen, int rows, int n_ids,
                                int vocab, int reset, void* stream, char* err, size_t errlen) {
-  if (rows < 1 || vocab < 1 || (!cu && n_ids != rows)) {
+  if (rows < 1 || vocab < 1 || n_ids < 0 || !counts || !seen || (n_ids > 0 && !ids)) {
+    set_err(err, errlen, "barlink: count_tokens needs ids, and tables of rows and a vocabulary");
+    return -1;
+  }
+  if (!cu && n_ids != rows) {
     set_err(err, errlen, "barlink: count_tokens needs one id per row, or row offsets");
     return -1;
   }
@@ -681,7 +690,7 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
 }
 
 extern "C" int bl_logit_rules(const blRulesArgs* r, void* stream, char* err, size_t errlen) {
-  if (r->rows < 1 || r->n < 1 || !r->out == !r->idx || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
+  if (r->rows < 1 || r->n < 1 || !r->logits || r->n_bias < 0 || r->offset < 0 || !r->out == !r->idx || !r->idx != !r->val || (r->penalties && (!r->counts || !r->seen)) ||
       (r->n_bias > 0 && (!r->bias_ids || !r->bias)) || r->vocab < 0 ||
       (r->mask && int64_t(r->mask_words) * 32 < r->vocab)) {
     set_err(err, errlen, "barlink: logit rules need logits, an output, and the tables of the rules that are set");

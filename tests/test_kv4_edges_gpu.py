@@ -159,3 +159,12 @@ def test_the_engine_reports_a_wait_that_ran_out(ext, polls):
     eng.finish([0, 1])
     eng.start(prompt, [40, 20])
     assert torch.equal(eng.step_host(first), want)
+
+
+def test_a_cache_without_blocks():
+    """Nothing is there: zeros."""
+    cache = ops.kv4_cache(0, 2, 128)
+    slots = torch.tensor([0, -1, 5], dtype=torch.int32, device="cuda")
+    assert not any(bool(t.any()) for t in ops.kv4_read(cache, slots, 128))
+    q = _randn(260, 3, 4 * 128).bfloat16()
+    assert not bool(ops.paged_attn_decode_q4(q, cache, slots[:, None].contiguous(), slots.abs(), 4, 2, 128, 0.1).any())

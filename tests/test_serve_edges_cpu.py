@@ -1,8 +1,11 @@
 # SPDX-License-Identifier: MIT
 """Serving on the 4-bit cache where a run leaves the ordinary, on the CPU path: blocks run out, requests outgrow their tables."""
+import ctypes
+
 import pytest
 import torch
 
+import barlink_sm86_b200 as bl
 from barlink_sm86_b200 import ops
 from barlink_sm86_b200.models import DecodeEngine, Qwen2Config, Qwen2Model
 
@@ -69,3 +72,38 @@ def test_a_context_longer_than_the_table():
         with pytest.raises(ValueError):
             eng.set_context(length)
     assert eng.ctx_lens.tolist() == [64, 64]
+
+
+def test_plain_c_entries_refuse_what_they_cannot_read():
+    """No pointer, or one that a 16-byte access would not take, gets as far as a launch; sizes that no workspace has are 0 bytes."""
+    p, i, f, d, s, e = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_size_t, ctypes.create_string_buffer(512)
+    lib = ctypes.CDLL(bl.load_extension().__file__)
+
+    def refused(name, types, *args):
+        fn = getattr(lib, name)
+        fn.argtypes = [*types, p, ctypes.c_char_p, s]
+        e.value = b""
+        return fn(*args, None, e, 512) == -1 and e.value.startswith(b"barlink: ")
+
+    read = ("bl_kv4_read", [p] * 4 + [i] * 5)
+    for ptrs in ((None, 16, 16, 16), (16, None, 16, 16), (16, 16, None, 16), (16, 16, 16, None), (24, 16, 16, 16), (16, 16, 8, 16), (16, 16, 16, 4)):
+        assert refused(*read, *ptrs, 1, 1, 128, 16, 1)
+    lib.bl_paged_attn_decode_q4_ws.restype = s
+    for sizes in ((1, 4, 0, 128), (1, 0, 1, 128), (0, 4, 1, 128), (-1, 4, 1, 128)):
+        assert lib.bl_paged_attn_decode_q4_ws(*sizes) == 0
+    attn = ("bl_paged_attn_decode_q4", [p, i] + [p] * 4 + [i] * 7 + [f, p, s])
+    sizes = (1, 4, 1, 128, 16, 1, 1)
+    for q, *ptrs in ((None, 16, 16, 16, 16), (16, None, 16, 16, 16), (16, 16, None, 16, 16), (16, 16, 16, None, 16), (16, 16, 16, 16, None)):
+        assert refused(*attn, q, 512, *ptrs, *sizes, 0.1, 16, 1 << 30)
+    assert refused(*attn, 16, 512, 16, 16, 16, 16, -1, *sizes[1:], 0.1, 16, 1 << 30)
+    layout = ("bl_paged_layout", [p] * 10 + [i] * 6)
+    for k in range(10):
+        assert refused(*layout, *(None if j == k else 16 for j in range(10)), 1, 1, 1, 1, 16, 0)
+    count = ("bl_count_tokens", [p] * 5 + [i] * 4)
+    for ptrs in ((None, 16, None, 16, 16), (16, 16, None, None, 16), (16, 16, None, 16, None)):
+        assert refused(*count, *ptrs, 1, 1, 10, 1)
+    assert refused(*count, 16, 16, None, 16, 16, 1, -1, 10, 0) and refused(*count, 16, None, None, 16, 16, 2, 1, 10, 0)
+    write = ("bl_rope_kv_write_q4", [p, p, i, s] + [p] * 5 + [i] * 6 + [d])
+    for ptrs in ((None, 16, 16, 16, 16), (16, None, 16, 16, 16), (16, 16, None, 16, 16), (16, 16, 16, 16, None), (8, 16, 16, 16, 16), (16, 16, 16, 16, 8)):
+        qkv, out, pos, slots, cache = ptrs
+        assert refused(*write, qkv, None, 0, 0, None, out, pos, slots, cache, 1, 1, 1, 128, 16, 1, 1e4)
