@@ -718,6 +718,14 @@ class DecodeEngine:
         out = self.ids.clone()
         if not ids.numel():
             return out
+        try:
+            return self._start(ids, lens, max_tokens, out)
+        except BaseException:
+            # (their blocks were dealt out before the model ran)
+            self.finish([b for b in range(self.batch) if lens[b]])
+            raise
+
+    def _start(self, ids, lens, max_tokens, out):
         dev = self.positions.device
         new = torch.tensor(lens, dtype=torch.int32).to(dev)
         lay = self._lay_out(new, ids.numel())

@@ -107,3 +107,30 @@ def test_plain_c_entries_refuse_what_they_cannot_read():
     for ptrs in ((None, 16, 16, 16, 16), (16, None, 16, 16, 16), (16, 16, None, 16, 16), (16, 16, 16, 16, None), (8, 16, 16, 16, 16), (16, 16, 16, 16, 8)):
         qkv, out, pos, slots, cache = ptrs
         assert refused(*write, qkv, None, 0, 0, None, out, pos, slots, cache, 1, 1, 1, 128, 16, 1, 1e4)
+
+
+def test_a_start_that_fails_leaves_the_engine_as_it_was(monkeypatch):
+    """An error of the model in the middle of the passes: no request holds blocks, and the same call can be made again."""
+    m = _model()
+    want = DecodeEngine(m, 3, 64, kv_bits=4)
+    want.ids.copy_(want.start(_ids(50), [30, 0, 20]))
+    eng = DecodeEngine(m, 3, 64, kv_bits=4)
+    run, calls = m.prefill_packed, []
+
+    def fails(*a):
+        calls.append(a)
+        if len(calls) == 2:
+            raise MemoryError("no memory")
+        return run(*a)
+
+    monkeypatch.setattr(m, "prefill_packed", fails)
+    eng.ids.copy_(eng.start(_ids(9), [0, 9, 0]))
+    eng.step()
+    with pytest.raises(MemoryError):
+        eng.start(_ids(50), [30, 0, 20], max_tokens=30)
+    assert eng.ctx_lens.tolist() == [0, 10, 0] and eng.running == [False, True, False] and eng.new_lens.tolist() == [0, 1, 0]
+    assert int(eng.cache.free_range[1]) == 11
+    out = eng.start(_ids(50), [30, 0, 20], max_tokens=30)
+    assert out.tolist()[::2] == want.ids.tolist()[::2]
+    eng.ids.copy_(out)
+    assert eng.step().tolist()[::2] == want.step().tolist()[::2]
