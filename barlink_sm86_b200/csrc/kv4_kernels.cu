@@ -976,7 +976,9 @@ extern "C" int bl_rope_kv_write_q4(const void* qkv, const void* slabs, int nspli
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Many rows: four to a block, a warp each that goes through the heads (8191 rows of 36 heads: 35 us; two warps a row and three heads at
   // a time 37 to 48, by registers); few rows (a decode step) and slabs: a row's heads dealt out to blocks, each thread with one octet.
-  const bool many = rows > 4 * sm_count() && !a.slabs;
+  // us, a row and four to a block: 36 heads of 128, 592 rows 5.9 and 7.1, 2000 rows 13.4 and 17.4, 3200 19.6 and 18.7, 4000 24.1 and 18.9; 56
+  // heads, 2000 rows 18.2 and 26.7, 3200 29.8 and 29.4; 12 heads of 64, 900 rows 3.8 and 4.3, 1200 5.3 and 4.4.
+  const bool many = rows > (hd == 128 ? 22 : 7) * sm_count() && !a.slabs;
   const int heads = nq + 2 * nkv, step = 128 / (hd / 16);
   const dim3 grid(many ? (rows + 3) / 4 : rows, many ? 1 : (heads + step - 1) / step), block(128);
   if (hd == 128) {

@@ -168,3 +168,17 @@ def test_a_cache_without_blocks():
     assert not any(bool(t.any()) for t in ops.kv4_read(cache, slots, 128))
     q = _randn(260, 3, 4 * 128).bfloat16()
     assert not bool(ops.paged_attn_decode_q4(q, cache, slots[:, None].contiguous(), slots.abs(), 4, 2, 128, 0.1).any())
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(3, 2, 128), (5, 1, 64)])
+@pytest.mark.parametrize("more", [0, 1, 2, 7])
+def test_write_on_both_sides_of_the_line(nq, nkv, hd, more):
+    """As many rows as get blocks of their own, and more: the same rows and bytes as in parts."""
+    rows = (22 if hd == 128 else 7) * torch.cuda.get_device_properties(0).multi_processor_count + more
+    x = _randn(270, rows, (nq + 2 * nkv) * hd).bfloat16()
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda") * 11
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    caches = [ops.kv4_cache(rows // 16 + 1, nkv, hd).fill_(0xFF) for _ in range(2)]
+    whole = ops.rope_kv_write_q4(x.clone(), pos, slots, caches[0], nq, nkv, hd, 16, 1e6)
+    parts = [ops.rope_kv_write_q4(x[i:i + 500].clone(), pos[i:i + 500], slots[i:i + 500], caches[1], nq, nkv, hd, 16, 1e6) for i in range(0, rows, 500)]
+    assert torch.equal(whole, torch.cat(parts)) and torch.equal(*caches)
