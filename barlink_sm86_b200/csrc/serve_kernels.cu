@@ -25,7 +25,9 @@ namespace bl {
 // block tables, row offsets, positions and slots
 // ---------------------------------------------------------------------------
 constexpr int kLayoutMaxBatch = 8192;
-constexpr int kLayoutAlone = 2048;  // rows up to which the one block writes them itself
+// Rows up to which the one block writes them itself.  us, alone and with a second kernel: 64 requests with 2048 rows 6.1 and 6.7, with 4096
+// 8.8 and 6.8; 256 requests 5.5 and 6.4, 9.6 and 7.2.
+constexpr int kLayoutAlone = 2048;
 
 struct RequestLayout {
   const int* new_lens;  // tokens that a request gets now; below 0: it has ended
@@ -417,8 +419,12 @@ __device__ __forceinline__ void warp_best(float& best, int& bi) {
 // us: one pass that branches into the penalties for every vector with a seen token 30; the seen words dealt out to warps 20.
 constexpr int kRulesThreads = 512;
 constexpr int kRulesShare = 8;    // blocks of a row at most
-constexpr int kRulesLap = 5;      // vectors that a thread takes at a time
-constexpr int kRulesList = 6144;  // seen tokens of a block that are put off; what is beyond is dealt with on the spot
+// Vectors that a thread takes at a time.  us with 2, 3, 4, 5, 6, 8: 64 x 152064 7.9, 8.1, 8.2, 7.8, 8.6, 13.7; 256 x 152064 25.1, 23.9, 24.1, 23.8,
+// 25.8, 47; 64 x 50257 5.8, 6.1, 5.8, 5.9, 6.4, 9.4; 64 x 32000, where few threads have as many, 4.1, 4.4, 4.8, 4.9, 5.4, 7.5.
+constexpr int kRulesLap = 5;
+// Seen tokens of a block that are put off; what is beyond is dealt with on the spot.  1024 to 8192 take the same time, rows of 8000 tokens
+// among them.
+constexpr int kRulesList = 6144;
 template <typename T, bool PICK>  // the arg max, or the logits under the rules
 __global__ void __launch_bounds__(kRulesThreads, 2) k_logit_rules(const Rules a) {
   extern __shared__ uint32_t s_rules[];  // with biases: a bit per column that an entry names; the entries' columns and values
@@ -638,8 +644,9 @@ extern "C" int bl_paged_layout_counting(const int* new_lens, const int* past_len
     return -1;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // (a decode step: a block whose barriers are cheap)
-  const bool few = batch <= 256 && tokens <= 512;
+  // A decode step: a block whose barriers are cheap, while it has a row and a request for each thread at most.  us, 256 and 1024 threads:
+  // 64 requests of one token 3.1 and 3.7, 256 3.3 and 3.9, 256 of two 4.2 and 3.9, 512 4.9 and 4.1.
+  const bool few = batch <= 256 && tokens <= 256;
   launch_k(few ? k_paged_layout<256> : k_paged_layout<1024>, dim3(1), dim3(few ? 256 : 1024), smem, st, a);
   SERVE_LAUNCH_CHECK("paged_layout");
   if (tokens > kLayoutAlone) {
