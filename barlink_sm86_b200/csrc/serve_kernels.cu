@@ -673,8 +673,8 @@ extern "C" int bl_count_tokens(const int* ids, const int* cu, const int* prompt_
     return -1;
   }
   if (reset) {
-    // Slices as large as let two blocks share an SM, smaller ones while there are fewer than four for an SM: one row of 152064 in
-    // 8 and 32 slices 3.0 and 2.0 us, 64 rows 9.4 and 12.5.
+    // Four blocks for an SM, by slices of 1024 to kCountSlice tokens and up to 32 for a row: one row of 152064 in 8 and 32 slices 3.0 and 2.0 us,
+    // 64 rows 9.4 and 12.5.  (64 rows: 9 slices of 16896, 576 blocks, of which shared memory lets three on an SM, 444 at once.)
     const int want = 4 * sm_count() / rows, most = want < 1 ? 1 : want > 32 ? 32 : want;
     const int64_t even = ((int64_t(vocab) + most - 1) / most + 127) / 128 * 128;
     const int slice = even < 1024 ? 1024 : even < kCountSlice ? int(even) : kCountSlice;

@@ -627,7 +627,8 @@ class DecodeEngine:
     kv_bits=4 holds the cache in 4 bits and deals its blocks out on the GPU: requests then have lengths of their own
     (`start`), come and go while the others run (`start`, `finish`), and the captured step takes the blocks that it
     needs (n_blocks of block_size tokens in all; `blocks_missing`, `tokens_lost`).  rules (ops.LogitRules, one row per request): the greedy token is
-    that of the logits under them, and their counts follow the tokens that are produced.
+    that of the logits under them, and their counts follow the tokens that are produced.  Either takes the plain decode path, also where the
+    folded or the fused one would run without it.
     """
 
     def __init__(self, model: Qwen2Model, batch: int, max_len: int, use_graph: bool = True,

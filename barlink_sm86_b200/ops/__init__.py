@@ -442,7 +442,9 @@ def kv4_read(cache, slots, hd, block_size=16):
 def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, out=None):
     """`paged_attn_decode` over a 4-bit cache: q bf16 [batch, >= nq * hd] (the first nq * hd columns; rows start on 16-byte boundaries),
     block_tables int32 [batch, max_blocks], ctx_lens int32 [batch].  At most 16 query heads per KV head.  A table entry that names no
-    block leaves its tokens out; a request without tokens gets zeros.  scale > 0.  Returns bf16 [batch, nq * hd]."""
+    block leaves its tokens out; a request without tokens gets zeros.  scale > 0.  Queries are below 2^117 in absolute value.  A group
+    whose steps lie 2^14 or more below those of the head's other groups loses places, because probabilities times steps are fp16.
+    Returns bf16 [batch, nq * hd]."""
     if not scale > 0:
         raise ValueError("attention over the 4-bit cache needs a positive scale")
     if q.is_cuda:
@@ -467,7 +469,8 @@ class PagedLayout(NamedTuple):
 
 def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size=16, into=None, rows_per_request=0,
                  lost=None):
-    """Block tables, row offsets, positions and slots of a step, from the requests' lengths, on the GPU and in one launch.
+    """Block tables, row offsets, positions and slots of a step, from the requests' lengths, on the GPU and in one launch (two beyond
+    2048 rows).
 
     new_lens int32 [batch]: tokens that a request gets now (0 too); below 0: it has ended, and the blocks in its table go back to
     the free ones.  past_lens int32 [batch]: tokens in the cache before.  block_tables int32 [batch, max_blocks]: the entries of new pages
@@ -552,7 +555,7 @@ class LogitRules:
 def count_tokens(rules, ids, cu=None, prompt_lens=None, reset=False):
     """Adds tokens to the tables of `rules`: every one is seen, and one behind a row's first prompt_lens (int32 [rows]; None: 0) is
     counted as produced.  ids int32 [rows]: one token per row; with cu int32 [rows + 1]: row b's are ids[cu[b]:cu[b + 1]].  Ids below 0
-    or beyond the vocabulary are passed over.  reset: the tables are emptied first."""
+    or beyond the vocabulary are passed over.  reset: the tables are emptied first.  At most 65535 rows on a GPU."""
     if rules.counts is None or rules.seen is None:
         raise ValueError("count_tokens needs rules with the counts and seen tables")
     if rules.counts.is_cuda:
