@@ -284,9 +284,9 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ ca
 // Queries go in as fp16 of a power of two per head (exact: 2^-27 of the head's largest element is still whole).  The reference of
 // the running softmax is the greatest of x_t + e_t, e_t = log2 of the token's largest step, so that p step stays within fp16 whatever the
 // values' size, or of its largest |low| over 2^95, if that is more: a group of one value has no step, and p low has to stay within
-// fp32.  It moves only when p step exceeds it by 2^8, when a lane's four tokens have (next to) no steps, or when there is a low of 2^65
-// or more, which one vote per unit finds out.  Between the votes p is at most 2^29 where a token has less than 2^65, so that p low
-// is below 2^97 and its sums are finite, whatever the context's length.  (What that costs: beside a low above 2^95, groups with steps below
+// fp32.  It moves only when p step exceeds it by 2^8, when a lane's four tokens have next to no steps and lows that matter there, or when there
+// is a low of 2^65 or more, which one vote per unit finds out.  Between the votes p is at most 2^29 where a token has less than 2^65, so
+// that p low is below 2^97 and its sums are finite, whatever the context's length.  (What that costs: beside a low above 2^95, groups with steps below
 // 2^-14 of low / 2^95 lose places.)
 //
 // Work: the units (two tiles) of all (request, KV head) pairs in one row, cut into equal runs, one for each warp; a warp has a
@@ -664,20 +664,21 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
             }
       }
       // ---- probabilities; where one times step may leave fp16's range, a new reference first ----
-      float top;  // the largest of the steps here (bf16 above 0 compare as integers); 2^39 where they do not bound p low
+      float steps, top;  // the largest of the steps here (bf16 above 0 compare as integers); the same, or 2^39 where it does not bound p low
       {
         uint32_t m = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < NA / 2; ++i) m = __vmaxu2(m, __vmaxu2(vs0[u][i], vs1[u][i]));
-        top = fmaxf(bf16_lo(m), bf16_hi(m));
-        if (top < 9.5367431640625e-7f) top = 549755813888.f;  // (2^-20: p up to 2^-30 passes, tokens that are not there among them)
+        steps = fmaxf(bf16_lo(m), bf16_hi(m));
+        top = steps < 9.5367431640625e-7f ? 549755813888.f : steps;  // (2^-20: p up to 2^-30 passes, tokens that are not there among them)
       }
-      uint32_t vast;  // token `lane` of the unit has a low of 2^65 or more: the two highest bits of its exponent
+      const uint32_t lows = tile + (lane >> 4) * TB + q4_v_params(HD) + (lane & 15) * NA * 4 + NA * 2;  // of token `lane` of the unit
+      uint32_t vast;  // one of 2^65 or more is among them: the two highest bits of its exponent
       {
         uint32_t w[NA / 2];
-        lds_words<NA / 2>(tile + (lane >> 4) * TB + q4_v_params(HD) + (lane & 15) * NA * 4 + NA * 2, w);
+        lds_words<NA / 2>(lows, w);
         vast = w[0] & w[0] << 1;
         if constexpr (NA == 4) vast |= w[1] & w[1] << 1;
         vast &= lane < left && !(no_block >> (lane >> 4) & 1) ? 0x40004000u : 0u;
@@ -697,7 +698,17 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) k_paged_attn_q4(const Q4Attn
         return most;
       };
       const float most = weigh();
-      if (__any_sync(kAll, !(most * top <= 512.f) || vast)) {  // (NaN too: it is of one head, and would hide what the lane's others ask for)
+      // (NaN too: it is of one head, and would hide what the lane's others ask for)
+      bool move = __any_sync(kAll, !(most * top <= 512.f) || vast);
+      if (move && !__any_sync(kAll, !(most * fmaxf(steps, 6.4623485355705287e-27f) <= 512.f))) {
+        // next to no steps, and p at most 2^96: lows below 2^-2 (zeros, most of all) need no other reference
+        uint32_t w[NA / 2], large = 0;
+        lds_words<NA / 2>(lows, w);
+#pragma unroll
+        for (int i = 0; i < NA / 2; ++i) large |= __vcmpgeu2(w[i] & 0x7fff7fffu, 0x3e803e80u);
+        move = __any_sync(kAll, large && lane < left && !(no_block >> (lane >> 4) & 1));
+      }
+      if (move) {
         float e[2][2];  // log2 of a token's largest step, rounded down, or that of its largest low less 95
 #pragma unroll
         for (int u = 0; u < 2; ++u)
