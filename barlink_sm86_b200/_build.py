@@ -29,6 +29,7 @@ SOURCES = [
     "w4a16_kernels.cu",
     "kv4_kernels.cu",
     "serve_kernels.cu",
+    "score_kernels.cu",
     "backend.cc",
     "binding.cc",
     "binding_extra.cc",

@@ -8,6 +8,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <tuple>
 
 #include "bl_ops.h"
@@ -305,6 +306,43 @@ std::vector<at::Tensor> logit_rules(const at::Tensor& logits, bool pick, int64_t
   return r;
 }
 
+// (given, entropy, top_ids, top_val); raw: parts [rows, 3] in place of the entropy
+std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& ids, int64_t top, int64_t offset, int64_t vocab, bool raw) {
+  const bool fp32 = logits.scalar_type() == at::kFloat;
+  TORCH_CHECK(logits.is_cuda() && (fp32 || logits.scalar_type() == at::kBFloat16) && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1) &&
+                  (logits.size(0) < 2 || logits.stride(0) >= logits.size(1)),
+              "barlink: token_logprobs needs 2-D bfloat16 or float32 CUDA logits with dense rows");
+  TORCH_CHECK(ids.dim() >= 1 && ids.dim() <= 2 && ids.size(0) == logits.size(0), "barlink: ids must be int32 [rows] or [rows, tokens]");
+  TORCH_CHECK(top >= 0 && top <= 32, "barlink: token_logprobs gives 0 to 32 alternatives");
+  TORCH_CHECK(offset >= 0 && vocab >= 0 && offset + logits.size(1) <= 0x7fffffff, "barlink: token ids must fit 32 bits");
+  blScoreArgs a = {};
+  a.rows = small(logits.size(0), "rows");
+  a.n = small(logits.size(1), "columns");
+  a.fp32 = fp32;
+  a.vocab = int(std::min<int64_t>(vocab, 0x7fffffff));
+  a.offset = int(offset);
+  a.logits = logits.data_ptr();
+  a.ld = size_t(logits.stride(0));
+  a.ids = i32(ids, logits, -1, "ids");
+  a.n_ids = ids.dim() == 1 ? 1 : small(ids.size(1), "tokens of a row");
+  a.top = int(top);
+  a.raw = raw;
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t rows = a.rows, n[4] = {rows * a.n_ids, raw ? 3 * rows : rows, rows * top, rows * top};
+  int64_t at[5] = {0};
+  for (int i = 0; i < 4; ++i) at[i + 1] = at[i] + to16(4 * n[i]);
+  const at::Tensor all = fresh({at[4]}, at::kByte, logits);
+  std::vector<at::Tensor> r = {part_of(all, at::kFloat, at[0], ids.sizes()),
+                               raw ? part_of(all, at::kFloat, at[1], {rows, 3}) : part_of(all, at::kFloat, at[1], {rows}),
+                               part_of(all, at::kInt, at[2], {rows, top}), part_of(all, at::kFloat, at[3], {rows, top})};
+  a.given = r[0].data_ptr();
+  (raw ? a.parts : a.entropy) = r[1].data_ptr();
+  a.top_ids = r[2].data_ptr();
+  a.top_val = r[3].data_ptr();
+  if (a.rows > 0) BL_CHECK(bl_token_logprobs(&a, stream_of(logits), err, errlen));
+  return r;
+}
+
 }  // namespace
 
 void bind_serve(py::module_& m) {
@@ -325,4 +363,6 @@ void bind_serve(py::module_& m) {
   m.def("logit_rules", &logit_rules, py::arg("logits"), py::arg("pick"), py::arg("vocab"), py::arg("offset") = 0,
         py::arg("penalties") = py::none(), py::arg("counts") = py::none(), py::arg("seen") = py::none(), py::arg("bias_ids") = py::none(),
         py::arg("bias") = py::none(), py::arg("mask") = py::none(), py::arg("out") = py::none());
+  m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("ids"), py::arg("top") = 0, py::arg("offset") = 0, py::arg("vocab") = 0x7fffffff,
+        py::arg("raw") = false);
 }

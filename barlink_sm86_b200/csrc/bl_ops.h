@@ -500,6 +500,26 @@ typedef struct blRulesArgs {
 } blRulesArgs;
 int bl_logit_rules(const blRulesArgs* a, void* stream, char* err, size_t errlen);
 
+/* ---- scores of tokens (score_kernels.cu) -------------------------------------------------------------
+ * Logits [rows][n] (bf16, or fp32), token id = column + offset, columns behind the vocabulary left out.  With m = max x, S = sum e^(x - m),
+ * T = sum (x - m) e^(x - m): given = x_id - m - log S of every id (-inf where these columns have no such token), entropy = log S - T / S, and the
+ * `top` (0 to 32) greatest with theirs (the lowest index of equals, NaN passed over; id -1, -inf where nothing above -inf is left).
+ * raw: given and top_val are logits, and parts [rows][3] = m, S, T instead of the entropy (what shards of a vocabulary are joined from). */
+typedef struct blScoreArgs {
+  const void* logits;
+  size_t ld;
+  int rows, n, fp32;
+  int vocab, offset;
+  const void* ids; /* int32 [rows][n_ids] */
+  int n_ids, top, raw;
+  void* given;   /* fp32 [rows][n_ids] */
+  void* entropy; /* fp32 [rows] */
+  void* top_ids; /* int32 [rows][top] */
+  void* top_val; /* fp32 [rows][top] */
+  void* parts;   /* fp32 [rows][3], with raw */
+} blScoreArgs;
+int bl_token_logprobs(const blScoreArgs* a, void* stream, char* err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

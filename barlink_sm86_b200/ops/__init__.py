@@ -590,9 +590,53 @@ def logits_argmax(logits, rules, offset=0):
     return ref.pick(ref.logit_rules(logits, rules.vocab, offset, *rules._args()), offset)
 
 
+# ---------------------------------------------------------------- scores of tokens
+class TokenLogprobs(NamedTuple):
+    """See `token_logprobs`."""
+    logprobs: torch.Tensor      # fp32, the shape of ids
+    entropy: torch.Tensor       # fp32 [rows], in nats
+    top_ids: torch.Tensor       # int32 [rows, top]
+    top_logprobs: torch.Tensor  # fp32 [rows, top]
+
+
+def _check_logprobs(logits, ids, top, offset, vocab):
+    if logits.dim() != 2 or ids.dim() not in (1, 2) or ids.shape[0] != logits.shape[0] or ids.dtype != torch.int32:
+        raise ValueError("token_logprobs needs logits [rows, n] and int32 ids [rows] or [rows, tokens]")
+    if not 0 <= top <= 32 or offset < 0 or (vocab is not None and vocab < 0):
+        raise ValueError("token_logprobs gives 0 to 32 alternatives, of tokens from 0 on")
+
+
+def token_logprobs(logits, ids, top=0, offset=0, vocab=None):
+    """Log probabilities (natural logarithm) of the tokens `ids` (int32 [rows], or [rows, tokens] for several of each row) under logits [rows, n]
+    (bf16 or fp32; rows may lie apart), the entropy of every row's distribution, and its `top` (0 to 32) most likely tokens, the most likely
+    first and the lowest of equals, with theirs: a TokenLogprobs, all in fp32, from one pass over the logits.
+
+    Column i is token i + offset; columns at or beyond `vocab` (the padding of a head) are left out.  Logits of -inf (a mask's) have probability 0.  An
+    id that is none of the columns' has log probability -inf.  Where fewer than `top` tokens are above -inf the rest are -1 with -inf; a row with
+    nothing above -inf gives -inf everywhere and entropy 0.  A row with NaN or +inf has NaN for all its values.
+
+    Logits under rules: `logits_process` first.  Vocabularies in shards: `TPComm.token_logprobs_vocab_parallel`."""
+    if logits.is_cuda:
+        _count()
+        return TokenLogprobs(*_C().token_logprobs(logits, ids, top, offset, 2 ** 31 - 1 if vocab is None else vocab))
+    _check_logprobs(logits, ids, top, offset, vocab)
+    return TokenLogprobs(*ref.token_logprobs_of(*ref.token_logprob_parts(logits, ids, top, offset, 2 ** 31 - 1 if vocab is None else vocab)))
+
+
+def token_logprob_parts(logits, ids, top=0, offset=0, vocab=None):
+    """What a shard of a vocabulary knows: (logits of ids, -inf where these columns have none of them; fp32 [rows, 3]: greatest logit m, sum of e^(x - m), sum of
+    (x - m) e^(x - m); top ids; their logits).  `ref.join_token_logprobs` joins those of all shards, `ref.token_logprobs_of` turns the result into
+    log probabilities."""
+    if logits.is_cuda:
+        _count()
+        return tuple(_C().token_logprobs(logits, ids, top, offset, 2 ** 31 - 1 if vocab is None else vocab, raw=True))
+    _check_logprobs(logits, ids, top, offset, vocab)
+    return ref.token_logprob_parts(logits, ids, top, offset, 2 ** 31 - 1 if vocab is None else vocab)
+
+
 __all__ = [
     "linear", "linear_split", "k_splits", "TiledWeight", "tile_weight", "untile_weight", "rmsnorm", "rmsnorm_digits", "rope_kv_write", "rope", "silu_mul", "embedding", "argmax",
     "paged_attn_decode", "rope_attn_decode", "attention", "w8a16_linear", "w8a16_linear_split", "W8GroupScales", "prepare_w8_scales", "w4a16_linear", "w4a16_linear_split", "qknorm_rope", "layernorm_modulate", "gate_residual", "ref",
     "kv4_cache", "rope_kv_write_q4", "kv4_read", "paged_attn_decode_q4", "PagedLayout", "paged_layout", "LogitRules", "count_tokens",
-    "logits_process", "logits_argmax",
+    "logits_process", "logits_argmax", "TokenLogprobs", "token_logprobs", "token_logprob_parts",
 ]

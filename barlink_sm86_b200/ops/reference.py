@@ -503,3 +503,51 @@ def pick(x, offset=0):
     val = x.amax(-1)
     idx = (x == val[:, None]).int().argmax(-1) + offset
     return torch.where(val == -math.inf, torch.full_like(idx, -1), idx).to(torch.int32), val
+
+
+def token_logprob_parts(logits, ids, top=0, offset=0, vocab=2 ** 31 - 1):
+    """(logits of ids, parts fp32 [rows, 3] = m, S, T, top_ids, top logits), see ops.token_logprobs."""
+    n = max(0, min(logits.shape[1], vocab - offset))
+    x = logits[:, :n].double()
+    rows = x.shape[0]
+    m = torch.where(torch.isnan(x), -math.inf, x).amax(-1) if n else torch.full((rows,), -math.inf, dtype=torch.float64)
+    t = x - torch.where(m == -math.inf, 0.0, m)[:, None]
+    e = torch.exp(t)
+    parts = torch.stack([m, e.sum(-1), torch.where(t == -math.inf, 0.0, t * e).sum(-1)], 1).float()
+    at = ids.long().view(rows, -1) - offset
+    ok = (ids.view(rows, -1) >= 0) & (at >= 0) & (at < n)
+    given = torch.where(ok, x.gather(1, torch.where(ok, at, 0)), -math.inf) if n else torch.full(at.shape, -math.inf, dtype=torch.float64)
+    order = torch.sort(torch.where(torch.isnan(x), -math.inf, x), dim=-1, descending=True, stable=True)
+    val = torch.nn.functional.pad(order.values[:, :top], (0, max(0, top - n)), value=-math.inf)
+    idx = torch.nn.functional.pad(order.indices[:, :top] + offset, (0, max(0, top - n)), value=-1)
+    return given.view(ids.shape).float(), parts, torch.where(val == -math.inf, -1, idx).to(torch.int32), val.float()
+
+
+def token_logprobs_of(given, parts, top_ids, top_val):
+    """(logprobs, entropy, top_ids, top_logprobs) from what token_logprob_parts leaves."""
+    m, s, t = parts.double().unbind(-1)
+    none = (m == -math.inf) & (s == 0)
+
+    def logp(x):
+        rows = (-1,) + (1,) * (x.dim() - 1)
+        y = (x.double() - m.view(rows)) - torch.log(s).view(rows)
+        return torch.where(none.view(rows), -math.inf, y).float()
+
+    top = torch.where((top_ids < 0) & ~torch.isnan(s)[:, None], -math.inf, logp(top_val))
+    return logp(given), torch.where(none, 0.0, torch.log(s) - t / s).float(), top_ids, top
+
+
+def join_token_logprobs(shards):
+    """What token_logprob_parts leaves, of the shards of a vocabulary in their order -> the same of the whole."""
+    given = torch.stack([s[0] for s in shards]).amax(0)
+    parts = torch.stack([s[1] for s in shards]).double()
+    m = parts[..., 0].amax(0)
+    # (the distance of an empty shard is of no account: its sums are zero)
+    d = torch.where(parts[..., 0] == -math.inf, 0.0, parts[..., 0] - torch.where(m == -math.inf, 0.0, m))
+    e = torch.exp(d)
+    s = (e * parts[..., 1]).sum(0)
+    t = (e * (parts[..., 2] + torch.where(d == -math.inf, 0.0, d) * parts[..., 1])).sum(0)
+    top = shards[0][2].shape[-1]
+    order = torch.sort(torch.cat([x[3] for x in shards], 1), dim=-1, descending=True, stable=True)
+    ids = torch.cat([x[2] for x in shards], 1).gather(1, order.indices[:, :top])
+    return given, torch.stack([m, s, t], 1).float(), ids, order.values[:, :top]

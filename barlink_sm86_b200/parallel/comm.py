@@ -250,6 +250,25 @@ class TPComm:
             return out
         return r
 
+    def token_logprobs_vocab_parallel(self, logits_local, ids, vocab_per_rank, vocab, top=0):
+        """`ops.token_logprobs` over vocab-parallel logits [rows, vocab_per_rank] of all ranks (vocab: tokens in all; the columns behind are
+        padding): every rank sends a few words per row -- the sums of its columns, the logits of the given tokens, its most likely tokens -- and
+        all have the same result."""
+        lo = self.rank * vocab_per_rank
+        if self.world == 1 or self.no_comm:
+            return _ops.token_logprobs(logits_local, ids, top, lo, vocab)
+        given, parts, top_ids, top_val = _ops.token_logprob_parts(logits_local, ids, top, lo, vocab)
+        rows = parts.shape[0]
+        mine = torch.cat([parts, given.reshape(rows, -1), top_val, top_ids.view(torch.float32)], 1)
+        wide = mine.shape[1]
+        got = self.all_gather_cols(torch.nn.functional.pad(mine, (0, -wide % 4)))  # (whole 16-byte vectors)
+        n = given.numel() // max(rows, 1)
+        shards = []
+        for part in got.view(rows, self.world, wide + -wide % 4).unbind(1):
+            p, g, v, i, _ = part.split([3, n, top, top, -wide % 4], 1)
+            shards.append((g.reshape(given.shape), p, i.contiguous().view(torch.int32), v))
+        return _ops.TokenLogprobs(*ref.token_logprobs_of(*ref.join_token_logprobs(shards)))
+
     def barrier(self):
         if self.world > 1:
             dist.barrier(group=self.group)
