@@ -28,6 +28,7 @@ SOURCES = [
     "w8a16_kernels.cu",
     "w4a16_kernels.cu",
     "kv4_kernels.cu",
+    "chunk_attn_kernels.cu",
     "serve_kernels.cu",
     "score_kernels.cu",
     "backend.cc",

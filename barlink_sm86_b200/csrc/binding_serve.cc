@@ -183,6 +183,62 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
   return out;
 }
 
+// k_cache and v_cache bf16 [blocks, nkv, block, hd], or (v_cache none) the 4-bit cache
+at::Tensor paged_attn_chunk(const at::Tensor& q, const at::Tensor& cache, const OptTensor& v_cache, const at::Tensor& block_tables, const at::Tensor& cu_q,
+                            const at::Tensor& ctx_lens, int nq, int nkv, int hd, double scale, const OptTensor& out_opt) {
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 2 && (q.stride(1) == 1 || q.size(1) == 1) && (q.size(0) < 2 || q.stride(0) % 8 == 0) && aligned16(q),
+              "barlink: q/qkv must be a 2-D bfloat16 CUDA tensor whose rows start on 16-byte boundaries");
+  TORCH_CHECK(hd == 64 || hd == 128, "barlink: attention of a chunk over the paged cache is built for head_dim 64 and 128");
+  TORCH_CHECK(nkv >= 1 && nq >= 1 && nq % nkv == 0 && nq / nkv <= 128,
+              "barlink: attention of a chunk over the paged cache needs nq % nkv == 0 and at most 128 query heads per KV head");
+  const int tokens = small(q.size(0), "tokens"), batch = small(ctx_lens.numel(), "batch");
+  TORCH_CHECK(q.size(1) >= int64_t(nq) * hd && (tokens < 2 || q.stride(0) >= int64_t(nq) * hd) && q.stride(0) <= 0x7fffffff, "barlink: q rows too short");
+  TORCH_CHECK(cache.dim() == 4, "barlink: the paged cache must be a 4-D CUDA tensor");
+  int block_size;
+  if (v_cache) {
+    for (const at::Tensor* t : {&cache, &*v_cache}) {
+      check_on(*t, q, "cache");
+      TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->dim() == 4 && t->size(1) == nkv && t->size(3) == hd && aligned16(*t) &&
+                      t->sizes() == cache.sizes(),
+                  "barlink: k_cache and v_cache must be contiguous, 16-byte aligned bfloat16 [blocks, nkv, block_size, head_dim] of one shape");
+    }
+    block_size = small(cache.size(2), "block size");
+  } else {
+    block_size = small(cache.size(2) * 16, "block size");
+    check_cache(cache, q, nkv, hd, block_size);
+  }
+  TORCH_CHECK(block_size >= 16 && block_size % 16 == 0, "barlink: attention of a chunk over the paged cache needs a block size that is a multiple of 16");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == batch, "barlink: block_tables must be int32 [batch, max_blocks]");
+  const int* bt = i32(block_tables, q, -1, "block_tables");
+  const int* cu = i32(cu_q, q, int64_t(batch) + 1, "cu_q");
+  const int* cl = i32(ctx_lens, q, batch, "ctx_lens");
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = out_opt ? *out_opt : fresh({tokens, int64_t(nq) * hd}, at::kBFloat16, q);
+  check_on(out, q, "out");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == 2 && out.size(0) == tokens && out.size(1) == int64_t(nq) * hd &&
+                  aligned16(out),
+              "barlink: out must be a contiguous, 16-byte aligned bfloat16 [tokens, nq * hd]");
+  if (tokens > 0 && batch > 0) {
+    const size_t bytes = bl_paged_attn_chunk_ws(tokens, nq, nkv, hd);
+    at::Tensor ws = fresh({int64_t(bytes)}, at::kByte, q);
+    BL_CHECK(bl_paged_attn_chunk(q.data_ptr(), int(tokens > 1 ? q.stride(0) : int64_t(nq) * hd), v_cache ? cache.data_ptr() : nullptr,
+                                 v_cache ? v_cache->data_ptr() : nullptr, v_cache ? nullptr : cache.data_ptr(), bt, cu, cl, out.data_ptr(), tokens, batch, nq, nkv,
+                                 hd, block_size, small(cache.size(0), "blocks"), small(block_tables.size(1), "max_blocks"), float(scale), ws.data_ptr(), bytes,
+                                 stream_of(q), err, errlen));
+  }
+  return out;
+}
+// The error word of that kernel, into a pinned int32 tensor on the current stream of a device.
+void chunk_attn_error_into(const at::Tensor& out, int dev) {
+  TORCH_CHECK(out.is_cpu() && out.is_pinned() && out.scalar_type() == at::kInt && out.numel() == 1, "barlink: chunk_attn_error_into needs a pinned int32 element");
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  BL_CHECK(bl_chunk_attn_error_async(static_cast<unsigned*>(out.data_ptr()), at::cuda::getCurrentCUDAStream(dev).stream(), err, errlen));
+}
+void chunk_attn_error_clear(int dev) {
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  BL_CHECK(bl_chunk_attn_error_clear(err, errlen));
+}
+
 // [cu, positions, slots, ctx_lens, free_range]; `into`: the same five to write to
 std::vector<at::Tensor> paged_layout(const at::Tensor& new_lens, const at::Tensor& past_lens, const at::Tensor& block_tables,
                                      const at::Tensor& free_list, const at::Tensor& free_range, int64_t tokens, int block_size, int rows_per_request,
@@ -356,6 +412,11 @@ void bind_serve(py::module_& m) {
   m.def("kv4_error_clear", &kv4_error_clear, py::arg("device") = 0);
   m.def("kv4_error_into", &kv4_error_into, py::arg("out"), py::arg("device") = 0);
   m.def("kv4_wait_polls", &bl_kv4_wait_polls, py::arg("polls"));
+  m.def("paged_attn_chunk", &paged_attn_chunk, py::arg("q"), py::arg("cache"), py::arg("v_cache"), py::arg("block_tables"), py::arg("cu_q"),
+        py::arg("ctx_lens"), py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none());
+  m.def("chunk_attn_error_into", &chunk_attn_error_into, py::arg("out"), py::arg("device") = 0);
+  m.def("chunk_attn_error_clear", &chunk_attn_error_clear, py::arg("device") = 0);
+  m.def("chunk_attn_wait_polls", &bl_chunk_attn_wait_polls, py::arg("polls"));
   m.def("paged_layout", &paged_layout, py::arg("new_lens"), py::arg("past_lens"), py::arg("block_tables"), py::arg("free_list"),
         py::arg("free_range"), py::arg("tokens"), py::arg("block_size"), py::arg("rows_per_request") = 0, py::arg("into") = py::none(), py::arg("lost") = py::none());
   m.def("count_tokens", &count_tokens, py::arg("counts"), py::arg("seen"), py::arg("ids"), py::arg("cu") = py::none(),

@@ -500,6 +500,22 @@ typedef struct blRulesArgs {
 } blRulesArgs;
 int bl_logit_rules(const blRulesArgs* a, void* stream, char* err, size_t errlen);
 
+/* ---- attention of new tokens over a paged cache (chunk_attn_kernels.cu) -------------------------------------------
+ * q: rows q_stride elements apart, cu_q [batch + 1]: request b's rows are cu_q[b] .. cu_q[b + 1], its last tokens; ctx_lens [batch]: its tokens in all.  Row i of n
+ * sees keys 0 .. ctx - n + i; a row that sees none gets zeros; rows before cu_q[0] and behind cu_q[batch] are not written.  k_cache, v_cache:
+ * bf16 [n_blocks][nkv][block_size][hd]; or, with both null, cache4: as bl_rope_kv_write_q4 leaves it, keys and values as bl_kv4_read gives them.  A block-table
+ * entry that names no block leaves its tokens out.  hd 64 or 128, block_size a multiple of 16, at most 128 query heads per KV head, scale > 0.
+ * ws: bl_paged_attn_chunk_ws bytes of this call's own, 16-byte aligned.  A wait that runs out sets the current device's error word, which
+ * bl_chunk_attn_error_async copies to `out` (pinned) on a stream and bl_chunk_attn_error_clear sets back, and leaves NaN in the rows
+ * concerned.  bl_chunk_attn_wait_polls: as bl_kv4_wait_polls. */
+size_t bl_paged_attn_chunk_ws(int tokens, int nq, int nkv, int hd);
+int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_cache, const void* v_cache, const void* cache4, const int* block_tables,
+                        const int* cu_q, const int* ctx_lens, void* out, int tokens, int batch, int nq, int nkv, int hd, int block_size,
+                        int n_blocks, int max_blocks, float scale, void* ws, size_t ws_bytes, void* stream, char* err, size_t errlen);
+int bl_chunk_attn_error_async(unsigned* out, void* stream, char* err, size_t errlen);
+int bl_chunk_attn_error_clear(char* err, size_t errlen);
+unsigned bl_chunk_attn_wait_polls(unsigned polls);
+
 /* ---- scores of tokens (score_kernels.cu) -------------------------------------------------------------
  * Logits [rows][n] (bf16, or fp32), token id = column + offset, columns behind the vocabulary left out.  With m = max x, S = sum e^(x - m),
  * T = sum (x - m) e^(x - m): given = x_id - m - log S of every id (-inf where these columns have no such token), entropy = log S - T / S, and the

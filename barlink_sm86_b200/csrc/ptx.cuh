@@ -224,6 +224,13 @@ __device__ __forceinline__ void tma_load_2d_hint_s(uint32_t smem_dst, const void
       "l"(tmap), "r"(bar), "r"(x), "r"(y), "l"(hint)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_hint_s(uint32_t smem_dst, const void* tmap, uint32_t bar, int x, int y, int z, uint64_t hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_dst),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(hint)
+      : "memory");
+}
 // Loads for a whole converged warp, of which the elected lane issues (see elect_leader).
 __device__ __forceinline__ void tma_load_2d_hint_warp(uint32_t leader, uint32_t smem_dst, const void* tmap,
                                                       uint32_t bar, int x, int y, uint64_t hint) {

@@ -457,6 +457,57 @@ def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, o
     return y
 
 
+# ---------------------------------------------------------------- new tokens over a paged cache
+def _check_chunk(q, shape, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out):
+    if hd not in (64, 128) or nkv < 1 or nq < 1 or nq % nkv or nq // nkv > 128:
+        raise ValueError("attention of a chunk over the paged cache is built for head_dim 64 and 128 and up to 128 query heads per KV head")
+    if len(shape) != 3 or shape[0] != nkv or shape[1] < 16 or shape[1] % 16 or shape[2] != hd:
+        raise ValueError("the paged cache has nkv heads and a block size that is a multiple of 16")
+    if q.dim() != 2 or q.shape[1] < nq * hd or block_tables.dim() != 2 or block_tables.shape[0] != ctx_lens.numel() or cu_q.numel() != ctx_lens.numel() + 1:
+        raise ValueError("q must be [tokens, >= nq * hd], block_tables [batch, max_blocks], cu_q [batch + 1] and ctx_lens [batch]")
+    if any(t.dtype != torch.int32 for t in (block_tables, cu_q, ctx_lens)):
+        raise ValueError("block tables, row offsets and lengths are int32")
+    if out is not None and (tuple(out.shape) != (q.shape[0], nq * hd) or out.dtype != q.dtype):
+        raise ValueError("out must be [tokens, nq * hd] of q's type")
+    if not scale > 0:
+        raise ValueError("attention of a chunk over the paged cache needs a positive scale")
+
+
+def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None):
+    """Attention of new tokens of each request over its paged cache, their own keys and values included (write them first, `rope_kv_write`): a
+    prompt in pieces, a further turn, draft tokens to be checked, or a decode step (one token each).
+
+    q bf16 [tokens, >= nq * hd] (the first nq * hd columns; rows start on 16-byte boundaries).  cu_q int32 [batch + 1]: request b's new
+    tokens are rows cu_q[b] .. cu_q[b + 1] (none, too); ctx_lens int32 [batch]: its tokens in all, the new ones the last of them, so that new
+    token i of n sees the keys 0 .. ctx - n + i.  block_tables int32 [batch, max_blocks]; k_cache, v_cache bf16 [blocks, nkv, block_size, hd].
+
+    hd 64 or 128, block_size a multiple of 16, at most 128 query heads per KV head, scale > 0.  A table entry that names no block, and a
+    table that ends early, leave their tokens out; a token that sees no key gets zeros.  What the cache holds behind a request's last token
+    is of no account; within it, a value that is no finite number may also show in tokens just before it (up to 63).  Rows
+    that belong to no request are not written (nor set in a new tensor).  Returns bf16 [tokens, nq * hd]."""
+    if v_cache is None:
+        raise ValueError("paged_attn_chunk needs keys and values; the 4-bit cache is paged_attn_chunk_q4's")
+    if q.is_cuda:
+        _count(2)
+        return _C().paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+    _check_chunk(q, k_cache.shape[1:], block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have one shape")
+    out = torch.empty(q.shape[0], nq * hd, dtype=q.dtype) if out is None else out
+    return ref.paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+
+
+def paged_attn_chunk_q4(q, cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None):
+    """`paged_attn_chunk` over a 4-bit cache (`kv4_cache`, written by `rope_kv_write_q4`), with the keys and values that `kv4_read` gives: rounded to
+    bf16, which `paged_attn_decode_q4` does without (its results are closer by up to half a step of bf16 a key or value)."""
+    if q.is_cuda:
+        _count(2)
+        return _C().paged_attn_chunk(q, cache, None, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+    _check_chunk(q, (cache.shape[1], cache.shape[2] * 16, cache.shape[3] // 20), block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+    out = torch.empty(q.shape[0], nq * hd, dtype=q.dtype) if out is None else out
+    return ref.paged_attn_chunk_q4(q, cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+
+
 # ---------------------------------------------------------------- serving steps
 class PagedLayout(NamedTuple):
     """Where a step's tokens go, see `paged_layout`."""
@@ -637,6 +688,6 @@ def token_logprob_parts(logits, ids, top=0, offset=0, vocab=None):
 __all__ = [
     "linear", "linear_split", "k_splits", "TiledWeight", "tile_weight", "untile_weight", "rmsnorm", "rmsnorm_digits", "rope_kv_write", "rope", "silu_mul", "embedding", "argmax",
     "paged_attn_decode", "rope_attn_decode", "attention", "w8a16_linear", "w8a16_linear_split", "W8GroupScales", "prepare_w8_scales", "w4a16_linear", "w4a16_linear_split", "qknorm_rope", "layernorm_modulate", "gate_residual", "ref",
-    "kv4_cache", "rope_kv_write_q4", "kv4_read", "paged_attn_decode_q4", "PagedLayout", "paged_layout", "LogitRules", "count_tokens",
+    "kv4_cache", "rope_kv_write_q4", "kv4_read", "paged_attn_decode_q4", "paged_attn_chunk", "paged_attn_chunk_q4", "PagedLayout", "paged_layout", "LogitRules", "count_tokens",
     "logits_process", "logits_argmax", "TokenLogprobs", "token_logprobs", "token_logprob_parts",
 ]

@@ -420,6 +420,42 @@ def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale):
     return out
 
 
+def _paged_attn_chunk(q, n_blocks, bs, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, read):
+    """read(slots) -> k, v [rows, nkv, hd]"""
+    G = nq // nkv
+    for b in range(ctx_lens.numel()):
+        lo = min(max(int(cu_q[b]), 0), q.shape[0])
+        n = min(max(int(cu_q[b + 1]), lo), q.shape[0]) - lo
+        ctx = max(int(ctx_lens[b]), 0)
+        t = torch.arange(min(ctx, block_tables.shape[1] * bs))
+        blk = block_tables[b].long()[t // bs] if len(t) else t
+        ok = (blk >= 0) & (blk < n_blocks)
+        t, slots = t[ok], (blk * bs + t % bs)[ok]
+        k, v = (x.float() for x in read(slots))
+        qq = q[lo:lo + n, :nq * hd].reshape(n, nkv, G, hd).float()
+        s = torch.einsum("nhgd,thd->hgnt", qq, k) * scale
+        seen = t <= (ctx - n + torch.arange(n))[:, None]
+        s = torch.where(seen, s, torch.full_like(s, -math.inf))
+        p = torch.where(seen.any(-1)[:, None], torch.softmax(s, -1), torch.zeros_like(s))
+        out[lo:lo + n] = torch.einsum("hgnt,thd->nhgd", p, v).reshape(n, nq * hd).to(q.dtype)
+    return out
+
+
+def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out):
+    bs = k_cache.shape[2]
+
+    def read(slots):
+        return [c[slots // bs, :, slots % bs] for c in (k_cache, v_cache)]
+
+    return _paged_attn_chunk(q, k_cache.shape[0], bs, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, read)
+
+
+def paged_attn_chunk_q4(q, cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out):
+    bs = cache.shape[2] * 16
+    return _paged_attn_chunk(q, cache.shape[0], bs, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out,
+                             lambda slots: kv4_read(cache, slots, hd, bs))
+
+
 # ---------------------------------------------------------------- serving steps
 def paged_layout(new_lens, past_lens, block_tables, free_list, free_range, tokens, block_size, rows_per_request=0, lost=None):
     """See ops.paged_layout; block_tables, free_list and lost are updated in place."""
