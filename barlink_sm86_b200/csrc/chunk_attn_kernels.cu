@@ -4,19 +4,24 @@
 // included: token i of n new ones, of a request with c tokens in all, sees keys 0 .. c - n + i.
 //
 // The query heads that share a KV head, times T = 128 / (heads that share) tokens, are the 128 rows of a tile of tcgen05 products, so that a
-// chunk of a few tokens reads its keys once for all of them.  Two tiles (a "pair") of 128 rows walk the keys together in steps of 64:
+// chunk of a few tokens reads its keys once for all of them.  A block has places for two tiles; the keys come in steps of 128.  Where a request has
+// new tokens for more than a tile, the two hold neighbouring tiles ("a pair") and share every step's keys and values; where it has not (the
+// case that is bound by memory and by the chain scores -> softmax -> values) both hold the same tile and take the steps in turn, and their
+// sums are joined at the end.
 //
-//   warp 0      asks for keys and values: boxes of up to 64 tokens of a block by TMA, or 16-token tiles of the 4-bit cache by bulk copies
-//   warp 1      issues S = Q K^T (128 x 64 into TMEM, two buffers a tile) and O += P V (128 x hd in TMEM)
-//   warp 2      asks for queries: one three-dimensional box is a tile (64 dims, the heads, T tokens)
-//   warps 4-7   softmax of the first tile's rows, one row a thread: P (bf16) goes over S in TMEM, from where it is an operand
-//   warps 8-11  the same for the second tile
+//   warp 0      asks for keys, warp 3 for values: boxes of up to 64 tokens of a block by TMA; 4-bit cache: parts of 16-token tiles by bulk copies
+//   warp 3      also walks the list, and asks for queries: one three-dimensional box is a tile (64 dims, the heads, T tokens)
+//   warps 1, 2  issue S = Q K^T (128 x 64 into TMEM) and O += P V (128 x hd in TMEM) of a place each, the next S right behind P V
+//   warps 4-7   softmax of the first place's rows, one row a thread: P (bf16) goes over S in TMEM, from where it is an operand
+//   warps 8-11  the same for the second place
 //   warps 12-15 (4-bit cache) expand codes into bf16 tiles in the layout that TMA would leave
 //
+// A step's scores come in halves of 64 keys, each with columns of its own, so that a place's softmax always finds scores while its products go on.  S of
+// a half goes into the columns from which P V of the same half of the step before, issued ahead of it and not waited for, takes P: one thread
+// issues both, and the tensor pipe works off a thread's products in the order in which they are issued.
+//
 // Steps of all pairs of all requests and KV heads make one list, of which every block takes an equal run: lengths are known on the GPU only.  A pair
-// that is cut leaves its pieces (sums, maxima) to a second kernel.  The chain of a run does not stop at a pair's end: scores are two steps
-// ahead, also of the next pair; where a pair has one tile only (few new tokens: the case that is bound by memory) pairs take the two tiles'
-// places in turn, and one's last products and output pass beside the next one's first scores.
+// that is cut leaves its pieces (sums, maxima) to a second kernel.
 //
 // Tokens of table entries that name no block are left out (their boxes start behind the cache, so TMA fills in zeros).  What stands in the cache
 // behind a request's last token may be anything: the values of the rest of its box are set to zero in shared memory.
@@ -37,11 +42,13 @@
 namespace bl {
 
 constexpr int kChRows = 128;   // of a tile
-constexpr int kChKeys = 64;    // of a step
+constexpr int kChKeys = 128;   // of a step
 constexpr int kChGran = 16;    // tokens that lie together in either cache
-constexpr int kChStages = 4;   // K tiles and V tiles in flight, a ring each
-constexpr int kChRaw = 3;      // steps of the 4-bit cache in flight
-constexpr uint32_t kChTmemCols = 512;  // S of tile t, use parity p: 128 t + 64 p, P in its first half; O of tile t: 256 + 128 t
+constexpr int kChGrans = kChKeys / kChGran;
+constexpr int kChRaw = 3;      // half steps of the 4-bit cache in flight
+constexpr int kChHalf = kChKeys / 2;
+constexpr uint32_t kChTmemCols = 512;  // S of place t, half h of a step: 128 t + 64 h, P in its first half; O of place t: 256 + 128 t
+constexpr int kChPoly = 1;             // of four pairs of exponentials, those on the FMA pipe
 constexpr float kChRescale = 8.f;      // log2 units
 constexpr uint32_t kChPolls = 1u << 24;
 
@@ -50,7 +57,7 @@ __device__ uint32_t g_chunk_err;  // set by a wait that ran out; one word per de
 struct ChunkMeta {
   int count;                // pieces of the pair that begins in this run and ends in another; 0: none does
   int first;                // its first piece; piece k of the others is the first of run me + k
-  int b, h, q0, tok0, ntok; // request, KV head, first row of the request, first token, tokens of the pair
+  int h, row, ntok;         // KV head, first row of q and out, tokens of the pair
 };
 
 struct Chunk {
@@ -84,57 +91,129 @@ __device__ __forceinline__ int chunk_keys(const ChunkReq& r, int tok0, int ntok)
 // (a pair that sees nothing has a step all the same: its rows are written)
 __device__ __forceinline__ int chunk_steps(int keys) { return max(1, (keys + kChKeys - 1) / kChKeys); }
 
-// Where a run stands: a pair and its steps.
-struct ChunkAt {
-  int b, h, tok0;
-  int64_t start;   // of the pair in the list
-  ChunkReq r;
-  int ntok, keys, steps;
-  __device__ __forceinline__ void fill(const Chunk& a) {
-    ntok = min(2 * a.T, r.n - tok0);
-    keys = chunk_keys(r, tok0, ntok);
-    steps = chunk_steps(keys);
-  }
-  // the next pair (there is one)
-  __device__ __forceinline__ void next(const Chunk& a) {
-    start += steps;
-    tok0 += 2 * a.T;
-    if (tok0 >= r.n) {
-      tok0 = 0;
-      if (++h == a.nkv) {
-        h = 0;
-        do {
-          ++b;
-          if (b < a.batch) r = chunk_req(a, b);
-        } while (b < a.batch && r.n == 0);
-      }
-    }
-    fill(a);
-  }
+// A run's share of a pair, as the warp that walks the list leaves it for the others.
+struct ChunkSeg {
+  int b, h;
+  int row, ntok;    // first row of q and out, tokens
+  int keys;         // that the last token sees
+  int lim, cap;     // the first token sees min(lim, cap) keys, and each one more, up to cap
+  int j0, n, i0;    // first step, steps (0: the run is over), number of the first one in the run
+  int piece;        // -1: the whole pair
+  int pad;
 };
+constexpr int kChSegs = 4;
 
 template <int HD, bool Q4>
 struct ChunkShape {
   static constexpr int kThreads = Q4 ? 512 : 384;
   static constexpr uint32_t kQ = kChRows * HD * 2, kKV = kChKeys * HD * 2, kHalf = kChKeys * 128, kQHalf = kChRows * 128;
-  static constexpr uint32_t kRawBytes = (kChKeys / kQ4Tokens) * q4_tile_bytes(HD);
-  static constexpr uint32_t kOffK = 2 * kQ, kOffV = kOffK + kChStages * kKV, kOffRaw = kOffV + kChStages * kKV;
-  static constexpr uint32_t kOffBar = kOffRaw + (Q4 ? kChRaw * kRawBytes : 0);
-  static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // barriers and words; room to align
-  static_assert(kSmem <= 232448, "attention tiles do not fit the shared memory of one block");
+  static constexpr uint32_t kRawGran = 10 * HD, kRawBytes = (kChGrans / 2) * kRawGran;  // codes and params of a granule's keys, or of its values
+  static constexpr uint32_t kOffK = 2 * kQ, kOffV = kOffK + 2 * kKV, kOffRaw = kOffV + 2 * kKV;
+  static constexpr uint32_t kOffSums = kOffRaw + (Q4 ? 2 * kChRaw * kRawBytes : 0);  // (maximum, sum) of the second place's rows
+  static constexpr uint32_t kOffBar = kOffSums + kChRows * 8;
+  static constexpr uint32_t kSmem = kOffBar + 768 + 1024;  // barriers, words, shares of pairs; room to align
+  static_assert(kSmem <= 232448 - 256, "attention tiles do not fit the shared memory of one block");
 };
 
 struct ChunkBars {
   uint64_t q_full[2], q_empty[2];
-  uint64_t k_full[kChStages], k_empty[kChStages], v_full[kChStages], v_empty[kChStages];
-  uint64_t raw_full[kChRaw], raw_empty[kChRaw];
-  uint64_t s_ready[2][2], p_ready[2][2];  // [tile][use parity]
-  uint64_t pv_done[2], o_final[2], o_free[2];
-  uint64_t drained;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t raw_full[2][kChRaw], raw_empty[2][kChRaw];  // keys, values
+  uint64_t s_ready[2][2], p_ready[2][2];        // by place and half
+  uint64_t pv_done[2], o_final[2], o_free[2];   // by place
+  uint64_t met[2];   // see the products
+  uint64_t sums;     // the second place's (maximum, sum) are there
+  uint64_t drained[2];
+  uint64_t seg_full[kChSegs], seg_empty[kChSegs];
+  ChunkSeg segs[kChSegs];
   uint32_t tmem, abort;
   uint32_t gone[8];  // granules of a step (by its number in the run, modulo 8) that have no block
 };
-static_assert(sizeof(ChunkBars) <= 512, "barriers");
+static_assert(sizeof(ChunkBars) <= 768, "barriers");
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+// 2^x of two numbers on the FMA pipe: x = n + f, |f| <= 1/2, 2^f by the polynomial of degree 3 whose relative error is least (7.5e-5; P is rounded to
+// 2^-8 behind it), 2^n by its bits.  Exactly 0 below -127, -inf included; NaN stays.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
+  const float2 magic = make_float2(12583039.f, 12583039.f);  // 1.5 * 2^23 + 127: adding it leaves n + 127 in the lowest bits
+  const float2 t = add2(x, magic);
+  const float2 f = add2(x, fma2(t, make_float2(-1.f, -1.f), magic));
+  float2 p = fma2(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.242611125f, 0.242611125f));
+  p = fma2(p, f, make_float2(0.693260968f, 0.693260968f));
+  p = fma2(p, f, make_float2(0.999928057f, 0.999928057f));
+  return mul2(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+// S of a tile: hd / 16 products, in both operands 64 dims to a half tile of 128 rows (16 KiB).  (Few instructions: predicates are made once, and only the low
+// words of the operands' descriptors change.)
+template <int HD>
+__device__ __forceinline__ void umma_f16_ss_row_warp(uint32_t leader, uint32_t d, uint64_t qa, uint64_t kb, uint32_t idesc) {
+  const uint32_t qlo = uint32_t(qa), qhi = uint32_t(qa >> 32), klo = uint32_t(kb), khi = uint32_t(kb >> 32);
+  uint32_t acc = 0;
+  asm volatile(
+      "{\n\t.reg .pred q, f, t;\n\t.reg .b64 x, y;\n\t.reg .b32 u, v;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 f, %7, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 u, %1, 0;\n\tadd.u32 v, %3, 0;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, f;\n\t"
+      "add.u32 u, %1, 2;\n\tadd.u32 v, %3, 2;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, t;\n\t"
+      "add.u32 u, %1, 4;\n\tadd.u32 v, %3, 4;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, t;\n\t"
+      "add.u32 u, %1, 6;\n\tadd.u32 v, %3, 6;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, t;\n\t"
+      "}" ::"r"(d),
+      "r"(qlo), "r"(qhi), "r"(klo), "r"(khi), "r"(idesc), "r"(leader), "r"(acc)
+      : "memory");
+  if constexpr (HD == 128) {
+    acc = 1;
+    asm volatile(
+      "{\n\t.reg .pred q, f, t;\n\t.reg .b64 x, y;\n\t.reg .b32 u, v;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 f, %7, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 u, %1, 1024;\n\tadd.u32 v, %3, 1024;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, f;\n\t"
+      "add.u32 u, %1, 1026;\n\tadd.u32 v, %3, 1026;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, t;\n\t"
+      "add.u32 u, %1, 1028;\n\tadd.u32 v, %3, 1028;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, t;\n\t"
+      "add.u32 u, %1, 1030;\n\tadd.u32 v, %3, 1030;\n\tmov.b64 x, {u, %2};\n\tmov.b64 y, {v, %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, t;\n\t"
+      "}" ::"r"(d),
+      "r"(qlo), "r"(qhi), "r"(klo), "r"(khi), "r"(idesc), "r"(leader), "r"(acc)
+      : "memory");
+  }
+}
+// P V of half a step: four products of 16 keys, P in 32 columns of TMEM, 16 keys of V 2 KiB apart
+__device__ __forceinline__ void umma_f16_ts4_warp(uint32_t leader, uint32_t d, uint32_t pa, uint64_t vb, uint32_t idesc, uint32_t accumulate) {
+  const uint32_t vlo = uint32_t(vb), vhi = uint32_t(vb >> 32);
+  asm volatile(
+      "{\n\t.reg .pred q, f, t;\n\t.reg .b64 y;\n\t.reg .b32 x, v;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 f, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 x, %1, 0;\n\tadd.u32 v, %2, 0;\n\tmov.b64 y, {v, %3};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %4, f;\n\t"
+      "add.u32 x, %1, 8;\n\tadd.u32 v, %2, 128;\n\tmov.b64 y, {v, %3};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %4, t;\n\t"
+      "add.u32 x, %1, 16;\n\tadd.u32 v, %2, 256;\n\tmov.b64 y, {v, %3};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %4, t;\n\t"
+      "add.u32 x, %1, 24;\n\tadd.u32 v, %2, 384;\n\tmov.b64 y, {v, %3};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %4, t;\n\t"
+      "}" ::"r"(d),
+      "r"(pa), "r"(vlo), "r"(vhi), "r"(idesc), "r"(leader), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Keeps the compiler from making a copy of a loop for either value of a flag (what does not fit the instruction cache is fetched once a step).
+__device__ __forceinline__ bool one_copy(bool flag) {
+  int f = flag;
+  asm volatile("" : "+r"(f));
+  return f != 0;
+}
 
 template <int HD, bool Q4>
 __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
@@ -147,8 +226,8 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   ChunkBars& bars = *reinterpret_cast<ChunkBars*>(gen + S::kOffBar);
   volatile uint32_t* s_abort = &bars.abort;
-  __shared__ int64_t s_scan[S::kThreads / 32];
-  __shared__ ChunkAt s_at;
+  __shared__ int s_scan[S::kThreads / 32];
+  __shared__ int s_first[4];  // request, KV head, first token of the pair, step
 
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -156,25 +235,32 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&bars.q_full[t], 1);
       mbar_init(&bars.q_empty[t], 1);
-      for (int p = 0; p < 2; ++p) {
-        mbar_init(&bars.s_ready[t][p], 1);
-        mbar_init(&bars.p_ready[t][p], kChRows);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars.s_ready[t][h], 1);
+        mbar_init(&bars.p_ready[t][h], kChRows / 32);
       }
       mbar_init(&bars.pv_done[t], 1);
       mbar_init(&bars.o_final[t], 1);
-      mbar_init(&bars.o_free[t], kChRows);
+      mbar_init(&bars.o_free[t], kChRows / 32);
     }
-    for (int s = 0; s < kChStages; ++s) {
+    for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.k_full[s], Q4 ? 4 : 1);
-      mbar_init(&bars.k_empty[s], 1);
       mbar_init(&bars.v_full[s], Q4 ? 4 : 1);
-      mbar_init(&bars.v_empty[s], 1);
+      mbar_init(&bars.k_empty[s], 2);
+      mbar_init(&bars.v_empty[s], 2);
+      mbar_init(&bars.met[s], 1);
     }
-    for (int s = 0; s < kChRaw; ++s) {
-      mbar_init(&bars.raw_full[s], 1);
-      mbar_init(&bars.raw_empty[s], 4);
+    for (int s = 0; s < kChRaw; ++s)
+      for (int v = 0; v < 2; ++v) {
+        mbar_init(&bars.raw_full[v][s], 1);
+        mbar_init(&bars.raw_empty[v][s], 4);
+      }
+    mbar_init(&bars.sums, kChRows / 32);
+    for (int t = 0; t < 2; ++t) mbar_init(&bars.drained[t], 1);
+    for (int i = 0; i < kChSegs; ++i) {
+      mbar_init(&bars.seg_full[i], 1);
+      mbar_init(&bars.seg_empty[i], Q4 ? 15 : 11);  // all warps but the one that walks the list
     }
-    mbar_init(&bars.drained, 1);
     bars.abort = 0;
     for (int i = 0; i < 8; ++i) bars.gone[i] = 0;
     mbar_fence_init();
@@ -191,59 +277,84 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   // lengths, tables, queries and the cache may come from the kernel just before this one
   pdl_wait();
 
-  // ---- this block's run [lo, lo + count) of the list ----------------------------------------------------------------
-  const int runs = gridDim.x, me = blockIdx.x;
-  int64_t lo, run;
-  int count;
-  {
-    const int per = (a.batch + S::kThreads - 1) / S::kThreads;
-    const int b0 = min(int(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
-    auto units_of = [&](const ChunkReq& r) {  // of one KV head
-      int64_t u = 0;
-      for (int t = 0; t < r.n; t += 2 * a.T) u += chunk_steps(chunk_keys(r, t, min(2 * a.T, r.n - t)));
-      return u;
-    };
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(chunk_req(a, b)) * a.nkv;
-    int64_t upto = mine;
+  // ---- this block's run [lo, lo + count) of the list (one lane a request; a request's pairs are dealt out to the warp's lanes) ----
+  const int runs = gridDim.x, me = blockIdx.x, pair = 2 * a.T;
+  const int per = (a.batch + S::kThreads - 1) / S::kThreads, b0 = int(threadIdx.x) * per;
+  auto steps_of = [&](int n, int past, int cap, int p) {  // of pair p of a request
+    const int t = p * pair;
+    return t < n ? max(1, (min(max(past + min(t + pair, n), 0), cap) + kChKeys - 1) / kChKeys) : 0;
+  };
+  int run = 0, lo = 0, count = 0, src = 0, at = 0, mine = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+    for (int k = 0; k < per; ++k) {
+      ChunkReq r = {0, 0, 0, 0};
+      if (b0 + k < a.batch) r = chunk_req(a, b0 + k);
+      int u = steps_of(r.n, r.past, r.cap, 0);
+#pragma unroll 1
+      for (uint32_t many = __ballot_sync(kAll, r.n > pair); many; many &= many - 1) {
+        const int of = __ffs(many) - 1, n = __shfl_sync(kAll, r.n, of), past = __shfl_sync(kAll, r.past, of), cap = __shfl_sync(kAll, r.cap, of);
+        int sum = 0;
+#pragma unroll 1
+        for (int p = lane; p * pair < n; p += 32) sum += steps_of(n, past, cap, p);
+        sum = __reduce_add_sync(kAll, sum);
+        if (lane == of) u = sum;
+      }
+      if (pass == 0) {
+        mine += u * a.nkv;
+        continue;
+      }
+      // the request that holds the first step; its KV head, and the pair
+      u = __shfl_sync(kAll, u, src);
+      if (lo >= at + u * a.nkv) {
+        at += u * a.nkv;
+        continue;
+      }
+      const int h = (lo - at) / u, n = __shfl_sync(kAll, r.n, src), past = __shfl_sync(kAll, r.past, src), cap = __shfl_sync(kAll, r.cap, src);
+      at += h * u;
+#pragma unroll 1
+      for (int p = lane;; p += 32) {
+        const int st = steps_of(n, past, cap, p);
+        int cum = st;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(kAll, cum, o);
+          if (lane >= o) cum += v;
+        }
+        const uint32_t in = __ballot_sync(kAll, lo < at + cum);
+        if (in) {
+          if (lane == __ffs(in) - 1) {
+            s_first[1] = h;
+            s_first[2] = p * pair;
+            s_first[3] = lo - (at + cum - st);
+          }
+          if (lane == src) s_first[0] = b0 + k;
+          break;
+        }
+        at += __shfl_sync(kAll, cum, 31);
+      }
+      break;
+    }
+    if (pass) break;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(kAll, upto, o);
-      if (lane >= o) upto += u;
+      const int v = __shfl_up_sync(kAll, upto, o);
+      if (lane >= o) upto += v;
     }
     if (lane == 31) s_scan[warp] = upto;
     __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < S::kThreads / 32; ++w) {
-      if (w < warp) upto += s_scan[w];
-      total += s_scan[w];
-    }
+    // (at most sixteen warps)
+    const int w = lane < S::kThreads / 32 ? s_scan[lane] : 0, total = __reduce_add_sync(kAll, w);
+    upto += __reduce_add_sync(kAll, lane < warp ? w : 0);
     run = (total + runs - 1) / runs;
-    lo = min(int64_t(me) * run, total);
-    count = int(min(run, total - lo));
-    int64_t at = upto - mine;
-    if (count > 0 && at <= lo && lo < upto) {  // one thread's requests hold the first step
-      ChunkAt s;
-      s.b = b0;
-      int64_t units;
-      for (;; ++s.b) {
-        s.r = chunk_req(a, s.b);
-        units = units_of(s.r);
-        if (lo < at + units * a.nkv) break;
-        at += units * a.nkv;
-      }
-      s.h = int((lo - at) / units);
-      s.start = at + s.h * units;
-      s.tok0 = 0;
-      s.fill(a);
-      while (lo >= s.start + s.steps) {
-        s.start += s.steps;
-        s.tok0 += 2 * a.T;
-        s.fill(a);
-      }
-      s_at = s;
-    }
+    lo = min(me * run, total);
+    count = min(run, total - lo);
+    const uint32_t holds = __ballot_sync(kAll, count > 0 && upto - mine <= lo && lo < upto);
+    if (!holds) break;
+    src = __ffs(holds) - 1;  // one lane of one warp
+    at = __shfl_sync(kAll, upto - mine, src);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -255,34 +366,41 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     if (warp == 1) tmem_dealloc(tmem_base, kChTmemCols);
     return;
   }
-  const ChunkAt first = s_at;
-  // Every role walks the pairs of the run by itself: (pair, its first and last step + 1 in this run, its step 0 in the run's numbers, place).
-  // place: the tile whose rows are a pair's only ones; 2: both tiles.  Pairs of one tile take the two places in turn.
-  auto walk = [&](auto&& f) {
-    ChunkAt s = first;
-    int turn = 0;
-    for (int i = 0;;) {
-      const int j0 = int(lo + i - s.start), j1 = min(s.steps, j0 + count - i);
-      int place = 2;
-      if (s.ntok <= a.T) {
-        place = turn;
-        turn ^= 1;
+  // Step j of a share has slot j & 1 of the keys and of the values, so that a share with one tile has a slot to a place; a role knows a slot's phase by
+  // how often it has been filled.
+  // Every role goes through the run's shares of pairs: f(share, whether it has two tiles).  After a wait that ran out they go on without work.
+  bool ok = true;
+  auto each = [&](auto&& f) {
+#pragma unroll 1
+    for (int k = 0;; ++k) {
+      uint32_t never = 0;
+      if (!mbar_wait_small_warp(&bars.seg_full[k % kChSegs], uint32_t(k / kChSegs) & 1u, &never, 1u << 22)) {
+        *s_abort = 1;
+        return;
       }
-      if (!f(s, j0, j1, i, place)) return;
-      i += j1 - j0;
-      if (i >= count) return;
-      s.next(a);
+      const ChunkSeg s = bars.segs[k % kChSegs];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.seg_empty[k % kChSegs]);
+      if (s.n == 0) return;
+      f(s, s.ntok > a.T);
     }
   };
 
-  if (warp == 0) {
-    // ------------------------------ keys and values ------------------------------
-    int kst = 0, issued_k = 0, issued_v = 0;  // (stages follow from the step's number)
-    bool ok = true;
+  if (warp == 0 || warp == 3) {
+    // ------------------------------ keys (warp 0); the list, queries and values (warp 3) ------------------------------
+    const uint32_t leader = elect_leader();
+    const int values = warp == 3;
+    uint64_t* full = Q4 ? bars.raw_full[values] : values ? bars.v_full : bars.k_full;
+    uint64_t* empty = Q4 ? bars.raw_empty[values] : values ? bars.v_empty : bars.k_empty;
+    const CUtensorMap* tmap = values ? &tmap_v : &tmap_k;
+    const uint32_t ring = base + (Q4 ? S::kOffRaw + values * kChRaw * S::kRawBytes : values ? S::kOffV : S::kOffK);
+    int rs = 0, issued = 0;  // (4-bit cache: a ring of its own)
+    uint32_t rphase = 1, fills[2] = {0, 0};
+    int asked_of[2] = {0, 0};  // fills of a slot
     uint32_t gone_before = 0;  // bit s: bars.gone[s] is set
-    walk([&](const ChunkAt& s, int j0, int j1, int i0, int) {
+    auto load = [&](const ChunkSeg& s) {
       const int* table = a.tables + size_t(s.b) * a.max_blocks;
-      // lane l: granule l of eight steps -- the row of the cache where it begins (tile of the 4-bit cache), -1: nothing visible, -2: no block
+      // lane l: granule l of four steps -- the row of the cache where it begins (tile of the 4-bit cache), -1: nothing visible, -2: no block
       auto look = [&](int j) {
         const int tok = j * kChKeys + lane * kChGran;
         int at = -1;
@@ -292,369 +410,422 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         }
         return at;
       };
-      int ahead = look(j0), where = 0;
+      int ahead = look(s.j0), where = 0;
       const int none = a.n_blocks * a.nkv * a.block_size;  // behind the cache
-      for (int j = j0; j < j1; ++j) {
-        const int part = (j - j0) & 7, i = i0 + j - j0;
+#pragma unroll 1
+      for (int j = 0; j < s.n; ++j) {
+        const int part = j & 3, i = s.i0 + j;
         if (part == 0) {
           where = ahead;
-          ahead = look(j + 8);
+          ahead = look(s.j0 + j + 4);
         }
-        const uint32_t lost = __ballot_sync(kAll, where == -2) >> (4 * part) & 15u;
-        if constexpr (!Q4) {
-          const int gr = lane & 3, half = lane >> 2 & 1;
-          const int at = __shfl_sync(kAll, where, 4 * part + gr);
-          const int y = at >= 0 ? at : none;
-          const bool mine = lane < 4 * (HD / 64) && gr % (a.box / kChGran) == 0;
-          const uint32_t off = uint32_t(half) * S::kHalf + uint32_t(gr) * (kChGran * 128);
-          kst = i % kChStages;
-          const uint32_t phase = uint32_t(i / kChStages) & 1u;
-          ok = mbar_wait_bounded_warp(&bars.k_empty[kst], phase ^ 1u, s_abort, a.polls);
-          if (!ok) break;
-          if (lane == 0) {
-            if (lost || (gone_before >> (i & 7) & 1u)) bars.gone[i & 7] = lost;
-            mbar_expect_tx(&bars.k_full[kst], S::kKV);
+        const uint32_t lost = __ballot_sync(kAll, where == -2) >> (kChGrans * part) & 255u;
+#pragma unroll 1
+        for (int u = 0; u < (Q4 ? 2 : 1); ++u) {
+          const int st = Q4 ? rs : j & 1;
+          const uint32_t phase = Q4 ? rphase : (st ? fills[1] : fills[0]) + uint32_t(j >> 1) + 1u;
+          if (!(ok = mbar_wait_small_warp(&empty[st], phase & 1u, s_abort, a.polls))) return;
+          if (!values && u == 0) {
+            if (lane == 0 && (lost || (gone_before >> (i & 7) & 1u))) bars.gone[i & 7] = lost;
+            gone_before = (gone_before & ~(1u << (i & 7))) | uint32_t(lost != 0) << (i & 7);
+            __syncwarp();
           }
-          gone_before = (gone_before & ~(1u << (i & 7))) | uint32_t(lost != 0) << (i & 7);
-          __syncwarp();
-          if (mine) tma_load_2d_hint_s(base + S::kOffK + kst * S::kKV + off, &tmap_k, smem_u32(&bars.k_full[kst]), half * 64, y, kHintEvictLast);
-          issued_k = i + 1;
-          ok = mbar_wait_bounded_warp(&bars.v_empty[kst], phase ^ 1u, s_abort, a.polls);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&bars.v_full[kst], S::kKV);
-          __syncwarp();
-          if (mine) tma_load_2d_hint_s(base + S::kOffV + kst * S::kKV + off, &tmap_v, smem_u32(&bars.v_full[kst]), half * 64, y, kHintEvictLast);
-          issued_v = i + 1;
-        } else {
-          const int at = __shfl_sync(kAll, where, 4 * part + (lane & 3));
-          const uint32_t has = __ballot_sync(kAll, at >= 0) & 15u;
-          const int rs = i % kChRaw;
-          ok = mbar_wait_bounded_warp(&bars.raw_empty[rs], (uint32_t(i / kChRaw) & 1u) ^ 1u, s_abort, a.polls);
-          if (!ok) break;
-          if (lane == 0) {
-            bars.gone[i & 7] = lost | (has ^ 15u) << 8;
-            mbar_expect_tx(&bars.raw_full[rs], uint32_t(__popc(has)) * q4_tile_bytes(HD));
+          if constexpr (!Q4) {
+            // (the whole warp stays together and one lane issues)
+            mbar_expect_tx_warp(leader, &full[st], S::kKV);
+#pragma unroll 1
+            for (int gr = 0; gr < kChGrans; gr += a.box / kChGran) {
+              const int at = __shfl_sync(kAll, where, kChGrans * part + gr);
+#pragma unroll
+              for (int h = 0; h < HD / 64; ++h)
+                tma_load_2d_hint_warp(leader, ring + st * S::kKV + h * S::kHalf + gr * (kChGran * 128), tmap, smem_u32(&full[st]), h * 64, at >= 0 ? at : none,
+                                      kHintEvictLast);
+            }
+          } else {
+            // lanes 0..3 ask for the codes of a granule, 4..7 for its steps and least elements; one that is not there leaves what stood there before
+            const int at = __shfl_sync(kAll, where, kChGrans * part + 4 * u + (lane & 3));
+            const uint32_t has = __ballot_sync(kAll, at >= 0) & 15u;
+            mbar_expect_tx_warp(leader, &full[st], uint32_t(__popc(has)) * S::kRawGran);
+            const bool params = lane >= 4;
+            const uint8_t* from = a.cache4 + size_t(max(at, 0)) * q4_tile_bytes(HD) + (values ? (params ? q4_v_params(HD) : q4_v_codes(HD)) : params ? q4_k_params(HD) : 0);
+            bulk_load_warp(lane < 8 && at >= 0, ring + st * S::kRawBytes + (lane & 3) * S::kRawGran + (params ? 8 * HD : 0), from, params ? 2 * HD : 8 * HD,
+                           smem_u32(&full[st]), kHintEvictFirst);
           }
-          __syncwarp();
-          bulk_load_warp(lane < 4 && at >= 0, base + S::kOffRaw + rs * S::kRawBytes + lane * q4_tile_bytes(HD),
-                         a.cache4 + size_t(max(at, 0)) * q4_tile_bytes(HD), q4_tile_bytes(HD), smem_u32(&bars.raw_full[rs]), kHintEvictFirst);
-          issued_k = i + 1;
+          ++issued;
+          if (!Q4) ++asked_of[st];
+          if (++rs == kChRaw) {
+            rs = 0;
+            rphase ^= 1u;
+          }
         }
       }
-      return ok;
-    });
-    // The block's shared memory is another's behind it: whatever is still on its way lands first, also after a wait that ran out.
-    auto drain = [&](uint64_t* full, int issued, int stages) {
-      for (int i = max(0, issued - stages); i < issued; ++i)
-        for (uint32_t p = 0; p < (1u << 20); ++p)
-          if (mbar_try_wait(&full[i % stages], uint32_t(i / stages) & 1u)) break;
+      fills[0] += uint32_t(s.n + 1) >> 1;
+      fills[1] += uint32_t(s.n) >> 1;
     };
+    if (!values) {
+      each([&](const ChunkSeg& s, bool) {
+        if (ok) load(s);
+      });
+    } else {
+      const uint32_t bytes = uint32_t(a.G) * a.T * HD * 2;
+      int asked[2] = {0, 0};  // tiles asked for, by place
+      ChunkMeta m = {};       // what the second kernel needs to know
+      int b = s_first[0], h = s_first[1], tok0 = s_first[2], j0 = s_first[3];
+      ChunkReq r = chunk_req(a, b);
+#pragma unroll 1
+      for (int k = 0, i = 0;; ++k) {
+        ChunkSeg s = {};
+        if (i < count) {
+          s.b = b;
+          s.h = h;
+          s.row = r.q0 + tok0;
+          s.ntok = min(pair, r.n - tok0);
+          s.keys = chunk_keys(r, tok0, s.ntok);
+          s.lim = r.past + tok0 + 1;
+          s.cap = r.cap;
+          const int steps = chunk_steps(s.keys);
+          s.j0 = j0;
+          s.n = min(steps - j0, count - i);
+          s.i0 = i;
+          s.piece = s.n == steps ? -1 : 2 * me + (i == 0 ? 0 : 1);
+          if (j0 == 0 && s.n < steps) m = {int((lo + i + steps - 1) / run) - me + 1, s.piece, h, s.row, s.ntok};
+          i += s.n;
+          j0 = 0;
+          tok0 += pair;
+          if (tok0 >= r.n) {
+            tok0 = 0;
+            if (++h == a.nkv && i < count) {
+              h = 0;
+              do r = chunk_req(a, ++b);
+              while (r.n == 0);  // (there are more steps, so there is another)
+            }
+          }
+        }
+        uint32_t never = 0;
+        if (!mbar_wait_small_warp(&bars.seg_empty[k % kChSegs], (uint32_t(k / kChSegs) & 1u) ^ 1u, &never, 1u << 22)) {
+          *s_abort = 1;
+          break;
+        }
+        if (lane == 0) {
+          bars.segs[k % kChSegs] = s;
+          mbar_arrive(&bars.seg_full[k % kChSegs]);
+        }
+        __syncwarp();
+        if (s.n == 0) break;
+        const bool two = s.ntok > a.T;
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || (t == 1 && !two && s.n < 2)) break;
+          if (!(ok = mbar_wait_small_warp(&bars.q_empty[t], (uint32_t(asked[t]) & 1u) ^ 1u, s_abort, a.polls))) break;
+          if (lane == 0) {
+            mbar_expect_tx(&bars.q_full[t], bytes);
+#pragma unroll
+            for (int hh = 0; hh < HD / 64; ++hh)
+              tma_load_3d_hint_s(base + t * S::kQ + hh * S::kQHalf, &tmap_q, smem_u32(&bars.q_full[t]), hh * 64, s.h * a.G, s.row + (two ? t * a.T : 0), kHintEvictFirst);
+          }
+          ++asked[t];
+        }
+        if (ok) load(s);
+      }
+      if (lane == 0) a.meta[me] = m;
+      if (*s_abort)
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t)
+          if (asked[t] > 0)
+#pragma unroll 1
+            for (uint32_t p = 0; p < (1u << 20); ++p)
+              if (mbar_try_wait(&bars.q_full[t], uint32_t(asked[t] - 1) & 1u)) break;
+    }
+    // The block's shared memory is another's behind it: whatever is still on its way lands first, also after a wait that ran out.
     if (*s_abort) {
-      if constexpr (Q4) {
-        drain(bars.raw_full, issued_k, kChRaw);
-      } else {
-        drain(bars.k_full, issued_k, kChStages);
-        drain(bars.v_full, issued_v, kChStages);
+#pragma unroll 1
+      for (int i = 0; i < (Q4 ? kChRaw : 2); ++i) {
+        // (a slot that was never filled has nothing on its way; of the others the last fill counts)
+        const int n = Q4 ? (issued + kChRaw - 1 - i) / kChRaw : asked_of[i];
+#pragma unroll 1
+        for (uint32_t p = 0; n > 0 && p < (1u << 20); ++p)
+          if (mbar_try_wait(&full[i], uint32_t(n - 1) & 1u)) break;
       }
     }
-  } else if (warp == 2) {
-    // ------------------------------ queries ------------------------------
-    const uint32_t bytes = uint32_t(a.G) * a.T * HD * 2;
-    int n[2] = {0, 0};  // tiles asked for, by place
-    walk([&](const ChunkAt& s, int, int, int, int place) {
-      for (int t = 0; t < 2; ++t) {
-        if (place != 2 && place != t) continue;
-        if (!mbar_wait_bounded_warp(&bars.q_empty[t], (uint32_t(n[t]) & 1u) ^ 1u, s_abort, a.polls)) return false;
-        if (lane == 0) {
-          mbar_expect_tx(&bars.q_full[t], bytes);
-#pragma unroll
-          for (int h = 0; h < HD / 64; ++h)
-            tma_load_3d_hint_s(base + t * S::kQ + h * S::kQHalf, &tmap_q, smem_u32(&bars.q_full[t]), h * 64, s.h * a.G,
-                               s.r.q0 + s.tok0 + (place == 2 ? t * a.T : 0), kHintEvictFirst);
-        }
-        ++n[t];
-      }
-      return true;
-    });
-    if (*s_abort)
-      for (int t = 0; t < 2; ++t)
-        if (n[t] > 0)
-          for (uint32_t p = 0; p < (1u << 20); ++p)
-            if (mbar_try_wait(&bars.q_full[t], uint32_t(n[t] - 1) & 1u)) break;
-  } else if (warp == 1) {
-    // ------------------------------ products ------------------------------
+  } else if (warp < 3) {
+    // ------------------------------ products, a place's by a warp ------------------------------
+    // (a wait takes as long as the tensor cores have queued products for: two warps, and one's products fill the other's waits)
     const uint32_t leader = elect_leader();
-    const uint32_t idesc_s = umma_idesc_f16(kChRows, kChKeys, 1);
+    const int t = warp - 1;
+    const uint32_t idesc_s = umma_idesc_f16(kChRows, kChHalf, 1);
     const uint32_t idesc_o = umma_idesc_f16(kChRows, HD, 1) | kUmmaBMajorN;
-    auto issue_s = [&](int t, int p, int st) {
-      const uint64_t dq = umma_desc_k_sw128(base + t * S::kQ), dk = umma_desc_k_sw128(base + S::kOffK + st * S::kKV);
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-        umma_f16_ss_warp(leader, tmem_base + uint32_t(t * 128 + p * kChKeys), dq + uint64_t((ks >> 2) * (S::kQHalf / 16) + 2 * (ks & 3)),
-                         dk + uint64_t((ks >> 2) * (S::kHalf / 16) + 2 * (ks & 3)), idesc_s, ks > 0 ? 1u : 0u);
-      umma_commit_warp(leader, &bars.s_ready[t][p]);
-    };
-    auto issue_pv = [&](int t, int p, int st, bool acc) {
-      const uint64_t dv = umma_desc_mn_sw128(base + S::kOffV + st * S::kKV, S::kHalf);
-#pragma unroll
-      for (int ks = 0; ks < kChKeys / 16; ++ks)
-        umma_f16_ts_warp(leader, tmem_base + 256u + uint32_t(t * 128), tmem_base + uint32_t(t * 128 + p * kChKeys + 8 * ks), dv + uint64_t(128 * ks), idesc_o,
-                         (acc || ks > 0) ? 1u : 0u);
-      umma_commit_warp(leader, &bars.pv_done[t]);
-    };
-    bool ok = true;
-    // scores, two steps ahead of the products with values
-    ChunkAt sa = first;
-    int s_i = 0, s_pair = 0, s_turn = 0;           // step of the run, where its pair begins there, whose turn it is
-    int s_uses[2] = {0, 0}, s_tiles[2] = {0, 0};   // uses and query tiles of either place so far
-    int s_j0 = int(lo - sa.start), s_j1 = min(sa.steps, s_j0 + count), s_place = sa.ntok <= a.T ? s_turn : 2;
-    if (s_place != 2) s_turn ^= 1;
-    auto scores = [&] {
-      if (s_i >= count) return true;
-      if (s_i - s_pair >= s_j1 - s_j0) {
-        s_pair = s_i;
-        sa.next(a);
-        s_j0 = 0;
-        s_j1 = min(sa.steps, count - s_i);
-        s_place = 2;
-        if (sa.ntok <= a.T) {
-          s_place = s_turn;
-          s_turn ^= 1;
-        }
-      }
-      const int st = s_i % kChStages;
-      if (!mbar_wait_bounded_warp(&bars.k_full[st], uint32_t(s_i / kChStages) & 1u, s_abort, a.polls)) return false;
-      const bool begins = s_i == s_pair, ends = s_i - s_pair + 1 == s_j1 - s_j0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (s_place != 2 && s_place != t) continue;
-        if (begins && !mbar_wait_bounded_warp(&bars.q_full[t], uint32_t(s_tiles[t]++) & 1u, s_abort, a.polls)) return false;
-        tc_fence_after_sync();
-        issue_s(t, s_uses[t]++ & 1, st);
-        if (ends) umma_commit_warp(leader, &bars.q_empty[t]);
-      }
-      umma_commit_warp(leader, &bars.k_empty[st]);
-      ++s_i;
-      return true;
-    };
-    ok = scores() && scores();
-    int uses[2] = {0, 0}, pairs[2] = {0, 0};
-    if (ok)
-      walk([&](const ChunkAt& s, int j0, int j1, int i0, int place) {
-        for (int j = j0; j < j1; ++j) {
-          const int i = i0 + j - j0, st = i % kChStages;
-          bool waited = false;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (place != 2 && place != t) continue;
-            const int p = uses[t] & 1;
-            bool here = mbar_wait_bounded(&bars.p_ready[t][p], uint32_t(uses[t] >> 1) & 1u, s_abort, a.polls);
-            if (!waited) here = here && mbar_wait_bounded(&bars.v_full[st], uint32_t(i / kChStages) & 1u, s_abort, a.polls);
-            // the sums of the place's pair before have been read
-            if (j == j0) here = here && mbar_wait_bounded(&bars.o_free[t], (uint32_t(pairs[t]) & 1u) ^ 1u, s_abort, a.polls);
-            if (!__all_sync(kAll, here)) return ok = false;
-            if (!Q4 && !waited && (j + 1) * kChKeys > s.keys && s.keys % a.box) {
-              // the rest of the last box: probabilities are zero there, values may be anything
-              const int r0 = s.keys - j * kChKeys, r1 = (r0 + a.box - 1) / a.box * a.box;
-              for (int k = lane + r0 * (HD / 8); k < r1 * (HD / 8); k += 32) {
-                const int r = k / (HD / 8), c = k % (HD / 8);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(base + S::kOffV + st * S::kKV + (c >> 3) * S::kHalf + r * 128 + (c & 7) * 16), "r"(0)
-                             : "memory");
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-            }
-            waited = true;
-            tc_fence_after_sync();
-            issue_pv(t, p, st, j > j0);
-            if (j + 1 == j1) {
-              umma_commit_warp(leader, &bars.o_final[t]);
-              ++pairs[t];
-            }
-            ++uses[t];
+    const uint64_t desc_q = umma_desc_k_sw128(base + t * S::kQ), desc_k = umma_desc_k_sw128(base + S::kOffK), desc_v = umma_desc_mn_sw128(base + S::kOffV, S::kHalf);
+    const uint32_t s_at = tmem_base + uint32_t(t * 128), o_at = s_at + 256u;
+    uint32_t uses[2] = {0, 0}, tiles = 0, fills[2] = {0, 0};  // halves of steps, pairs of this place so far; fills of either slot ahead of this share
+    uint32_t meets = 0;
+    bool apart = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = mbar_wait_quick_warp(bar, parity & 1u, s_abort, a.polls); };
+    auto share = [&](const ChunkSeg& s, bool two) {
+      const int every = two ? 1 : 2, n = s.n, begin = two ? 0 : t;  // this place's steps
+      if (begin >= n) return;
+      auto filled = [&](int j) { return ((j & 1) ? fills[1] : fills[0]) + uint32_t(j >> 1); };
+      const int last = (n - 1 - begin) / every * every + begin;       // this place's last step
+      const bool cut = s.keys - (s.j0 + last) * kChKeys <= kChHalf;   // of which there is the first half only
+      if (!wait(&bars.q_full[t], tiles)) return;
+#pragma unroll 1
+      for (int js = begin;; js += every) {
+        const int j = js - every, sk = js & 1, sv = j & 1;
+        const bool product = js != begin, more = js <= last;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          // the scores of half h of step js, ahead of which that half of the place's step before is multiplied by its values
+          const bool of = product && !(h == 1 && cut && j == last), next = more && !(h == 1 && cut && js == last), fresh = of && h == 0 && j == begin;
+          if (of) {
+            if (!wait(&bars.p_ready[t][h], h ? uses[1]++ : uses[0]++)) return;
+            if (h == 0 && !wait(&bars.v_full[sv], filled(j))) return;
           }
-          umma_commit_warp(leader, &bars.v_empty[st]);
-          if (!scores()) return ok = false;
+          // (ahead of the product, behind which a wait takes longer; but the 4-bit cache's next keys may have to wait for the values that it reads)
+          if ((!Q4 || !product) && h == 0 && more && !wait(&bars.k_full[sk], filled(js))) return;
+          if (of) {
+            if (!Q4 && h == 0 && j == last) {
+              const int r0 = s.keys - (s.j0 + j) * kChKeys;
+              if (r0 < kChKeys && r0 % a.box) {
+                // the rest of the last box: probabilities are zero there, values may be anything
+                const int r1 = (r0 + a.box - 1) / a.box * a.box;
+#pragma unroll 1
+                for (int k = lane + r0 * (HD / 8); k < r1 * (HD / 8); k += 32) {
+                  const int r = k / (HD / 8), c = k % (HD / 8);
+                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(base + S::kOffV + sv * S::kKV + (c >> 3) * S::kHalf + r * 128 + (c & 7) * 16), "r"(0)
+                               : "memory");
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+              }
+            }
+            // a place's first product of a pair: the sums of the pair before have been read
+            if (fresh && !wait(&bars.o_free[t], tiles ^ 1u)) return;
+            tc_fence_after_sync();
+            umma_f16_ts4_warp(leader, o_at, s_at + uint32_t(kChHalf * h), desc_v + uint64_t(sv * int(S::kKV / 16) + h * (kChHalf * 128 / 16)), idesc_o, fresh ? 0u : 1u);
+            umma_commit_warp(leader, &bars.pv_done[t]);
+          }
+          if (h == 1 && product) {
+            umma_commit_warp(leader, &bars.v_empty[sv]);
+            if (!two) umma_commit_warp(leader, &bars.v_empty[sv]);  // (for the other place)
+          }
+          if (next) {
+            if (Q4 && product && h == 0 && !wait(&bars.k_full[sk], filled(js))) return;
+            tc_fence_after_sync();
+            umma_f16_ss_row_warp<HD>(leader, s_at + uint32_t(kChHalf * h), desc_q, desc_k + uint64_t(sk * int(S::kKV / 16) + h * (kChHalf * 128 / 16)), idesc_s);
+            umma_commit_warp(leader, &bars.s_ready[t][h]);
+          }
+          if (h == 1 && more) {
+            umma_commit_warp(leader, &bars.k_empty[sk]);
+            if (!two) umma_commit_warp(leader, &bars.k_empty[sk]);
+          }
         }
-        return true;
-      });
+        if (!more) break;
+      }
+      // the place's last product of this pair, and its last use of the queries
+      umma_commit_warp(leader, &bars.o_final[t]);
+      umma_commit_warp(leader, &bars.q_empty[t]);
+      ++tiles;
+    };
+    each([&](const ChunkSeg& s, bool two) {
+      // Where the places go on together after steps apart, each has to know that the other has seen its slot's fills: a phase is told from
+      // the one before it, not from older ones.
+      if (two && apart) {
+        if (lane == 0) mbar_arrive(&bars.met[t]);
+        if (ok) wait(&bars.met[t ^ 1], meets);
+        ++meets;
+      }
+      apart = !two;
+      if (ok) share(s, two);
+      fills[0] += uint32_t(s.n + 1) >> 1;
+      fills[1] += uint32_t(s.n) >> 1;
+    });
     if (!ok) {
       // products on their way read shared memory and write TMEM, which are given back below
-      umma_commit_warp(leader, &bars.drained);
-      mbar_wait_bounded_warp(&bars.drained, 0, s_abort, 1u << 20);
+      umma_commit_warp(leader, &bars.drained[t]);
+      mbar_wait_small_warp(&bars.drained[t], 0, s_abort, 1u << 20);
     }
   } else if (warp >= 12) {
     // ------------------------------ codes of the 4-bit cache to bf16 tiles ------------------------------
     if constexpr (Q4) {
       constexpr int NA = HD / kQ4Group;
       const int tid = threadIdx.x - 384;
-      walk([&](const ChunkAt& s, int j0, int j1, int i0, int) {
-        for (int j = j0; j < j1; ++j) {
-          const int i = i0 + j - j0, rs = i % kChRaw, st = i % kChStages;
-          if (!mbar_wait_bounded_warp(&bars.raw_full[rs], uint32_t(i / kChRaw) & 1u, s_abort, a.polls)) return false;
-          const uint32_t none = bars.gone[i & 7] >> 8;  // granules without copies
-          const int left = s.keys - j * kChKeys;        // tokens of this step
-          const uint32_t raw = base + S::kOffRaw + rs * S::kRawBytes;
-          auto words = [&](uint32_t addr, uint32_t (&w)[NA]) {
-            if constexpr (NA == 4)
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
-            else
-              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-          };
-          // (16 bits 0x430c are the bf16 number 128 + c)
-          auto value = [&](uint32_t two, __nv_bfloat162 step, __nv_bfloat162 low) {
-            const uint32_t c = (two & 0x000f000fu) | 0x43004300u, k = 0xc300c300u;  // - 128
-            const __nv_bfloat162 v = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(&k)), step, low);
-            return *reinterpret_cast<const uint32_t*>(&v);
-          };
-          auto twice = [](uint32_t w, int hi) {
-            const uint32_t v = __byte_perm(w, 0, hi ? 0x3232 : 0x1010);
-            return *reinterpret_cast<const __nv_bfloat162*>(&v);
-          };
-          auto store = [&](uint32_t tile, int key, int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(tile + (chunk >> 3) * S::kHalf + key * 128 + (((chunk & 7) ^ (key & 7)) << 4)), "r"(x), "r"(y), "r"(z), "r"(w)
-                         : "memory");
-          };
-          if (!mbar_wait_bounded_warp(&bars.k_empty[st], (uint32_t(i / kChStages) & 1u) ^ 1u, s_abort, a.polls)) return false;
-          const uint32_t kt = base + S::kOffK + st * S::kKV, vt = base + S::kOffV + st * S::kKV;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int key = u * 32 + (tid >> 2), t = tid & 3, g = key >> 4;
-            uint32_t w[NA] = {}, par[NA] = {};
-            if (key < left && !(none >> g & 1u)) {
-              words(raw + g * q4_tile_bytes(HD) + (key & 15) * (HD / 2) + t * NA * 4, w);
-              words(raw + g * q4_tile_bytes(HD) + q4_k_params(HD) + (key & 15) * NA * 4, par);
-            }
-#pragma unroll
-            for (int n = 0; n < NA; ++n) {
-              const __nv_bfloat162 step = twice(par[n >> 1], n & 1), low = twice(par[NA / 2 + (n >> 1)], n & 1);
-              // nibbles (0, 4), (1, 5), (2, 6), (3, 7)
-              const uint32_t p0 = value(w[n], step, low), p1 = value(w[n] >> 4, step, low), p2 = value(w[n] >> 8, step, low), p3 = value(w[n] >> 12, step, low);
-              store(kt, key, 4 * n + t, __byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.k_full[st]);
-          if (!mbar_wait_bounded_warp(&bars.v_empty[st], (uint32_t(i / kChStages) & 1u) ^ 1u, s_abort, a.polls)) return false;
+      auto words = [&](uint32_t addr, uint32_t (&w)[NA]) {
+        if constexpr (NA == 4)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+        else
+          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+      };
+      // (16 bits 0x430c are the bf16 number 128 + c; low + step * c is rounded once)
+      auto value = [&](uint32_t two, __nv_bfloat162 step, __nv_bfloat162 low) {
+        const uint32_t c = (two & 0x000f000fu) | 0x43004300u, k = 0xc300c300u;  // - 128
+        const __nv_bfloat162 v = __hfma2(__hadd2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(&k)), step, low);
+        return *reinterpret_cast<const uint32_t*>(&v);
+      };
+      auto pair_of = [](uint32_t x, uint32_t y, uint32_t how) {
+        const uint32_t v = __byte_perm(x, y, how);
+        return *reinterpret_cast<const __nv_bfloat162*>(&v);
+      };
+      auto store = [&](uint32_t tile, int key, int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(tile + (chunk >> 3) * S::kHalf + key * 128 + (((chunk & 7) ^ (key & 7)) << 4)), "r"(x), "r"(y), "r"(z), "r"(w)
+                     : "memory");
+      };
+      int rs = 0;
+      uint32_t rphase = 0, fills[2] = {0, 0};
+      each([&](const ChunkSeg& s, bool) {
+        if (!ok) return;
+        const int* table = a.tables + size_t(s.b) * a.max_blocks;
+        #pragma unroll 1
+        for (int j = 0; j < s.n; ++j) {
+          const int left = s.keys - (s.j0 + j) * kChKeys;  // tokens of this step
+          // granules that are there (as the copying warps saw it)
+          uint32_t has;
           {
-            // two tokens, eight dims of every group
-            const int pair = tid >> 2, q = tid & 3, g = pair >> 3, key = 2 * pair;
-            uint32_t w0[NA] = {}, w1[NA] = {}, pa[NA] = {}, pb[NA] = {};
-            const bool one = key < left && !(none >> g & 1u), two = key + 1 < left && !(none >> g & 1u);
-            const uint32_t tile = raw + g * q4_tile_bytes(HD);
-            if (one) {
-              words(tile + q4_v_codes(HD) + (pair & 7) * HD + 2 * q * NA * 4, w0);
-              words(tile + q4_v_codes(HD) + (pair & 7) * HD + (2 * q + 1) * NA * 4, w1);
-              words(tile + q4_v_params(HD) + (key & 15) * NA * 4, pa);
-            }
-            if (two) words(tile + q4_v_params(HD) + (key & 15) * NA * 4 + NA * 4, pb);
-#pragma unroll
-            for (int n = 0; n < NA; ++n) {
-              // (the first token's nibble beside the second's)
-              const uint32_t s2 = __byte_perm(pa[n >> 1], pb[n >> 1], n & 1 ? 0x7632 : 0x5410), l2 = __byte_perm(pa[NA / 2 + (n >> 1)], pb[NA / 2 + (n >> 1)], n & 1 ? 0x7632 : 0x5410);
-              const __nv_bfloat162 step = *reinterpret_cast<const __nv_bfloat162*>(&s2), low = *reinterpret_cast<const __nv_bfloat162*>(&l2);
-              uint32_t v[8];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                v[e] = value(w0[n] >> (4 * e), step, low);
-                v[4 + e] = value(w1[n] >> (4 * e), step, low);
-              }
-              const int chunk = 4 * n + q;
-              store(vt, key, chunk, __byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[4], v[5], 0x5410), __byte_perm(v[6], v[7], 0x5410));
-              store(vt, key + 1, chunk, __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632), __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
-            }
+            const int tok = (s.j0 + j) * kChKeys + (lane & 7) * kChGran;
+            const int blk = tok < s.keys ? table[tok / a.block_size] : -1;
+            has = __ballot_sync(kAll, blk >= 0 && blk < a.n_blocks);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&bars.v_full[st]);
-            mbar_arrive(&bars.raw_empty[rs]);
+          const int rs0 = rs, st = j & 1;
+          const uint32_t rphase0 = rphase, phase = ((st ? fills[1] : fills[0]) + uint32_t(j >> 1) + 1u) & 1u;
+#pragma unroll 1
+          for (int values = 0; values < 2; ++values) {
+            rs = rs0;
+            rphase = rphase0;
+            const uint32_t tile = base + (values ? S::kOffV : S::kOffK) + st * S::kKV;
+            if (!mbar_wait_quick_warp(values ? &bars.v_empty[st] : &bars.k_empty[st], phase, s_abort, a.polls)) { ok = false; return; }
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+              if (!mbar_wait_quick_warp(&bars.raw_full[values][rs], rphase, s_abort, a.polls)) { ok = false; return; }
+              const uint32_t raw = base + S::kOffRaw + (values * kChRaw + rs) * S::kRawBytes;
+              if (!values) {
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                  const int in = v * 32 + (tid >> 2), t = tid & 3, g = in >> 4, key = 64 * u + in;
+                  const uint32_t gran = raw + g * S::kRawGran;
+                  uint32_t w[NA] = {}, par[NA] = {};
+                  if (key < left && (has >> (4 * u + g) & 1u)) {
+                    words(gran + (in & 15) * (HD / 2) + t * NA * 4, w);
+                    words(gran + 8 * HD + (in & 15) * NA * 4, par);
+                  }
+#pragma unroll
+                  for (int m = 0; m < NA; ++m) {
+                    const __nv_bfloat162 step = pair_of(par[m >> 1], 0, m & 1 ? 0x3232 : 0x1010), low = pair_of(par[NA / 2 + (m >> 1)], 0, m & 1 ? 0x3232 : 0x1010);
+                    // nibbles (0, 4), (1, 5), (2, 6), (3, 7)
+                    const uint32_t p0 = value(w[m], step, low), p1 = value(w[m] >> 4, step, low), p2 = value(w[m] >> 8, step, low), p3 = value(w[m] >> 12, step, low);
+                    store(tile, key, 4 * m + t, __byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
+                  }
+                }
+              } else {
+                // two tokens, eight dims of every group
+                const int in = 2 * (tid >> 2), q = tid & 3, g = in >> 4, key = 64 * u + in;
+                const uint32_t gran = raw + g * S::kRawGran;
+                uint32_t w0[NA] = {}, w1[NA] = {}, pa[NA] = {}, pb[NA] = {};
+                if (key < left && (has >> (4 * u + g) & 1u)) {
+                  words(gran + (in >> 1 & 7) * HD + 2 * q * NA * 4, w0);
+                  words(gran + (in >> 1 & 7) * HD + (2 * q + 1) * NA * 4, w1);
+                  words(gran + 8 * HD + (in & 15) * NA * 4, pa);
+                  if (key + 1 < left) words(gran + 8 * HD + (in & 15) * NA * 4 + NA * 4, pb);
+                }
+#pragma unroll
+                for (int m = 0; m < NA; ++m) {
+                  // (the first token's beside the second's)
+                  const uint32_t how = m & 1 ? 0x7632 : 0x5410;
+                  const __nv_bfloat162 step = pair_of(pa[m >> 1], pb[m >> 1], how), low = pair_of(pa[NA / 2 + (m >> 1)], pb[NA / 2 + (m >> 1)], how);
+                  uint32_t v[8];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    v[e] = value(w0[m] >> (4 * e), step, low);
+                    v[4 + e] = value(w1[m] >> (4 * e), step, low);
+                  }
+                  const int chunk = 4 * m + q;
+                  store(tile, key, chunk, __byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[4], v[5], 0x5410), __byte_perm(v[6], v[7], 0x5410));
+                  store(tile, key + 1, chunk, __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632), __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
+                }
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars.raw_empty[values][rs]);
+              if (++rs == kChRaw) {
+                rs = 0;
+                rphase ^= 1u;
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(values ? &bars.v_full[st] : &bars.k_full[st]);
           }
         }
-        return true;
+        fills[0] += uint32_t(s.n + 1) >> 1;
+        fills[1] += uint32_t(s.n) >> 1;
       });
     }
   } else if (warp >= 4) {
     // ------------------------------ softmax ------------------------------
     const int t = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;  // TMEM lanes that this warp may touch
     const int tok = row / a.G, g = row - tok * a.G;
-    const uint32_t lane_addr = tmem_base + (uint32_t(quarter * 32) << 16);
-    const uint32_t o_addr = lane_addr + 256u + uint32_t(t * 128);
-    int uses = 0, pairs = 0;
-    bool ok = true;
-    walk([&](const ChunkAt& s, int j0, int j1, int i0, int place) {
-      if (place != 2 && place != t) return true;
-      const int tk = s.tok0 + (place == 2 ? t * a.T : 0) + tok;  // token of the request
-      const bool valid = tok < a.T && tk < s.r.n;
-      const int lim = min(s.r.past + tk + 1, s.r.cap);           // keys [0, lim) are visible
+    const uint32_t s_base = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(t * 128);
+    const uint32_t o_addr = tmem_base + (uint32_t(quarter * 32) << 16) + 256u + uint32_t(t * 128);
+    float2* s_sums = reinterpret_cast<float2*>(gen + S::kOffSums);
+    uint32_t uses[2] = {0, 0}, pairs = 0, others = 0, joins = 0, products = 0;
+    each([&](const ChunkSeg& s, bool two) {
+      const int n = s.n, tk = (two ? t * a.T : 0) + tok;  // token of the pair
+      const bool valid = tok < a.T && tk < s.ntok;
+      const int lim = min(s.lim + tk, s.cap);             // keys [0, lim) are visible
       const bool busy = __any_sync(kAll, valid);
+      const int mine = two ? n : (n + 1 - t) >> 1;        // steps of this place
+      // halves of steps; the last may be without its second one
+      const int halves = 2 * mine - (mine > 0 && s.keys - (s.j0 + (two ? n - 1 : 2 * mine - 2 + t)) * kChKeys <= kChHalf ? 1 : 0);
       float m_used = -INFINITY, l = 0.f;
-      for (int j = j0; j < j1 && ok; ++j, ++uses) {
-        const int p = uses & 1;
-        if (!mbar_wait_bounded_warp(&bars.s_ready[t][p], uint32_t(uses >> 1) & 1u, s_abort, a.polls)) {
+#pragma unroll 1
+      for (int k = 0; k < halves && ok; ++k, ++products) {
+        const int j = one_copy(two) ? k >> 1 : (k & ~1) + t, half = k & 1;
+        if (!mbar_wait_quick_warp(&bars.s_ready[t][half], (half ? uses[1] : uses[0]) & 1u, s_abort, a.polls)) {
           ok = false;
           break;
         }
-        if (!busy) {  // rows of no token: whatever their probabilities are
-          mbar_arrive(&bars.p_ready[t][p]);
+        half ? ++uses[1] : ++uses[0];
+        if (!one_copy(busy)) {  // rows of no token: whatever their probabilities are
+          if (lane == 0) mbar_arrive(&bars.p_ready[t][half]);
           continue;
         }
         tc_fence_after_sync();
-        const uint32_t s_addr = lane_addr + uint32_t(t * 128 + p * kChKeys);
-        float x[kChKeys];
-        {
-          uint32_t r0[32], r1[32];
-          tmem_ld_32x32(s_addr, r0);
-          tmem_ld_32x32(s_addr + 32, r1);
-          tmem_ld_wait();
-          const float2 sl = make_float2(a.scale_log2, a.scale_log2);
+        const uint32_t s_addr = s_base + uint32_t(kChHalf * half);
+        const uint32_t lost = *const_cast<volatile uint32_t*>(&bars.gone[(s.i0 + j) & 7]) >> (kChGrans / 2 * half) & 15u;
+        const int seen = lim - (s.j0 + j) * kChKeys - kChHalf * half;  // of these keys
+        uint32_t r0[32], r1[32];
+        tmem_ld_32x32(s_addr, r0);
+        tmem_ld_32x32(s_addr + 32, r1);
+        tmem_ld_wait();
+        if (lost || __any_sync(kAll, valid && seen < kChHalf)) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float2 u = mul2(make_float2(__uint_as_float(r0[c]), __uint_as_float(r0[c + 1])), sl);
-            const float2 v = mul2(make_float2(__uint_as_float(r1[c]), __uint_as_float(r1[c + 1])), sl);
-            x[c] = u.x;
-            x[c + 1] = u.y;
-            x[c + 32] = v.x;
-            x[c + 33] = v.y;
+          for (int c = 0; c < 32; ++c) {
+            if (c >= seen || (lost >> (c / kChGran) & 1u)) r0[c] = 0xff800000u;
+            if (32 + c >= seen || (lost >> (2 + c / kChGran) & 1u)) r1[c] = 0xff800000u;
           }
         }
-        const int kbase = j * kChKeys;
-        if (kbase + kChKeys > lim) {
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < kChKeys; ++c)
-            if (kbase + c >= lim) x[c] = -INFINITY;
-        }
-        const uint32_t lost = *const_cast<volatile uint32_t*>(&bars.gone[(i0 + j - j0) & 7]) & 15u;
-        if (lost) {
+        for (int c = 0; c < 32; c += 4)
 #pragma unroll
-          for (int c = 0; c < kChKeys; ++c)
-            if (lost >> (c / kChGran) & 1u) x[c] = -INFINITY;
-        }
-        // four chains: the maximum is on the way from the scores to everything else
-        float mx4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int c = 4; c < kChKeys; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], x[c]);
-        const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
-        const bool grow = m_new > m_used + kChRescale;  // also true on the first finite maximum
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r0[c + e]), __uint_as_float(r1[c + e]));
+        const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2);
+        // also true on the first finite maximum; rows of no token have no say (the warp's others would be rounded as they have it)
+        const bool grow = valid && m_new > m_used + kChRescale;
         if (__any_sync(kAll, grow)) {
           const float alpha = (m_new == -INFINITY) ? 1.f : ex2_approx(m_used - m_new);
-          if (j > j0) {
-            // P V of the use before may still be running.  Parity tells its phase apart from its neighbours: the one behind needs this warp's own
-            // P, and the one before is over, since it was issued ahead of the scores of this use by the same thread.
-            if (!mbar_wait_bounded_warp(&bars.pv_done[t], uint32_t(uses - 1) & 1u, s_abort, a.polls)) {
+          if (k > 0) {
+            // P V of the half before may still be running.  Parity tells its phase from its neighbours: the one behind needs this warp's own P,
+            // and the one before it was issued ahead of these scores.
+            if (!mbar_wait_quick_warp(&bars.pv_done[t], (products - 1) & 1u, s_abort, a.polls)) {
               ok = false;
               break;
             }
             tc_fence_after_sync();
 #pragma unroll 1
-            for (int c0 = 0; c0 < HD; c0 += 32) {
-              uint32_t r[32];
-              tmem_ld_32x32(o_addr + c0, r);
+            for (int c0 = 0; c0 < HD; c0 += 16) {
+              uint32_t r[16];
+              tmem_ld_32x16(o_addr + c0, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
-              tmem_st_32x32(o_addr + c0, r);
+              for (int c = 0; c < 16; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+              tmem_st_32x16(o_addr + c0, r);
             }
             tmem_st_wait();
           }
@@ -662,69 +833,99 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           m_used = m_new;
         }
         const float mref = (m_used == -INFINITY) ? 0.f : m_used;
-        const float2 neg = make_float2(-mref, -mref);
+        const float2 neg = make_float2(-mref, -mref), sl = make_float2(a.scale_log2, a.scale_log2);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t pk[kChKeys / 2];
+        auto weigh = [&](const uint32_t (&r)[32], uint32_t to) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int c = 0; c < kChKeys; c += 2) {
-          const float2 u = add2(make_float2(x[c], x[c + 1]), neg);
-          const float2 e = make_float2(ex2_approx(u.x), ex2_approx(u.y));
-          sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], e);
-          // (P in bf16: the products want it; off by half a step, 2^-9, of every term)
-          pk[c >> 1] = pack_bf16x2(e.x, e.y);
-        }
+          for (int c = 0; c < 32; c += 2) {
+            const float2 u = fma2(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl, neg);
+            const float2 e = (c >> 1) % 4 < kChPoly ? ex2_poly(u) : make_float2(ex2_approx(u.x), ex2_approx(u.y));
+            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], e);
+            // (P in bf16: the products want it; off by half a step, 2^-8 at most, of every term)
+            pk[c >> 1] = pack_bf16x2(e.x, e.y);
+          }
+          tmem_st_32x16(to, pk);  // over the scores: P of 32 keys takes the columns of 16
+        };
+        weigh(r0, s_addr);
+        weigh(r1, s_addr + 16);
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
-        tmem_st_32x32(s_addr, pk);  // over the scores that it was made of
         tmem_st_wait();
         tc_fence_before_sync();
-        mbar_arrive(&bars.p_ready[t][p]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_ready[t][half]);
       }
       // ---- the pair's rows, or a piece of them ----
-      if (ok && !mbar_wait_bounded_warp(&bars.o_final[t], uint32_t(pairs) & 1u, s_abort, a.polls)) ok = false;
+      if (mine == 0) return;
+      if (ok && !mbar_wait_quick_warp(&bars.o_final[t], pairs & 1u, s_abort, a.polls)) ok = false;
       ++pairs;
-      const bool whole = j0 == 0 && j1 == s.steps;
-      const int piece = 2 * me + (i0 == 0 ? 0 : 1), at = (place == 2 ? t * kChRows : 0) + row;
-      const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : 0.f;
-      __nv_bfloat16* orow = a.out + (size_t(s.r.q0 + tk) * a.nq + size_t(s.h) * a.G + g) * HD;
-      float* prow = a.part + (size_t(piece) * a.row_cap + at) * HD;
-      tc_fence_after_sync();
-#pragma unroll 1
-      for (int c0 = 0; c0 < HD; c0 += 32) {
-        uint32_t r[32];
-        if (ok) {
-          tmem_ld_32x32(o_addr + c0, r);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) r[c] = 0x7fffffffu;
-        }
-        if (valid && whole) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 8)
-            *reinterpret_cast<uint4*>(orow + c0 + c) = make_uint4(
-                pack_bf16x2(__uint_as_float(r[c]) * inv, __uint_as_float(r[c + 1]) * inv), pack_bf16x2(__uint_as_float(r[c + 2]) * inv, __uint_as_float(r[c + 3]) * inv),
-                pack_bf16x2(__uint_as_float(r[c + 4]) * inv, __uint_as_float(r[c + 5]) * inv), pack_bf16x2(__uint_as_float(r[c + 6]) * inv, __uint_as_float(r[c + 7]) * inv));
-        } else if (valid) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(prow + c0 + c) = make_uint4(r[c], r[c + 1], r[c + 2], r[c + 3]);
-        }
+      const bool join = !two && n > 1;  // the sums of the same rows in two places
+      if (join && t == 1) {
+        s_sums[row] = make_float2(m_used, ok ? l : NAN);
+        tc_fence_before_sync();
         __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.sums);
+        return;
       }
-      if (!whole && valid)
-        reinterpret_cast<float2*>(a.part + size_t(2 * runs) * a.row_cap * HD)[size_t(piece) * a.row_cap + at] = make_float2(m_used, ok ? l : NAN);
+      float w0 = 1.f, w1 = 0.f;
+      if (join) {
+        if (ok && !(mbar_wait_quick_warp(&bars.sums, joins & 1u, s_abort, a.polls) && mbar_wait_quick_warp(&bars.o_final[1], others & 1u, s_abort, a.polls))) ok = false;
+        ++joins;
+        const float2 ml = s_sums[row];
+        const float m = fmaxf(m_used, ml.x), ref = m == -INFINITY ? 0.f : m;
+        w0 = ex2_approx(m_used - ref);
+        w1 = ex2_approx(ml.x - ref);
+        l = l * w0 + ml.y * w1;
+        m_used = m;
+      }
+      if (t == 0 && (two || join)) ++others;
+      const bool whole = s.piece < 0;
+      const int at = (two ? t * kChRows : 0) + row;
+      const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : NAN;
+      w0 = ok ? w0 * inv : NAN;
+      w1 *= inv;
+      __nv_bfloat16* orow = a.out + (size_t(s.row + tk) * a.nq + size_t(s.h) * a.G + g) * HD;
+      // (pieces: four dims of all rows beside one another, so that a warp's stores are whole lines)
+      float4* prow = reinterpret_cast<float4*>(a.part) + size_t(s.piece) * (HD / 4) * a.row_cap + at;
+      tc_fence_after_sync();
+      if (busy) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += 16) {
+          uint32_t r[16], q[16];
+          tmem_ld_32x16(o_addr + c0, r);
+          if (one_copy(join)) {
+            tmem_ld_32x16(o_addr + 128u + c0, q);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) q[c] = 0;
+          }
+          tmem_ld_wait();
+          float v[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) v[c] = fmaf(__uint_as_float(q[c]), w1, __uint_as_float(r[c]) * w0);
+          if (one_copy(valid && whole)) {
+#pragma unroll
+            for (int c = 0; c < 16; c += 8)
+              *reinterpret_cast<uint4*>(orow + c0 + c) =
+                  make_uint4(pack_bf16x2(v[c], v[c + 1]), pack_bf16x2(v[c + 2], v[c + 3]), pack_bf16x2(v[c + 4], v[c + 5]), pack_bf16x2(v[c + 6], v[c + 7]));
+          } else if (one_copy(valid)) {
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) prow[size_t((c0 + c) / 4) * a.row_cap] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+          }
+          __syncwarp();
+        }
+        if (!whole && valid)
+          reinterpret_cast<float2*>(a.part + size_t(2 * runs) * a.row_cap * HD)[size_t(s.piece) * a.row_cap + at] = make_float2(m_used, ok ? l : NAN);
+      }
       tc_fence_before_sync();
-      mbar_arrive(&bars.o_free[t]);
-      return true;  // (a run that gave up goes on to leave NaN everywhere)
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars.o_free[t]);
+        if (join) mbar_arrive(&bars.o_free[1]);
+      }
+      // (a run that gave up goes on to leave NaN everywhere)
     });
-  } else if (lane == 0) {
-    // ------------------------------ what the second kernel needs to know ------------------------------
-    ChunkMeta m = {};
-    walk([&](const ChunkAt& s, int j0, int j1, int i0, int) {
-      if (j0 == 0 && j1 < s.steps) m = {int((s.start + s.steps - 1) / run) - me + 1, 2 * me + (i0 == 0 ? 0 : 1), s.b, s.h, s.r.q0, s.tok0, s.ntok};
-      return true;
-    });
-    a.meta[me] = m;
   }
 
   tc_fence_before_sync();
@@ -736,76 +937,49 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   if (threadIdx.x == 0 && *s_abort) g_chunk_err = 1;
 }
 
-// Pieces of a pair that was cut: block (run where it begins, rows).  Eight warps take a row each, or, with more pieces, share a row.
+// Pieces of a pair that was cut: block (run where it begins, 32 rows), a lane a row, a warp HD / 8 of its dims.
 constexpr int kChMergeWarps = 8;
 template <int HD>
 __global__ void __launch_bounds__(kChMergeWarps * 32) k_chunk_merge(const Chunk a) {
-  constexpr int D = HD / 32;
-  __shared__ float s_o[kChMergeWarps][HD], s_m[kChMergeWarps], s_l[kChMergeWarps];
+  constexpr int V = HD / 4 / kChMergeWarps;  // vectors of four dims
   pdl_launch_dependents();
   pdl_wait();
-  const int me = blockIdx.x, runs = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int me = blockIdx.x, runs = gridDim.x, warp = threadIdx.x >> 5;
   const ChunkMeta m = a.meta[me];
+  const int r = blockIdx.y * 32 + (threadIdx.x & 31), tok = r / a.G, g = r - tok * a.G;
   // (every run leaves its words; lengths that another stream changes meanwhile, which nobody may, could leave some that fit nothing)
-  if (m.count <= 0 || m.count > runs - me || m.ntok > 2 * a.T) return;
-  const int ways = m.count <= 2 ? 1 : m.count <= 5 ? 2 : m.count <= 12 ? 4 : 8, per = kChMergeWarps / ways, w = warp % ways;
-  const int rows = m.ntok * a.G;
-  const float2* sums = reinterpret_cast<const float2*>(a.part + size_t(2 * runs) * a.row_cap * HD);
-  for (int r0 = blockIdx.y * per; r0 < rows; r0 += gridDim.y * per) {
-    const int r = r0 + warp / ways;
-    const bool there = r < rows;
-    const int tok = r / a.G, g = r - tok * a.G, at = (tok >= a.T ? kChRows + (tok - a.T) * a.G : tok * a.G) + g;
-    float M = -INFINITY, L = 0.f, acc[D];
+  if (m.count <= 0 || m.count > runs - me || m.ntok > 2 * a.T || tok >= m.ntok) return;
+  const int at = (tok >= a.T ? kChRows + (tok - a.T) * a.G : tok * a.G) + g;
+  const float2* sums = reinterpret_cast<const float2*>(a.part + size_t(2 * runs) * a.row_cap * HD) + at;
+  const float4* part = reinterpret_cast<const float4*>(a.part) + size_t(warp * V) * a.row_cap + at;
+  float M = -INFINITY, L = 0.f;
+  float4 acc[V];
 #pragma unroll
-    for (int d = 0; d < D; ++d) acc[d] = 0.f;
-    if (there) {
-#pragma unroll 4
-      for (int k = w; k < m.count; k += ways) {
-        const size_t p = size_t(k == 0 ? m.first : 2 * (me + k)) * a.row_cap + at;
-        const float2 ml = sums[p];
-        float v[D];
-        if constexpr (D == 4) {
-          const float4 u = *reinterpret_cast<const float4*>(a.part + p * HD + 4 * lane);
-          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-        } else {
-          const float2 u = *reinterpret_cast<const float2*>(a.part + p * HD + 2 * lane);
-          v[0] = u.x; v[1] = u.y;
-        }
-        const float n = fmaxf(M, ml.x), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(ml.x - ref);
-        M = n;
-        L = L * s0 + ml.y * s1;
+  for (int d = 0; d < V; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int k = 0; k < m.count; ++k) {
+    const size_t p = size_t(k == 0 ? m.first : 2 * (me + k)) * a.row_cap;
+    const float2 ml = sums[p];
+    float4 v[V];
 #pragma unroll
-        for (int d = 0; d < D; ++d) acc[d] = acc[d] * s0 + v[d] * s1;
-      }
-    }
-    if (ways > 1) {
+    for (int d = 0; d < V; ++d) v[d] = part[p * (HD / 4) + size_t(d) * a.row_cap];
+    const float n = fmaxf(M, ml.x), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(ml.x - ref);
+    M = n;
+    L = L * s0 + ml.y * s1;
 #pragma unroll
-      for (int d = 0; d < D; ++d) s_o[warp][D * lane + d] = acc[d];
-      if (lane == 0) {
-        s_m[warp] = M;
-        s_l[warp] = L;
-      }
-      __syncthreads();
-      if (w == 0) {
-        for (int i = 1; i < ways; ++i) {
-          const float n = fmaxf(M, s_m[warp + i]), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(s_m[warp + i] - ref);
-          M = n;
-          L = L * s0 + s_l[warp + i] * s1;
-#pragma unroll
-          for (int d = 0; d < D; ++d) acc[d] = acc[d] * s0 + s_o[warp + i][D * lane + d] * s1;
-        }
-      }
-      __syncthreads();
-    }
-    if (there && w == 0) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      __nv_bfloat16* to = a.out + (size_t(m.q0 + m.tok0 + tok) * a.nq + size_t(m.h) * a.G + g) * HD + D * lane;
-      if constexpr (D == 4)
-        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-      else
-        *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    for (int d = 0; d < V; ++d) {
+      acc[d].x = acc[d].x * s0 + v[d].x * s1;
+      acc[d].y = acc[d].y * s0 + v[d].y * s1;
+      acc[d].z = acc[d].z * s0 + v[d].z * s1;
+      acc[d].w = acc[d].w * s0 + v[d].w * s1;
     }
   }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  __nv_bfloat16* to = a.out + (size_t(m.row + tok) * a.nq + size_t(m.h) * a.G + g) * HD + 4 * V * warp;
+#pragma unroll
+  for (int d = 0; d < V; d += 2)
+    *reinterpret_cast<uint4*>(to + 4 * d) = make_uint4(pack_bf16x2(acc[d].x * inv, acc[d].y * inv), pack_bf16x2(acc[d].z * inv, acc[d].w * inv),
+                                                       pack_bf16x2(acc[d + 1].x * inv, acc[d + 1].y * inv), pack_bf16x2(acc[d + 1].z * inv, acc[d + 1].w * inv));
 }
 
 }  // namespace bl
@@ -855,6 +1029,10 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   if (n_blocks < 1) return refuse("needs a cache with a block");
   if (int64_t(n_blocks) * nkv * block_size > 0x7fffffffLL - kChKeys) return refuse("needs a cache whose rows (tokens times KV heads) fit 32 bits");
   if (int64_t(max_blocks) * block_size > 0x3fffffffLL) return refuse("needs tables of less than 2^30 tokens");
+  {
+    const int64_t pairs = tokens / (2 * chunk_tile_tokens(nq / nkv)) + int64_t(batch), steps = int64_t(max_blocks) * block_size / kChKeys + 1;
+    if (pairs * nkv > 0x7fffffffLL / steps - sm_count()) return refuse("has too many tokens for its tables: steps of 128 keys, over all tiles and KV heads, must fit 31 bits");
+  }
   if (q_stride % 8 || q_stride < 0 || (tokens > 1 && q_stride < int64_t(nq) * hd)) return refuse("needs rows of q on 16-byte boundaries that hold nq heads");
   if (!q || (cache4 ? k_cache || v_cache : !k_cache || !v_cache) || (!block_tables && max_blocks) || !cu_q || !ctx_lens || !out)
     return refuse("needs queries, one kind of cache, block tables, row offsets, context lengths and an output");
@@ -906,7 +1084,7 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   auto go = [&](auto* kernel, auto* merge, unsigned smem, unsigned threads, bool (&done)[64]) {
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), int(smem), done);
     if (e == cudaSuccess) e = launch_k(kernel, dim3(runs), dim3(threads), smem, st, tq, tk, tv, a);
-    if (e == cudaSuccess) e = launch_k(merge, dim3(runs, a.row_cap < 32 ? a.row_cap : 32), dim3(kChMergeWarps * 32), 0, st, a);
+    if (e == cudaSuccess) e = launch_k(merge, dim3(runs, (a.row_cap + 31) / 32), dim3(kChMergeWarps * 32), 0, st, a);
     return e;
   };
   cudaError_t e;
