@@ -5,16 +5,17 @@
 //   m = max x,  S = sum e^(x - m),  T = sum (x - m) e^(x - m)
 //   logprob(id) = x_id - m - log S,  entropy = log S - T / S
 //
-// One pass: a thread takes its share of a row into registers (up to kScoreLap vectors of 16 bytes, all asked for at once), finds their
-// maximum, adds up S and T relative to it, and looks through the same registers again for the most likely tokens.  Sums of
-// threads, warps and the blocks of a cluster, which share a row, are joined afterwards.
+// One pass: a block goes through its share of a row in laps, a thread with kScoreLap vectors of 16 bytes in registers and those of the next lap on
+// their way; it finds their maximum and adds up S and T relative to it.  Sums of laps, threads, warps and the blocks of a cluster, which share a
+// row, are joined afterwards.
 //
-// The `top` greatest: 64 groups of four threads each put forward the greatest element (of equals the first); the top-th greatest of these is
-// one that at least `top` elements reach, so whatever is below it is out.  Those that reach it, hardly more than `top` on logits, are
-// ranked by counting, which gives the order and leaves ties to the lowest index.
+// The `top` greatest: in the first lap 64 groups of four threads each put forward the greatest logit; the top-th greatest of these is one that at least
+// `top` logits reach, so whatever is below it is out; that is the border for all
+// laps.  Those that reach it, hardly more than `top` a lap on logits, are ranked by counting, which gives the order and leaves ties to the lowest index.
 #include <math.h>
 #include <stdio.h>
 
+#include "attn_tc.cuh"
 #include "bl_ops.h"
 #include "heap.h"
 #include "launch.h"
@@ -23,10 +24,11 @@
 namespace bl {
 
 constexpr int kScoreThreads = 256;
-constexpr int kScoreLap = 10;        // vectors of a thread in registers: 8 blocks of a row of 152064 bf16 logits need one lap
+constexpr int kScoreLap = 5;         // vectors of a thread and lap
 constexpr int kScoreTop = 32;        // alternatives at most
 constexpr int kScoreGroups = 64;
 constexpr int kScoreList = 1024;     // tokens that reach the border
+static_assert(8 * kScoreTop == kScoreThreads, "a thread for every token that a cluster puts forward");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Score {
@@ -70,15 +72,24 @@ __device__ __forceinline__ ScoreSum score_xor(ScoreSum a, int lane_mask) {
 }
 
 // Order of tokens: the greater logit, of equals the lower index.  0: none (-inf and NaN among them).
-__device__ __forceinline__ uint64_t score_key(float x, int idx) {
+__device__ __forceinline__ uint32_t score_order(float x) {
   if (!(x > -INFINITY)) return 0;
   const uint32_t u = __float_as_uint(x + 0.f);  // (-0 counts as 0)
-  return uint64_t(u ^ (u >> 31 ? 0xffffffffu : 0x80000000u)) << 32 | uint32_t(~idx);
+  return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ float score_key_value(uint64_t k) {
-  const uint32_t u = uint32_t(k >> 32);
-  return k == 0 ? -INFINITY : __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u);
+__device__ __forceinline__ uint64_t score_key(float x, int idx) {
+  const uint32_t u = score_order(x);
+  return u ? uint64_t(u) << 32 | uint32_t(~idx) : 0;
 }
+__device__ __forceinline__ float2 score_fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float score_unorder(uint32_t u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
+__device__ __forceinline__ float score_key_value(uint64_t k) { return k == 0 ? -INFINITY : score_unorder(uint32_t(k >> 32)); }
 __device__ __forceinline__ int score_key_index(uint64_t k) { return k == 0 ? -1 : int(~uint32_t(k)); }
 
 template <bool FP32>
@@ -94,13 +105,6 @@ struct ScoreVec {
   static __device__ __forceinline__ float load(const void* row, size_t i) {
     return FP32 ? static_cast<const float*>(row)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]);
   }
-  static __device__ __forceinline__ void set(uint4& v, int e, const void* row, size_t i) {
-    uint32_t& w = (&v.x)[FP32 ? e : e >> 1];
-    if constexpr (FP32)
-      w = static_cast<const uint32_t*>(row)[i];
-    else
-      w = e & 1 ? (w & 0xffffu) | uint32_t(static_cast<const uint16_t*>(row)[i]) << 16 : (w & 0xffff0000u) | static_cast<const uint16_t*>(row)[i];
-  }
   // the greatest element; NaN is passed over
   static __device__ __forceinline__ float most(const uint4& v) {
     if constexpr (FP32) return fmaxf(fmaxf(at(v, 0), at(v, 1)), fmaxf(at(v, 2), at(v, 3)));
@@ -114,173 +118,195 @@ struct ScoreVec {
 // the place of `key` among keys[0..n) (all different but for 0): how many are greater
 __device__ __forceinline__ int score_rank(uint64_t key, const uint64_t* keys, int n) {
   int above = 0;
+#pragma unroll 4
   for (int i = 0; i < n; ++i) above += keys[i] > key;
   return above;
 }
 
 template <bool FP32, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads) k_token_logprobs(const Score a) {
+__global__ void __launch_bounds__(kScoreThreads, 4) k_token_logprobs(const Score a) {
   using V = ScoreVec<FP32>;
   constexpr int kWarps = kScoreThreads / 32;
   __shared__ float s_sum[kWarps][3];
   __shared__ float s_parts[8][3];                          // of the cluster's blocks, in the first one
   __shared__ uint64_t s_best[TOP ? 8 * kScoreTop : 1];     // their most likely tokens
-  __shared__ uint64_t s_group[TOP ? kScoreGroups : 1];
-  __shared__ uint64_t s_list[TOP ? kScoreList + kScoreTop : 1];
-  __shared__ uint64_t s_kept[TOP ? kScoreTop : 1];         // the greatest of this block so far
-  __shared__ uint64_t s_border, s_round[TOP ? kWarps : 1];
+  __shared__ uint32_t s_group[TOP ? kScoreGroups : 1];
+  __shared__ uint64_t s_list[TOP ? kScoreList : 1];
+  __shared__ uint64_t s_round[TOP ? kWarps : 1];
+  __shared__ float s_border;
   __shared__ int s_count;
   pdl_launch_dependents();
   const int share = cluster_nctarank(), rank = cluster_ctarank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / share;
+  if constexpr (TOP) {
+    s_best[tid] = 0;  // (as many as threads)
+    if (tid == 0) s_count = 0;
+  }
+  if (share > 1) cluster_arrive();
   pdl_wait();
   const uint8_t* x = static_cast<const uint8_t*>(a.logits) + size_t(row) * a.ld * (FP32 ? 4 : 2);
-  // Vectors on 16-byte boundaries; the row starts `shift` elements into the first one.
-  const int shift = int(reinterpret_cast<uintptr_t>(x) & 15) / (FP32 ? 4 : 2);
-  const uint4* vecs = reinterpret_cast<const uint4*>(x - (reinterpret_cast<uintptr_t>(x) & 15));
-  const int n_vecs = a.n > 0 ? int((int64_t(a.n) + shift + V::N - 1) / V::N) : 0;
+  // Whole vectors on 16-byte boundaries, and up to N - 1 elements ahead of them and behind, which are the first and the last block's, one to a thread.
+  const int shift = int(reinterpret_cast<uintptr_t>(x) & 15) / (FP32 ? 4 : 2), head = min(a.n, (V::N - shift) % V::N);
+  const uint4* vecs = reinterpret_cast<const uint4*>(x + size_t(head) * (FP32 ? 4 : 2));
+  const int n_vecs = (a.n - head) / V::N, rest = (a.n - head) % V::N;
   const int per = (n_vecs + share - 1) / share, v0 = min(rank * per, n_vecs), v1 = min(v0 + per, n_vecs);
+  const int single = rank == 0 && tid < head ? tid : rank == share - 1 && tid >= V::N && tid - V::N < rest ? a.n - rest + tid - V::N : -1;
   // the logits of the given tokens, asked for ahead of everything else
   const bool gives = rank == 0 && tid < a.n_ids;
   auto logit_of = [&](int id) {
     const int64_t c = int64_t(id) - a.offset;
     return id >= 0 && c >= 0 && c < a.n ? V::load(x, size_t(c)) : -INFINITY;
   };
+  const float extra = single >= 0 ? V::load(x, size_t(single)) : -INFINITY;
   const float mine = gives ? logit_of(a.ids[size_t(row) * a.n_ids + tid]) : 0.f;
-  if constexpr (TOP) {
-    if (tid < kScoreTop) s_kept[tid] = 0;
-  }
-
-  ScoreSum sum = {-INFINITY, 0.f, 0.f};
-  for (int lap = v0; lap < v1 || lap == v0; lap += kScoreLap * kScoreThreads) {
-    uint4 v[kScoreLap];
+  auto ask = [&](uint4 (&v)[kScoreLap], int lap) {
+    const uint4* from = vecs + lap + tid;
+    if (lap + kScoreLap * kScoreThreads <= v1) {
 #pragma unroll
-    for (int j = 0; j < kScoreLap; ++j) {
-      const int i = lap + j * kScoreThreads + tid;
-      v[j] = V::none();
-      if (i < v1) {
-        const int64_t at = int64_t(i) * V::N - shift;
-        if (at >= 0 && at + V::N <= a.n) {
-          v[j] = ld_nc_v4(vecs + i);
-        } else {
+      for (int j = 0; j < kScoreLap; ++j) v[j] = ld_nc_v4(from + j * kScoreThreads);
+    } else {
 #pragma unroll
-          for (int e = 0; e < V::N; ++e)
-            if (at + e >= 0 && at + e < a.n) V::set(v[j], e, x, size_t(at + e));
-        }
+      for (int j = 0; j < kScoreLap; ++j) {
+        v[j] = V::none();
+        if (lap + tid + j * kScoreThreads < v1) v[j] = ld_nc_v4(from + j * kScoreThreads);
       }
     }
-    float most = -INFINITY;
+  };
+
+  ScoreSum sum = {-INFINITY, 0.f, 0.f};
+  uint4 next[kScoreLap];
+  ask(next, v0);
+  float border = -INFINITY;
+#pragma unroll 1
+  for (int lap = v0; lap < v1; lap += kScoreLap * kScoreThreads) {
+    uint4 v[kScoreLap];
 #pragma unroll
-    for (int j = 0; j < kScoreLap; ++j) most = fmaxf(most, V::most(v[j]));
+    for (int j = 0; j < kScoreLap; ++j) v[j] = next[j];
+    if (lap + kScoreLap * kScoreThreads < v1) ask(next, lap + kScoreLap * kScoreThreads);
+    float each[kScoreLap], most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kScoreLap; ++j) most = fmaxf(most, each[j] = V::most(v[j]));
     {
-      ScoreSum s = {most, 0.f, 0.f};
       const float ref = most == -INFINITY ? 0.f : most;
+      const float2 neg = make_float2(-ref, -ref), log2e = make_float2(kLog2e, kLog2e);
+      float2 ss = make_float2(0.f, 0.f), tt = make_float2(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < kScoreLap; ++j)
 #pragma unroll
-        for (int e = 0; e < V::N; ++e) {
-          const float t = (V::at(v[j], e) - ref) * kLog2e, p = score_ex2(t);
-          s.s += p;
-          s.t += fmaxf(t, -1e30f) * p;  // (-inf weighs nothing; NaN is in p)
+        for (int e = 0; e < V::N; e += 2) {
+          // (the difference first: it is exact or nearly so, where two rounded products would not be)
+          const float2 t = mul2(add2(make_float2(V::at(v[j], e), V::at(v[j], e + 1)), neg), log2e);
+          const float2 p = make_float2(score_ex2(t.x), score_ex2(t.y));
+          ss = add2(ss, p);
+          // (-inf weighs nothing; NaN is in p)
+          tt = score_fma2(make_float2(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)), p, tt);
         }
-      sum = score_join(sum, s);
+      sum = score_join(sum, ScoreSum{most, ss.x + ss.y, tt.x + tt.y});
     }
     if constexpr (TOP) {
-      // ---- the border: what the groups put forward ----
-      int first = 0x7fffffff;
-      if (most > -INFINITY) {
+      // ---- the border ----
+      if (lap == v0) {
+        uint32_t key = score_order(most);
+        key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
+        key = max(key, __shfl_xor_sync(0xffffffffu, key, 2));
+        if ((tid & 3) == 0) s_group[tid >> 2] = key;
+        if (tid == 0) s_border = -INFINITY;  // fewer than `top` groups with anything: everything is looked at
+        __syncthreads();
+        int above = 0;
 #pragma unroll
-        for (int j = kScoreLap - 1; j >= 0; --j)
-          if (V::most(v[j]) == most) {
-#pragma unroll
-            for (int e = V::N - 1; e >= 0; --e)
-              if (V::at(v[j], e) == most) first = (lap + j * kScoreThreads + tid) * V::N - shift + e;
-          }
+        for (int i = 0; i < kScoreGroups / 4; ++i) {
+          const int g = (tid & 3) + 4 * i;
+          above += s_group[g] > key || (s_group[g] == key && g < (tid >> 2));
+        }
+        above += __shfl_xor_sync(0xffffffffu, above, 1);
+        above += __shfl_xor_sync(0xffffffffu, above, 2);
+        if (key && above == a.top - 1 && (tid & 3) == 0) s_border = score_unorder(key);
+        __syncthreads();
+        border = s_border;  // (a border for all laps)
       }
-      uint64_t key = most > -INFINITY ? score_key(most, first) : 0;
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
-        key = key > other ? key : other;
-      }
-      if ((tid & 3) == 0) s_group[tid >> 2] = key;
-      if (tid == 0) {
-        s_border = 1;  // fewer than `top` groups with anything: everything is looked at
-        s_count = 0;
-      }
-      __syncthreads();
-      int above = 0;
-#pragma unroll
-      for (int i = 0; i < kScoreGroups / 4; ++i) above += s_group[(tid & 3) * (kScoreGroups / 4) + i] > key;
-      above += __shfl_xor_sync(0xffffffffu, above, 1);
-      above += __shfl_xor_sync(0xffffffffu, above, 2);
-      if (key && above == a.top - 1 && (tid & 3) == 0) s_border = key;
-      __syncthreads();
-      const uint64_t border = s_border;
-      const float bv = border == 1 ? -INFINITY : score_key_value(border);
       // ---- those that reach it ----
+      uint32_t hits = 0;
 #pragma unroll
-      for (int j = 0; j < kScoreLap; ++j) {
-        if (!(V::most(v[j]) >= bv)) continue;
-        const int at = (lap + j * kScoreThreads + tid) * V::N - shift;
+      for (int j = 0; j < kScoreLap; ++j)
+        if (each[j] >= border && each[j] > -INFINITY) hits |= 1u << j;
+#pragma unroll 1
+      for (; hits; hits &= hits - 1) {
+        const int jj = __ffs(hits) - 1, at = head + (lap + jj * kScoreThreads + tid) * V::N;
+        uint4 w = v[0];
+#pragma unroll
+        for (int j = 1; j < kScoreLap; ++j)
+          if (jj == j) w = v[j];
+        uint32_t these = 0;
 #pragma unroll
         for (int e = 0; e < V::N; ++e) {
-          const float f = V::at(v[j], e);
-          if (f >= bv) {
-            const uint64_t k = score_key(f, at + e);
-            if (k >= border) {
-              const int to = atomicAdd(&s_count, 1);
-              if (to < kScoreList) s_list[to] = k;
-            }
-          }
+          const float f = V::at(w, e);
+          these |= uint32_t((f >= border) & (f > -INFINITY)) << e;
+        }
+        int to = atomicAdd(&s_count, __popc(these));
+#pragma unroll 1
+        for (; these; these &= these - 1, ++to) {
+          const int e = __ffs(these) - 1, q = FP32 ? e : e >> 1;
+          const uint32_t word = q == 0 ? w.x : q == 1 ? w.y : q == 2 ? w.z : w.w;
+          const float f = FP32 ? __uint_as_float(word) : __uint_as_float(e & 1 ? word & 0xffff0000u : word << 16);
+          if (to < kScoreList) s_list[to] = score_key(f, at + e);
         }
       }
-      __syncthreads();
-      int n = s_count;
-      if (n > kScoreList) {
-        // Too many for the list (more than a thousand of a block's logits above the border: none that a model computes): the greatest, the
-        // greatest below it, and so on.
-        uint64_t last = ~uint64_t(0);
-        for (n = 0; n < a.top; ++n) {
-          uint64_t best = 0;
-#pragma unroll
-          for (int j = 0; j < kScoreLap; ++j)
-#pragma unroll
-            for (int e = 0; e < V::N; ++e) {
-              const uint64_t k = score_key(V::at(v[j], e), (lap + j * kScoreThreads + tid) * V::N - shift + e);
-              if (k < last && k > best) best = k;
-            }
-#pragma unroll
-          for (int o = 16; o; o >>= 1) {
-            const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-            best = best > other ? best : other;
-          }
-          if (lane == 0) s_round[warp] = best;
-          __syncthreads();
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) best = best > s_round[w] ? best : s_round[w];
-          if (tid == 0) s_list[n] = best;
-          last = best;
-          __syncthreads();
-        }
-      }
-      // with what earlier laps left
-      if (lap > v0 && tid < a.top) s_list[n + tid] = s_kept[tid];
-      if (lap > v0) n += a.top;
-      __syncthreads();
-      if (lap > v0 && tid < kScoreTop) s_kept[tid] = 0;
-      if (lap > v0) __syncthreads();
-      for (int i = tid; i < n; i += kScoreThreads) {
-        const uint64_t k = s_list[i];
-        if (k == 0) continue;
-        const int at = score_rank(k, s_list, n);
-        if (at < a.top) s_kept[at] = k;
-      }
-      __syncthreads();
     }
   }
 
-  // ---- threads, warps, blocks of the cluster ----
+  if (extra > -INFINITY || extra != extra) sum = score_join(sum, ScoreSum{extra, extra - extra + 1.f, 0.f});
+  // ---- this block's most likely tokens, in order, into the first block ----
+  if constexpr (TOP) {
+    if (v0 >= v1) __syncthreads();  // (no lap: the count is zero all the same)
+    if (extra >= border && extra > -INFINITY) {
+      const int to = atomicAdd(&s_count, 1);
+      if (to < kScoreList) s_list[to] = score_key(extra, single);
+    }
+    __syncthreads();
+    int n = s_count;
+    if (n > kScoreList) {
+      // Too many for the list (more than a thousand at the border or above: equal ones, or the greatest of a few threads): the greatest, the greatest
+      // below it, and so on, from memory.
+      uint64_t last = ~uint64_t(0);
+#pragma unroll 1
+      for (n = 0; n < a.top; ++n) {
+        uint64_t best = 0;
+#pragma unroll 1
+        for (int i = head + v0 * V::N + tid; i < head + v1 * V::N; i += kScoreThreads) {
+          const uint64_t k = score_key(V::load(x, size_t(i)), i);
+          if (k < last && k > best) best = k;
+        }
+        const uint64_t k = score_key(extra, single);
+        if (k < last && k > best) best = k;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+          best = best > other ? best : other;
+        }
+        if (lane == 0) s_round[warp] = best;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) best = best > s_round[w] ? best : s_round[w];
+        if (tid == 0) s_list[n] = best;
+        last = best;
+        __syncthreads();
+      }
+    }
+    if (share > 1) cluster_wait();  // (for the arrivals at the start) the first block runs, and its places are empty
+    const uint32_t to = map_to_cta(smem_u32(s_best), 0);
+#pragma unroll 1
+    for (int i = tid; i < n; i += kScoreThreads) {
+      const uint64_t k = s_list[i];
+      const int at = k ? score_rank(k, s_list, n) : kScoreTop;
+      if (at < a.top) {
+        st_cluster_u32(to + 8 * (rank * a.top + at), uint32_t(k));
+        st_cluster_u32(to + 8 * (rank * a.top + at) + 4, uint32_t(k >> 32));
+      }
+    }
+  } else if (share > 1) {
+    cluster_wait();
+  }
+  // ---- sums of threads, warps, blocks ----
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum = score_xor(sum, o);
   if (lane == 0) {
@@ -293,35 +319,22 @@ __global__ void __launch_bounds__(kScoreThreads) k_token_logprobs(const Score a)
     sum = lane < kWarps ? ScoreSum{s_sum[lane][0], s_sum[lane][1], s_sum[lane][2]} : ScoreSum{-INFINITY, 0.f, 0.f};
 #pragma unroll
     for (int o = kWarps / 2; o; o >>= 1) sum = score_xor(sum, o);
-  }
-  if (share > 1) {
-    cluster_sync_all();  // the first block runs: its shared memory may be written
-    if (tid == 0) {
+    if (lane == 0) {
       const uint32_t to = map_to_cta(smem_u32(&s_parts[rank][0]), 0);
       st_cluster_u32(to, __float_as_uint(sum.m));
       st_cluster_u32(to + 4, __float_as_uint(sum.s));
       st_cluster_u32(to + 8, __float_as_uint(sum.t));
     }
-    if constexpr (TOP) {
-      if (tid < a.top) {
-        const uint32_t to = map_to_cta(smem_u32(&s_best[rank * a.top + tid]), 0);
-        st_cluster_u32(to, uint32_t(s_kept[tid]));
-        st_cluster_u32(to + 4, uint32_t(s_kept[tid] >> 32));
-      }
-    }
+  }
+  if (share > 1) {
     cluster_sync_all();
     if (rank != 0) return;
-    sum = {s_parts[0][0], s_parts[0][1], s_parts[0][2]};
-    for (int i = 1; i < share; ++i) sum = score_join(sum, ScoreSum{s_parts[i][0], s_parts[i][1], s_parts[i][2]});
   } else {
-    if (tid == 0) {
-      s_parts[0][0] = sum.m;
-      s_parts[0][1] = sum.s;
-      s_parts[0][2] = sum.t;
-    }
     __syncthreads();
-    sum = {s_parts[0][0], s_parts[0][1], s_parts[0][2]};
   }
+  sum = (lane & 7) < share ? ScoreSum{s_parts[lane & 7][0], s_parts[lane & 7][1], s_parts[lane & 7][2]} : ScoreSum{-INFINITY, 0.f, 0.f};
+#pragma unroll
+  for (int o = 4; o; o >>= 1) sum = score_xor(sum, o);
 
   // ---- results; a row without anything above -inf: no token has a probability, and nothing is uncertain ----
   const float log_s = logf(sum.s);
@@ -340,26 +353,32 @@ __global__ void __launch_bounds__(kScoreThreads) k_token_logprobs(const Score a)
     }
   }
   if constexpr (TOP) {
-    const uint64_t* keys = share > 1 ? s_best : s_kept;
-    const int n = share > 1 ? share * a.top : a.top;
-    if (share > 1) {
-      // places that no token takes
-      if (tid < kScoreTop) s_kept[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kScoreThreads) {
-        const uint64_t k = keys[i];
-        const int at = k ? score_rank(k, keys, n) : kScoreTop;
-        if (at < a.top) s_kept[at] = k;
+    const uint64_t k = tid < share * a.top ? s_best[tid] : 0;
+    const int there = __syncthreads_count(k != 0);
+    const size_t to = size_t(row) * a.top;
+    if (k) {
+      // every block's are in order: how many are greater is found by halving, in all of them at once
+      int lo[8] = {0}, at = 0;
+#pragma unroll 1
+      for (int step = kScoreTop; step; step >>= 1) {
+        if (step > a.top) continue;
+        uint64_t other[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) other[b] = s_best[min(b, share - 1) * a.top + min(lo[b] + step, a.top) - 1];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) lo[b] += (b < share) & (lo[b] + step <= a.top) & (other[b] > k) ? step : 0;
       }
-      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < 8; ++b) at += lo[b];
+      if (at < a.top) {
+        a.top_ids[to + at] = score_key_index(k) + a.offset;
+        a.top_val[to + at] = out(score_key_value(k));
+      }
     }
-    if (tid < a.top) {
-      const uint64_t k = s_kept[tid];
-      const int idx = score_key_index(k);
-      const size_t to = size_t(row) * a.top + tid;
-      a.top_ids[to] = idx < 0 ? -1 : idx + a.offset;
+    if (tid >= there && tid < a.top) {
+      a.top_ids[to + tid] = -1;
       // (a row with NaN or +inf has no probabilities, also where nothing else is left)
-      a.top_val[to] = k || sum.s != sum.s ? out(score_key_value(k)) : -INFINITY;
+      a.top_val[to + tid] = sum.s != sum.s && !a.raw ? NAN : -INFINITY;
     }
   }
 }
@@ -396,10 +415,10 @@ extern "C" int bl_token_logprobs(const blScoreArgs* s, void* stream, char* err, 
   a.top_ids = static_cast<int*>(s->top_ids);
   a.top_val = static_cast<float*>(s->top_val);
   a.parts = static_cast<float*>(s->parts);
-  // A lap's worth of a row to a block, eight blocks to a row at most.
-  const int lap = kScoreThreads * kScoreLap * (s->fp32 ? 4 : 8);
+  // Blocks of a row: as many as it has laps (eight at most) where there are few rows, fewer the more rows there are.
+  const int lap = kScoreThreads * kScoreLap * (s->fp32 ? 4 : 8), slots = sm_count() * 4;
   int share = 1;
-  while (share < 8 && int64_t(share) * lap < a.n) share *= 2;
+  while (share < 8 && int64_t(share) * lap < a.n && int64_t(s->rows) * share * 2 <= slots) share *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto* kernel = s->fp32 ? (s->top ? k_token_logprobs<true, true> : k_token_logprobs<true, false>)
                          : (s->top ? k_token_logprobs<false, true> : k_token_logprobs<false, false>);
