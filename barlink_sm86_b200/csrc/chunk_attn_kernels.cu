@@ -14,7 +14,7 @@
 //   warps 1, 2  issue S = Q K^T (128 x 64 into TMEM) and O += P V (128 x hd in TMEM) of a place each, the next S right behind P V
 //   warps 4-7   softmax of the first place's rows, one row a thread: P (bf16) goes over S in TMEM, from where it is an operand
 //   warps 8-11  the same for the second place
-//   warps 12-15 (4-bit cache) expand codes into bf16 tiles in the layout that TMA would leave
+//   warps 12-19 (4-bit cache) expand codes into bf16 tiles in the layout that TMA would leave
 //
 // A step's scores come in halves of 64 keys, each with columns of its own, so that a place's softmax always finds scores while its products go on.  S of
 // a half goes into the columns from which P V of the same half of the step before, issued ahead of it and not waited for, takes P: one thread
@@ -99,13 +99,13 @@ struct ChunkSeg {
   int lim, cap;     // the first token sees min(lim, cap) keys, and each one more, up to cap
   int j0, n, i0;    // first step, steps (0: the run is over), number of the first one in the run
   int piece;        // -1: the whole pair
-  int pad;
+  int cut;          // the last step has its first half only
 };
 constexpr int kChSegs = 4;
 
 template <int HD, bool Q4>
 struct ChunkShape {
-  static constexpr int kThreads = Q4 ? 512 : 384;
+  static constexpr int kThreads = Q4 ? 640 : 384;
   static constexpr uint32_t kQ = kChRows * HD * 2, kKV = kChKeys * HD * 2, kHalf = kChKeys * 128, kQHalf = kChRows * 128;
   static constexpr uint32_t kRawGran = 10 * HD, kRawBytes = (kChGrans / 2) * kRawGran;  // codes and params of a granule's keys, or of its values
   static constexpr uint32_t kOffK = 2 * kQ, kOffV = kOffK + 2 * kKV, kOffRaw = kOffV + 2 * kKV;
@@ -117,7 +117,7 @@ struct ChunkShape {
 
 struct ChunkBars {
   uint64_t q_full[2], q_empty[2];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t k_full[2][2], k_empty[2][2], v_full[2][2], v_empty[2][2];  // by slot and half
   uint64_t raw_full[2][kChRaw], raw_empty[2][kChRaw];  // keys, values
   uint64_t s_ready[2][2], p_ready[2][2];        // by place and half
   uint64_t pv_done[2], o_final[2], o_free[2];   // by place
@@ -127,6 +127,9 @@ struct ChunkBars {
   uint64_t seg_full[kChSegs], seg_empty[kChSegs];
   ChunkSeg segs[kChSegs];
   uint32_t tmem, abort;
+  uint32_t never;    // set where a wait for the list ran out
+  uint32_t there[2][4];  // by group of four warps: whether its last wait, and the one before, came through
+  uint32_t has[2][kChRaw];  // 4-bit cache: granules that a raw half has copies of
   uint32_t gone[8];  // granules of a step (by its number in the run, modulo 8) that have no block
 };
 static_assert(sizeof(ChunkBars) <= 768, "barriers");
@@ -226,6 +229,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   ChunkBars& bars = *reinterpret_cast<ChunkBars*>(gen + S::kOffBar);
   volatile uint32_t* s_abort = &bars.abort;
+  const uint32_t abort_at = smem_u32(&bars.abort), never_at = smem_u32(&bars.never);
   __shared__ int s_scan[S::kThreads / 32];
   __shared__ int s_first[4];  // request, KV head, first token of the pair, step
 
@@ -244,10 +248,12 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       mbar_init(&bars.o_free[t], kChRows / 32);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars.k_full[s], Q4 ? 4 : 1);
-      mbar_init(&bars.v_full[s], Q4 ? 4 : 1);
-      mbar_init(&bars.k_empty[s], 2);
-      mbar_init(&bars.v_empty[s], 2);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars.k_full[s][h], Q4 ? 4 : 1);
+        mbar_init(&bars.v_full[s][h], Q4 ? 4 : 1);
+        mbar_init(&bars.k_empty[s][h], 2);
+        mbar_init(&bars.v_empty[s][h], 2);
+      }
       mbar_init(&bars.met[s], 1);
     }
     for (int s = 0; s < kChRaw; ++s)
@@ -259,9 +265,10 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     for (int t = 0; t < 2; ++t) mbar_init(&bars.drained[t], 1);
     for (int i = 0; i < kChSegs; ++i) {
       mbar_init(&bars.seg_full[i], 1);
-      mbar_init(&bars.seg_empty[i], Q4 ? 15 : 11);  // all warps but the one that walks the list
+      mbar_init(&bars.seg_empty[i], Q4 ? 7 : 11);  // three warps, and the groups of four or their warps
     }
     bars.abort = 0;
+    bars.never = 0;
     for (int i = 0; i < 8; ++i) bars.gone[i] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_q);
@@ -366,21 +373,61 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     if (warp == 1) tmem_dealloc(tmem_base, kChTmemCols);
     return;
   }
-  // Step j of a share has slot j & 1 of the keys and of the values, so that a share with one tile has a slot to a place; a role knows a slot's phase by
-  // how often it has been filled.
-  // Every role goes through the run's shares of pairs: f(share, whether it has two tiles).  After a wait that ran out they go on without work.
+  // Step j of a share has slot j & 1 of the keys and of the values, so that a share with one tile has a slot to a place; a slot is filled and emptied by
+  // halves, of which a pair's last step may have the first only, and a role knows a half's phase by how often it has been filled.
+  struct Fills {
+    uint32_t n[2][2] = {{0, 0}, {0, 0}};
+    __device__ __forceinline__ uint32_t of(int j, int h) const {  // ahead of step j
+      return (j & 1 ? (h ? n[1][1] : n[1][0]) : (h ? n[0][1] : n[0][0])) + uint32_t(j >> 1);
+    }
+    __device__ __forceinline__ void add(const ChunkSeg& s) {
+      const uint32_t a = uint32_t(s.n + 1) >> 1, b = uint32_t(s.n) >> 1;
+      n[0][0] += a;
+      n[1][0] += b;
+      n[0][1] += a - (s.cut && (s.n & 1) ? 1 : 0);
+      n[1][1] += b - (s.cut && !(s.n & 1) ? 1 : 0);
+    }
+  };
   bool ok = true;
+  // With the 4-bit cache, groups of four warps (softmax, conversion) wait as one: their first warp looks at the barrier, the others wait for it where
+  // waiting takes no issue slots (with twenty warps that look at barriers pauses between looks made the kernel faster, which with twelve they do
+  // not).  All four have the same answer, so that they stay together also after a wait that ran out.
+  auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(warp >> 2) : "memory"); };
+  int nth = 0;
+  auto group_wait = [&](uint64_t* bar, uint32_t parity) {
+    if constexpr (!Q4) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
+    if ((warp & 3) == 0) {
+      const bool there = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
+      if (lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
+    }
+    group_sync();
+    // (two words in turn: the first warp may be at the next wait before the last one has read this one's answer)
+    const bool there = *const_cast<volatile uint32_t*>(&bars.there[nth][(warp >> 2) - 1]) != 0;
+    nth ^= 1;
+    return there;
+  };
+  // Every role goes through the run's shares of pairs: f(share, whether it has two tiles).  After a wait that ran out they go on without work.
   auto each = [&](auto&& f) {
 #pragma unroll 1
     for (int k = 0;; ++k) {
-      uint32_t never = 0;
-      if (!mbar_wait_small_warp(&bars.seg_full[k % kChSegs], uint32_t(k / kChSegs) & 1u, &never, 1u << 22)) {
+      bool there = true;
+      if (!Q4 || warp < 4 || (warp & 3) == 0) there = mbar_wait_call(smem_u32(&bars.seg_full[k % kChSegs]), uint32_t(k / kChSegs) & 1u, never_at, 1u << 22);
+      if (Q4 && warp >= 4) {
+        if ((warp & 3) == 0 && lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
+        group_sync();
+        there = *const_cast<volatile uint32_t*>(&bars.there[nth][(warp >> 2) - 1]) != 0;
+        nth ^= 1;
+      }
+      if (!there) {
         *s_abort = 1;
         return;
       }
       const ChunkSeg s = bars.segs[k % kChSegs];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.seg_empty[k % kChSegs]);
+      if (Q4 && warp >= 4)
+        group_sync();
+      else
+        __syncwarp();
+      if (lane == 0 && (!Q4 || warp < 4 || (warp & 3) == 0)) mbar_arrive(&bars.seg_empty[k % kChSegs]);
       if (s.n == 0) return;
       f(s, s.ntok > a.T);
     }
@@ -390,13 +437,14 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     // ------------------------------ keys (warp 0); the list, queries and values (warp 3) ------------------------------
     const uint32_t leader = elect_leader();
     const int values = warp == 3;
-    uint64_t* full = Q4 ? bars.raw_full[values] : values ? bars.v_full : bars.k_full;
-    uint64_t* empty = Q4 ? bars.raw_empty[values] : values ? bars.v_empty : bars.k_empty;
+    uint64_t (*full)[2] = values ? bars.v_full : bars.k_full;
+    uint64_t (*empty)[2] = values ? bars.v_empty : bars.k_empty;
     const CUtensorMap* tmap = values ? &tmap_v : &tmap_k;
     const uint32_t ring = base + (Q4 ? S::kOffRaw + values * kChRaw * S::kRawBytes : values ? S::kOffV : S::kOffK);
     int rs = 0, issued = 0;  // (4-bit cache: a ring of its own)
-    uint32_t rphase = 1, fills[2] = {0, 0};
-    int asked_of[2] = {0, 0};  // fills of a slot
+    uint32_t rphase = 1;
+    Fills fills;
+    uint32_t asked00 = 0, asked01 = 0, asked10 = 0, asked11 = 0;  // of either slot's halves
     uint32_t gone_before = 0;  // bit s: bars.gone[s] is set
     auto load = [&](const ChunkSeg& s) {
       const int* table = a.tables + size_t(s.b) * a.max_blocks;
@@ -420,60 +468,67 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           ahead = look(s.j0 + j + 4);
         }
         const uint32_t lost = __ballot_sync(kAll, where == -2) >> (kChGrans * part) & 255u;
+        const int st = j & 1;
 #pragma unroll 1
-        for (int u = 0; u < (Q4 ? 2 : 1); ++u) {
-          const int st = Q4 ? rs : j & 1;
-          const uint32_t phase = Q4 ? rphase : (st ? fills[1] : fills[0]) + uint32_t(j >> 1) + 1u;
-          if (!(ok = mbar_wait_small_warp(&empty[st], phase & 1u, s_abort, a.polls))) return;
-          if (!values && u == 0) {
+        for (int h = 0; h < 2 - (s.cut && j == s.n - 1 ? 1 : 0); ++h) {
+          uint64_t* bar = Q4 ? &bars.raw_full[values][rs] : &full[st][h];
+          if (!(ok = mbar_wait_call(smem_u32(Q4 ? &bars.raw_empty[values][rs] : &empty[st][h]), (Q4 ? rphase : fills.of(j, h) + 1u) & 1u, abort_at, a.polls))) return;
+          if (!values && h == 0) {
             if (lane == 0 && (lost || (gone_before >> (i & 7) & 1u))) bars.gone[i & 7] = lost;
             gone_before = (gone_before & ~(1u << (i & 7))) | uint32_t(lost != 0) << (i & 7);
             __syncwarp();
           }
           if constexpr (!Q4) {
             // (the whole warp stays together and one lane issues)
-            mbar_expect_tx_warp(leader, &full[st], S::kKV);
+            mbar_expect_tx_warp(leader, bar, S::kKV / 2);
 #pragma unroll 1
-            for (int gr = 0; gr < kChGrans; gr += a.box / kChGran) {
+            for (int gr = kChGrans / 2 * h; gr < kChGrans / 2 * (h + 1); gr += a.box / kChGran) {
               const int at = __shfl_sync(kAll, where, kChGrans * part + gr);
 #pragma unroll
-              for (int h = 0; h < HD / 64; ++h)
-                tma_load_2d_hint_warp(leader, ring + st * S::kKV + h * S::kHalf + gr * (kChGran * 128), tmap, smem_u32(&full[st]), h * 64, at >= 0 ? at : none,
-                                      kHintEvictLast);
+              for (int d = 0; d < HD / 64; ++d)
+                tma_load_2d_hint_warp(leader, ring + st * S::kKV + d * S::kHalf + gr * (kChGran * 128), tmap, smem_u32(bar), d * 64, at >= 0 ? at : none, kHintEvictLast);
+            }
+            ++issued;
+            if (st) {
+              if (h) ++asked11; else ++asked10;
+            } else {
+              if (h) ++asked01; else ++asked00;
             }
           } else {
             // lanes 0..3 ask for the codes of a granule, 4..7 for its steps and least elements; one that is not there leaves what stood there before
-            const int at = __shfl_sync(kAll, where, kChGrans * part + 4 * u + (lane & 3));
+            const int at = __shfl_sync(kAll, where, kChGrans * part + 4 * h + (lane & 3));
             const uint32_t has = __ballot_sync(kAll, at >= 0) & 15u;
-            mbar_expect_tx_warp(leader, &full[st], uint32_t(__popc(has)) * S::kRawGran);
+            if (lane == 0) bars.has[values][rs] = has;
+            __syncwarp();
+            mbar_expect_tx_warp(leader, bar, uint32_t(__popc(has)) * S::kRawGran);
             const bool params = lane >= 4;
             const uint8_t* from = a.cache4 + size_t(max(at, 0)) * q4_tile_bytes(HD) + (values ? (params ? q4_v_params(HD) : q4_v_codes(HD)) : params ? q4_k_params(HD) : 0);
-            bulk_load_warp(lane < 8 && at >= 0, ring + st * S::kRawBytes + (lane & 3) * S::kRawGran + (params ? 8 * HD : 0), from, params ? 2 * HD : 8 * HD,
-                           smem_u32(&full[st]), kHintEvictFirst);
-          }
-          ++issued;
-          if (!Q4) ++asked_of[st];
-          if (++rs == kChRaw) {
-            rs = 0;
-            rphase ^= 1u;
+            bulk_load_warp(lane < 8 && at >= 0, ring + rs * S::kRawBytes + (lane & 3) * S::kRawGran + (params ? 8 * HD : 0), from, params ? 2 * HD : 8 * HD,
+                           smem_u32(bar), kHintEvictFirst);
+            ++issued;
+            if (++rs == kChRaw) {
+              rs = 0;
+              rphase ^= 1u;
+            }
           }
         }
       }
-      fills[0] += uint32_t(s.n + 1) >> 1;
-      fills[1] += uint32_t(s.n) >> 1;
+      fills.add(s);
     };
-    if (!values) {
-      each([&](const ChunkSeg& s, bool) {
-        if (ok) load(s);
-      });
-    } else {
-      const uint32_t bytes = uint32_t(a.G) * a.T * HD * 2;
-      int asked[2] = {0, 0};  // tiles asked for, by place
-      ChunkMeta m = {};       // what the second kernel needs to know
-      int b = s_first[0], h = s_first[1], tok0 = s_first[2], j0 = s_first[3];
-      ChunkReq r = chunk_req(a, b);
+    const uint32_t bytes = uint32_t(a.G) * a.T * HD * 2;
+    int asked[2] = {0, 0};  // query tiles asked for, by place
+    ChunkMeta m = {};       // what the second kernel needs to know
+    int b = s_first[0], h = s_first[1], tok0 = s_first[2], j0 = s_first[3];
+    ChunkReq r = chunk_req(a, b);
 #pragma unroll 1
-      for (int k = 0, i = 0;; ++k) {
+    for (int k = 0, i = 0;; ++k) {
+      const uint32_t slot = k % kChSegs, turn = uint32_t(k / kChSegs) & 1u;
+      if (!mbar_wait_call(smem_u32(values ? &bars.seg_empty[slot] : &bars.seg_full[slot]), values ? turn ^ 1u : turn, never_at, 1u << 22)) {
+        *s_abort = 1;
+        break;
+      }
+      if (values && lane == 0) {
+        // the next share of a pair
         ChunkSeg s = {};
         if (i < count) {
           s.b = b;
@@ -487,8 +542,9 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           s.j0 = j0;
           s.n = min(steps - j0, count - i);
           s.i0 = i;
+          s.cut = s.keys - (j0 + s.n - 1) * kChKeys <= kChHalf;
           s.piece = s.n == steps ? -1 : 2 * me + (i == 0 ? 0 : 1);
-          if (j0 == 0 && s.n < steps) m = {int((lo + i + steps - 1) / run) - me + 1, s.piece, h, s.row, s.ntok};
+          if (j0 == 0 && s.n < steps) m = {(lo + i + steps - 1) / run - me + 1, s.piece, h, s.row, s.ntok};
           i += s.n;
           j0 = 0;
           tok0 += pair;
@@ -501,50 +557,48 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
             }
           }
         }
-        uint32_t never = 0;
-        if (!mbar_wait_small_warp(&bars.seg_empty[k % kChSegs], (uint32_t(k / kChSegs) & 1u) ^ 1u, &never, 1u << 22)) {
-          *s_abort = 1;
-          break;
-        }
-        if (lane == 0) {
-          bars.segs[k % kChSegs] = s;
-          mbar_arrive(&bars.seg_full[k % kChSegs]);
-        }
-        __syncwarp();
-        if (s.n == 0) break;
+        bars.segs[slot] = s;
+        mbar_arrive(&bars.seg_full[slot]);
+      }
+      __syncwarp();
+      const ChunkSeg s = bars.segs[slot];
+      __syncwarp();
+      if (!values && lane == 0) mbar_arrive(&bars.seg_empty[slot]);
+      if (s.n == 0) break;
+      if (values) {
         const bool two = s.ntok > a.T;
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
           if (!ok || (t == 1 && !two && s.n < 2)) break;
-          if (!(ok = mbar_wait_small_warp(&bars.q_empty[t], (uint32_t(asked[t]) & 1u) ^ 1u, s_abort, a.polls))) break;
+          if (!(ok = mbar_wait_call(smem_u32(&bars.q_empty[t]), (uint32_t(t ? asked[1] : asked[0]) & 1u) ^ 1u, abort_at, a.polls))) break;
           if (lane == 0) {
             mbar_expect_tx(&bars.q_full[t], bytes);
 #pragma unroll
             for (int hh = 0; hh < HD / 64; ++hh)
               tma_load_3d_hint_s(base + t * S::kQ + hh * S::kQHalf, &tmap_q, smem_u32(&bars.q_full[t]), hh * 64, s.h * a.G, s.row + (two ? t * a.T : 0), kHintEvictFirst);
           }
-          ++asked[t];
+          t ? ++asked[1] : ++asked[0];
         }
-        if (ok) load(s);
       }
-      if (lane == 0) a.meta[me] = m;
-      if (*s_abort)
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t)
-          if (asked[t] > 0)
-#pragma unroll 1
-            for (uint32_t p = 0; p < (1u << 20); ++p)
-              if (mbar_try_wait(&bars.q_full[t], uint32_t(asked[t] - 1) & 1u)) break;
+      if (ok) load(s);
     }
-    // The block's shared memory is another's behind it: whatever is still on its way lands first, also after a wait that ran out.
-    if (*s_abort) {
+    if (values && lane == 0) a.meta[me] = m;
+    if (*s_abort && values)
 #pragma unroll 1
-      for (int i = 0; i < (Q4 ? kChRaw : 2); ++i) {
-        // (a slot that was never filled has nothing on its way; of the others the last fill counts)
-        const int n = Q4 ? (issued + kChRaw - 1 - i) / kChRaw : asked_of[i];
+      for (int t = 0; t < 2; ++t)
+#pragma unroll 1
+        for (uint32_t p = 0; asked[t] > 0 && p < (1u << 20); ++p)
+          if (mbar_try_wait(&bars.q_full[t], uint32_t(asked[t] - 1) & 1u)) break;
+    // The block's shared memory is another's behind it: whatever is still on its way lands first, also after a wait that ran out.
+    if (*s_abort && issued > 0) {
+#pragma unroll 1
+      for (int i = 0; i < (Q4 ? kChRaw : 4); ++i) {
+        uint64_t* bar = Q4 ? &bars.raw_full[values][i] : &full[i >> 1][i & 1];
+        // (what was never asked for has nothing on its way; of the rest the last time counts)
+        const uint32_t n = Q4 ? uint32_t((issued + kChRaw - 1 - i) / kChRaw) : i == 0 ? asked00 : i == 1 ? asked01 : i == 2 ? asked10 : asked11;
 #pragma unroll 1
         for (uint32_t p = 0; n > 0 && p < (1u << 20); ++p)
-          if (mbar_try_wait(&full[i], uint32_t(n - 1) & 1u)) break;
+          if (mbar_try_wait(bar, (n - 1) & 1u)) break;
       }
     }
   } else if (warp < 3) {
@@ -556,35 +610,35 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     const uint32_t idesc_o = umma_idesc_f16(kChRows, HD, 1) | kUmmaBMajorN;
     const uint64_t desc_q = umma_desc_k_sw128(base + t * S::kQ), desc_k = umma_desc_k_sw128(base + S::kOffK), desc_v = umma_desc_mn_sw128(base + S::kOffV, S::kHalf);
     const uint32_t s_at = tmem_base + uint32_t(t * 128), o_at = s_at + 256u;
-    uint32_t uses[2] = {0, 0}, tiles = 0, fills[2] = {0, 0};  // halves of steps, pairs of this place so far; fills of either slot ahead of this share
+    uint32_t uses[2] = {0, 0}, tiles = 0;  // halves of steps, pairs of this place so far
+    Fills fills;
     uint32_t meets = 0;
     bool apart = false;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = mbar_wait_quick_warp(bar, parity & 1u, s_abort, a.polls); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls); };
     auto share = [&](const ChunkSeg& s, bool two) {
       const int every = two ? 1 : 2, n = s.n, begin = two ? 0 : t;  // this place's steps
       if (begin >= n) return;
-      auto filled = [&](int j) { return ((j & 1) ? fills[1] : fills[0]) + uint32_t(j >> 1); };
       const int last = (n - 1 - begin) / every * every + begin;       // this place's last step
-      const bool cut = s.keys - (s.j0 + last) * kChKeys <= kChHalf;   // of which there is the first half only
+      const bool cut = s.cut && last == n - 1;                        // of which there is the first half only
       if (!wait(&bars.q_full[t], tiles)) return;
 #pragma unroll 1
       for (int js = begin;; js += every) {
         const int j = js - every, sk = js & 1, sv = j & 1;
-        const bool product = js != begin, more = js <= last;
+        const bool product = one_copy(js != begin), more = js <= last;
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           // the scores of half h of step js, ahead of which that half of the place's step before is multiplied by its values
           const bool of = product && !(h == 1 && cut && j == last), next = more && !(h == 1 && cut && js == last), fresh = of && h == 0 && j == begin;
           if (of) {
             if (!wait(&bars.p_ready[t][h], h ? uses[1]++ : uses[0]++)) return;
-            if (h == 0 && !wait(&bars.v_full[sv], filled(j))) return;
+            if (!wait(&bars.v_full[sv][h], fills.of(j, h))) return;
           }
           // (ahead of the product, behind which a wait takes longer; but the 4-bit cache's next keys may have to wait for the values that it reads)
-          if ((!Q4 || !product) && h == 0 && more && !wait(&bars.k_full[sk], filled(js))) return;
+          if ((!Q4 || !product) && next && !wait(&bars.k_full[sk][h], fills.of(js, h))) return;
           if (of) {
-            if (!Q4 && h == 0 && j == last) {
+            if (!Q4 && j == last) {
               const int r0 = s.keys - (s.j0 + j) * kChKeys;
-              if (r0 < kChKeys && r0 % a.box) {
+              if (r0 > kChHalf * h && r0 < kChHalf * (h + 1) && r0 % a.box) {
                 // the rest of the last box: probabilities are zero there, values may be anything
                 const int r1 = (r0 + a.box - 1) / a.box * a.box;
 #pragma unroll 1
@@ -602,27 +656,22 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
             tc_fence_after_sync();
             umma_f16_ts4_warp(leader, o_at, s_at + uint32_t(kChHalf * h), desc_v + uint64_t(sv * int(S::kKV / 16) + h * (kChHalf * 128 / 16)), idesc_o, fresh ? 0u : 1u);
             umma_commit_warp(leader, &bars.pv_done[t]);
-          }
-          if (h == 1 && product) {
-            umma_commit_warp(leader, &bars.v_empty[sv]);
-            if (!two) umma_commit_warp(leader, &bars.v_empty[sv]);  // (for the other place)
+            umma_commit_warp(leader, &bars.v_empty[sv][h]);
+            if (!two) umma_commit_warp(leader, &bars.v_empty[sv][h]);  // (for the other place)
           }
           if (next) {
-            if (Q4 && product && h == 0 && !wait(&bars.k_full[sk], filled(js))) return;
+            if (Q4 && product && !wait(&bars.k_full[sk][h], fills.of(js, h))) return;
             tc_fence_after_sync();
             umma_f16_ss_row_warp<HD>(leader, s_at + uint32_t(kChHalf * h), desc_q, desc_k + uint64_t(sk * int(S::kKV / 16) + h * (kChHalf * 128 / 16)), idesc_s);
             umma_commit_warp(leader, &bars.s_ready[t][h]);
+            umma_commit_warp(leader, &bars.k_empty[sk][h]);
+            if (!two) umma_commit_warp(leader, &bars.k_empty[sk][h]);
           }
-          if (h == 1 && more) {
-            umma_commit_warp(leader, &bars.k_empty[sk]);
-            if (!two) umma_commit_warp(leader, &bars.k_empty[sk]);
-          }
+          if (h == 1 && js == last) umma_commit_warp(leader, &bars.q_empty[t]);  // (the place's last use of the queries)
         }
         if (!more) break;
       }
-      // the place's last product of this pair, and its last use of the queries
       umma_commit_warp(leader, &bars.o_final[t]);
-      umma_commit_warp(leader, &bars.q_empty[t]);
       ++tiles;
     };
     each([&](const ChunkSeg& s, bool two) {
@@ -635,25 +684,24 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       apart = !two;
       if (ok) share(s, two);
-      fills[0] += uint32_t(s.n + 1) >> 1;
-      fills[1] += uint32_t(s.n) >> 1;
+      fills.add(s);
     });
     if (!ok) {
       // products on their way read shared memory and write TMEM, which are given back below
       umma_commit_warp(leader, &bars.drained[t]);
-      mbar_wait_small_warp(&bars.drained[t], 0, s_abort, 1u << 20);
+      mbar_wait_call(smem_u32(&bars.drained[t]), 0, never_at, 1u << 20);
     }
   } else if (warp >= 12) {
     // ------------------------------ codes of the 4-bit cache to bf16 tiles ------------------------------
     if constexpr (Q4) {
       constexpr int NA = HD / kQ4Group;
-      const int tid = threadIdx.x - 384;
       auto words = [&](uint32_t addr, uint32_t (&w)[NA]) {
         if constexpr (NA == 4)
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
         else
           asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
       };
+      auto pair_order = [](int i) { return (i >> 2) * 4 + (i >> 1 & 1) + (i & 1) * 2; };  // 0 2 1 3 4 6 5 7: neighbours are four tokens apart
       // (16 bits 0x430c are the bf16 number 128 + c; low + step * c is rounded once)
       auto value = [&](uint32_t two, __nv_bfloat162 step, __nv_bfloat162 low) {
         const uint32_t c = (two & 0x000f000fu) | 0x43004300u, k = 0xc300c300u;  // - 128
@@ -668,92 +716,84 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(tile + (chunk >> 3) * S::kHalf + key * 128 + (((chunk & 7) ^ (key & 7)) << 4)), "r"(x), "r"(y), "r"(z), "r"(w)
                      : "memory");
       };
+      const int values = warp >= 16, cwarp = warp & 3;  // warps 12 to 15 keys, 16 to 19 values
       int rs = 0;
-      uint32_t rphase = 0, fills[2] = {0, 0};
+      uint32_t rphase = 0;
+      Fills fills;
       each([&](const ChunkSeg& s, bool) {
         if (!ok) return;
-        const int* table = a.tables + size_t(s.b) * a.max_blocks;
-        #pragma unroll 1
+#pragma unroll 1
         for (int j = 0; j < s.n; ++j) {
           const int left = s.keys - (s.j0 + j) * kChKeys;  // tokens of this step
-          // granules that are there (as the copying warps saw it)
-          uint32_t has;
-          {
-            const int tok = (s.j0 + j) * kChKeys + (lane & 7) * kChGran;
-            const int blk = tok < s.keys ? table[tok / a.block_size] : -1;
-            has = __ballot_sync(kAll, blk >= 0 && blk < a.n_blocks);
-          }
-          const int rs0 = rs, st = j & 1;
-          const uint32_t rphase0 = rphase, phase = ((st ? fills[1] : fills[0]) + uint32_t(j >> 1) + 1u) & 1u;
+          const int st = j & 1;
+          const uint32_t tile = base + (values ? S::kOffV : S::kOffK) + st * S::kKV;
 #pragma unroll 1
-          for (int values = 0; values < 2; ++values) {
-            rs = rs0;
-            rphase = rphase0;
-            const uint32_t tile = base + (values ? S::kOffV : S::kOffK) + st * S::kKV;
-            if (!mbar_wait_quick_warp(values ? &bars.v_empty[st] : &bars.k_empty[st], phase, s_abort, a.polls)) { ok = false; return; }
+          for (int u = 0; u < 2 - (s.cut && j == s.n - 1 ? 1 : 0); ++u) {
+            if (!group_wait(&bars.raw_full[values][rs], rphase) || !group_wait(values ? &bars.v_empty[st][u] : &bars.k_empty[st][u], fills.of(j, u) + 1u)) {
+              ok = false;
+              return;
+            }
+            const uint32_t has = *const_cast<volatile uint32_t*>(&bars.has[values][rs]);
+            const uint32_t raw = base + S::kOffRaw + (values * kChRaw + rs) * S::kRawBytes;
+            if (!values) {
 #pragma unroll 1
-            for (int u = 0; u < 2; ++u) {
-              if (!mbar_wait_quick_warp(&bars.raw_full[values][rs], rphase, s_abort, a.polls)) { ok = false; return; }
-              const uint32_t raw = base + S::kOffRaw + (values * kChRaw + rs) * S::kRawBytes;
-              if (!values) {
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                  const int in = v * 32 + (tid >> 2), t = tid & 3, g = in >> 4, key = 64 * u + in;
-                  const uint32_t gran = raw + g * S::kRawGran;
-                  uint32_t w[NA] = {}, par[NA] = {};
-                  if (key < left && (has >> (4 * u + g) & 1u)) {
-                    words(gran + (in & 15) * (HD / 2) + t * NA * 4, w);
-                    words(gran + 8 * HD + (in & 15) * NA * 4, par);
-                  }
-#pragma unroll
-                  for (int m = 0; m < NA; ++m) {
-                    const __nv_bfloat162 step = pair_of(par[m >> 1], 0, m & 1 ? 0x3232 : 0x1010), low = pair_of(par[NA / 2 + (m >> 1)], 0, m & 1 ? 0x3232 : 0x1010);
-                    // nibbles (0, 4), (1, 5), (2, 6), (3, 7)
-                    const uint32_t p0 = value(w[m], step, low), p1 = value(w[m] >> 4, step, low), p2 = value(w[m] >> 8, step, low), p3 = value(w[m] >> 12, step, low);
-                    store(tile, key, 4 * m + t, __byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
-                  }
-                }
-              } else {
-                // two tokens, eight dims of every group
-                const int in = 2 * (tid >> 2), q = tid & 3, g = in >> 4, key = 64 * u + in;
+              for (int v = 0; v < 2; ++v) {
+                // a token, eight dims of every group; of eight neighbouring lanes four have a token four further on, so that a store of theirs meets all banks
+                const int in = 32 * v + cwarp * 8 + (lane >> 3) + (lane & 4), t = lane & 3, g = in >> 4, key = 64 * u + in;
                 const uint32_t gran = raw + g * S::kRawGran;
-                uint32_t w0[NA] = {}, w1[NA] = {}, pa[NA] = {}, pb[NA] = {};
-                if (key < left && (has >> (4 * u + g) & 1u)) {
-                  words(gran + (in >> 1 & 7) * HD + 2 * q * NA * 4, w0);
-                  words(gran + (in >> 1 & 7) * HD + (2 * q + 1) * NA * 4, w1);
-                  words(gran + 8 * HD + (in & 15) * NA * 4, pa);
-                  if (key + 1 < left) words(gran + 8 * HD + (in & 15) * NA * 4 + NA * 4, pb);
+                uint32_t w[NA] = {}, par[NA] = {};
+                if (key < left && (has >> g & 1u)) {
+                  words(gran + (in & 15) * (HD / 2) + t * NA * 4, w);
+                  words(gran + 8 * HD + (in & 15) * NA * 4, par);
                 }
 #pragma unroll
                 for (int m = 0; m < NA; ++m) {
-                  // (the first token's beside the second's)
-                  const uint32_t how = m & 1 ? 0x7632 : 0x5410;
-                  const __nv_bfloat162 step = pair_of(pa[m >> 1], pb[m >> 1], how), low = pair_of(pa[NA / 2 + (m >> 1)], pb[NA / 2 + (m >> 1)], how);
-                  uint32_t v[8];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    v[e] = value(w0[m] >> (4 * e), step, low);
-                    v[4 + e] = value(w1[m] >> (4 * e), step, low);
-                  }
-                  const int chunk = 4 * m + q;
-                  store(tile, key, chunk, __byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[4], v[5], 0x5410), __byte_perm(v[6], v[7], 0x5410));
-                  store(tile, key + 1, chunk, __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632), __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
+                  const __nv_bfloat162 step = pair_of(par[m >> 1], 0, m & 1 ? 0x3232 : 0x1010), low = pair_of(par[NA / 2 + (m >> 1)], 0, m & 1 ? 0x3232 : 0x1010);
+                  // nibbles (0, 4), (1, 5), (2, 6), (3, 7)
+                  const uint32_t p0 = value(w[m], step, low), p1 = value(w[m] >> 4, step, low), p2 = value(w[m] >> 8, step, low), p3 = value(w[m] >> 12, step, low);
+                  store(tile, key, 4 * m + t, __byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
                 }
               }
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars.raw_empty[values][rs]);
-              if (++rs == kChRaw) {
-                rs = 0;
-                rphase ^= 1u;
+            } else {
+              // two tokens, eight dims of every group; lanes as above
+              const int in = 2 * (cwarp * 8 + pair_order(lane >> 2)), q = lane & 3, g = in >> 4, key = 64 * u + in;
+              const uint32_t gran = raw + g * S::kRawGran;
+              uint32_t w0[NA] = {}, w1[NA] = {}, pa[NA] = {}, pb[NA] = {};
+              if (key < left && (has >> g & 1u)) {
+                words(gran + (in >> 1 & 7) * HD + 2 * q * NA * 4, w0);
+                words(gran + (in >> 1 & 7) * HD + (2 * q + 1) * NA * 4, w1);
+                words(gran + 8 * HD + (in & 15) * NA * 4, pa);
+                if (key + 1 < left) words(gran + 8 * HD + (in & 15) * NA * 4 + NA * 4, pb);
+              }
+#pragma unroll
+              for (int m = 0; m < NA; ++m) {
+                // (the first token's beside the second's)
+                const uint32_t how = m & 1 ? 0x7632 : 0x5410;
+                const __nv_bfloat162 step = pair_of(pa[m >> 1], pb[m >> 1], how), low = pair_of(pa[NA / 2 + (m >> 1)], pb[NA / 2 + (m >> 1)], how);
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  v[e] = value(w0[m] >> (4 * e), step, low);
+                  v[4 + e] = value(w1[m] >> (4 * e), step, low);
+                }
+                const int chunk = 4 * m + q;
+                store(tile, key, chunk, __byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[4], v[5], 0x5410), __byte_perm(v[6], v[7], 0x5410));
+                store(tile, key + 1, chunk, __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632), __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
               }
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(values ? &bars.v_full[st] : &bars.k_full[st]);
+            if (lane == 0) {
+              mbar_arrive(values ? &bars.v_full[st][u] : &bars.k_full[st][u]);
+              mbar_arrive(&bars.raw_empty[values][rs]);
+            }
+            if (++rs == kChRaw) {
+              rs = 0;
+              rphase ^= 1u;
+            }
           }
         }
-        fills[0] += uint32_t(s.n + 1) >> 1;
-        fills[1] += uint32_t(s.n) >> 1;
+        fills.add(s);
       });
     }
   } else if (warp >= 4) {
@@ -771,12 +811,12 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       const bool busy = __any_sync(kAll, valid);
       const int mine = two ? n : (n + 1 - t) >> 1;        // steps of this place
       // halves of steps; the last may be without its second one
-      const int halves = 2 * mine - (mine > 0 && s.keys - (s.j0 + (two ? n - 1 : 2 * mine - 2 + t)) * kChKeys <= kChHalf ? 1 : 0);
+      const int halves = 2 * mine - (s.cut && mine > 0 && (two || ((n - 1) & 1) == t) ? 1 : 0);
       float m_used = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int k = 0; k < halves && ok; ++k, ++products) {
         const int j = one_copy(two) ? k >> 1 : (k & ~1) + t, half = k & 1;
-        if (!mbar_wait_quick_warp(&bars.s_ready[t][half], (half ? uses[1] : uses[0]) & 1u, s_abort, a.polls)) {
+        if (!group_wait(&bars.s_ready[t][half], half ? uses[1] : uses[0])) {
           ok = false;
           break;
         }
@@ -789,22 +829,42 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         const uint32_t s_addr = s_base + uint32_t(kChHalf * half);
         const uint32_t lost = *const_cast<volatile uint32_t*>(&bars.gone[(s.i0 + j) & 7]) >> (kChGrans / 2 * half) & 15u;
         const int seen = lim - (s.j0 + j) * kChKeys - kChHalf * half;  // of these keys
-        uint32_t r0[32], r1[32];
-        tmem_ld_32x32(s_addr, r0);
-        tmem_ld_32x32(s_addr + 32, r1);
-        tmem_ld_wait();
         if (lost || __any_sync(kAll, valid && seen < kChHalf)) {
+          // keys that a row does not see, or that no block holds: their scores are written over
+#pragma unroll 1
+          for (int c0 = 0; c0 < kChHalf; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld_32x16(s_addr + c0, r);
+            tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (c >= seen || (lost >> (c / kChGran) & 1u)) r0[c] = 0xff800000u;
-            if (32 + c >= seen || (lost >> (2 + c / kChGran) & 1u)) r1[c] = 0xff800000u;
+            for (int c = 0; c < 16; ++c)
+              if (c0 + c >= seen || (lost >> (c0 / kChGran) & 1u)) r[c] = 0xff800000u;
+            tmem_st_32x16(s_addr + c0, r);
+          }
+          tmem_st_wait();
+        }
+        // (4-bit cache: 32 scores at a time, read once more for the exponentials: its 640 threads have 96 registers each)
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t r0[32], r1[Q4 ? 1 : 32];
+        tmem_ld_32x32(s_addr, r0);
+        if constexpr (!Q4) {
+          tmem_ld_32x32(s_addr + 32, r1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r0[c + e]), __uint_as_float(r1[c + e]));
+        } else {
+#pragma unroll 1
+          for (int c0 = 0; c0 < kChHalf; c0 += 32) {
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; c += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r0[c + e]), __uint_as_float(r0[c + 4 + e]));
+            tmem_ld_32x32(s_addr + (c0 ^ 32), r0);
           }
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 32; c += 4)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r0[c + e]), __uint_as_float(r1[c + e]));
         const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2);
         // also true on the first finite maximum; rows of no token have no say (the warp's others would be rounded as they have it)
         const bool grow = valid && m_new > m_used + kChRescale;
@@ -813,10 +873,8 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           if (k > 0) {
             // P V of the half before may still be running.  Parity tells its phase from its neighbours: the one behind needs this warp's own P,
             // and the one before it was issued ahead of these scores.
-            if (!mbar_wait_quick_warp(&bars.pv_done[t], (products - 1) & 1u, s_abort, a.polls)) {
-              ok = false;
-              break;
-            }
+            // (a warp by itself: one whose wait runs out goes on with its group, and leaves NaN)
+            if (!mbar_wait_quick_warp(&bars.pv_done[t], (products - 1) & 1u, abort_at, a.polls)) l = NAN;
             tc_fence_after_sync();
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += 16) {
@@ -840,15 +898,24 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             const float2 u = fma2(make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl, neg);
-            const float2 e = (c >> 1) % 4 < kChPoly ? ex2_poly(u) : make_float2(ex2_approx(u.x), ex2_approx(u.y));
+            const float2 e = !Q4 && (c >> 1) % 4 < kChPoly ? ex2_poly(u) : make_float2(ex2_approx(u.x), ex2_approx(u.y));
             sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], e);
             // (P in bf16: the products want it; off by half a step, 2^-8 at most, of every term)
             pk[c >> 1] = pack_bf16x2(e.x, e.y);
           }
           tmem_st_32x16(to, pk);  // over the scores: P of 32 keys takes the columns of 16
         };
-        weigh(r0, s_addr);
-        weigh(r1, s_addr + 16);
+        if constexpr (!Q4) {
+          weigh(r0, s_addr);
+          weigh(r1, s_addr + 16);
+        } else {
+#pragma unroll 1
+          for (int c0 = 0; c0 < kChHalf; c0 += 32) {
+            tmem_ld_wait();
+            weigh(r0, s_addr + c0 / 2);
+            if (c0 == 0) tmem_ld_32x32(s_addr + 32, r0);
+          }
+        }
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
         tmem_st_wait();
@@ -858,7 +925,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       // ---- the pair's rows, or a piece of them ----
       if (mine == 0) return;
-      if (ok && !mbar_wait_quick_warp(&bars.o_final[t], pairs & 1u, s_abort, a.polls)) ok = false;
+      if (ok && !group_wait(&bars.o_final[t], pairs)) ok = false;
       ++pairs;
       const bool join = !two && n > 1;  // the sums of the same rows in two places
       if (join && t == 1) {
@@ -870,7 +937,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       float w0 = 1.f, w1 = 0.f;
       if (join) {
-        if (ok && !(mbar_wait_quick_warp(&bars.sums, joins & 1u, s_abort, a.polls) && mbar_wait_quick_warp(&bars.o_final[1], others & 1u, s_abort, a.polls))) ok = false;
+        if (ok && !(group_wait(&bars.sums, joins) && group_wait(&bars.o_final[1], others))) ok = false;
         ++joins;
         const float2 ml = s_sums[row];
         const float m = fmaxf(m_used, ml.x), ref = m == -INFINITY ? 0.f : m;

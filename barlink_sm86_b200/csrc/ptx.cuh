@@ -188,34 +188,33 @@ __device__ __forceinline__ bool mbar_wait_bounded_warp(uint64_t* bar, uint32_t p
                                                        uint32_t max_polls = 1u << 24) {
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, max_polls));
 }
-// The same in little code: the compiler unrolls the loop above, and what a warp runs once a step it fetches once a step.
-__device__ __forceinline__ bool mbar_wait_small_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t max_polls) {
-  bool there = false;
+// The same for a kernel of many roles: the waiting itself is a function (shared-memory addresses in, the same answer for all lanes out), so that its
+// code stands once and what is run once a step is little enough to stay in the instruction cache.
+static __device__ __noinline__ bool mbar_wait_call(uint32_t bar, uint32_t parity, uint32_t abort_flag, uint32_t max_polls) {
+  uint32_t there = 0;
 #pragma unroll 1
   for (uint32_t i = 0; i < max_polls && !there; ++i) {
-    there = mbar_try_wait(bar, parity);
-    if ((i & 255u) == 255u && *abort_flag) break;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(there)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if ((i & 255u) == 255u) {
+      uint32_t f;
+      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(f) : "r"(abort_flag) : "memory");
+      if (f) break;
+    }
   }
-  if (!there) *abort_flag = 1;
-  return __all_sync(0xffffffffu, there);
+  if (!there) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(1) : "memory");
+  return __all_sync(0xffffffffu, there != 0);
 }
 // Looking once without suspending first.  Where a phase is over already, try_wait takes some 160 cycles and test_wait 15; where it is not, try_wait
 // wakes up some 300 after it is.
-__device__ __forceinline__ bool mbar_wait_quick_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t max_polls) {
+__device__ __forceinline__ bool mbar_wait_quick_warp(uint64_t* bar, uint32_t parity, uint32_t abort_flag, uint32_t max_polls) {
   if (max_polls > 0 && __all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
-  return mbar_wait_small_warp(bar, parity, abort_flag, max_polls);
-}
-// Looking again and again so: for the one warp of a block that everything waits for.  (All warps of a block looking so take the issue slots of
-// those that work.)
-__device__ __forceinline__ bool mbar_wait_spin_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t max_polls) {
-  bool there = false;
-#pragma unroll 1
-  for (uint32_t i = 0; i < max_polls && !there; ++i) {
-    there = mbar_test_wait(bar, parity);
-    if ((i & 255u) == 255u && *abort_flag) break;
-  }
-  if (!there) *abort_flag = 1;
-  return __all_sync(0xffffffffu, there);
+  return mbar_wait_call(smem_u32(bar), parity, abort_flag, max_polls);
 }
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
