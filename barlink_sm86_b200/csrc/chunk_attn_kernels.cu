@@ -49,6 +49,8 @@ constexpr int kChRaw = 3;      // half steps of the 4-bit cache in flight
 constexpr int kChHalf = kChKeys / 2;
 constexpr uint32_t kChTmemCols = 512;  // S of place t, half h of a step: 128 t + 64 h, P in its first half; O of place t: 256 + 128 t
 constexpr int kChPoly = 1;             // of four pairs of exponentials, those on the FMA pipe
+// What a pair costs beside its steps (queries, sums, a chain that starts anew), in steps: that many empty ones follow it in the list.
+constexpr int chunk_over(bool q4) { return q4 ? 4 : 3; }
 constexpr float kChRescale = 8.f;      // log2 units
 constexpr uint32_t kChPolls = 1u << 24;
 
@@ -105,7 +107,7 @@ constexpr int kChSegs = 4;
 
 template <int HD, bool Q4>
 struct ChunkShape {
-  static constexpr int kThreads = Q4 ? 640 : 384;
+  static constexpr int kThreads = Q4 ? 640 : 384, kOver = chunk_over(Q4);
   static constexpr uint32_t kQ = kChRows * HD * 2, kKV = kChKeys * HD * 2, kHalf = kChKeys * 128, kQHalf = kChRows * 128;
   static constexpr uint32_t kRawGran = 10 * HD, kRawBytes = (kChGrans / 2) * kRawGran;  // codes and params of a granule's keys, or of its values
   static constexpr uint32_t kOffK = 2 * kQ, kOffV = kOffK + 2 * kKV, kOffRaw = kOffV + 2 * kKV;
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   const int per = (a.batch + S::kThreads - 1) / S::kThreads, b0 = int(threadIdx.x) * per;
   auto steps_of = [&](int n, int past, int cap, int p) {  // of pair p of a request
     const int t = p * pair;
-    return t < n ? max(1, (min(max(past + min(t + pair, n), 0), cap) + kChKeys - 1) / kChKeys) : 0;
+    return t < n ? max(1, (min(max(past + min(t + pair, n), 0), cap) + kChKeys - 1) / kChKeys) + S::kOver : 0;
   };
   int run = 0, lo = 0, count = 0, src = 0, at = 0, mine = 0;
 #pragma unroll 1
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     int b = s_first[0], h = s_first[1], tok0 = s_first[2], j0 = s_first[3];
     ChunkReq r = chunk_req(a, b);
 #pragma unroll 1
-    for (int k = 0, i = 0;; ++k) {
+    for (int k = 0, i = 0, done = 0;; ++k) {
       const uint32_t slot = k % kChSegs, turn = uint32_t(k / kChSegs) & 1u;
       if (!mbar_wait_call(smem_u32(values ? &bars.seg_empty[slot] : &bars.seg_full[slot]), values ? turn ^ 1u : turn, never_at, 1u << 22)) {
         *s_abort = 1;
@@ -530,7 +532,8 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       if (values && lane == 0) {
         // the next share of a pair
         ChunkSeg s = {};
-        if (i < count) {
+#pragma unroll 1
+        while (i < count && s.n == 0) {
           s.b = b;
           s.h = h;
           s.row = r.q0 + tok0;
@@ -540,12 +543,13 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           s.cap = r.cap;
           const int steps = chunk_steps(s.keys);
           s.j0 = j0;
-          s.n = min(steps - j0, count - i);
-          s.i0 = i;
+          s.n = min(max(steps - j0, 0), count - i);  // (0: the run begins behind the pair's steps)
+          s.i0 = done;
           s.cut = s.keys - (j0 + s.n - 1) * kChKeys <= kChHalf;
           s.piece = s.n == steps ? -1 : 2 * me + (i == 0 ? 0 : 1);
           if (j0 == 0 && s.n < steps) m = {(lo + i + steps - 1) / run - me + 1, s.piece, h, s.row, s.ntok};
-          i += s.n;
+          done += s.n;
+          i += steps + S::kOver - j0;
           j0 = 0;
           tok0 += pair;
           if (tok0 >= r.n) {
@@ -958,27 +962,29 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       tc_fence_after_sync();
       if (busy) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < HD; c0 += 16) {
-          uint32_t r[16], q[16];
-          tmem_ld_32x16(o_addr + c0, r);
+        for (int c0 = 0; c0 < HD; c0 += 32) {
+          uint32_t r[2][16], q[2][16];
+#pragma unroll
+          for (int d = 0; d < 2; ++d) tmem_ld_32x16(o_addr + c0 + 16 * d, r[d]);
           if (one_copy(join)) {
-            tmem_ld_32x16(o_addr + 128u + c0, q);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) tmem_ld_32x16(o_addr + 128u + c0 + 16 * d, q[d]);
           } else {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) q[c] = 0;
+            for (int c = 0; c < 32; ++c) q[c >> 4][c & 15] = 0;
           }
           tmem_ld_wait();
-          float v[16];
+          float v[32];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) v[c] = fmaf(__uint_as_float(q[c]), w1, __uint_as_float(r[c]) * w0);
+          for (int c = 0; c < 32; ++c) v[c] = fmaf(__uint_as_float(q[c >> 4][c & 15]), w1, __uint_as_float(r[c >> 4][c & 15]) * w0);
           if (one_copy(valid && whole)) {
 #pragma unroll
-            for (int c = 0; c < 16; c += 8)
+            for (int c = 0; c < 32; c += 8)
               *reinterpret_cast<uint4*>(orow + c0 + c) =
                   make_uint4(pack_bf16x2(v[c], v[c + 1]), pack_bf16x2(v[c + 2], v[c + 3]), pack_bf16x2(v[c + 4], v[c + 5]), pack_bf16x2(v[c + 6], v[c + 7]));
           } else if (one_copy(valid)) {
 #pragma unroll
-            for (int c = 0; c < 16; c += 4) prow[size_t((c0 + c) / 4) * a.row_cap] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+            for (int c = 0; c < 32; c += 4) prow[size_t((c0 + c) / 4) * a.row_cap] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
           }
           __syncwarp();
         }
@@ -1097,7 +1103,7 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   if (int64_t(n_blocks) * nkv * block_size > 0x7fffffffLL - kChKeys) return refuse("needs a cache whose rows (tokens times KV heads) fit 32 bits");
   if (int64_t(max_blocks) * block_size > 0x3fffffffLL) return refuse("needs tables of less than 2^30 tokens");
   {
-    const int64_t pairs = tokens / (2 * chunk_tile_tokens(nq / nkv)) + int64_t(batch), steps = int64_t(max_blocks) * block_size / kChKeys + 1;
+    const int64_t pairs = tokens / (2 * chunk_tile_tokens(nq / nkv)) + int64_t(batch), steps = int64_t(max_blocks) * block_size / kChKeys + 1 + chunk_over(true);
     if (pairs * nkv > 0x7fffffffLL / steps - sm_count()) return refuse("has too many tokens for its tables: steps of 128 keys, over all tiles and KV heads, must fit 31 bits");
   }
   if (q_stride % 8 || q_stride < 0 || (tokens > 1 && q_stride < int64_t(nq) * hd)) return refuse("needs rows of q on 16-byte boundaries that hold nq heads");
