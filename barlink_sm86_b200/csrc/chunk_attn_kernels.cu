@@ -408,6 +408,12 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     nth ^= 1;
     return there;
   };
+  // All roles are through; behind it `abort` stays as it is.
+  auto settle = [&] {
+    tc_fence_before_sync();
+    asm volatile("bar.sync 0;" ::: "memory");
+    return *s_abort != 0;
+  };
   // Every role goes through the run's shares of pairs: f(share, whether it has two tiles).  After a wait that ran out they go on without work.
   auto each = [&](auto&& f) {
 #pragma unroll 1
@@ -587,14 +593,15 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       if (ok) load(s);
     }
     if (values && lane == 0) a.meta[me] = m;
-    if (*s_abort && values)
+    // The block's shared memory is another's behind it: after a wait that ran out, anyone's, whatever is still on its way lands first.
+    const bool gave_up = settle();
+    if (gave_up && values)
 #pragma unroll 1
       for (int t = 0; t < 2; ++t)
 #pragma unroll 1
         for (uint32_t p = 0; asked[t] > 0 && p < (1u << 20); ++p)
           if (mbar_try_wait(&bars.q_full[t], uint32_t(asked[t] - 1) & 1u)) break;
-    // The block's shared memory is another's behind it: whatever is still on its way lands first, also after a wait that ran out.
-    if (*s_abort && issued > 0) {
+    if (gave_up && issued > 0) {
 #pragma unroll 1
       for (int i = 0; i < (Q4 ? kChRaw : 4); ++i) {
         uint64_t* bar = Q4 ? &bars.raw_full[values][i] : &full[i >> 1][i & 1];
@@ -683,14 +690,15 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       // the one before it, not from older ones.
       if (two && apart) {
         if (lane == 0) mbar_arrive(&bars.met[t]);
-        if (ok) wait(&bars.met[t ^ 1], meets);
+        // (a place that has given up meets the other without having seen anything)
+        if (ok && wait(&bars.met[t ^ 1], meets) && *s_abort) ok = false;
         ++meets;
       }
       apart = !two;
       if (ok) share(s, two);
       fills.add(s);
     });
-    if (!ok) {
+    if (settle()) {
       // products on their way read shared memory and write TMEM, which are given back below
       umma_commit_warp(leader, &bars.drained[t]);
       mbar_wait_call(smem_u32(&bars.drained[t]), 0, never_at, 1u << 20);
@@ -799,6 +807,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         }
         fills.add(s);
       });
+      settle();
     }
   } else if (warp >= 4) {
     // ------------------------------ softmax ------------------------------
@@ -999,10 +1008,10 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       // (a run that gave up goes on to leave NaN everywhere)
     });
+    settle();
   }
 
-  tc_fence_before_sync();
-  __syncthreads();
+  if (*s_abort) __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, kChTmemCols);

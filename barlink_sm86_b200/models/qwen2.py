@@ -413,6 +413,22 @@ class Qwen2Model:
 
         return self._run_layers(ids.to(torch.int32), positions, attn_factory)
 
+    def extend_packed(self, ids, positions, slots, cu, ctx_lens, cache):
+        """New tokens of requests that may have tokens in the cache already, packed: ids, positions, slots int32 [tokens], cu int32
+        [batch + 1], ctx_lens int32 [batch] (tokens in all, the new ones the last of them) -> final normed hidden [tokens, hidden].  Keys and
+        values go to `cache` (PagedKV or PagedKV4) at `slots`; a token attends to its request's cache up to itself."""
+        nq, nkv, hd = self.nq, self.nkv, self.hd
+
+        def attn_factory(li):
+            def attn(qkv, bias=None):
+                qkv = self._rope_write(cache, li, qkv, positions, slots, bias)
+                if isinstance(cache, PagedKV4):
+                    return ops.paged_attn_chunk_q4(qkv, cache.kv[li], cache.block_tables, cu, ctx_lens, nq, nkv, hd, self.scale)
+                return ops.paged_attn_chunk(qkv, cache.k[li], cache.v[li], cache.block_tables, cu, ctx_lens, nq, nkv, hd, self.scale)
+            return attn
+
+        return self._run_layers(ids.to(torch.int32), positions, attn_factory)
+
     # ---- decode: one token per sequence against the paged cache ------------
     def decode_hidden(self, ids, positions, slots, ctx_lens, cache: PagedKV, splits=0):
         nq, nkv, hd = self.nq, self.nkv, self.hd
@@ -598,8 +614,9 @@ class Qwen2Model:
         full = self.comm.all_gather_cols(self.logits_local(hidden))
         return full[:, : self.cfg.vocab]
 
-    def next_tokens(self, hidden, out=None, dlin=False, rules=None):
+    def next_tokens(self, hidden, out=None, dlin=False, rules=None, logprobs=None):
         """Greedy next token per row (local arg max + a few bytes per row exchanged), under `rules` (ops.LogitRules) if given.
+        logprobs: also its log probability, the entropy and that many alternatives (ops.TokenLogprobs; of the model's logits, without the rules): a pair.
         dlin: the head may run on the decode-linear kernel; it does when its row tiles fit the GPU
         at once (a vocabulary shard of 149 tiles takes the persistent GEMM two laps of its 148 CTAs)."""
         head = self.w.lm_head
@@ -610,7 +627,16 @@ class Qwen2Model:
             logits = load_extension().dlin(hidden, head, epi="store")
         else:
             logits = self.logits_local(hidden)
-        return self.comm.argmax_vocab_parallel(logits, self.w.vocab_local, out, rules)
+        nxt = self.comm.argmax_vocab_parallel(logits, self.w.vocab_local, out, rules)
+        if logprobs is None:
+            return nxt
+        return nxt, self.comm.token_logprobs_vocab_parallel(logits, nxt, self.w.vocab_local, self.cfg.vocab, logprobs)
+
+    def token_logprobs(self, hidden, ids, top=0, max_rows=1024):
+        """ops.TokenLogprobs of `ids` (int32 [rows]) under the logits of hidden [rows, hidden], at most max_rows rows' logits at a time."""
+        parts = [self.comm.token_logprobs_vocab_parallel(self.logits_local(hidden[r:r + max_rows]), ids[r:r + max_rows], self.w.vocab_local, self.cfg.vocab, top)
+                 for r in range(0, hidden.shape[0], max_rows)]
+        return ops.TokenLogprobs(*(torch.cat(t, 0) for t in zip(*parts)))
 
 
 class DecodeEngine:
@@ -627,13 +653,17 @@ class DecodeEngine:
     kv_bits=4 holds the cache in 4 bits and deals its blocks out on the GPU: requests then have lengths of their own
     (`start`), come and go while the others run (`start`, `finish`), and the captured step takes the blocks that it
     needs (n_blocks of block_size tokens in all; `blocks_missing`, `tokens_lost`).  rules (ops.LogitRules, one row per request): the greedy token is
-    that of the logits under them, and their counts follow the tokens that are produced.  Either takes the plain decode path, also where the
-    folded or the fused one would run without it.
+    that of the logits under them, and their counts follow the tokens that are produced.  logprobs=k: every step leaves the log probability of
+    the token that it chose, the entropy and the k most likely tokens in `logprobs` (ops.TokenLogprobs, of the logits without the rules; until the next
+    step).  Any of these takes the plain decode path, also where the folded or the fused one would run without it.
+
+    `extend` gives requests further tokens on top of what they have in the cache (either kind): a turn of a conversation, a long prompt in
+    pieces; `score` does that and tells how likely each of the tokens was.
     """
 
     def __init__(self, model: Qwen2Model, batch: int, max_len: int, use_graph: bool = True,
                  attn_splits: int = 0, kv_bits: int = 16, rules: Optional[ops.LogitRules] = None, block_size: int = 16,
-                 n_blocks: Optional[int] = None):
+                 n_blocks: Optional[int] = None, logprobs: Optional[int] = None):
         self.m = model
         self.batch, self.max_len = batch, max_len
         dev, dt = model.device, model.dtype
@@ -643,7 +673,10 @@ class DecodeEngine:
             raise ValueError("block_size and n_blocks are for the 4-bit cache")
         if rules is not None and any(t is not None and t.shape[0] != batch for t in rules._args()):
             raise ValueError("rules must have one row per request")
+        if logprobs is not None and not 0 <= logprobs <= 32:
+            raise ValueError("logprobs must be 0 to 32 alternatives")
         self.kv_bits, self.rules = kv_bits, rules
+        self.top, self.logprobs = logprobs, None
         # (a mask or biases alone go by no counts)
         self.counted = rules is not None and rules.counts is not None and rules.seen is not None
         if kv_bits == 4:
@@ -761,6 +794,125 @@ class DecodeEngine:
             self.running[r] = True
         return out
 
+    def extend(self, ids, lens, max_tokens: int = 8192):
+        """Further tokens, packed: ids int32 [tokens]; lens (one per request, 0: none).  They follow what a request has in the cache (the token that `step`
+        chose last is not in it yet, and goes first if the text goes on from there), run through the model at most `max_tokens` per pass, also
+        within a request, and their keys and values go to the cache.  Returns the next token of every request that got some (int32 [batch]; the
+        current input of the others); the next `step` consumes these once they are in `ids`.  With the 4-bit cache a request that rests starts
+        anew, and if the model raises, those that got tokens are finished.  Waits for the GPU."""
+        return self._extend(ids, lens, max_tokens, None)[0]
+
+    def score(self, ids, lens, top: int = 0, max_tokens: int = 8192):
+        """`extend`, and how likely the tokens were: (next tokens, ops.TokenLogprobs with a row per token of ids).  A row is about the token that
+        follows it: the next one of the same request, and behind a request's last one the next token that is returned."""
+        return self._extend(ids, lens, max_tokens, top)
+
+    def _extend(self, ids, lens, max_tokens, top):
+        lens = [int(n) for n in lens]
+        if len(lens) != self.batch or any(n < 0 or n > self.max_len for n in lens) or sum(lens) != ids.numel() or max_tokens < 1:
+            raise ValueError("lens must be one length per request, up to max_len, and add up to the ids")
+        if top is not None and not 0 <= top <= 32:
+            raise ValueError("score gives 0 to 32 alternatives")
+        dev = self.positions.device
+        out = self.ids.clone()
+        if not ids.numel():
+            if top is None:
+                return out, None
+            none = torch.zeros(0, dtype=torch.float32, device=dev)
+            return out, ops.TokenLogprobs(none, none, torch.zeros(0, top, dtype=torch.int32, device=dev), none.new_zeros(0, top))
+        ids = ids.to(device=dev, dtype=torch.int32)
+        new = torch.tensor(lens, dtype=torch.int32).to(dev)
+        fresh = []
+        past = (self.ctx_lens if self.kv_bits == 4 else self.positions).clone()
+        # (in the whole cache the next token has to have a place too)
+        if int(torch.where(new > 0, past + new, 0).max()) > self.max_len - (self.kv_bits == 16):
+            raise ValueError("a request has room for max_len tokens (bf16 cache: the next one among them)")
+        if self.kv_bits == 4:
+            fresh = [b for b in range(self.batch) if lens[b] and not self.running[b]]
+            lay = self._lay_out(new, ids.numel())
+            positions, slots = lay.positions, lay.slots
+        else:
+            cu = torch.tensor([0] + lens, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+            of = torch.repeat_interleave(torch.arange(self.batch, device=dev), new.long(), output_size=ids.numel())
+            positions = (past[of] + torch.arange(ids.numel(), device=dev) - cu[of]).to(torch.int32)
+            bs = self.cache.block_size
+            slots = (self.cache.block_tables[of, (positions // bs).long()] * bs + positions % bs).to(torch.int32)
+        try:
+            nxt, scores = self._run_extend(ids, lens, new, past, positions, slots, max_tokens, top, fresh, out)
+        except BaseException:
+            # (their blocks were dealt out before the model ran)
+            if self.kv_bits == 4:
+                self.finish([b for b in range(self.batch) if lens[b]])
+            raise
+        if self.kv_bits == 4:
+            self.new_lens.masked_fill_(new > 0, 1)
+            for b in range(self.batch):
+                self.running[b] = self.running[b] or lens[b] > 0
+        else:
+            self.positions.add_(new)
+            self._refresh()
+        return nxt, scores
+
+    def _run_extend(self, ids, lens, new, past, positions, slots, max_tokens, top, fresh, out):
+        dev, total = ids.device, ids.numel()
+        first = [0]
+        for n in lens:
+            first.append(first[-1] + n)
+        rows = [b for b in range(self.batch) if lens[b]]
+        if self.counted:
+            gone = torch.zeros(self.batch, dtype=torch.bool)
+            gone[fresh] = True
+            gone = gone.to(dev)
+            self.rules.counts.masked_fill_(gone[:, None], 0)
+            self.rules.seen.masked_fill_(gone[:, None], 0)
+            ops.count_tokens(self.rules, ids, torch.tensor(first, dtype=torch.int32).to(dev), new)
+        lasts, kept = [], []
+        for t0 in range(0, total, max_tokens):
+            t1 = min(t0 + max_tokens, total)
+            # this pass's share of every request, and what a request has in the cache with it
+            share = [max(0, min(first[b + 1], t1) - max(first[b], t0)) for b in range(self.batch)]
+            done = [min(max(t1 - first[b], 0), lens[b]) for b in range(self.batch)]
+            cu = torch.tensor([0] + share, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+            ctx = past + torch.tensor(done, dtype=torch.int32).to(dev)
+            hidden = self.m.extend_packed(ids[t0:t1].contiguous(), positions[t0:t1].contiguous(), slots[t0:t1].contiguous(), cu, ctx, self.cache)
+            ends = [first[b + 1] - 1 - t0 for b in rows if t0 < first[b + 1] <= t1]
+            if ends:
+                lasts.append(hidden[torch.tensor(ends).to(dev)])
+            if top is not None:
+                kept.append(hidden)
+        # (rules have a row per request: all requests' logits, of which those with new tokens count)
+        at = torch.tensor(rows).to(dev)
+        last = torch.zeros(self.batch, lasts[0].shape[1], dtype=lasts[0].dtype, device=dev)
+        last[at] = torch.cat(lasts, 0)
+        nxt = self.m.next_tokens(last, rules=self.rules)
+        out[at] = nxt[at]
+        if self.counted:
+            ops.count_tokens(self.rules, torch.where(new > 0, nxt, -1))
+        if top is None:
+            self._check_chunk()
+            return out, None
+        follows = torch.cat([ids[1:], ids[:1]])
+        follows[torch.tensor([first[b + 1] - 1 for b in rows]).to(dev)] = out[at]
+        parts, t0 = [], 0
+        for hidden in kept:
+            parts.append(self.m.token_logprobs(hidden, follows[t0:t0 + hidden.shape[0]].contiguous(), top))
+            t0 += hidden.shape[0]
+        # (behind the last collective: a rank that raises leaves none of the others waiting)
+        self._check_chunk()
+        return out, ops.TokenLogprobs(*(torch.cat(t, 0) for t in zip(*parts)))
+
+    def _check_chunk(self):
+        """Waits for the passes so far.  RuntimeError if attention over the cache gave up waiting in one of them."""
+        if self.m.device.type != "cuda":
+            return
+        from .. import load_extension
+        ext, dev = load_extension(), self.positions.device.index
+        ext.chunk_attn_error_into(self.h_err, dev)
+        torch.cuda.current_stream(self.m.device).synchronize()
+        if int(self.h_err):
+            ext.chunk_attn_error_clear(dev)
+            raise RuntimeError("attention over the paged cache gave up waiting for its copies: the tokens of this call are not to be used")
+
     def set_context(self, length: int):
         """Declare that every sequence already has `length` tokens in the cache."""
         if self.kv_bits == 4:
@@ -811,12 +963,14 @@ class DecodeEngine:
             ops.paged_layout(self.new_lens, self.ctx_lens, c.block_tables, c.free_list, c.free_range, self.batch, c.block_size,
                              self.layout, rows_per_request=1, lost=self.lost)
         hidden = self.m.decode_hidden(self.ids, self.positions, self.slots, self.ctx_lens, c, self.attn_splits)
-        self.m.next_tokens(hidden, self.out_ids, rules=self.rules)
+        nxt = self.m.next_tokens(hidden, self.out_ids, rules=self.rules, logprobs=self.top)
+        if self.top is not None:
+            self.logprobs = nxt[1]
         if self.counted:
             ops.count_tokens(self.rules, self.out_ids if self.kv_bits != 4 else torch.where(self.new_lens > 0, self.out_ids, -1))
 
     def _step_body(self):
-        if self.kv_bits == 4 or self.rules is not None:
+        if self.kv_bits == 4 or self.rules is not None or self.top is not None:
             self._step_ruled()
             nxt = self.out_ids
             if self.kv_bits == 4:
