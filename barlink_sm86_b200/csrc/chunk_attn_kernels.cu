@@ -396,10 +396,10 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   // not).  All four have the same answer, so that they stay together also after a wait that ran out.
   auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(warp >> 2) : "memory"); };
   int nth = 0;
-  auto group_wait = [&](uint64_t* bar, uint32_t parity) {
+  auto group_wait = [&](uint64_t* bar, uint32_t parity, uint64_t* also = nullptr, uint32_t its = 0) {
     if constexpr (!Q4) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
     if ((warp & 3) == 0) {
-      const bool there = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
+      const bool there = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls) && (!also || mbar_wait_quick_warp(also, its & 1u, abort_at, a.polls));
       if (lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
     }
     group_sync();
@@ -724,10 +724,11 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         const uint32_t v = __byte_perm(x, y, how);
         return *reinterpret_cast<const __nv_bfloat162*>(&v);
       };
-      auto store = [&](uint32_t tile, int key, int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(tile + (chunk >> 3) * S::kHalf + key * 128 + (((chunk & 7) ^ (key & 7)) << 4)), "r"(x), "r"(y), "r"(z), "r"(w)
-                     : "memory");
+      // eight dims, 4 m + t of 8, of a key whose row's place for dims 8 t (swizzled) is `at`: t < 4, so that bit 2 of 4 m is bit 6 of the address
+      auto store = [&](uint32_t at, int m, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"((m & 1 ? at ^ 64u : at) + (m >> 1) * S::kHalf), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
       };
+      auto place = [](uint32_t tile, int key, int t) { return tile + uint32_t(key * 128 + ((t ^ (key & 7)) << 4)); };
       const int values = warp >= 16, cwarp = warp & 3;  // warps 12 to 15 keys, 16 to 19 values
       int rs = 0;
       uint32_t rphase = 0;
@@ -741,7 +742,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           const uint32_t tile = base + (values ? S::kOffV : S::kOffK) + st * S::kKV;
 #pragma unroll 1
           for (int u = 0; u < 2 - (s.cut && j == s.n - 1 ? 1 : 0); ++u) {
-            if (!group_wait(&bars.raw_full[values][rs], rphase) || !group_wait(values ? &bars.v_empty[st][u] : &bars.k_empty[st][u], fills.of(j, u) + 1u)) {
+            if (!group_wait(&bars.raw_full[values][rs], rphase, values ? &bars.v_empty[st][u] : &bars.k_empty[st][u], fills.of(j, u) + 1u)) {
               ok = false;
               return;
             }
@@ -752,7 +753,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
               for (int v = 0; v < 2; ++v) {
                 // a token, eight dims of every group; of eight neighbouring lanes four have a token four further on, so that a store of theirs meets all banks
                 const int in = 32 * v + cwarp * 8 + (lane >> 3) + (lane & 4), t = lane & 3, g = in >> 4, key = 64 * u + in;
-                const uint32_t gran = raw + g * S::kRawGran;
+                const uint32_t gran = raw + g * S::kRawGran, to = place(tile, key, t);
                 uint32_t w[NA] = {}, par[NA] = {};
                 if (key < left && (has >> g & 1u)) {
                   words(gran + (in & 15) * (HD / 2) + t * NA * 4, w);
@@ -763,13 +764,13 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
                   const __nv_bfloat162 step = pair_of(par[m >> 1], 0, m & 1 ? 0x3232 : 0x1010), low = pair_of(par[NA / 2 + (m >> 1)], 0, m & 1 ? 0x3232 : 0x1010);
                   // nibbles (0, 4), (1, 5), (2, 6), (3, 7)
                   const uint32_t p0 = value(w[m], step, low), p1 = value(w[m] >> 4, step, low), p2 = value(w[m] >> 8, step, low), p3 = value(w[m] >> 12, step, low);
-                  store(tile, key, 4 * m + t, __byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
+                  store(to, m, __byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
                 }
               }
             } else {
               // two tokens, eight dims of every group; lanes as above
               const int in = 2 * (cwarp * 8 + pair_order(lane >> 2)), q = lane & 3, g = in >> 4, key = 64 * u + in;
-              const uint32_t gran = raw + g * S::kRawGran;
+              const uint32_t gran = raw + g * S::kRawGran, to0 = place(tile, key, q), to1 = place(tile, key + 1, q);
               uint32_t w0[NA] = {}, w1[NA] = {}, pa[NA] = {}, pb[NA] = {};
               if (key < left && (has >> g & 1u)) {
                 words(gran + (in >> 1 & 7) * HD + 2 * q * NA * 4, w0);
@@ -788,9 +789,8 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
                   v[e] = value(w0[m] >> (4 * e), step, low);
                   v[4 + e] = value(w1[m] >> (4 * e), step, low);
                 }
-                const int chunk = 4 * m + q;
-                store(tile, key, chunk, __byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[4], v[5], 0x5410), __byte_perm(v[6], v[7], 0x5410));
-                store(tile, key + 1, chunk, __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632), __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
+                store(to0, m, __byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[4], v[5], 0x5410), __byte_perm(v[6], v[7], 0x5410));
+                store(to1, m, __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632), __byte_perm(v[4], v[5], 0x7632), __byte_perm(v[6], v[7], 0x7632));
               }
             }
             fence_proxy_async_smem();
