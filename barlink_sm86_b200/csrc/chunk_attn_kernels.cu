@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(warp >> 2) : "memory"); };
   int nth = 0;
   auto group_wait = [&](uint64_t* bar, uint32_t parity, uint64_t* also = nullptr, uint32_t its = 0) {
-    if constexpr (!Q4) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
+    if (!Q4 || warp < 12) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
     if ((warp & 3) == 0) {
       const bool there = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls) && (!also || mbar_wait_quick_warp(also, its & 1u, abort_at, a.polls));
       if (lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
