@@ -62,6 +62,20 @@ struct ChunkMeta {
   int h, row, ntok;         // KV head, first row of q and out, tokens of the pair
 };
 
+// n / d for 0 <= n < 2^31 by a product: with m = ceil(2^(31 + s) / d) and 2^s >= d, m d is above 2^(31 + s) by less than 2^s, which n times over stays
+// below one quotient's step.
+struct ChunkDiv {
+  uint32_t m;
+  int s;
+  __device__ __forceinline__ int operator()(int n) const { return int(uint64_t(uint32_t(n)) * m >> (31 + s)); }
+};
+// n / d where the quotient is below 2^16 (the quotient in fp32 is off by less than one)
+__device__ __forceinline__ int small_div(int n, int d) {
+  int q = int(__fdividef(float(n), float(d)));
+  const int r = n - q * d;
+  return r < 0 ? q - 1 : r >= d ? q + 1 : q;
+}
+
 struct Chunk {
   const int* cu;
   const int* ctx_lens;
@@ -73,6 +87,7 @@ struct Chunk {
   int tokens, batch, nq, nkv, G, T, block_size, n_blocks, max_blocks, row_cap, box;
   float scale_log2;
   uint32_t polls;
+  ChunkDiv by_runs, by_block;
 };
 
 // A request's share of the list: tokens, positions, what its table can hold.
@@ -104,6 +119,15 @@ struct ChunkSeg {
   int cut;          // the last step has its first half only
 };
 constexpr int kChSegs = 4;
+
+// Steps of all pairs of a request, and what they cost beside them: a warp's work.  (A function: two places call it.)
+static __device__ __noinline__ int chunk_all_steps(int n, int past, int cap, int pair, int over) {
+  const ChunkReq r = {0, n, past, cap};
+  int sum = 0;
+#pragma unroll 1
+  for (int p = threadIdx.x & 31; p * pair < n; p += 32) sum += chunk_steps(chunk_keys(r, p * pair, min(pair, n - p * pair))) + over;
+  return __reduce_add_sync(0xffffffffu, sum);
+}
 
 template <int HD, bool Q4>
 struct ChunkShape {
@@ -233,7 +257,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   volatile uint32_t* s_abort = &bars.abort;
   const uint32_t abort_at = smem_u32(&bars.abort), never_at = smem_u32(&bars.never);
   __shared__ int s_scan[S::kThreads / 32];
-  __shared__ int s_first[4];  // request, KV head, first token of the pair, step
+  int* s_upto = reinterpret_cast<int*>(gen + S::kOffK);  // (ahead of the first copy)
 
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -286,95 +310,44 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   // lengths, tables, queries and the cache may come from the kernel just before this one
   pdl_wait();
 
-  // ---- this block's run [lo, lo + count) of the list (one lane a request; a request's pairs are dealt out to the warp's lanes) ----
+  // ---- the list's length, up to each thread's requests (one lane a request; a request's pairs are dealt out to the warp's lanes) ----
   const int runs = gridDim.x, me = blockIdx.x, pair = 2 * a.T;
-  const int per = (a.batch + S::kThreads - 1) / S::kThreads, b0 = int(threadIdx.x) * per;
-  auto steps_of = [&](int n, int past, int cap, int p) {  // of pair p of a request
+  const int per = (a.batch + S::kThreads - 1) / S::kThreads;
+  auto steps_of = [&](const ChunkReq& r, int p) {  // of pair p of a request
     const int t = p * pair;
-    return t < n ? max(1, (min(max(past + min(t + pair, n), 0), cap) + kChKeys - 1) / kChKeys) + S::kOver : 0;
+    return t < r.n ? chunk_steps(chunk_keys(r, t, min(pair, r.n - t))) + S::kOver : 0;
   };
-  int run = 0, lo = 0, count = 0, src = 0, at = 0, mine = 0;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
+  {
+    int upto = 0;
 #pragma unroll 1
     for (int k = 0; k < per; ++k) {
+      const int b = int(threadIdx.x) * per + k;
       ChunkReq r = {0, 0, 0, 0};
-      if (b0 + k < a.batch) r = chunk_req(a, b0 + k);
-      int u = steps_of(r.n, r.past, r.cap, 0);
+      if (b < a.batch) r = chunk_req(a, b);
+      int u = steps_of(r, 0);
 #pragma unroll 1
       for (uint32_t many = __ballot_sync(kAll, r.n > pair); many; many &= many - 1) {
-        const int of = __ffs(many) - 1, n = __shfl_sync(kAll, r.n, of), past = __shfl_sync(kAll, r.past, of), cap = __shfl_sync(kAll, r.cap, of);
-        int sum = 0;
-#pragma unroll 1
-        for (int p = lane; p * pair < n; p += 32) sum += steps_of(n, past, cap, p);
-        sum = __reduce_add_sync(kAll, sum);
+        const int of = __ffs(many) - 1;
+        const int sum = chunk_all_steps(__shfl_sync(kAll, r.n, of), __shfl_sync(kAll, r.past, of), __shfl_sync(kAll, r.cap, of), pair, S::kOver);
         if (lane == of) u = sum;
       }
-      if (pass == 0) {
-        mine += u * a.nkv;
-        continue;
-      }
-      // the request that holds the first step; its KV head, and the pair
-      u = __shfl_sync(kAll, u, src);
-      if (lo >= at + u * a.nkv) {
-        at += u * a.nkv;
-        continue;
-      }
-      const int h = (lo - at) / u, n = __shfl_sync(kAll, r.n, src), past = __shfl_sync(kAll, r.past, src), cap = __shfl_sync(kAll, r.cap, src);
-      at += h * u;
-#pragma unroll 1
-      for (int p = lane;; p += 32) {
-        const int st = steps_of(n, past, cap, p);
-        int cum = st;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(kAll, cum, o);
-          if (lane >= o) cum += v;
-        }
-        const uint32_t in = __ballot_sync(kAll, lo < at + cum);
-        if (in) {
-          if (lane == __ffs(in) - 1) {
-            s_first[1] = h;
-            s_first[2] = p * pair;
-            s_first[3] = lo - (at + cum - st);
-          }
-          if (lane == src) s_first[0] = b0 + k;
-          break;
-        }
-        at += __shfl_sync(kAll, cum, 31);
-      }
-      break;
+      upto += u * a.nkv;
     }
-    if (pass) break;
-    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(kAll, upto, o);
       if (lane >= o) upto += v;
     }
+    s_upto[threadIdx.x] = upto;
+    fence_proxy_async_smem();  // (copies go there behind the barriers)
     if (lane == 31) s_scan[warp] = upto;
-    __syncthreads();
-    // (at most sixteen warps)
-    const int w = lane < S::kThreads / 32 ? s_scan[lane] : 0, total = __reduce_add_sync(kAll, w);
-    upto += __reduce_add_sync(kAll, lane < warp ? w : 0);
-    run = (total + runs - 1) / runs;
-    lo = min(me * run, total);
-    count = min(run, total - lo);
-    const uint32_t holds = __ballot_sync(kAll, count > 0 && upto - mine <= lo && lo < upto);
-    if (!holds) break;
-    src = __ffs(holds) - 1;  // one lane of one warp
-    at = __shfl_sync(kAll, upto - mine, src);
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = bars.tmem;
-  if (count == 0) {
-    if (threadIdx.x == 0) a.meta[me].count = 0;
-    __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, kChTmemCols);
-    return;
-  }
+  // Warp 3 finds the run's first step while the others wait here for its first share.
+  auto begin = [] { asm volatile("bar.sync 0;" ::: "memory"); };
   // Step j of a share has slot j & 1 of the keys and of the values, so that a share with one tile has a slot to a place; a slot is filled and emptied by
   // halves, of which a pair's last step may have the first only, and a role knows a half's phase by how often it has been filled.
   struct Fills {
@@ -416,10 +389,11 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   };
   // Every role goes through the run's shares of pairs: f(share, whether it has two tiles).  After a wait that ran out they go on without work.
   auto each = [&](auto&& f) {
+    begin();
 #pragma unroll 1
     for (int k = 0;; ++k) {
       bool there = true;
-      if (!Q4 || warp < 4 || (warp & 3) == 0) there = mbar_wait_call(smem_u32(&bars.seg_full[k % kChSegs]), uint32_t(k / kChSegs) & 1u, never_at, 1u << 22);
+      if (k > 0 && (!Q4 || warp < 4 || (warp & 3) == 0)) there = mbar_wait_call(smem_u32(&bars.seg_full[k % kChSegs]), uint32_t(k / kChSegs) & 1u, never_at, 1u << 22);
       if (Q4 && warp >= 4) {
         if ((warp & 3) == 0 && lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
         group_sync();
@@ -461,7 +435,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         const int tok = j * kChKeys + lane * kChGran;
         int at = -1;
         if (tok < s.keys) {
-          const int page = tok / a.block_size, blk = table[page], in = tok - page * a.block_size;
+          const int page = a.by_block(tok), blk = table[page], in = tok - page * a.block_size;
           at = blk < 0 || blk >= a.n_blocks ? -2 : Q4 ? (blk * a.nkv + s.h) * (a.block_size / kQ4Tokens) + in / kQ4Tokens : (blk * a.nkv + s.h) * a.block_size + in;
         }
         return at;
@@ -526,12 +500,62 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     const uint32_t bytes = uint32_t(a.G) * a.T * HD * 2;
     int asked[2] = {0, 0};  // query tiles asked for, by place
     ChunkMeta m = {};       // what the second kernel needs to know
-    int b = s_first[0], h = s_first[1], tok0 = s_first[2], j0 = s_first[3];
-    ChunkReq r = chunk_req(a, b);
+    // ---- this block's run [lo, lo + count) of the list, and where it begins ----
+    int b = 0, h = 0, tok0 = 0, j0 = 0, run = 0, lo = 0, count = 0;
+    ChunkReq r = {0, 0, 0, 0};
+    if (values) {
+      const int w = lane < S::kThreads / 32 ? s_scan[lane] : 0;  // (at most twenty warps)
+      int at = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kAll, at, o);
+        if (lane >= o) at += v;
+      }
+      const int total = __shfl_sync(kAll, at, 31);
+      run = a.by_runs(total + runs - 1);
+      lo = min(me * run, total);
+      count = min(run, total - lo);
+      if (count > 0) {
+        const int of = __ffs(__ballot_sync(kAll, lo < at)) - 1;
+        at = __shfl_sync(kAll, at - w, of);
+        const int upto = at + s_upto[of * 32 + lane], src = __ffs(__ballot_sync(kAll, lo < upto)) - 1;
+        if (src > 0) at = __shfl_sync(kAll, upto, src - 1);
+        // the request that holds the first step; its KV head, and the pair
+        int u = 0;
+        b = (of * 32 + src) * per - 1;
+        do {
+          at += u * a.nkv;
+          r = chunk_req(a, ++b);
+          u = r.n > pair ? chunk_all_steps(r.n, r.past, r.cap, pair, S::kOver) : steps_of(r, 0);
+        } while (lo >= at + u * a.nkv && b + 1 < a.batch);
+        // (lengths that another stream changes meanwhile, which nobody may, are to leave nothing worse than wrong rows)
+        u = max(u, 1);
+        h = min(small_div(lo - at, u), a.nkv - 1);
+        at += h * u;
+#pragma unroll 1
+        for (int p = lane; r.n > pair && (p - lane) * pair < r.n; p += 32) {
+          const int st = steps_of(r, p);
+          int cum = st;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(kAll, cum, o);
+            if (lane >= o) cum += v;
+          }
+          const uint32_t in = __ballot_sync(kAll, lo < at + cum);
+          if (in) {
+            at += __shfl_sync(kAll, cum - st, __ffs(in) - 1);
+            tok0 = __shfl_sync(kAll, p, __ffs(in) - 1) * pair;
+            break;
+          }
+          at += __shfl_sync(kAll, cum, 31);
+        }
+        j0 = lo - at;
+      }
+    }
 #pragma unroll 1
     for (int k = 0, i = 0, done = 0;; ++k) {
       const uint32_t slot = k % kChSegs, turn = uint32_t(k / kChSegs) & 1u;
-      if (!mbar_wait_call(smem_u32(values ? &bars.seg_empty[slot] : &bars.seg_full[slot]), values ? turn ^ 1u : turn, never_at, 1u << 22)) {
+      if (k >= (values ? kChSegs : 1) && !mbar_wait_call(smem_u32(values ? &bars.seg_empty[slot] : &bars.seg_full[slot]), values ? turn ^ 1u : turn, never_at, 1u << 22)) {
         *s_abort = 1;
         break;
       }
@@ -553,7 +577,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           s.i0 = done;
           s.cut = s.keys - (j0 + s.n - 1) * kChKeys <= kChHalf;
           s.piece = s.n == steps ? -1 : 2 * me + (i == 0 ? 0 : 1);
-          if (j0 == 0 && s.n < steps) m = {(lo + i + steps - 1) / run - me + 1, s.piece, h, s.row, s.ntok};
+          if (j0 == 0 && s.n < steps) m = {small_div(lo + i + steps - 1, run) - me + 1, s.piece, h, s.row, s.ntok};
           done += s.n;
           i += steps + S::kOver - j0;
           j0 = 0;
@@ -562,8 +586,10 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
             tok0 = 0;
             if (++h == a.nkv && i < count) {
               h = 0;
-              do r = chunk_req(a, ++b);
-              while (r.n == 0);  // (there are more steps, so there is another)
+              do
+                if (++b < a.batch) r = chunk_req(a, b);
+              while (b < a.batch && r.n == 0);
+              if (b >= a.batch) i = count;  // (not with steps left, but see above)
             }
           }
         }
@@ -571,6 +597,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         mbar_arrive(&bars.seg_full[slot]);
       }
       __syncwarp();
+      if (k == 0) begin();
       const ChunkSeg s = bars.segs[slot];
       __syncwarp();
       if (!values && lane == 0) mbar_arrive(&bars.seg_empty[slot]);
@@ -811,6 +838,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------ softmax ------------------------------
+    constexpr int kCols = Q4 ? 16 : 32;  // of the sums, at a time
     const int t = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;  // TMEM lanes that this warp may touch
     const int tok = row / a.G, g = row - tok * a.G;
     const uint32_t s_base = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(t * 128);
@@ -971,29 +999,29 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       tc_fence_after_sync();
       if (busy) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < HD; c0 += 32) {
-          uint32_t r[2][16], q[2][16];
+        for (int c0 = 0; c0 < HD; c0 += kCols) {
+          uint32_t r[kCols / 16][16], q[kCols / 16][16];
 #pragma unroll
-          for (int d = 0; d < 2; ++d) tmem_ld_32x16(o_addr + c0 + 16 * d, r[d]);
+          for (int d = 0; d < kCols / 16; ++d) tmem_ld_32x16(o_addr + c0 + 16 * d, r[d]);
           if (one_copy(join)) {
 #pragma unroll
-            for (int d = 0; d < 2; ++d) tmem_ld_32x16(o_addr + 128u + c0 + 16 * d, q[d]);
+            for (int d = 0; d < kCols / 16; ++d) tmem_ld_32x16(o_addr + 128u + c0 + 16 * d, q[d]);
           } else {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) q[c >> 4][c & 15] = 0;
+            for (int c = 0; c < kCols; ++c) q[c >> 4][c & 15] = 0;
           }
           tmem_ld_wait();
-          float v[32];
+          float v[kCols];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = fmaf(__uint_as_float(q[c >> 4][c & 15]), w1, __uint_as_float(r[c >> 4][c & 15]) * w0);
+          for (int c = 0; c < kCols; ++c) v[c] = fmaf(__uint_as_float(q[c >> 4][c & 15]), w1, __uint_as_float(r[c >> 4][c & 15]) * w0);
           if (one_copy(valid && whole)) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 8)
+            for (int c = 0; c < kCols; c += 8)
               *reinterpret_cast<uint4*>(orow + c0 + c) =
                   make_uint4(pack_bf16x2(v[c], v[c + 1]), pack_bf16x2(v[c + 2], v[c + 3]), pack_bf16x2(v[c + 4], v[c + 5]), pack_bf16x2(v[c + 6], v[c + 7]));
           } else if (one_copy(valid)) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) prow[size_t((c0 + c) / 4) * a.row_cap] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+            for (int c = 0; c < kCols; c += 4) prow[size_t((c0 + c) / 4) * a.row_cap] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
           }
           __syncwarp();
         }
@@ -1140,6 +1168,14 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   a.box = block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : 16;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.polls = g_chunk_polls.load();
+  auto divide_by = [](uint32_t d) {
+    ChunkDiv r = {0, 0};
+    while ((uint64_t(1) << r.s) < d) ++r.s;
+    r.m = uint32_t(((uint64_t(1) << (31 + r.s)) + d - 1) / d);
+    return r;
+  };
+  a.by_runs = divide_by(runs);
+  a.by_block = divide_by(block_size);
 
   const DriverApi* d = driver(err, errlen);
   if (!d) return -1;
