@@ -1048,7 +1048,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
 }
 
 // Pieces of a pair that was cut: block (run where it begins, 32 rows), a lane a row, a warp HD / 8 of its dims.
-constexpr int kChMergeWarps = 8;
+constexpr int kChMergeWarps = 8, kChMergeAhead = 4;  // pieces that are asked for at once
 template <int HD>
 __global__ void __launch_bounds__(kChMergeWarps * 32) k_chunk_merge(const Chunk a) {
   constexpr int V = HD / 4 / kChMergeWarps;  // vectors of four dims
@@ -1066,22 +1066,34 @@ __global__ void __launch_bounds__(kChMergeWarps * 32) k_chunk_merge(const Chunk 
   float4 acc[V];
 #pragma unroll
   for (int d = 0; d < V; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int k = 0; k < m.count; ++k) {
-    const size_t p = size_t(k == 0 ? m.first : 2 * (me + k)) * a.row_cap;
-    const float2 ml = sums[p];
-    float4 v[V];
+#pragma unroll 1
+  for (int k = 0; k < m.count; k += kChMergeAhead) {
+    float2 ml[kChMergeAhead];
+    float4 v[kChMergeAhead][V];
 #pragma unroll
-    for (int d = 0; d < V; ++d) v[d] = part[p * (HD / 4) + size_t(d) * a.row_cap];
-    const float n = fmaxf(M, ml.x), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(ml.x - ref);
-    M = n;
-    L = L * s0 + ml.y * s1;
+    for (int e = 0; e < kChMergeAhead; ++e) {
+      ml[e] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int d = 0; d < V; ++d) {
-      acc[d].x = acc[d].x * s0 + v[d].x * s1;
-      acc[d].y = acc[d].y * s0 + v[d].y * s1;
-      acc[d].z = acc[d].z * s0 + v[d].z * s1;
-      acc[d].w = acc[d].w * s0 + v[d].w * s1;
+      for (int d = 0; d < V; ++d) v[e][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k + e < m.count) {
+        const size_t p = size_t(k + e == 0 ? m.first : 2 * (me + k + e)) * a.row_cap;
+        ml[e] = sums[p];
+#pragma unroll
+        for (int d = 0; d < V; ++d) v[e][d] = part[p * (HD / 4) + size_t(d) * a.row_cap];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kChMergeAhead; ++e) {
+      const float n = fmaxf(M, ml[e].x), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(ml[e].x - ref);
+      M = n;
+      L = L * s0 + ml[e].y * s1;
+#pragma unroll
+      for (int d = 0; d < V; ++d) {
+        acc[d].x = acc[d].x * s0 + v[e][d].x * s1;
+        acc[d].y = acc[d].y * s0 + v[e][d].y * s1;
+        acc[d].z = acc[d].z * s0 + v[e][d].z * s1;
+        acc[d].w = acc[d].w * s0 + v[e][d].w * s1;
+      }
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
