@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
 #pragma unroll 1
         for (int h = 0; h < 2 - (s.cut && j == s.n - 1 ? 1 : 0); ++h) {
           uint64_t* bar = Q4 ? &bars.raw_full[values][rs] : &full[st][h];
-          if (!(ok = mbar_wait_call(smem_u32(Q4 ? &bars.raw_empty[values][rs] : &empty[st][h]), (Q4 ? rphase : fills.of(j, h) + 1u) & 1u, abort_at, a.polls))) return;
+          if (!(ok = mbar_wait_quick_warp(Q4 ? &bars.raw_empty[values][rs] : &empty[st][h], (Q4 ? rphase : fills.of(j, h) + 1u) & 1u, abort_at, a.polls))) return;
           if (!values && h == 0) {
             if (lane == 0 && (lost || (gone_before >> (i & 7) & 1u))) bars.gone[i & 7] = lost;
             gone_before = (gone_before & ~(1u << (i & 7))) | uint32_t(lost != 0) << (i & 7);
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
           if (!ok || (t == 1 && !two && s.n < 2)) break;
-          if (!(ok = mbar_wait_call(smem_u32(&bars.q_empty[t]), (uint32_t(t ? asked[1] : asked[0]) & 1u) ^ 1u, abort_at, a.polls))) break;
+          if (!(ok = mbar_wait_quick_warp(&bars.q_empty[t], (uint32_t(t ? asked[1] : asked[0]) & 1u) ^ 1u, abort_at, a.polls))) break;
           if (lane == 0) {
             mbar_expect_tx(&bars.q_full[t], bytes);
 #pragma unroll
