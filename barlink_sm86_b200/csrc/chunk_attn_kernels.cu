@@ -50,7 +50,7 @@ constexpr int kChHalf = kChKeys / 2;
 constexpr uint32_t kChTmemCols = 512;  // S of place t, half h of a step: 128 t + 64 h, P in its first half; O of place t: 256 + 128 t
 constexpr int kChPoly = 1;             // of four pairs of exponentials, those on the FMA pipe
 // What a pair costs beside its steps (queries, sums, a chain that starts anew), in steps: that many empty ones follow it in the list.
-constexpr int chunk_over(bool q4) { return q4 ? 4 : 3; }
+constexpr int chunk_over(bool q4) { return q4 ? 4 : 2; }
 constexpr float kChRescale = 8.f;      // log2 units
 constexpr uint32_t kChPolls = 1u << 24;
 
@@ -87,7 +87,7 @@ struct Chunk {
   int tokens, batch, nq, nkv, G, T, block_size, n_blocks, max_blocks, row_cap, box;
   float scale_log2;
   uint32_t polls;
-  ChunkDiv by_runs, by_block;
+  ChunkDiv by_runs, by_block, by_pair;
 };
 
 // A request's share of the list: tokens, positions, what its table can hold.
@@ -107,6 +107,16 @@ __device__ __forceinline__ ChunkReq chunk_req(const Chunk& a, int b) {
 __device__ __forceinline__ int chunk_keys(const ChunkReq& r, int tok0, int ntok) { return min(max(r.past + tok0 + ntok, 0), r.cap); }
 // (a pair that sees nothing has a step all the same: its rows are written)
 __device__ __forceinline__ int chunk_steps(int keys) { return max(1, (keys + kChKeys - 1) / kChKeys); }
+__device__ __forceinline__ int chunk_pairs(const Chunk& a, const ChunkReq& r) { return a.by_pair(r.n + 2 * a.T - 1); }
+// Where pair p of a request begins in its part of the list: floor(sum of the keys of the pairs before / 128) + p (1 + over).  A pair of x keys has no more
+// than floor(x / 128) + 1 steps, so that there is room for them and for `over` or one more empty ones; and the sum (keys grow evenly from pair to pair,
+// between 0 and what the table holds) needs no loop.
+__device__ __forceinline__ int chunk_upto(const Chunk& a, const ChunkReq& r, int p, int over) {
+  const int q1 = r.cap > r.past ? min(p, a.by_pair(r.cap - r.past - 1)) : 0;  // pairs 1 .. q1 end below the table's end,
+  const int q0 = r.past < 0 ? min(q1, a.by_pair(-r.past)) : 0;                // 1 .. q0 ahead of the first key
+  const int64_t keys = int64_t(q1 - q0) * r.past + a.T * (int64_t(q1) * (q1 + 1) - int64_t(q0) * (q0 + 1)) + int64_t(p - q1) * r.cap;
+  return int(keys >> 7) + p * (1 + over);
+}
 
 // A run's share of a pair, as the warp that walks the list leaves it for the others.
 struct ChunkSeg {
@@ -119,15 +129,6 @@ struct ChunkSeg {
   int cut;          // the last step has its first half only
 };
 constexpr int kChSegs = 4;
-
-// Steps of all pairs of a request, and what they cost beside them: a warp's work.  (A function: two places call it.)
-static __device__ __noinline__ int chunk_all_steps(int n, int past, int cap, int pair, int over) {
-  const ChunkReq r = {0, n, past, cap};
-  int sum = 0;
-#pragma unroll 1
-  for (int p = threadIdx.x & 31; p * pair < n; p += 32) sum += chunk_steps(chunk_keys(r, p * pair, min(pair, n - p * pair))) + over;
-  return __reduce_add_sync(0xffffffffu, sum);
-}
 
 template <int HD, bool Q4>
 struct ChunkShape {
@@ -310,28 +311,17 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   // lengths, tables, queries and the cache may come from the kernel just before this one
   pdl_wait();
 
-  // ---- the list's length, up to each thread's requests (one lane a request; a request's pairs are dealt out to the warp's lanes) ----
+  // ---- the list's length, up to each thread's requests ----
   const int runs = gridDim.x, me = blockIdx.x, pair = 2 * a.T;
   const int per = (a.batch + S::kThreads - 1) / S::kThreads;
-  auto steps_of = [&](const ChunkReq& r, int p) {  // of pair p of a request
-    const int t = p * pair;
-    return t < r.n ? chunk_steps(chunk_keys(r, t, min(pair, r.n - t))) + S::kOver : 0;
-  };
   {
     int upto = 0;
 #pragma unroll 1
     for (int k = 0; k < per; ++k) {
       const int b = int(threadIdx.x) * per + k;
-      ChunkReq r = {0, 0, 0, 0};
-      if (b < a.batch) r = chunk_req(a, b);
-      int u = steps_of(r, 0);
-#pragma unroll 1
-      for (uint32_t many = __ballot_sync(kAll, r.n > pair); many; many &= many - 1) {
-        const int of = __ffs(many) - 1;
-        const int sum = chunk_all_steps(__shfl_sync(kAll, r.n, of), __shfl_sync(kAll, r.past, of), __shfl_sync(kAll, r.cap, of), pair, S::kOver);
-        if (lane == of) u = sum;
-      }
-      upto += u * a.nkv;
+      if (b >= a.batch) break;
+      const ChunkReq r = chunk_req(a, b);
+      upto += chunk_upto(a, r, chunk_pairs(a, r), S::kOver) * a.nkv;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -501,7 +491,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     int asked[2] = {0, 0};  // query tiles asked for, by place
     ChunkMeta m = {};       // what the second kernel needs to know
     // ---- this block's run [lo, lo + count) of the list, and where it begins ----
-    int b = 0, h = 0, tok0 = 0, j0 = 0, run = 0, lo = 0, count = 0;
+    int b = 0, h = 0, p = 0, p_at = 0, j0 = 0, run = 0, lo = 0, count = 0;  // (pair p, which begins at p_at)
     ChunkReq r = {0, 0, 0, 0};
     if (values) {
       const int w = lane < S::kThreads / 32 ? s_scan[lane] : 0;  // (at most twenty warps)
@@ -526,30 +516,21 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         do {
           at += u * a.nkv;
           r = chunk_req(a, ++b);
-          u = r.n > pair ? chunk_all_steps(r.n, r.past, r.cap, pair, S::kOver) : steps_of(r, 0);
+          u = chunk_upto(a, r, chunk_pairs(a, r), S::kOver);
         } while (lo >= at + u * a.nkv && b + 1 < a.batch);
         // (lengths that another stream changes meanwhile, which nobody may, are to leave nothing worse than wrong rows)
         u = max(u, 1);
         h = min(small_div(lo - at, u), a.nkv - 1);
-        at += h * u;
+        const int in = lo - at - h * u;
 #pragma unroll 1
-        for (int p = lane; r.n > pair && (p - lane) * pair < r.n; p += 32) {
-          const int st = steps_of(r, p);
-          int cum = st;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(kAll, cum, o);
-            if (lane >= o) cum += v;
-          }
-          const uint32_t in = __ballot_sync(kAll, lo < at + cum);
-          if (in) {
-            at += __shfl_sync(kAll, cum - st, __ffs(in) - 1);
-            tok0 = __shfl_sync(kAll, p, __ffs(in) - 1) * pair;
-            break;
-          }
-          at += __shfl_sync(kAll, cum, 31);
+        for (int many = chunk_pairs(a, r); many > 1;) {
+          const int stride = (many + 31) / 32;
+          const int top = 31 - __clz(__ballot_sync(kAll, lane * stride < many && chunk_upto(a, r, p + lane * stride, S::kOver) <= in) | 1);
+          p += top * stride;
+          many = min(stride, many - top * stride);
         }
-        j0 = lo - at;
+        p_at = chunk_upto(a, r, p, S::kOver);
+        j0 = in - p_at;
       }
     }
 #pragma unroll 1
@@ -566,6 +547,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         while (i < count && s.n == 0) {
           s.b = b;
           s.h = h;
+          const int tok0 = p * pair;
           s.row = r.q0 + tok0;
           s.ntok = min(pair, r.n - tok0);
           s.keys = chunk_keys(r, tok0, s.ntok);
@@ -579,11 +561,11 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           s.piece = s.n == steps ? -1 : 2 * me + (i == 0 ? 0 : 1);
           if (j0 == 0 && s.n < steps) m = {small_div(lo + i + steps - 1, run) - me + 1, s.piece, h, s.row, s.ntok};
           done += s.n;
-          i += steps + S::kOver - j0;
+          i -= p_at + j0;
+          i += p_at = chunk_upto(a, r, ++p, S::kOver);
           j0 = 0;
-          tok0 += pair;
-          if (tok0 >= r.n) {
-            tok0 = 0;
+          if (tok0 + pair >= r.n) {
+            p = p_at = 0;
             if (++h == a.nkv && i < count) {
               h = 0;
               do
@@ -1188,6 +1170,7 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   };
   a.by_runs = divide_by(runs);
   a.by_block = divide_by(block_size);
+  a.by_pair = divide_by(2 * a.T);
 
   const DriverApi* d = driver(err, errlen);
   if (!d) return -1;
