@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(warp >> 2) : "memory"); };
   int nth = 0;
   auto group_wait = [&](uint64_t* bar, uint32_t parity, uint64_t* also = nullptr, uint32_t its = 0) {
-    if (!Q4 || warp < 12) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
+    if (!Q4) return mbar_spin_warp(bar, parity & 1u, s_abort, a.polls);
+    if (warp < 12) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
     if ((warp & 3) == 0) {
       const bool there = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls) && (!also || mbar_wait_quick_warp(also, its & 1u, abort_at, a.polls));
       if (lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     Fills fills;
     uint32_t meets = 0;
     bool apart = false;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = mbar_spin_warp(bar, parity & 1u, s_abort, a.polls); };
     auto share = [&](const ChunkSeg& s, bool two) {
       const int every = two ? 1 : 2, n = s.n, begin = two ? 0 : t;  // this place's steps
       if (begin >= n) return;

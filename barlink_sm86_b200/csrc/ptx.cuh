@@ -216,6 +216,16 @@ __device__ __forceinline__ bool mbar_wait_quick_warp(uint64_t* bar, uint32_t par
   if (max_polls > 0 && __all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   return mbar_wait_call(smem_u32(bar), parity, abort_flag, max_polls);
 }
+// Looking all the time, without a call behind which the thread's registers have to be put back: for warps that everyone waits for.  A poll is 16 looks.
+__device__ __forceinline__ bool mbar_spin_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t max_polls) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < max_polls << 4; ++i) {
+    if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    if ((i & 255u) == 255u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
