@@ -23,6 +23,19 @@
 // Steps of all pairs of all requests and KV heads make one list, of which every block takes an equal run: lengths are known on the GPU only.  A pair
 // that is cut leaves its pieces (sums, maxima) to a second kernel.
 //
+// Measured, as captured and replayed (heads / KV heads x dims; ideal: bytes at the rate of a copy, or products at that of a large matrix product):
+//   bf16   5 tokens on 333, 28/4x128             11 us          two launches and one step's chain: 5 us until the first keys are there, 2 for the pieces
+//          64 requests of up to 8 on 1100        26 us (10)     1.8 pairs a block, of four steps each: the first one's start and every pair's end
+//          9 of up to 700 on 5001, 14/2x128      87 us (42)     the chain below, and pairs' ends
+//          2048 on 16383, 40/8x128              553 us (387)    1.17 PFLOP/s; 630 us where it runs for long and the clock drops
+//   4-bit  4 on 900, 28/4x128                  13.5 us
+//          64 of up to 6 on 1100                 33 us (3.4)    conversion: 750 warp instructions a step and quarter of the SM for K and V
+//          2 of up to 13 on 100000, 40/8x128    135 us (29)     the same
+//          1500 on 9000, 28/4x128               218 us (106)    issue slots (half of them used) and the chain
+// Where new tokens fill tiles a step of two tiles takes some 3900 cycles of an SM; its products 2560 (S of 64 keys at a time reads its operands from shared
+// memory at three quarters of the rate of 128, which would leave a place no scores to go on with), its exponentials 1540 of the unit for them.  The rest is
+// the chain of a place's half step: products seen to be done, scores read, largest one, exponentials, P seen to be there.
+//
 // Tokens of table entries that name no block are left out (their boxes start behind the cache, so TMA fills in zeros).  What stands in the cache
 // behind a request's last token may be anything: the values of the rest of its box are set to zero in shared memory.
 //
@@ -48,8 +61,12 @@ constexpr int kChGrans = kChKeys / kChGran;
 constexpr int kChRaw = 3;      // half steps of the 4-bit cache in flight
 constexpr int kChHalf = kChKeys / 2;
 constexpr uint32_t kChTmemCols = 512;  // S of place t, half h of a step: 128 t + 64 h, P in its first half; O of place t: 256 + 128 t
-constexpr int kChPoly = 1;             // of four pairs of exponentials, those on the FMA pipe
-// What a pair costs beside its steps (queries, sums, a chain that starts anew), in steps: that many empty ones follow it in the list.
+// Of four pairs of exponentials, those on the FMA pipe (bf16 cache).  2048 tokens on 16383: none 573 us, one 553, two 589; 9 requests of up to 700 on 5001: 94,
+// 87, 91.  The 4-bit cache's blocks have no issue slots for them (1500 on 9000: none 214 us, one 224).
+constexpr int kChPoly = 1;
+// What a pair costs beside its steps (queries, sums, a chain that starts anew), in steps: that many empty ones, or one more, follow it in the list.
+// 64 requests of up to 8 tokens on 1100 without any 36.5 us, with 2 or 3 25.7; 9 of up to 700 on 5001 without 138, 3: 91, 2: 89.5; 4-bit cache, 64 of up to 6 on
+// 1100 without 42, 3: 33.0, 4: 32.6, 8: 41.
 constexpr int chunk_over(bool q4) { return q4 ? 4 : 2; }
 constexpr float kChRescale = 8.f;      // log2 units
 constexpr uint32_t kChPolls = 1u << 24;
@@ -164,13 +181,6 @@ static_assert(sizeof(ChunkBars) <= 768, "barriers");
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
 // 2^x of two numbers on the FMA pipe: x = n + f, |f| <= 1/2, 2^f by the polynomial of degree 3 whose relative error is least (7.5e-5; P is rounded to
@@ -354,9 +364,10 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     }
   };
   bool ok = true;
-  // With the 4-bit cache, groups of four warps (softmax, conversion) wait as one: their first warp looks at the barrier, the others wait for it where
-  // waiting takes no issue slots (with twenty warps that look at barriers pauses between looks made the kernel faster, which with twelve they do
-  // not).  All four have the same answer, so that they stay together also after a wait that ran out.
+  // Softmax warps of the bf16 cache look at a barrier all the time (9 requests of up to 700 on 5001: 87 us; pausing between looks: 89).  Those of the 4-bit cache
+  // pause, as its warps are short of issue slots (1500 on 9000: 217 us; looking all the time: 225), and its groups of four that convert codes wait as one: their
+  // first warp looks, the others wait for it where waiting takes no issue slots.  All four have the same answer, so that they stay together also after a
+  // wait that ran out.
   auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(warp >> 2) : "memory"); };
   int nth = 0;
   auto group_wait = [&](uint64_t* bar, uint32_t parity, uint64_t* also = nullptr, uint32_t its = 0) {
