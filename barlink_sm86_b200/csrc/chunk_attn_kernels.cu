@@ -29,7 +29,7 @@
 //          9 of up to 700 on 5001, 14/2x128      87 us (42)     the chain below, and pairs' ends
 //          2048 on 16383, 40/8x128              553 us (387)    1.17 PFLOP/s; 630 us where it runs for long and the clock drops
 //   4-bit  4 on 900, 28/4x128                  13.5 us
-//          64 of up to 6 on 1100                 33 us (3.4)    conversion: 750 warp instructions a step and quarter of the SM for K and V
+//          64 of up to 6 on 1100                 33 us (3.4)    conversion: some 800 warp instructions a step and quarter of the SM for K and V
 //          2 of up to 13 on 100000, 40/8x128    135 us (29)     the same
 //          1500 on 9000, 28/4x128               218 us (106)    issue slots (half of them used) and the chain
 // Where new tokens fill tiles a step of two tiles takes some 3900 cycles of an SM; its products 2560 (S of 64 keys at a time reads its operands from shared
@@ -518,21 +518,22 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       lo = min(me * run, total);
       count = min(run, total - lo);
       if (count > 0) {
-        const int of = __ffs(__ballot_sync(kAll, lo < at)) - 1;
+        // (Lengths that another stream changes meanwhile, which nobody may, or row offsets that fall, whose sum may pass 31 bits, are to leave nothing
+        // worse than wrong rows: what is found stays in range.)
+        const int of = max(__ffs(__ballot_sync(kAll, lo < at)) - 1, 0);
         at = __shfl_sync(kAll, at - w, of);
-        const int upto = at + s_upto[of * 32 + lane], src = __ffs(__ballot_sync(kAll, lo < upto)) - 1;
+        const int upto = at + s_upto[of * 32 + lane], src = max(__ffs(__ballot_sync(kAll, lo < upto)) - 1, 0);
         if (src > 0) at = __shfl_sync(kAll, upto, src - 1);
         // the request that holds the first step; its KV head, and the pair
         int u = 0;
-        b = (of * 32 + src) * per - 1;
+        b = min((of * 32 + src) * per, a.batch - 1) - 1;
         do {
           at += u * a.nkv;
           r = chunk_req(a, ++b);
           u = chunk_upto(a, r, chunk_pairs(a, r), S::kOver);
         } while (lo >= at + u * a.nkv && b + 1 < a.batch);
-        // (lengths that another stream changes meanwhile, which nobody may, are to leave nothing worse than wrong rows)
         u = max(u, 1);
-        h = min(small_div(lo - at, u), a.nkv - 1);
+        h = min(max(small_div(lo - at, u), 0), a.nkv - 1);
         const int in = lo - at - h * u;
 #pragma unroll 1
         for (int many = chunk_pairs(a, r); many > 1;) {

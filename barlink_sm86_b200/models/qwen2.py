@@ -820,7 +820,7 @@ class DecodeEngine:
                 return out, None
             none = torch.zeros(0, dtype=torch.float32, device=dev)
             return out, ops.TokenLogprobs(none, none, torch.zeros(0, top, dtype=torch.int32, device=dev), none.new_zeros(0, top))
-        ids = ids.to(device=dev, dtype=torch.int32)
+        ids = ids.to(device=dev, dtype=torch.int32).reshape(-1)
         new = torch.tensor(lens, dtype=torch.int32).to(dev)
         fresh = []
         past = (self.ctx_lens if self.kv_bits == 4 else self.positions).clone()

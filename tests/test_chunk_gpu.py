@@ -203,6 +203,26 @@ def test_rows_of_no_request_stay(heads, q4):
     assert torch.equal(got[7:52], want) and (got[:7] == 3.25).all() and (got[52:] == 3.25).all()
 
 
+@pytest.mark.parametrize("q4", [False, True])
+def test_requests_that_share_blocks(q4):
+    """A prefix that several requests have, and a block twice in one table: blocks are read only."""
+    c = Case((28, 4, 128), 16, [(5, 300), (40, 300), (1, 300)], q4)
+    c.table[1, :12] = c.table[0, :12]
+    c.table[2] = c.table[0]
+    c.table[0, 3] = c.table[0, 2]
+    c.check(c.run())
+
+
+def test_row_offsets_that_fall():
+    """Rows that two requests claim hold one's result or the other's, whichever was there last; all others are right."""
+    c = Case((8, 2, 64), 16, [(30, 64), (20, 200), (30, 90)])
+    want, size = c.want()
+    c.cu[2] = 10  # the second has none, the third 70 rows from 10 on
+    got = c.run()
+    err, room = (got.double() - want).abs(), 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -10) * size
+    assert bool((err <= room)[:10].all()) and bool(got.isfinite().all())
+
+
 def test_row_offsets_that_leave_the_rows():
     """Offsets outside q and lengths out of any range: nothing outside the tensors is touched."""
     c = Case((14, 2, 128), 16, [(30, 100), (10, 60)], seed=8)

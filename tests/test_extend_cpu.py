@@ -187,6 +187,14 @@ def test_refusals(kv_bits):
     assert torch.equal(nxt, eng.ids) and lp.logprobs.shape == (0,) and lp.top_ids.shape == (0, 2)
 
 
+def test_ids_of_any_shape():
+    m = _model()
+    a, b = DecodeEngine(m, 2, 32), DecodeEngine(m, 2, 32)
+    ids = torch.stack([_text(1, 9), _text(2, 9)])
+    out = a.extend(ids.long(), [9, 9], max_tokens=5)
+    assert torch.equal(out, b.extend(ids.reshape(-1), [9, 9], max_tokens=5)) and torch.equal(out, DecodeEngine(m, 2, 32).prefill(ids))
+
+
 def _run(comm):
     # (an odd vocabulary: the second rank's slice ends in padding)
     m = _model(comm, 501)
