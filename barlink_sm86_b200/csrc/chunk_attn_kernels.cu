@@ -43,6 +43,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "attn_tc.cuh"
@@ -1174,7 +1175,7 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   a.tokens = tokens; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks; a.max_blocks = max_blocks;
   a.box = block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : 16;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.polls = g_chunk_polls.load();
+  a.polls = std::min(g_chunk_polls.load(), 1u << 27);  // (a poll of the warps that look all the time is 16 looks)
   auto divide_by = [](uint32_t d) {
     ChunkDiv r = {0, 0};
     while ((uint64_t(1) << r.s) < d) ++r.s;

@@ -135,8 +135,9 @@ def test_a_wait_that_runs_out(ext, polls, heads, lens, q4):
         assert torch.equal(bad.all(1), bad.any(1)) and (not bool(bad.any()) or _word(ext) == 1)
         assert torch.equal(torch.where(bad, 0, got.view(-1, heads[2])), torch.where(bad, 0, want.view(-1, heads[2])))
         ext.chunk_attn_error_clear(0)
-    polls(1 << 24)
-    assert torch.equal(run(), want) and _word(ext) == 0
+    for n in (1 << 24, (1 << 32) - 1):
+        polls(n)
+        assert torch.equal(run(), want) and _word(ext) == 0
 
 
 @pytest.mark.parametrize("kv_bits", [16, 4])
