@@ -173,7 +173,6 @@ struct ChunkBars {
   ChunkSeg segs[kChSegs];
   uint32_t tmem, abort;
   uint32_t never;    // set where a wait for the list ran out
-  uint32_t there[2][4];  // by group of four warps: whether its last wait, and the one before, came through
   uint32_t has[2][kChRaw];  // 4-bit cache: granules that a raw half has copies of
   uint32_t gone[8];  // granules of a step (by its number in the run, modulo 8) that have no block
 };
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     for (int t = 0; t < 2; ++t) mbar_init(&bars.drained[t], 1);
     for (int i = 0; i < kChSegs; ++i) {
       mbar_init(&bars.seg_full[i], 1);
-      mbar_init(&bars.seg_empty[i], Q4 ? 7 : 11);  // three warps, and the groups of four or their warps
+      mbar_init(&bars.seg_empty[i], S::kThreads / 32 - 1);  // all warps but the one that fills them
     }
     bars.abort = 0;
     bars.never = 0;
@@ -365,24 +364,11 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     }
   };
   bool ok = true;
-  // Softmax warps of the bf16 cache look at a barrier all the time (9 requests of up to 700 on 5001: 87 us; pausing between looks: 89).  Those of the 4-bit cache
-  // pause, as its warps are short of issue slots (1500 on 9000: 217 us; looking all the time: 225), and its groups of four that convert codes wait as one: their
-  // first warp looks, the others wait for it where waiting takes no issue slots.  All four have the same answer, so that they stay together also after a
-  // wait that ran out.
-  auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(warp >> 2) : "memory"); };
-  int nth = 0;
-  auto group_wait = [&](uint64_t* bar, uint32_t parity, uint64_t* also = nullptr, uint32_t its = 0) {
-    if (!Q4) return mbar_spin_warp(bar, parity & 1u, s_abort, a.polls);
-    if (warp < 12) return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
-    if ((warp & 3) == 0) {
-      const bool there = mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls) && (!also || mbar_wait_quick_warp(also, its & 1u, abort_at, a.polls));
-      if (lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
-    }
-    group_sync();
-    // (two words in turn: the first warp may be at the next wait before the last one has read this one's answer)
-    const bool there = *const_cast<volatile uint32_t*>(&bars.there[nth][(warp >> 2) - 1]) != 0;
-    nth ^= 1;
-    return there;
+  // Softmax warps of the bf16 cache look at a barrier all the time (9 requests of up to 700 on 5001: 87 us; pausing between looks: 89).  With the 4-bit cache, whose
+  // warps are short of issue slots, they pause, as its converting warps do (1500 on 9000: 217 us; looking all the time: 225).
+  auto wait_for = [&](uint64_t* bar, uint32_t parity) {
+    if constexpr (!Q4) return mbar_spin_warp(bar, parity & 1u, s_abort, a.polls);
+    return mbar_wait_quick_warp(bar, parity & 1u, abort_at, a.polls);
   };
   // All roles are through; behind it `abort` stays as it is.
   auto settle = [&] {
@@ -395,24 +381,13 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     begin();
 #pragma unroll 1
     for (int k = 0;; ++k) {
-      bool there = true;
-      if (k > 0 && (!Q4 || warp < 4 || (warp & 3) == 0)) there = mbar_wait_call(smem_u32(&bars.seg_full[k % kChSegs]), uint32_t(k / kChSegs) & 1u, never_at, 1u << 22);
-      if (Q4 && warp >= 4) {
-        if ((warp & 3) == 0 && lane == 0) bars.there[nth][(warp >> 2) - 1] = there;
-        group_sync();
-        there = *const_cast<volatile uint32_t*>(&bars.there[nth][(warp >> 2) - 1]) != 0;
-        nth ^= 1;
-      }
-      if (!there) {
+      if (k > 0 && !mbar_wait_call(smem_u32(&bars.seg_full[k % kChSegs]), uint32_t(k / kChSegs) & 1u, never_at, 1u << 22)) {
         *s_abort = 1;
         return;
       }
       const ChunkSeg s = bars.segs[k % kChSegs];
-      if (Q4 && warp >= 4)
-        group_sync();
-      else
-        __syncwarp();
-      if (lane == 0 && (!Q4 || warp < 4 || (warp & 3) == 0)) mbar_arrive(&bars.seg_empty[k % kChSegs]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.seg_empty[k % kChSegs]);
       if (s.n == 0) return;
       f(s, s.ntok > a.T);
     }
@@ -765,7 +740,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           const uint32_t tile = base + (values ? S::kOffV : S::kOffK) + st * S::kKV;
 #pragma unroll 1
           for (int u = 0; u < 2 - (s.cut && j == s.n - 1 ? 1 : 0); ++u) {
-            if (!group_wait(&bars.raw_full[values][rs], rphase, values ? &bars.v_empty[st][u] : &bars.k_empty[st][u], fills.of(j, u) + 1u)) {
+            if (!wait_for(&bars.raw_full[values][rs], rphase) || !wait_for(values ? &bars.v_empty[st][u] : &bars.k_empty[st][u], fills.of(j, u) + 1u)) {
               ok = false;
               return;
             }
@@ -853,7 +828,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
 #pragma unroll 1
       for (int k = 0; k < halves && ok; ++k, ++products) {
         const int j = one_copy(two) ? k >> 1 : (k & ~1) + t, half = k & 1;
-        if (!group_wait(&bars.s_ready[t][half], half ? uses[1] : uses[0])) {
+        if (!wait_for(&bars.s_ready[t][half], half ? uses[1] : uses[0])) {
           ok = false;
           break;
         }
@@ -962,7 +937,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       // ---- the pair's rows, or a piece of them ----
       if (mine == 0) return;
-      if (ok && !group_wait(&bars.o_final[t], pairs)) ok = false;
+      if (ok && !wait_for(&bars.o_final[t], pairs)) ok = false;
       ++pairs;
       const bool join = !two && n > 1;  // the sums of the same rows in two places
       if (join && t == 1) {
@@ -974,7 +949,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       float w0 = 1.f, w1 = 0.f;
       if (join) {
-        if (ok && !(group_wait(&bars.sums, joins) && group_wait(&bars.o_final[1], others))) ok = false;
+        if (ok && !(wait_for(&bars.sums, joins) && wait_for(&bars.o_final[1], others))) ok = false;
         ++joins;
         const float2 ml = s_sums[row];
         const float m = fmaxf(m_used, ml.x), ref = m == -INFINITY ? 0.f : m;
