@@ -799,7 +799,8 @@ class DecodeEngine:
         chose last is not in it yet, and goes first if the text goes on from there), run through the model at most `max_tokens` per pass, also
         within a request, and their keys and values go to the cache.  Returns the next token of every request that got some (int32 [batch]; the
         current input of the others); the next `step` consumes these once they are in `ids`.  With the 4-bit cache a request that rests starts
-        anew, and if the model raises, those that got tokens are finished.  Waits for the GPU."""
+        anew, and if the call raises, those that got tokens are finished; the bf16 cache's requests are then as they were, and so are the rules' tables.
+        Waits for the GPU."""
         return self._extend(ids, lens, max_tokens, None)[0]
 
     def score(self, ids, lens, top: int = 0, max_tokens: int = 8192):
@@ -859,13 +860,6 @@ class DecodeEngine:
         for n in lens:
             first.append(first[-1] + n)
         rows = [b for b in range(self.batch) if lens[b]]
-        if self.counted:
-            gone = torch.zeros(self.batch, dtype=torch.bool)
-            gone[fresh] = True
-            gone = gone.to(dev)
-            self.rules.counts.masked_fill_(gone[:, None], 0)
-            self.rules.seen.masked_fill_(gone[:, None], 0)
-            ops.count_tokens(self.rules, ids, torch.tensor(first, dtype=torch.int32).to(dev), new)
         lasts, kept = [], []
         for t0 in range(0, total, max_tokens):
             t1 = min(t0 + max_tokens, total)
@@ -884,22 +878,42 @@ class DecodeEngine:
         at = torch.tensor(rows).to(dev)
         last = torch.zeros(self.batch, lasts[0].shape[1], dtype=lasts[0].dtype, device=dev)
         last[at] = torch.cat(lasts, 0)
+        tables = [self.rules.counts, self.rules.seen] if self.counted else []
+        before = [t[at] for t in tables]
+        try:
+            return out, self._choose(ids, first, new, fresh, at, last, kept, top, out)
+        except BaseException:
+            # (the tokens are not to be used: they leave no trace in the rules' tables either)
+            for t, rows_before in zip(tables, before):
+                t.index_copy_(0, at, rows_before)
+            raise
+
+    def _choose(self, ids, first, new, fresh, at, last, kept, top, out):
+        """The next tokens of the requests `at`, from their last hidden states, into out; scores of all passes' hidden states `kept`."""
+        dev = ids.device
+        if self.counted:
+            gone = torch.zeros(self.batch, dtype=torch.bool)
+            gone[fresh] = True
+            gone = gone.to(dev)
+            self.rules.counts.masked_fill_(gone[:, None], 0)
+            self.rules.seen.masked_fill_(gone[:, None], 0)
+            ops.count_tokens(self.rules, ids, torch.tensor(first, dtype=torch.int32).to(dev), new)
         nxt = self.m.next_tokens(last, rules=self.rules)
         out[at] = nxt[at]
         if self.counted:
             ops.count_tokens(self.rules, torch.where(new > 0, nxt, -1))
-        if top is None:
-            self._check_chunk()
-            return out, None
-        follows = torch.cat([ids[1:], ids[:1]])
-        follows[torch.tensor([first[b + 1] - 1 for b in rows]).to(dev)] = out[at]
-        parts, t0 = [], 0
-        for hidden in kept:
-            parts.append(self.m.token_logprobs(hidden, follows[t0:t0 + hidden.shape[0]].contiguous(), top))
-            t0 += hidden.shape[0]
+        scores = None
+        if top is not None:
+            follows = torch.cat([ids[1:], ids[:1]])
+            follows[torch.tensor(first[1:]).to(dev)[at] - 1] = out[at]
+            parts, t0 = [], 0
+            for hidden in kept:
+                parts.append(self.m.token_logprobs(hidden, follows[t0:t0 + hidden.shape[0]].contiguous(), top))
+                t0 += hidden.shape[0]
+            scores = ops.TokenLogprobs(*(torch.cat(t, 0) for t in zip(*parts)))
         # (behind the last collective: a rank that raises leaves none of the others waiting)
         self._check_chunk()
-        return out, ops.TokenLogprobs(*(torch.cat(t, 0) for t in zip(*parts)))
+        return scores
 
     def _check_chunk(self):
         """Waits for the passes so far.  RuntimeError if attention over the cache gave up waiting in one of them."""
