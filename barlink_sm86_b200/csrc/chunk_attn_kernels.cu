@@ -39,6 +39,10 @@
 // Tokens of table entries that name no block are left out (their boxes start behind the cache, so TMA fills in zeros).  What stands in the cache
 // behind a request's last token may be anything: the values of the rest of its box are set to zero in shared memory.
 //
+// A pair's products go through the keys of its last token, so that a row meets up to 2 T - 1 values that it does not see; they weigh nothing, but 0 x
+// infinity is NaN.  Rows that end up with a number that is none are looked at by the second kernel: where such a value is hidden from the row, the
+// dims concerned are computed once more from what it sees.
+//
 // Every wait is bounded.  A run that gives up waits for its copies and products, leaves NaN for the rows of its run and sets the error word.
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -78,6 +82,7 @@ struct ChunkMeta {
   int count;                // pieces of the pair that begins in this run and ends in another; 0: none does
   int first;                // its first piece; piece k of the others is the first of run me + k
   int h, row, ntok;         // KV head, first row of q and out, tokens of the pair
+  int odd;                  // whether this run wrote a row that holds an infinity or NaN
 };
 
 // n / d for 0 <= n < 2^31 by a product: with m = ceil(2^(31 + s) / d) and 2^s >= d, m d is above 2^(31 + s) by less than 2^s, which n times over stays
@@ -99,9 +104,12 @@ struct Chunk {
   const int* ctx_lens;
   const int* tables;
   const uint8_t* cache4;
+  const __nv_bfloat16 *q, *k, *v;
   __nv_bfloat16* out;
   float* part;   // [2 * runs][row_cap][hd], then [2 * runs][row_cap] (maximum, sum)
   ChunkMeta* meta;
+  size_t q_stride;
+  int again;     // rows that hold an infinity or NaN are looked at (q is still there)
   int tokens, batch, nq, nkv, G, T, block_size, n_blocks, max_blocks, row_cap, box;
   float scale_log2;
   uint32_t polls;
@@ -341,6 +349,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     s_upto[threadIdx.x] = upto;
     fence_proxy_async_smem();  // (copies go there behind the barriers)
     if (lane == 31) s_scan[warp] = upto;
+    if (threadIdx.x == 0) a.meta[me].odd = 0;  // (ahead of the barrier; whoever sets it is behind)
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -548,7 +557,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           s.i0 = done;
           s.cut = s.keys - (j0 + s.n - 1) * kChKeys <= kChHalf;
           s.piece = s.n == steps ? -1 : 2 * me + (i == 0 ? 0 : 1);
-          if (j0 == 0 && s.n < steps) m = {small_div(lo + i + steps - 1, run) - me + 1, s.piece, h, s.row, s.ntok};
+          if (j0 == 0 && s.n < steps) m = {small_div(lo + i + steps - 1, run) - me + 1, s.piece, h, s.row, s.ntok, 0};
           done += s.n;
           i -= p_at + j0;
           i += p_at = chunk_upto(a, r, ++p, S::kOver);
@@ -590,7 +599,14 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       }
       if (ok) load(s);
     }
-    if (values && lane == 0) a.meta[me] = m;
+    if (values && lane == 0) {
+      ChunkMeta& to = a.meta[me];  // (all but `odd`)
+      to.count = m.count;
+      to.first = m.first;
+      to.h = m.h;
+      to.row = m.row;
+      to.ntok = m.ntok;
+    }
     // The block's shared memory is another's behind it: after a wait that ran out, anyone's, whatever is still on its way lands first.
     const bool gave_up = settle();
     if (gave_up && values)
@@ -969,6 +985,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
       float4* prow = reinterpret_cast<float4*>(a.part) + size_t(s.piece) * (HD / 4) * a.row_cap + at;
       tc_fence_after_sync();
       if (busy) {
+        float2 odd = make_float2(0.f, 0.f);  // NaN from the first number that is none
 #pragma unroll 1
         for (int c0 = 0; c0 < HD; c0 += kCols) {
           uint32_t r[kCols / 16][16], q[kCols / 16][16];
@@ -985,6 +1002,8 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
           float v[kCols];
 #pragma unroll
           for (int c = 0; c < kCols; ++c) v[c] = fmaf(__uint_as_float(q[c >> 4][c & 15]), w1, __uint_as_float(r[c >> 4][c & 15]) * w0);
+#pragma unroll
+          for (int c = 0; c < kCols; c += 2) odd = fma2(make_float2(v[c], v[c + 1]), make_float2(0.f, 0.f), odd);
           if (one_copy(valid && whole)) {
 #pragma unroll
             for (int c = 0; c < kCols; c += 8)
@@ -998,6 +1017,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
         }
         if (!whole && valid)
           reinterpret_cast<float2*>(a.part + size_t(2 * runs) * a.row_cap * HD)[size_t(s.piece) * a.row_cap + at] = make_float2(m_used, ok ? l : NAN);
+        if (whole && valid && odd.x + odd.y != 0.f) a.meta[me].odd = 1;
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -1018,10 +1038,154 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
   if (threadIdx.x == 0 && *s_abort) g_chunk_err = 1;
 }
 
+// Numbers of one token's key or value as a lane of a warp holds them: dims V lane .. V lane + V - 1, V = HD / 32.
+template <int HD>
+struct ChunkLane {
+  static constexpr int V = HD / 32, NA = HD / kQ4Group;
+  static __device__ __forceinline__ void of(const __nv_bfloat16* row, float (&x)[V]) {
+    uint32_t w[V / 2];
+    if constexpr (V == 4) {
+      const uint2 u = *reinterpret_cast<const uint2*>(row + V * (threadIdx.x & 31));
+      w[0] = u.x;
+      w[1] = u.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(row + V * (threadIdx.x & 31));
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+  // token `r` of a tile of the 4-bit cache
+  static __device__ __forceinline__ void of4(const uint8_t* tile, int r, bool value, float (&x)[V]) {
+    const int d = V * (threadIdx.x & 31), ga = d / kQ4Group, in = d % kQ4Group;
+    const uint8_t* codes = value ? tile + q4_v_codes(HD) + (r >> 1) * HD + ((in >> 2) * NA + ga) * 4 : tile + r * (HD / 2) + ((in >> 3) * NA + ga) * 4;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes) >> 4 * (value ? (r & 1) * 4 + (in & 3) : in & 7);
+    const __nv_bfloat16* par = reinterpret_cast<const __nv_bfloat16*>(tile + (value ? q4_v_params(HD) : q4_k_params(HD)) + r * NA * 4);
+    const float step = __bfloat162float(par[ga]), low = __bfloat162float(par[NA + ga]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = __bfloat162float(__float2bfloat16(fmaf(step, float(w >> (4 * e) & 15u), low)));
+  }
+};
+__device__ __forceinline__ bool chunk_odd(float x) { return !(fabsf(x) < INFINITY); }
+
+// A warp looks at one row (token, query head) of the result.  Dims that hold an infinity or NaN, where a value of the pair's keys that the row does not
+// see is one, are computed from the keys that it sees; where one of these is none either, the dim stays as it is.  As plain as can be, as no row of a sound
+// cache comes here: 0.2 us a key and row (4-bit cache 0.4).  One NaN behind 2048 tokens on 16383, 40/8x128: 1880 rows, 12 ms (26).
+template <int HD, bool Q4>
+__device__ __noinline__ void chunk_again(const Chunk& a, int row, int head) {
+  using L = ChunkLane<HD>;
+  constexpr int V = L::V, kAhead = 8;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31, h = head / a.G;
+  __nv_bfloat16* to = a.out + (size_t(row) * a.nq + head) * HD;
+  float x[V];
+  L::of(to, x);
+  uint32_t bad = 0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) bad |= uint32_t(chunk_odd(x[e])) << e;
+  if (!__any_sync(kAll, bad)) return;
+  int b = -1;
+#pragma unroll 1
+  for (int b0 = 0; b0 < a.batch && b < 0; b0 += 32) {
+    bool here = false;
+    if (b0 + lane < a.batch) {
+      const ChunkReq r = chunk_req(a, b0 + lane);
+      here = row >= r.q0 && row - r.q0 < r.n;
+    }
+    const uint32_t found = __ballot_sync(kAll, here);
+    if (found) b = b0 + __ffs(found) - 1;
+  }
+  if (b < 0) return;  // a row of no request: whatever stands there
+  const ChunkReq r = chunk_req(a, b);
+  const int tok = row - r.q0, tok0 = tok / (2 * a.T) * (2 * a.T);
+  const int lim = max(min(r.past + tok + 1, r.cap), 0), keys = chunk_keys(r, tok0, min(2 * a.T, r.n - tok0));
+  const int* table = a.tables + size_t(b) * a.max_blocks;
+  // token t of the head: the row of the cache, -1: no block has it
+  auto look = [&](int t) {
+    const int page = t / a.block_size, blk = table[page];
+    return blk < 0 || blk >= a.n_blocks ? -1 : (blk * a.nkv + h) * a.block_size + t - page * a.block_size;
+  };
+  // (-1: of some row, so that loads wait for no branch)
+  auto load = [&](int at, bool value, float (&y)[V]) {
+    at = max(at, 0);
+    if constexpr (Q4)
+      L::of4(a.cache4 + size_t(at / kQ4Tokens) * q4_tile_bytes(HD), at % kQ4Tokens, value, y);
+    else
+      L::of((value ? a.v : a.k) + size_t(at) * HD, y);
+  };
+  // ---- values that the row does not see ----
+  uint32_t hidden = 0;
+#pragma unroll 1
+  for (int t0 = lim; t0 < keys; t0 += 32) {
+    const int mine = t0 + lane < keys ? look(t0 + lane) : -1;
+#pragma unroll kAhead
+    for (int k = 0; k < 32; ++k) {
+      const int at = __shfl_sync(kAll, mine, k);
+      float y[V];
+      load(at, true, y);
+#pragma unroll
+      for (int e = 0; e < V; ++e) hidden |= uint32_t(at >= 0 && chunk_odd(y[e])) << e;
+    }
+  }
+  bad &= hidden;
+  if (!__any_sync(kAll, bad)) return;
+  // ---- the row from what it sees, the last key first ----
+  float q[V], acc[V] = {}, m = -INFINITY, l = 0.f;
+  L::of(a.q + size_t(row) * a.q_stride + size_t(head) * HD, q);
+#pragma unroll 1
+  for (int t1 = lim; t1 > 0; t1 -= 32) {
+    const int mine = t1 - 1 - lane >= 0 ? look(t1 - 1 - lane) : -1;
+#pragma unroll 1
+    for (int k0 = 0; k0 < 32; k0 += kAhead) {
+      float s[kAhead], y[kAhead][V], v[kAhead][V], top = m;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int at = __shfl_sync(kAll, mine, k0 + k);
+        load(at, false, y[k]);
+        load(at, true, v[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const bool there = __shfl_sync(kAll, mine, k0 + k) >= 0;
+        s[k] = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          s[k] = fmaf(q[e], y[k][e], s[k]);
+          v[k][e] = there ? v[k][e] : 0.f;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s[k] += __shfl_xor_sync(kAll, s[k], o);
+        s[k] = there ? s[k] * a.scale_log2 : -INFINITY;
+        top = fmaxf(top, s[k]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top, alpha = ex2_approx(m - ref);
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] *= alpha;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const float p = ex2_approx(s[k] - ref);
+        l += p;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(p, v[k][e], acc[e]);
+      }
+    }
+    // dims of which the row sees a value that is none
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (chunk_odd(acc[e])) bad &= ~(1u << e);
+    if (!__any_sync(kAll, bad)) return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (bad >> e & 1u) to[V * lane + e] = __float2bfloat16(acc[e] * inv);
+}
+
 // Pieces of a pair that was cut: block (run where it begins, 32 rows), a lane a row, a warp HD / 8 of its dims.
 constexpr int kChMergeWarps = 8, kChMergeAhead = 4;  // pieces that are asked for at once
 template <int HD>
-__global__ void __launch_bounds__(kChMergeWarps * 32) k_chunk_merge(const Chunk a) {
+__global__ void __launch_bounds__(kChMergeWarps * 32, 2) k_chunk_merge(const __grid_constant__ Chunk a) {
   constexpr int V = HD / 4 / kChMergeWarps;  // vectors of four dims
   pdl_launch_dependents();
   pdl_wait();
@@ -1029,50 +1193,94 @@ __global__ void __launch_bounds__(kChMergeWarps * 32) k_chunk_merge(const Chunk 
   const ChunkMeta m = a.meta[me];
   const int r = blockIdx.y * 32 + (threadIdx.x & 31), tok = r / a.G, g = r - tok * a.G;
   // (every run leaves its words; lengths that another stream changes meanwhile, which nobody may, could leave some that fit nothing)
-  if (m.count <= 0 || m.count > runs - me || m.ntok > 2 * a.T || tok >= m.ntok) return;
-  const int at = (tok >= a.T ? kChRows + (tok - a.T) * a.G : tok * a.G) + g;
-  const float2* sums = reinterpret_cast<const float2*>(a.part + size_t(2 * runs) * a.row_cap * HD) + at;
-  const float4* part = reinterpret_cast<const float4*>(a.part) + size_t(warp * V) * a.row_cap + at;
-  float M = -INFINITY, L = 0.f;
-  float4 acc[V];
+  int odd = m.odd;  // 1: rows that the run's first kernel wrote, 2: rows joined here
+  const bool cut = m.count > 0 && m.count <= runs - me && m.ntok <= 2 * a.T;
+  if (cut && tok < m.ntok) {
+    const int at = (tok >= a.T ? kChRows + (tok - a.T) * a.G : tok * a.G) + g;
+    const float2* sums = reinterpret_cast<const float2*>(a.part + size_t(2 * runs) * a.row_cap * HD) + at;
+    const float4* part = reinterpret_cast<const float4*>(a.part) + size_t(warp * V) * a.row_cap + at;
+    float M = -INFINITY, L = 0.f;
+    float4 acc[V];
 #pragma unroll
-  for (int d = 0; d < V; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int d = 0; d < V; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-  for (int k = 0; k < m.count; k += kChMergeAhead) {
-    float2 ml[kChMergeAhead];
-    float4 v[kChMergeAhead][V];
+    for (int k = 0; k < m.count; k += kChMergeAhead) {
+      float2 ml[kChMergeAhead];
+      float4 v[kChMergeAhead][V];
 #pragma unroll
-    for (int e = 0; e < kChMergeAhead; ++e) {
-      ml[e] = make_float2(-INFINITY, 0.f);
+      for (int e = 0; e < kChMergeAhead; ++e) {
+        ml[e] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int d = 0; d < V; ++d) v[e][d] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k + e < m.count) {
-        const size_t p = size_t(k + e == 0 ? m.first : 2 * (me + k + e)) * a.row_cap;
-        ml[e] = sums[p];
+        for (int d = 0; d < V; ++d) v[e][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k + e < m.count) {
+          const size_t p = size_t(k + e == 0 ? m.first : 2 * (me + k + e)) * a.row_cap;
+          ml[e] = sums[p];
 #pragma unroll
-        for (int d = 0; d < V; ++d) v[e][d] = part[p * (HD / 4) + size_t(d) * a.row_cap];
+          for (int d = 0; d < V; ++d) v[e][d] = part[p * (HD / 4) + size_t(d) * a.row_cap];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kChMergeAhead; ++e) {
+        const float n = fmaxf(M, ml[e].x), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(ml[e].x - ref);
+        M = n;
+        L = L * s0 + ml[e].y * s1;
+#pragma unroll
+        for (int d = 0; d < V; ++d) {
+          acc[d].x = acc[d].x * s0 + v[e][d].x * s1;
+          acc[d].y = acc[d].y * s0 + v[e][d].y * s1;
+          acc[d].z = acc[d].z * s0 + v[e][d].z * s1;
+          acc[d].w = acc[d].w * s0 + v[e][d].w * s1;
+        }
       }
     }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    __nv_bfloat16* to = a.out + (size_t(m.row + tok) * a.nq + size_t(m.h) * a.G + g) * HD + 4 * V * warp;
 #pragma unroll
-    for (int e = 0; e < kChMergeAhead; ++e) {
-      const float n = fmaxf(M, ml[e].x), ref = n == -INFINITY ? 0.f : n, s0 = ex2_approx(M - ref), s1 = ex2_approx(ml[e].x - ref);
-      M = n;
-      L = L * s0 + ml[e].y * s1;
+    for (int d = 0; d < V; d += 2)
+      *reinterpret_cast<uint4*>(to + 4 * d) = make_uint4(pack_bf16x2(acc[d].x * inv, acc[d].y * inv), pack_bf16x2(acc[d].z * inv, acc[d].w * inv),
+                                                         pack_bf16x2(acc[d + 1].x * inv, acc[d + 1].y * inv), pack_bf16x2(acc[d + 1].z * inv, acc[d + 1].w * inv));
 #pragma unroll
-      for (int d = 0; d < V; ++d) {
-        acc[d].x = acc[d].x * s0 + v[e][d].x * s1;
-        acc[d].y = acc[d].y * s0 + v[e][d].y * s1;
-        acc[d].z = acc[d].z * s0 + v[e][d].z * s1;
-        acc[d].w = acc[d].w * s0 + v[e][d].w * s1;
-      }
+    for (int d = 0; d < V; ++d)
+      if (chunk_odd(acc[d].x * inv) || chunk_odd(acc[d].y * inv) || chunk_odd(acc[d].z * inv) || chunk_odd(acc[d].w * inv)) odd |= 2;
+  }
+  // ---- numbers that are none ----
+  auto again = [&](int row, int head) {
+    if (a.cache4)
+      chunk_again<HD, true>(a, row, head);
+    else
+      chunk_again<HD, false>(a, row, head);
+  };
+  if (!__syncthreads_or(odd) || !a.again) return;
+  if (__syncthreads_or(odd & 2)) {
+#pragma unroll 1
+    for (int i = warp; i < 32; i += kChMergeWarps) {
+      const int rr = blockIdx.y * 32 + i, t = rr / a.G;
+      if (t < m.ntok) again(m.row + t, m.h * a.G + rr - t * a.G);
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  __nv_bfloat16* to = a.out + (size_t(m.row + tok) * a.nq + size_t(m.h) * a.G + g) * HD + 4 * V * warp;
-#pragma unroll
-  for (int d = 0; d < V; d += 2)
-    *reinterpret_cast<uint4*>(to + 4 * d) = make_uint4(pack_bf16x2(acc[d].x * inv, acc[d].y * inv), pack_bf16x2(acc[d].z * inv, acc[d].w * inv),
-                                                       pack_bf16x2(acc[d + 1].x * inv, acc[d + 1].y * inv), pack_bf16x2(acc[d + 1].z * inv, acc[d + 1].w * inv));
+  if (odd & 1) {
+    // all rows, shared out among the runs that have some
+    int many = 0, mine = 0;
+#pragma unroll 1
+    for (int i = 0; i < runs; ++i) {
+      const int has = a.meta[i].odd != 0;
+      many += has;
+      mine += i < me && has;
+    }
+    const int64_t rows = int64_t(a.tokens) * a.nq;
+#pragma unroll 1
+    for (int64_t i = (int64_t(mine) * gridDim.y + blockIdx.y) * kChMergeWarps + warp; i < rows; i += int64_t(many) * gridDim.y * kChMergeWarps) {
+      const int row = int(i / a.nq), head = int(i - int64_t(row) * a.nq);
+      // (pairs that were cut are their own blocks')
+      bool other = false;
+#pragma unroll 1
+      for (int k = threadIdx.x & 31; k < runs; k += 32) {
+        const ChunkMeta c = a.meta[k];
+        other |= c.count > 0 && row >= c.row && row - c.row < c.ntok && head / a.G == c.h;
+      }
+      if (!__any_sync(0xffffffffu, other)) again(row, head);
+    }
+  }
 }
 
 }  // namespace bl
@@ -1147,6 +1355,16 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   a.part = static_cast<float*>(ws);
   a.row_cap = chunk_row_cap(tokens, a.G);
   a.meta = reinterpret_cast<ChunkMeta*>(a.part + 2 * size_t(runs) * a.row_cap * (hd + 2));
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.k = static_cast<const __nv_bfloat16*>(k_cache);
+  a.v = static_cast<const __nv_bfloat16*>(v_cache);
+  a.q_stride = size_t(tokens > 1 ? q_stride : 0);
+  {
+    // (where the result takes the queries' place, none are left to compute anything with)
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+    const uintptr_t q1 = q0 + (size_t(tokens - 1) * a.q_stride + size_t(nq) * hd) * 2, o1 = o0 + size_t(tokens) * nq * hd * 2;
+    a.again = q1 <= o0 || o1 <= q0;
+  }
   a.tokens = tokens; a.batch = batch; a.nq = nq; a.nkv = nkv; a.block_size = block_size; a.n_blocks = n_blocks; a.max_blocks = max_blocks;
   a.box = block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : 16;
   a.scale_log2 = scale * 1.4426950408889634f;

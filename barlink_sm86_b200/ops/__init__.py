@@ -482,9 +482,10 @@ def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv,
     token i of n sees the keys 0 .. ctx - n + i.  block_tables int32 [batch, max_blocks]; k_cache, v_cache bf16 [blocks, nkv, block_size, hd].
 
     hd 64 or 128, block_size a multiple of 16, at most 128 query heads per KV head, scale > 0.  A table entry that names no block, and a
-    table that ends early, leave their tokens out; a token that sees no key gets zeros.  What the cache holds behind a request's last token
-    is of no account; within it, a value that is no finite number may also show in tokens just before it (up to 63).  Rows
-    that belong to no request are not written (nor set in a new tensor).  Returns bf16 [tokens, nq * hd]."""
+    table that ends early, leave their tokens out; a token that sees no key gets zeros.  What a token does not see is of no
+    account to it, infinities and NaN among it, whether it is behind the request's last token or behind this one.  (Where a value of the latter kind is
+    none, the numbers that it could have reached are computed once more, a row at a time, if out is no part of q's memory.)  Rows that belong to no
+    request are not written (nor set in a new tensor).  Returns bf16 [tokens, nq * hd]."""
     if v_cache is None:
         raise ValueError("paged_attn_chunk needs keys and values; the 4-bit cache is paged_attn_chunk_q4's")
     if q.is_cuda:

@@ -437,7 +437,12 @@ def _paged_attn_chunk(q, n_blocks, bs, block_tables, cu_q, ctx_lens, nq, nkv, hd
         seen = t <= (ctx - n + torch.arange(n))[:, None]
         s = torch.where(seen, s, torch.full_like(s, -math.inf))
         p = torch.where(seen.any(-1)[:, None], torch.softmax(s, -1), torch.zeros_like(s))
-        out[lo:lo + n] = torch.einsum("hgnt,thd->nhgd", p, v).reshape(n, nq * hd).to(q.dtype)
+        o = torch.einsum("hgnt,thd->nhgd", p, v)
+        if not torch.isfinite(v).all():
+            # (0 x infinity is NaN: a row is made from the values that it sees)
+            for i in range(n):
+                o[i] = torch.einsum("hgt,thd->hgd", p[:, :, i, seen[i]], v[seen[i]])
+        out[lo:lo + n] = o.reshape(n, nq * hd).to(q.dtype)
     return out
 
 
