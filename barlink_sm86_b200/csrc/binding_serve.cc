@@ -185,7 +185,7 @@ at::Tensor paged_attn_decode_q4(const at::Tensor& q, const at::Tensor& cache, co
 
 // k_cache and v_cache bf16 [blocks, nkv, block, hd], or (v_cache none) the 4-bit cache
 at::Tensor paged_attn_chunk(const at::Tensor& q, const at::Tensor& cache, const OptTensor& v_cache, const at::Tensor& block_tables, const at::Tensor& cu_q,
-                            const at::Tensor& ctx_lens, int nq, int nkv, int hd, double scale, const OptTensor& out_opt) {
+                            const at::Tensor& ctx_lens, int nq, int nkv, int hd, double scale, const OptTensor& out_opt, const OptTensor& error) {
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kBFloat16 && q.dim() == 2 && (q.stride(1) == 1 || q.size(1) == 1) && (q.size(0) < 2 || q.stride(0) % 8 == 0) && aligned16(q),
               "barlink: q/qkv must be a 2-D bfloat16 CUDA tensor whose rows start on 16-byte boundaries");
   TORCH_CHECK(hd == 64 || hd == 128, "barlink: attention of a chunk over the paged cache is built for head_dim 64 and 128");
@@ -212,6 +212,7 @@ at::Tensor paged_attn_chunk(const at::Tensor& q, const at::Tensor& cache, const 
   const int* bt = i32(block_tables, q, -1, "block_tables");
   const int* cu = i32(cu_q, q, int64_t(batch) + 1, "cu_q");
   const int* cl = i32(ctx_lens, q, batch, "ctx_lens");
+  unsigned* word = error ? reinterpret_cast<unsigned*>(const_cast<int*>(i32(*error, q, 1, "error"))) : nullptr;
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = out_opt ? *out_opt : fresh({tokens, int64_t(nq) * hd}, at::kBFloat16, q);
   check_on(out, q, "out");
@@ -221,14 +222,14 @@ at::Tensor paged_attn_chunk(const at::Tensor& q, const at::Tensor& cache, const 
   if (tokens > 0 && batch > 0) {
     const size_t bytes = bl_paged_attn_chunk_ws(tokens, nq, nkv, hd);
     at::Tensor ws = fresh({int64_t(bytes)}, at::kByte, q);
-    BL_CHECK(bl_paged_attn_chunk(q.data_ptr(), int(tokens > 1 ? q.stride(0) : int64_t(nq) * hd), v_cache ? cache.data_ptr() : nullptr,
+    BL_CHECK(bl_paged_attn_chunk_say(q.data_ptr(), int(tokens > 1 ? q.stride(0) : int64_t(nq) * hd), v_cache ? cache.data_ptr() : nullptr,
                                  v_cache ? v_cache->data_ptr() : nullptr, v_cache ? nullptr : cache.data_ptr(), bt, cu, cl, out.data_ptr(), tokens, batch, nq, nkv,
                                  hd, block_size, small(cache.size(0), "blocks"), small(block_tables.size(1), "max_blocks"), float(scale), ws.data_ptr(), bytes,
-                                 stream_of(q), err, errlen));
+                                 word, stream_of(q), err, errlen));
   }
   return out;
 }
-// The error word of that kernel, into a pinned int32 tensor on the current stream of a device.
+// The word that its calls without one of their own set, into a pinned int32 tensor on the current stream of a device.
 void chunk_attn_error_into(const at::Tensor& out, int dev) {
   TORCH_CHECK(out.is_cpu() && out.is_pinned() && out.scalar_type() == at::kInt && out.numel() == 1, "barlink: chunk_attn_error_into needs a pinned int32 element");
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
@@ -413,7 +414,7 @@ void bind_serve(py::module_& m) {
   m.def("kv4_error_into", &kv4_error_into, py::arg("out"), py::arg("device") = 0);
   m.def("kv4_wait_polls", &bl_kv4_wait_polls, py::arg("polls"));
   m.def("paged_attn_chunk", &paged_attn_chunk, py::arg("q"), py::arg("cache"), py::arg("v_cache"), py::arg("block_tables"), py::arg("cu_q"),
-        py::arg("ctx_lens"), py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none());
+        py::arg("ctx_lens"), py::arg("nq"), py::arg("nkv"), py::arg("hd"), py::arg("scale"), py::arg("out") = py::none(), py::arg("error") = py::none());
   m.def("chunk_attn_error_into", &chunk_attn_error_into, py::arg("out"), py::arg("device") = 0);
   m.def("chunk_attn_error_clear", &chunk_attn_error_clear, py::arg("device") = 0);
   m.def("chunk_attn_wait_polls", &bl_chunk_attn_wait_polls, py::arg("polls"));

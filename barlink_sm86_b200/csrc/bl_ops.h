@@ -505,13 +505,17 @@ int bl_logit_rules(const blRulesArgs* a, void* stream, char* err, size_t errlen)
  * sees keys 0 .. ctx - n + i; a row that sees none gets zeros; rows before cu_q[0] and behind cu_q[batch] are not written.  k_cache, v_cache:
  * bf16 [n_blocks][nkv][block_size][hd]; or, with both null, cache4: as bl_rope_kv_write_q4 leaves it, keys and values as bl_kv4_read gives them.  A block-table
  * entry that names no block leaves its tokens out.  hd 64 or 128, block_size a multiple of 16, at most 128 query heads per KV head, scale > 0.
- * ws: bl_paged_attn_chunk_ws bytes of this call's own, 16-byte aligned.  A wait that runs out sets the current device's error word, which
- * bl_chunk_attn_error_async copies to `out` (pinned) on a stream and bl_chunk_attn_error_clear sets back, and leaves NaN in the rows
- * concerned.  bl_chunk_attn_wait_polls: as bl_kv4_wait_polls. */
+ * ws: bl_paged_attn_chunk_ws bytes of this call's own, 16-byte aligned.  A wait that runs out leaves NaN in the rows concerned and sets
+ * a word to 1: `error` of bl_paged_attn_chunk_say (the caller's own, on the device; nobody else's calls set it, and no call sets it back), or, where there is none,
+ * the current device's, which bl_chunk_attn_error_async copies to `out` (pinned) on a stream and bl_chunk_attn_error_clear sets
+ * back.  bl_chunk_attn_wait_polls: as bl_kv4_wait_polls. */
 size_t bl_paged_attn_chunk_ws(int tokens, int nq, int nkv, int hd);
 int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_cache, const void* v_cache, const void* cache4, const int* block_tables,
                         const int* cu_q, const int* ctx_lens, void* out, int tokens, int batch, int nq, int nkv, int hd, int block_size,
                         int n_blocks, int max_blocks, float scale, void* ws, size_t ws_bytes, void* stream, char* err, size_t errlen);
+int bl_paged_attn_chunk_say(const void* q, int q_stride, const void* k_cache, const void* v_cache, const void* cache4, const int* block_tables,
+                            const int* cu_q, const int* ctx_lens, void* out, int tokens, int batch, int nq, int nkv, int hd, int block_size,
+                            int n_blocks, int max_blocks, float scale, void* ws, size_t ws_bytes, unsigned* error, void* stream, char* err, size_t errlen);
 int bl_chunk_attn_error_async(unsigned* out, void* stream, char* err, size_t errlen);
 int bl_chunk_attn_error_clear(char* err, size_t errlen);
 unsigned bl_chunk_attn_wait_polls(unsigned polls);

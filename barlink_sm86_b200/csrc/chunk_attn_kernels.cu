@@ -43,7 +43,7 @@
 // infinity is NaN.  Rows that end up with a number that is none are looked at by the second kernel: where such a value is hidden from the row, the
 // dims concerned are computed once more from what it sees.
 //
-// Every wait is bounded.  A run that gives up waits for its copies and products, leaves NaN for the rows of its run and sets the error word.
+// Every wait is bounded.  A run that gives up waits for its copies and products, leaves NaN for the rows of its run and sets the call's error word.
 #include <cuda_bf16.h>
 #include <stdint.h>
 
@@ -76,7 +76,7 @@ constexpr int chunk_over(bool q4) { return q4 ? 4 : 2; }
 constexpr float kChRescale = 8.f;      // log2 units
 constexpr uint32_t kChPolls = 1u << 24;
 
-__device__ uint32_t g_chunk_err;  // set by a wait that ran out; one word per device
+__device__ uint32_t g_chunk_err;  // set by a wait that ran out in a call without a word of its own; one per device
 
 struct ChunkMeta {
   int count;                // pieces of the pair that begins in this run and ends in another; 0: none does
@@ -108,6 +108,7 @@ struct Chunk {
   __nv_bfloat16* out;
   float* part;   // [2 * runs][row_cap][hd], then [2 * runs][row_cap] (maximum, sum)
   ChunkMeta* meta;
+  uint32_t* error;  // the caller's word, or none
   size_t q_stride;
   int again;     // rows that hold an infinity or NaN are looked at (q is still there)
   int tokens, batch, nq, nkv, G, T, block_size, n_blocks, max_blocks, row_cap, box;
@@ -1035,7 +1036,7 @@ __global__ void __launch_bounds__(ChunkShape<HD, Q4>::kThreads, 1)
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, kChTmemCols);
   }
-  if (threadIdx.x == 0 && *s_abort) g_chunk_err = 1;
+  if (threadIdx.x == 0 && *s_abort) *(a.error ? a.error : &g_chunk_err) = 1;
 }
 
 // Numbers of one token's key or value as a lane of a warp holds them: dims V lane .. V lane + V - 1, V = HD / 32.
@@ -1318,6 +1319,14 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
                                    const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int tokens, int batch, int nq,
                                    int nkv, int hd, int block_size, int n_blocks, int max_blocks, float scale, void* ws, size_t ws_bytes,
                                    void* stream, char* err, size_t errlen) {
+  return bl_paged_attn_chunk_say(q, q_stride, k_cache, v_cache, cache4, block_tables, cu_q, ctx_lens, out, tokens, batch, nq, nkv, hd, block_size, n_blocks,
+                                 max_blocks, scale, ws, ws_bytes, nullptr, stream, err, errlen);
+}
+
+extern "C" int bl_paged_attn_chunk_say(const void* q, int q_stride, const void* k_cache, const void* v_cache, const void* cache4,
+                                       const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int tokens, int batch, int nq,
+                                       int nkv, int hd, int block_size, int n_blocks, int max_blocks, float scale, void* ws, size_t ws_bytes,
+                                       unsigned* error, void* stream, char* err, size_t errlen) {
   auto refuse = [&](const char* why) {
     set_err(err, errlen, "barlink: attention of a chunk over the paged cache %s", why);
     return -1;
@@ -1341,6 +1350,7 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(ws)) & 15)
     return refuse("needs tensors on 16-byte boundaries");
   if (!(scale > 0.f) || scale > 3e38f) return refuse("needs a positive scale");
+  if (reinterpret_cast<uintptr_t>(error) & 3) return refuse("needs an error word on its own boundary");
   if (!ws || ws_bytes < bl_paged_attn_chunk_ws(tokens, nq, nkv, hd)) return refuse("needs the workspace that bl_paged_attn_chunk_ws says");
 
   const int runs = sm_count();
@@ -1355,6 +1365,7 @@ extern "C" int bl_paged_attn_chunk(const void* q, int q_stride, const void* k_ca
   a.part = static_cast<float*>(ws);
   a.row_cap = chunk_row_cap(tokens, a.G);
   a.meta = reinterpret_cast<ChunkMeta*>(a.part + 2 * size_t(runs) * a.row_cap * (hd + 2));
+  a.error = error;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.k = static_cast<const __nv_bfloat16*>(k_cache);
   a.v = static_cast<const __nv_bfloat16*>(v_cache);

@@ -413,18 +413,18 @@ class Qwen2Model:
 
         return self._run_layers(ids.to(torch.int32), positions, attn_factory)
 
-    def extend_packed(self, ids, positions, slots, cu, ctx_lens, cache):
+    def extend_packed(self, ids, positions, slots, cu, ctx_lens, cache, error=None):
         """New tokens of requests that may have tokens in the cache already, packed: ids, positions, slots int32 [tokens], cu int32
         [batch + 1], ctx_lens int32 [batch] (tokens in all, the new ones the last of them) -> final normed hidden [tokens, hidden].  Keys and
-        values go to `cache` (PagedKV or PagedKV4) at `slots`; a token attends to its request's cache up to itself."""
+        values go to `cache` (PagedKV or PagedKV4) at `slots`; a token attends to its request's cache up to itself.  error: as ops.paged_attn_chunk has it."""
         nq, nkv, hd = self.nq, self.nkv, self.hd
 
         def attn_factory(li):
             def attn(qkv, bias=None):
                 qkv = self._rope_write(cache, li, qkv, positions, slots, bias)
                 if isinstance(cache, PagedKV4):
-                    return ops.paged_attn_chunk_q4(qkv, cache.kv[li], cache.block_tables, cu, ctx_lens, nq, nkv, hd, self.scale)
-                return ops.paged_attn_chunk(qkv, cache.k[li], cache.v[li], cache.block_tables, cu, ctx_lens, nq, nkv, hd, self.scale)
+                    return ops.paged_attn_chunk_q4(qkv, cache.kv[li], cache.block_tables, cu, ctx_lens, nq, nkv, hd, self.scale, None, error)
+                return ops.paged_attn_chunk(qkv, cache.k[li], cache.v[li], cache.block_tables, cu, ctx_lens, nq, nkv, hd, self.scale, None, error)
             return attn
 
         return self._run_layers(ids.to(torch.int32), positions, attn_factory)
@@ -691,6 +691,7 @@ class DecodeEngine:
         self.ctx_lens = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.slots = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.out_ids = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.gave_up = torch.zeros(1, dtype=torch.int32, device=dev)  # set by this engine's attention of new tokens where a wait ran out
         self.use_graph = use_graph and dev.type == "cuda"
         self.graph = None
         self.attn_splits = attn_splits
@@ -841,6 +842,7 @@ class DecodeEngine:
         try:
             nxt, scores = self._run_extend(ids, lens, new, past, positions, slots, max_tokens, top, fresh, out)
         except BaseException:
+            self.gave_up.zero_()
             # (their blocks were dealt out before the model ran)
             if self.kv_bits == 4:
                 self.finish([b for b in range(self.batch) if lens[b]])
@@ -868,7 +870,7 @@ class DecodeEngine:
             done = [min(max(t1 - first[b], 0), lens[b]) for b in range(self.batch)]
             cu = torch.tensor([0] + share, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
             ctx = past + torch.tensor(done, dtype=torch.int32).to(dev)
-            hidden = self.m.extend_packed(ids[t0:t1].contiguous(), positions[t0:t1].contiguous(), slots[t0:t1].contiguous(), cu, ctx, self.cache)
+            hidden = self.m.extend_packed(ids[t0:t1].contiguous(), positions[t0:t1].contiguous(), slots[t0:t1].contiguous(), cu, ctx, self.cache, self.gave_up)
             ends = [first[b + 1] - 1 - t0 for b in rows if t0 < first[b + 1] <= t1]
             if ends:
                 lasts.append(hidden[torch.tensor(ends).to(dev)])
@@ -919,12 +921,9 @@ class DecodeEngine:
         """Waits for the passes so far.  RuntimeError if attention over the cache gave up waiting in one of them."""
         if self.m.device.type != "cuda":
             return
-        from .. import load_extension
-        ext, dev = load_extension(), self.positions.device.index
-        ext.chunk_attn_error_into(self.h_err, dev)
+        self.h_err.copy_(self.gave_up, non_blocking=True)
         torch.cuda.current_stream(self.m.device).synchronize()
         if int(self.h_err):
-            ext.chunk_attn_error_clear(dev)
             raise RuntimeError("attention over the paged cache gave up waiting for its copies: the tokens of this call are not to be used")
 
     def set_context(self, length: int):

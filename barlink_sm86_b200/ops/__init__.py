@@ -458,7 +458,7 @@ def paged_attn_decode_q4(q, cache, block_tables, ctx_lens, nq, nkv, hd, scale, o
 
 
 # ---------------------------------------------------------------- new tokens over a paged cache
-def _check_chunk(q, shape, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out):
+def _check_chunk(q, shape, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, error):
     if hd not in (64, 128) or nkv < 1 or nq < 1 or nq % nkv or nq // nkv > 128:
         raise ValueError("attention of a chunk over the paged cache is built for head_dim 64 and 128 and up to 128 query heads per KV head")
     if len(shape) != 3 or shape[0] != nkv or shape[1] < 16 or shape[1] % 16 or shape[2] != hd:
@@ -471,9 +471,11 @@ def _check_chunk(q, shape, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out
         raise ValueError("out must be [tokens, nq * hd] of q's type")
     if not scale > 0:
         raise ValueError("attention of a chunk over the paged cache needs a positive scale")
+    if error is not None and (error.dtype != torch.int32 or error.numel() != 1):
+        raise ValueError("error must be one int32 element")
 
 
-def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None):
+def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None, error=None):
     """Attention of new tokens of each request over its paged cache, their own keys and values included (write them first, `rope_kv_write`): a
     prompt in pieces, a further turn, draft tokens to be checked, or a decode step (one token each).
 
@@ -485,26 +487,30 @@ def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv,
     table that ends early, leave their tokens out; a token that sees no key gets zeros.  What a token does not see is of no
     account to it, infinities and NaN among it, whether it is behind the request's last token or behind this one.  (Where a value of the latter kind is
     none, the numbers that it could have reached are computed once more, a row at a time, if out is no part of q's memory.)  Rows that belong to no
-    request are not written (nor set in a new tensor).  Returns bf16 [tokens, nq * hd]."""
+    request are not written (nor set in a new tensor).  Returns bf16 [tokens, nq * hd].
+
+    The kernel's waits for its copies are bounded.  A call in which one ran out leaves NaN in the rows concerned and sets `error` (an int32 element on q's device, the
+    caller's own; it is never set back) to 1.  Without it the call sets a word that all such calls on the device share: `chunk_attn_error_into` and
+    `chunk_attn_error_clear` of the extension."""
     if v_cache is None:
         raise ValueError("paged_attn_chunk needs keys and values; the 4-bit cache is paged_attn_chunk_q4's")
     if q.is_cuda:
         _count(2)
-        return _C().paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
-    _check_chunk(q, k_cache.shape[1:], block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+        return _C().paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, error)
+    _check_chunk(q, k_cache.shape[1:], block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, error)
     if k_cache.shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have one shape")
     out = torch.empty(q.shape[0], nq * hd, dtype=q.dtype) if out is None else out
     return ref.paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
 
 
-def paged_attn_chunk_q4(q, cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None):
+def paged_attn_chunk_q4(q, cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None, error=None):
     """`paged_attn_chunk` over a 4-bit cache (`kv4_cache`, written by `rope_kv_write_q4`), with the keys and values that `kv4_read` gives: rounded to
     bf16, which `paged_attn_decode_q4` does without (its results are closer by up to half a step of bf16 a key or value)."""
     if q.is_cuda:
         _count(2)
-        return _C().paged_attn_chunk(q, cache, None, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
-    _check_chunk(q, (cache.shape[1], cache.shape[2] * 16, cache.shape[3] // 20), block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
+        return _C().paged_attn_chunk(q, cache, None, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, error)
+    _check_chunk(q, (cache.shape[1], cache.shape[2] * 16, cache.shape[3] // 20), block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out, error)
     out = torch.empty(q.shape[0], nq * hd, dtype=q.dtype) if out is None else out
     return ref.paged_attn_chunk_q4(q, cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out)
 
