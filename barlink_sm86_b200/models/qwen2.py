@@ -289,6 +289,12 @@ class PagedKV4:
         return sum(t.numel() for t in self.kv)
 
 
+def _no_scores(ids, top):
+    """ops.TokenLogprobs of no rows (ids: of none)."""
+    none = torch.zeros(ids.shape, dtype=torch.float32, device=ids.device)
+    return ops.TokenLogprobs(none, none.new_zeros(0), ids.new_zeros(0, top, dtype=torch.int32), none.new_zeros(0, top))
+
+
 class Qwen2Model:
     def __init__(self, cfg: Qwen2Config, comm: Optional[TPComm] = None, device="cpu",
                  dtype=torch.float32, seed=0, layers=None, quant="none", shard_of=None, source=None):
@@ -634,6 +640,8 @@ class Qwen2Model:
 
     def token_logprobs(self, hidden, ids, top=0, max_rows=1024):
         """ops.TokenLogprobs of `ids` (int32 [rows]) under the logits of hidden [rows, hidden], at most max_rows rows' logits at a time."""
+        if not hidden.shape[0]:
+            return _no_scores(ids, top)
         parts = [self.comm.token_logprobs_vocab_parallel(self.logits_local(hidden[r:r + max_rows]), ids[r:r + max_rows], self.w.vocab_local, self.cfg.vocab, top)
                  for r in range(0, hidden.shape[0], max_rows)]
         return ops.TokenLogprobs(*(torch.cat(t, 0) for t in zip(*parts)))
@@ -820,8 +828,7 @@ class DecodeEngine:
         if not ids.numel():
             if top is None:
                 return out, None
-            none = torch.zeros(0, dtype=torch.float32, device=dev)
-            return out, ops.TokenLogprobs(none, none, torch.zeros(0, top, dtype=torch.int32, device=dev), none.new_zeros(0, top))
+            return out, _no_scores(torch.zeros(0, dtype=torch.int32, device=dev), top)
         ids = ids.to(device=dev, dtype=torch.int32).reshape(-1)
         new = torch.tensor(lens, dtype=torch.int32).to(dev)
         fresh = []

@@ -555,8 +555,9 @@ def token_logprob_parts(logits, ids, top=0, offset=0, vocab=2 ** 31 - 1):
     t = x - torch.where(m == -math.inf, 0.0, m)[:, None]
     e = torch.exp(t)
     parts = torch.stack([m, e.sum(-1), torch.where(t == -math.inf, 0.0, t * e).sum(-1)], 1).float()
-    at = ids.long().view(rows, -1) - offset
-    ok = (ids.view(rows, -1) >= 0) & (at >= 0) & (at < n)
+    wide = ids.reshape(rows, 1 if ids.dim() == 1 else ids.shape[1])
+    at = wide.long() - offset
+    ok = (wide >= 0) & (at >= 0) & (at < n)
     given = torch.where(ok, x.gather(1, torch.where(ok, at, 0)), -math.inf) if n else torch.full(at.shape, -math.inf, dtype=torch.float64)
     order = torch.sort(torch.where(torch.isnan(x), -math.inf, x), dim=-1, descending=True, stable=True)
     val = torch.nn.functional.pad(order.values[:, :top], (0, max(0, top - n)), value=-math.inf)

@@ -255,14 +255,13 @@ class TPComm:
         padding): every rank sends a few words per row -- the sums of its columns, the logits of the given tokens, its most likely tokens -- and
         all have the same result."""
         lo = self.rank * vocab_per_rank
-        if self.world == 1 or self.no_comm:
+        if self.world == 1 or self.no_comm or not ids.shape[0]:
             return _ops.token_logprobs(logits_local, ids, top, lo, vocab)
         given, parts, top_ids, top_val = _ops.token_logprob_parts(logits_local, ids, top, lo, vocab)
-        rows = parts.shape[0]
-        mine = torch.cat([parts, given.reshape(rows, -1), top_val, top_ids.view(torch.float32)], 1)
+        rows, n = parts.shape[0], 1 if ids.dim() == 1 else ids.shape[1]
+        mine = torch.cat([parts, given.reshape(rows, n), top_val, top_ids.view(torch.float32)], 1)
         wide = mine.shape[1]
         got = self.all_gather_cols(torch.nn.functional.pad(mine, (0, -wide % 4)))  # (whole 16-byte vectors)
-        n = given.numel() // max(rows, 1)
         shards = []
         for part in got.view(rows, self.world, wide + -wide % 4).unbind(1):
             p, g, v, i, _ = part.split([3, n, top, top, -wide % 4], 1)
