@@ -25,13 +25,16 @@
 //
 // Measured, as captured and replayed (heads / KV heads x dims; ideal: bytes at the rate of a copy, or products at that of a large matrix product):
 //   bf16   5 tokens on 333, 28/4x128             11 us          two launches and one step's chain: 5 us until the first keys are there, 2 for the pieces
-//          64 requests of up to 8 on 1100        26 us (10)     1.8 pairs a block, of four steps each: the first one's start and every pair's end
-//          9 of up to 700 on 5001, 14/2x128      87 us (42)     the chain below, and pairs' ends
-//          2048 on 16383, 40/8x128              553 us (387)    1.17 PFLOP/s; 630 us where it runs for long and the clock drops
+//          64 requests of up to 8 on 1100        27 us (10)     1.8 pairs a block, of four steps each: the first one's start and every pair's end
+//          9 of up to 700 on 5001, 14/2x128      89 us (42)     the chain below, and pairs' ends; 80 to 89 with other lengths
+//          2048 on 16383, 40/8x128              559 us (387)    1.16 PFLOP/s; 650 us where it runs for long and the clock drops
 //   4-bit  4 on 900, 28/4x128                    13 us          as the first, and the first keys' conversion
-//          64 of up to 6 on 1100                 32 us (3.4)    conversion: some 800 warp instructions a step and quarter of the SM for K and V
-//          2 of up to 13 on 100000, 40/8x128    125 us (29)     the same
-//          1500 on 9000, 28/4x128               221 us (106)    issue slots (half of them used) and the chain
+//          64 of up to 6 on 1100                 32 us (3.4)    as the 64 above, with longer steps
+//          2 of up to 13 on 100000, 40/8x128    125 us (29)     3400 cycles a step (61 a block; 119 to 145 us with other lengths), in which a quarter of the SM
+//                                                              issues 2200 warp instructions: 800 to expand codes, the softmax, and looks at barriers.  35 % of
+//                                                              its slots stay empty: each half step's expansion is a chain of its own (a wait, loads, 200
+//                                                              instructions that depend on one another, stores, a fence), one warp for keys and one for values
+//          1500 on 9000, 28/4x128               221 us (106)    the same, and the softmax of full tiles
 // Where new tokens fill tiles a step of two tiles takes some 3900 cycles of an SM; its products 2560 (S of 64 keys at a time reads its operands from shared
 // memory at three quarters of the rate of 128, which would leave a place no scores to go on with), its exponentials 1540 of the unit for them.  The rest is
 // the chain of a place's half step: products seen to be done, scores read, largest one, exponentials, P seen to be there.

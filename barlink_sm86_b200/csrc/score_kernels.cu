@@ -10,11 +10,13 @@
 // row, are joined afterwards.
 //
 // The `top` greatest: in the first lap 64 groups of four threads each put forward the greatest logit; the top-th greatest of these is one that at least
-// `top` logits reach, so whatever is below it is out; that is the border for all laps.  Those that reach it, hardly more than `top` a lap on logits, are
-// ranked by counting, which gives the order and leaves ties to the lowest index.
+// `top` logits reach, so whatever is below it is out; that is the border for all laps.  Those that reach it, some 1.4 times `top` a lap on logits, are
+// ranked by counting, which gives the order and leaves ties to the lowest index.  Where a block takes many laps for a row they can be more than the list
+// holds (20 alternatives of 152064 fp32 logits, 30 laps: some 720 of 1024, 32: 1290); the greatest are then found one by one from memory, a pass each.
 //
-// Measured, as captured and replayed, 152064 bf16 logits a row: 2000 rows 99 us (6.1 TB/s, 0.94 of the rate of a copy; bound by memory); 64 rows and 5
-// alternatives 12.2 us, one row and 20 alternatives 8.3 us (latency: launch, a trip to memory, border, ranking, the cluster's join).
+// Measured, as captured and replayed, 152064 bf16 logits a row, no alternatives: 2000 rows 99 us (6.1 TB/s, 0.94 of the rate of a copy; bound by memory); 64 rows and 5
+// alternatives 12.2 us, one row and 20 alternatives 8.3 us (latency: launch, a trip to memory, border, ranking, the cluster's join).  2000 rows with 5, 20 and 32 alternatives
+// 143, 235 and 4451 us, fp32 (no alternatives 183) 213, 2953 and 31387: the last ones and that of 20 go by rows whose list overflows.
 #include <math.h>
 #include <stdio.h>
 

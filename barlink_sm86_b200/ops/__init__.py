@@ -477,7 +477,7 @@ def _check_chunk(q, shape, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out
 
 def paged_attn_chunk(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, nq, nkv, hd, scale, out=None, error=None):
     """Attention of new tokens of each request over its paged cache, their own keys and values included (write them first, `rope_kv_write`): a
-    prompt in pieces, a further turn, draft tokens to be checked, or a decode step (one token each).
+    prompt in pieces, a further turn, draft tokens to be checked, or a decode step (one token each; `paged_attn_decode` is made for these).
 
     q bf16 [tokens, >= nq * hd] (the first nq * hd columns; rows start on 16-byte boundaries).  cu_q int32 [batch + 1]: request b's new
     tokens are rows cu_q[b] .. cu_q[b + 1] (none, too); ctx_lens int32 [batch]: its tokens in all, the new ones the last of them, so that new
@@ -667,7 +667,8 @@ def _check_logprobs(logits, ids, top, offset, vocab):
 def token_logprobs(logits, ids, top=0, offset=0, vocab=None):
     """Log probabilities (natural logarithm) of the tokens `ids` (int32 [rows], or [rows, tokens] for several of each row) under logits [rows, n]
     (bf16 or fp32; rows may lie apart), the entropy of every row's distribution, and its `top` (0 to 32) most likely tokens, the most likely
-    first and the lowest of equals, with theirs: a TokenLogprobs, all in fp32, from one pass over the logits.
+    first and the lowest of equals, with theirs: a TokenLogprobs, all in fp32, from one pass over the logits (many alternatives on hundreds of
+    rows take further passes over some rows, up to one for each alternative).
 
     Column i is token i + offset; columns at or beyond `vocab` (the padding of a head) are left out.  Logits of -inf (a mask's) have probability 0.  An
     id that is none of the columns' has log probability -inf.  Where fewer than `top` tokens are above -inf the rest are -1 with -inf; a row with
